@@ -131,6 +131,11 @@ uint64_t sgb_launch_count(const sgb_ctx *ctx);
  * (sgb_decode_paged_q8kv_d128_noalloc caps m_q * q_heads * n_splits at 2048: 64 splits for 32 q heads.) */
 uint32_t sgb_decode_paged_splits_hint(const sgb_ctx *ctx, uint32_t n_kv_heads, uint32_t kv_len);
 
+/* Bytes of the `work` binding of attn_blocks_e4m3_d128 for a dispatch of that grid and push (partial results of requests that
+ * several warps share; its contents mean nothing between dispatches).  Enough for every smaller grid and max_q as well. */
+size_t sgb_attn_blocks_work_bytes(const sgb_ctx *ctx, uint32_t n_kv_heads, uint32_t q_per_kv, uint32_t requests, uint32_t n_tokens,
+                                  uint32_t max_q);
+
 /* ---- record once, replay: record_graph / submit_blocking (crates/sg-gpu/src/graph.rs:523-528, */
 /* 640-642).  Between begin and end every sgb_dispatch / sgb_step_write-free call is captured    */
 /* into a CUDA graph instead of running; the graph keeps its buffers alive.  A replay runs the   */

@@ -1,0 +1,86 @@
+// The 8-bit cache that many requests share: e4m3 numbers in tiles of 16 tokens of one kv head, one power of two per tile.
+//
+//   pool   u8 [block][kv head][16 tokens][128]    2048 consecutive bytes per (block, head); pool row = 16 * block + token in block
+//   exps   i8 [block][kv head]                    value = e4m3 * 2^e, e in [-15, 8] as the append writes it
+//   table  u32 [request][stride]                  token t of request r: row table[r][t / page] * page + t % page
+//
+// The scale is a power of two because e4m3 carries four significant bits whatever its scale: a free factor would buy nothing, and
+// a power of two makes quantising, growing a tile's scale and undoing it exact but for e4m3's own rounding.  Magnitudes above
+// 61440 count as 61440, the largest f16 of four significant bits, so that every cached value is an f16 number; 2^-15 is the least
+// scale because f16's own grid is 2^-24 and e4m3's is 2^-9.
+#pragma once
+
+#include "sgb_common.cuh"
+
+namespace sgb {
+
+constexpr int TILE_TOK = 16;
+constexpr uint32_t TILE_BYTES = TILE_TOK * 128;
+constexpr uint32_t NO_SLOT = 0xffffffffu;
+constexpr int LOWEST_EXP = -15;
+constexpr uint32_t MOST_REQUESTS = 65536;
+
+// What a dispatch over the cache knows of its requests.
+struct Requests {
+    const uint32_t* table;   // [n][stride]
+    const uint32_t* lens;    // [n] keys of each, this step's tokens among them
+    const uint32_t* starts;  // [n + 1] first query token of each
+    uint32_t n, stride, page_shift, pool_pages, tokens, max_q, window;
+    uint32_t* status;
+};
+struct Request {
+    uint32_t first, n, len;  // its query tokens, its keys
+};
+// Lengths come from the device: what does not fit the buffers is reported and taken as nothing (queries) or cut (keys).
+__device__ __forceinline__ Request request_at(const Requests& a, uint32_t r)
+{
+    Request q;
+    q.first = ld_global(a.starts + r);
+    const uint32_t end = ld_global(a.starts + r + 1);
+    q.len = ld_global(a.lens + r);
+    q.n = end - q.first;
+    if (end < q.first || end > a.tokens || q.n > a.max_q) {
+        report_error(a.status, DEV_ERR_BOUNDS, 601, r, end);
+        q.n = 0;
+    }
+    const uint64_t most = (uint64_t)a.stride << a.page_shift;
+    if (q.len > most) {
+        report_error(a.status, DEV_ERR_BOUNDS, 602, r, q.len);
+        q.len = (uint32_t)most;
+    }
+    return q;
+}
+// The pool's block that holds tokens 16 * tile .. of request r; a page that the pool does not have is reported and read as page 0.
+__device__ __forceinline__ uint32_t block_at(const Requests& a, uint32_t r, uint32_t tile)
+{
+    const uint32_t shift = a.page_shift - 4, lp = tile >> shift;
+    uint32_t page = 0;
+    if (lp < a.stride) {
+        page = ld_global(a.table + (size_t)r * a.stride + lp);
+    } else {
+        report_error(a.status, DEV_ERR_BOUNDS, 603, r, lp);
+    }
+    if (page >= a.pool_pages) {
+        report_error(a.status, DEV_ERR_BOUNDS, 604, r, page);
+        page = 0;
+    }
+    return (page << shift) + (tile & ((1u << shift) - 1));
+}
+
+// Two e4m3 bytes as two f16, exactly (one instruction at the rate of an integer one: 64 a clock and SM).
+__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((uint16_t)two_bytes));
+    return r;
+}
+__device__ __forceinline__ uint32_t f16x2_to_e4m3x2(uint32_t x)
+{
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(x));
+    return r;
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+__device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
+
+}  // namespace sgb

@@ -1,0 +1,366 @@
+// A serving step's bookkeeping and its writes into the 8-bit cache of blocks.cuh.
+//
+// kv_block_tables: from the lengths of all requests, which pages each keeps, gives back and takes, and where every new token goes.
+// kv_append_blocks_e4m3_d128: new keys and values into their slots, with one power of two per tile of 16 tokens and head.
+#include "blocks.cuh"
+#include "sgb_kernels.h"
+
+namespace sgb {
+
+namespace {
+
+// ---- block tables and slot maps ------------------------------------------------------------------------------------------------
+// need_r = ceil((ctx_r + new_r) / page).  A request takes part if need_r <= stride and its tokens end within the step's `tokens`.
+// Pages beyond need_r go to the end of the free list, in the order of requests and pages; then pages are taken from the list's
+// end, in the same order, by every request whose wants the list still covers when all before it are counted.  The others are
+// refused: they keep what they hold, their length is 0 and their tokens have no slot.
+//
+// Prefix sums over the requests and little else: bound by its own latency.  One CTA does the sums (1024 requests at a time); a
+// page's number is moved by one lane, a request's pages by one warp.
+constexpr int PLAN_THREADS = 1024, PLAN_WARPS = PLAN_THREADS / 32;
+
+struct PlanArgs {
+    const uint32_t *ctx, *add, *held, *count;
+    uint32_t *free_list, *table, *held_out, *free_out, *starts, *lens, *slots, *at;
+    uint32_t n, tokens, page_shift, stride, capacity;
+    uint32_t* status;
+};
+
+// Exclusive prefix sum over the CTA; `total` is everybody's.
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* warp_sums, uint64_t& total)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    uint64_t x = v;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const uint64_t t = __shfl_up_sync(0xffffffffu, x, off);
+        if (lane >= off) x += t;
+    }
+    __syncthreads();  // the last use of warp_sums is over
+    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();
+    uint64_t s = warp_sums[lane];
+    const uint64_t mine = s;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const uint64_t t = __shfl_up_sync(0xffffffffu, s, off);
+        if (lane >= off) s += t;
+    }
+    total = __shfl_sync(0xffffffffu, s, 31);
+    return __shfl_sync(0xffffffffu, s - mine, warp) + x - v;
+}
+
+// Slot and position of token t of the step.
+__device__ __forceinline__ void place_token(const PlanArgs& a, uint32_t t)
+{
+    uint32_t lo = 0, hi = a.n;  // the request whose tokens t is among: the last one with starts[r] <= t
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (ld_global(a.starts + mid) <= t) lo = mid; else hi = mid;
+    }
+    uint32_t slot = NO_SLOT, pos = 0;
+    if (t < ld_global(a.starts + a.n)) {
+        pos = ld_global(a.ctx + lo) + (t - ld_global(a.starts + lo));
+        if (ld_global(a.lens + lo) != 0) {
+            const uint64_t row = ((uint64_t)ld_global(a.table + (size_t)lo * a.stride + (pos >> a.page_shift)) << a.page_shift) +
+                                 (pos & ((1u << a.page_shift) - 1));
+            if (row < NO_SLOT) slot = (uint32_t)row;
+        }
+    }
+    a.slots[t] = slot;
+    a.at[t] = pos;
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) block_tables_kernel(const PlanArgs a)
+{
+    __shared__ uint64_t sums[PLAN_WARPS];
+    const int lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_launch_dependents();
+    uint32_t count = ld_global(a.count);
+    if (count > a.capacity) {
+        if (threadIdx.x == 0) report_error(a.status, DEV_ERR_BOUNDS, 611, count, a.capacity);
+        count = a.capacity;
+    }
+    struct Mine {
+        uint32_t held, need, add, len;
+        uint64_t end;
+        bool fits;
+    };
+    auto look = [&](uint32_t r, uint64_t& carry) {
+        Mine m{0, 0, 0, 0, 0, false};
+        uint64_t need = 0, len = 0;
+        if (r < a.n) {
+            m.add = ld_global(a.add + r);
+            len = (uint64_t)ld_global(a.ctx + r) + m.add;
+            need = (len + (1u << a.page_shift) - 1) >> a.page_shift;
+            m.held = ld_global(a.held + r);
+            if (m.held > a.stride) {
+                report_error(a.status, DEV_ERR_BOUNDS, 612, r, m.held);
+                m.held = a.stride;
+            }
+        }
+        uint64_t total;
+        m.end = carry + block_scan(m.add, sums, total) + m.add;
+        carry += total;
+        m.fits = r < a.n && need <= a.stride && m.end <= a.tokens && len < NO_SLOT;
+        m.need = m.fits ? (uint32_t)need : 0;
+        m.len = (uint32_t)len;
+        return m;
+    };
+
+    // Pages given back, and where every request's tokens start.
+    uint64_t ends = 0, given = 0;
+    for (uint32_t base = 0; base < a.n; base += PLAN_THREADS) {
+        const uint32_t r = base + threadIdx.x;
+        const Mine m = look(r, ends);
+        const uint32_t back = m.fits && m.held > m.need ? m.held - m.need : 0;
+        uint64_t total;
+        const uint64_t to = count + given + block_scan(back, sums, total);
+        given += total;
+        if (r < a.n) {
+            a.starts[r + 1] = (uint32_t)min(m.end, (uint64_t)a.tokens);
+            if (r == 0) a.starts[0] = 0;
+        }
+        for (uint32_t todo = __ballot_sync(0xffffffffu, back != 0); todo; todo &= todo - 1) {
+            const int src = __ffs(todo) - 1;
+            const uint32_t n = __shfl_sync(0xffffffffu, back, src), from = __shfl_sync(0xffffffffu, m.need, src);
+            const uint64_t at = __shfl_sync(0xffffffffu, to, src);
+            const uint32_t* row = a.table + (size_t)(base + (threadIdx.x & ~31) + src) * a.stride + from;
+            for (uint32_t j = lane; j < n; j += 32) {
+                if (at + j < a.capacity) a.free_list[at + j] = ld_global(row + j);
+                else report_error(a.status, DEV_ERR_BOUNDS, 613, (uint32_t)(at + j), a.capacity);
+            }
+        }
+    }
+    const uint64_t have = min(count + given, (uint64_t)a.capacity);
+    __syncthreads();  // the list is read from here on
+
+    // Pages taken.
+    uint64_t wanted = 0, used = 0, refused = 0, placed = 0;
+    ends = 0;
+    for (uint32_t base = 0; base < a.n; base += PLAN_THREADS) {
+        const uint32_t r = base + threadIdx.x;
+        const Mine m = look(r, ends);
+        const uint32_t want = m.fits && m.need > m.held ? m.need - m.held : 0;
+        uint64_t total;
+        const uint64_t before = wanted + block_scan(want, sums, total);
+        wanted += total;
+        const bool granted = m.fits && (want == 0 || before + want <= have);
+        if (r < a.n) {
+            a.held_out[r] = granted ? m.need : m.held;
+            a.lens[r] = granted ? m.len : 0;
+        }
+        for (uint32_t todo = __ballot_sync(0xffffffffu, granted && want != 0); todo; todo &= todo - 1) {
+            const int src = __ffs(todo) - 1;
+            const uint32_t n = __shfl_sync(0xffffffffu, want, src), to = __shfl_sync(0xffffffffu, m.held, src);
+            const uint64_t at = have - 1 - __shfl_sync(0xffffffffu, before, src);
+            uint32_t* row = a.table + (size_t)(base + (threadIdx.x & ~31) + src) * a.stride + to;
+            for (uint32_t j = lane; j < n; j += 32) row[j] = ld_global(a.free_list + (at - j));
+        }
+        uint64_t sum;
+        block_scan(granted ? want : 0, sums, sum);
+        used += sum;
+        block_scan(r < a.n && !granted, sums, sum);
+        refused += sum;
+        block_scan(granted ? m.add : 0, sums, sum);
+        placed += sum;
+    }
+    if (threadIdx.x == 0) {
+        a.free_out[0] = (uint32_t)(have - used);
+        a.free_out[1] = (uint32_t)refused;
+        a.free_out[2] = (uint32_t)placed;
+        a.free_out[3] = (uint32_t)used;
+    }
+}
+
+__global__ void __launch_bounds__(256) place_tokens_kernel(const PlanArgs a)
+{
+    pdl_wait();
+    pdl_launch_dependents();
+    const uint32_t t = blockIdx.x * 256 + threadIdx.x;
+    if (t < a.tokens) place_token(a, t);
+}
+
+// ---- append --------------------------------------------------------------------------------------------------------------------
+// A run is a stretch of tokens with consecutive slots of one block; its first token leads it.  For every run, kv head and side one
+// warp: A = max |x| over the run's rows, e = the least e >= -15 with A <= 448 * 2^e, no less than the tile's own exponent if
+// the run does not begin the tile; if that grows, the rows before the run are rounded again (q * 2^(old - e)); then the run's rows
+// are written as e4m3(x * 2^-e).  All products are by powers of two and exact in f16 wherever e4m3 does not round them to 0.
+// Two bytes read and one written per value: bound by bytes.
+constexpr int APPEND_THREADS = 256;
+
+struct AppendArgs {
+    const __half* src[2];
+    const uint32_t* slots;
+    uint8_t* pool[2];
+    int8_t* exps[2];
+    uint32_t n, n_kv, blocks;
+    uint32_t* status;
+};
+
+// The least e >= LOWEST_EXP with a <= 448 * 2^e: a = f * 2^k, 1 <= f < 2, 448 = 1.75 * 2^8.
+__device__ __forceinline__ int exponent_for(float a)
+{
+    const uint32_t bits = __float_as_uint(a);
+    const int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return max(e, LOWEST_EXP);
+}
+// 2^e as f16 pair, e in [-24, 15].
+__device__ __forceinline__ __half2 power_of_two(int e) { return __float2half2_rn(__int_as_float((e + 127) << 23)); }
+
+__device__ __forceinline__ void append_run(const AppendArgs& a, int side, uint32_t head, uint32_t t, uint32_t slot, uint32_t run)
+{
+    const uint32_t lane = threadIdx.x & 31, half = lane >> 4, c = lane & 15;
+    const uint32_t block = slot / TILE_TOK, at = slot % TILE_TOK;
+    const size_t tile = (size_t)block * a.n_kv + head;
+    const __half* src = a.src[side] + ((size_t)t * a.n_kv + head) * 128 + c * 8;
+    uint8_t* out = a.pool[side] + tile * TILE_BYTES;
+    uint4 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t j = 2 * i + half;
+        x[i] = make_uint4(0, 0, 0, 0);
+        if (j < run) x[i] = ld_global(reinterpret_cast<const uint4*>(src + (size_t)j * a.n_kv * 128));
+    }
+    int old = LOWEST_EXP;
+    if (at != 0) old = *(volatile const int8_t*)(a.exps[side] + tile);
+    __half2 m = __float2half2_rn(0.0f);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        m = __hmax2(m, __habs2(as_half2(x[i].x)));  // a NaN loses against a number
+        m = __hmax2(m, __habs2(as_half2(x[i].y)));
+        m = __hmax2(m, __habs2(as_half2(x[i].z)));
+        m = __hmax2(m, __habs2(as_half2(x[i].w)));
+    }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) m = __hmax2(m, as_half2(__shfl_xor_sync(0xffffffffu, as_u32(m), off)));
+    const float most = fminf(fmaxf(__low2float(m), __high2float(m)), 61440.0f);
+    const int e = max(exponent_for(most), old);
+    if (at != 0 && e > old) {
+        const __half2 f = power_of_two(max(old - e, -24));
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (4 * i + lane / 8 < at) {
+                uint4* p = reinterpret_cast<uint4*>(out + i * 512 + lane * 16);
+                uint4 v = ld_global(p);
+                uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const uint32_t lo = f16x2_to_e4m3x2(as_u32(__hmul2(as_half2(e4m3x2_to_f16x2(w[k] & 0xffffu)), f)));
+                    const uint32_t hi = f16x2_to_e4m3x2(as_u32(__hmul2(as_half2(e4m3x2_to_f16x2(w[k] >> 16)), f)));
+                    w[k] = lo | (hi << 16);
+                }
+                *p = v;
+            }
+        }
+    }
+    const __half2 f = power_of_two(-e), top = __float2half2_rn(61440.0f), low = __float2half2_rn(-61440.0f);
+    auto quantise = [&](uint32_t w) { return f16x2_to_e4m3x2(as_u32(__hmul2(__hmax2_nan(__hmin2_nan(as_half2(w), top), low), f))); };
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t j = 2 * i + half;
+        if (j < run)
+            *reinterpret_cast<uint2*>(out + (at + j) * 128 + c * 8) =
+                make_uint2(quantise(x[i].x) | (quantise(x[i].y) << 16), quantise(x[i].z) | (quantise(x[i].w) << 16));
+    }
+    if (lane == 0) a.exps[side][tile] = (int8_t)e;
+}
+
+// SPAN tokens of the slot map per warp, kv head and side.
+template <int SPAN>
+__global__ void __launch_bounds__(APPEND_THREADS) append_blocks_kernel(const AppendArgs a)
+{
+    pdl_wait();
+    pdl_launch_dependents();
+    const uint32_t lane = threadIdx.x & 31;
+    const uint64_t unit = (uint64_t)blockIdx.x * (APPEND_THREADS / 32) + threadIdx.x / 32;
+    const int side = (int)(unit & 1);
+    const uint32_t head = (uint32_t)((unit >> 1) % a.n_kv);
+    const uint64_t t0 = (unit >> 1) / a.n_kv * SPAN;
+    if (t0 >= a.n) return;
+    uint32_t mine = NO_SLOT, before = NO_SLOT;
+    if (lane < SPAN && t0 + lane < a.n) {
+        mine = ld_global(a.slots + t0 + lane);
+        if (t0 + lane > 0) before = ld_global(a.slots + t0 + lane - 1);
+    }
+    bool leads = false;
+    if (mine != NO_SLOT) {
+        if (mine / TILE_TOK >= a.blocks) {
+            report_error(a.status, DEV_ERR_BOUNDS, 621, mine, a.blocks);
+        } else if (before != NO_SLOT && before / TILE_TOK == mine / TILE_TOK && before + 1 != mine) {
+            report_error(a.status, DEV_ERR_BOUNDS, 622, before, mine);  // a tile's tokens stand in its order
+        } else {
+            leads = !(before != NO_SLOT && before + 1 == mine && mine % TILE_TOK != 0);
+        }
+    }
+    for (uint32_t todo = __ballot_sync(0xffffffffu, leads); todo; todo &= todo - 1) {
+        const int src = __ffs(todo) - 1;
+        const uint32_t slot = __shfl_sync(0xffffffffu, mine, src), t = (uint32_t)t0 + src;
+        bool follows = false;
+        if (lane < TILE_TOK - slot % TILE_TOK && (uint64_t)t + lane < a.n) follows = ld_global(a.slots + t + lane) == slot + lane;
+        const uint32_t run = __ffs(~__ballot_sync(0xffffffffu, follows)) - 1;
+        append_run(a, side, head, t, slot, run);
+    }
+}
+
+struct PushPlan {
+    uint32_t page, stride;
+};
+
+}  // namespace
+
+// kv_block_tables: ctx, add, held, count, free list, table, held out, free out, starts, lens, slots, positions.
+// push {page, table stride}.  grid [requests, tokens].
+int launch_kv_block_tables(const LaunchArgs& a)
+{
+    const PushPlan p = *(const PushPlan*)a.push;
+    const uint32_t n = a.groups[0], tokens = a.groups[1];
+    if (n == 0 || n > MOST_REQUESTS) return fail_validation(a, "block_tables: groups[0] (requests) must be 1..65536");
+    if (tokens == 0) return fail_validation(a, "block_tables: groups[1] (tokens of the step) must be > 0");
+    if (p.page < (uint32_t)TILE_TOK || (p.page & (p.page - 1))) return fail_validation(a, "block_tables: page must be a power of two, at least 16 tokens");
+    if (p.stride == 0) return fail_validation(a, "block_tables: the table's stride must be > 0");
+    if (int r = need_aligned(a, {4, 4, 4, 4, 4, 4, 4, 4, 4, 4, 4, 4})) return r;
+    const size_t per = 4 * (size_t)n;
+    const char* names[12] = {"ctx", "new", "held", "count", "free list", "table", "held out", "free out", "starts", "lens", "slots", "positions"};
+    const size_t bytes[12] = {per, per, per, 4, 4, per * p.stride, per, 16, per + 4, per, 4 * (size_t)tokens, 4 * (size_t)tokens};
+    for (int i = 0; i < 12; i++)
+        if (int r = need_bytes(a, i, bytes[i], names[i])) return r;
+    const auto u = [&](int i) { return (uint32_t*)a.b[i].ptr; };
+    const size_t capacity = a.b[4].bytes / 4;
+    PlanArgs k{u(0), u(1), u(2), u(3), u(4), u(5), u(6), u(7), u(8), u(9), u(10), u(11), n, tokens, (uint32_t)__builtin_ctz(p.page), p.stride,
+               (uint32_t)(capacity < NO_SLOT ? capacity : NO_SLOT), a.status};
+    cudaError_t e = launch_dependent(block_tables_kernel, dim3(1), dim3(PLAN_THREADS), 0, a.stream, k);
+    ++*a.launches;
+    if (int r = check_cuda(a, e, "kv_block_tables")) return r;
+    e = launch_dependent(place_tokens_kernel, dim3((unsigned)((tokens + 255ull) / 256)), dim3(256), 0, a.stream, k);
+    ++*a.launches;
+    return check_cuda(a, e, "kv_block_tables tokens");
+}
+
+// kv_append_blocks_e4m3_d128: k, v f16 [n x KV x 128], slots, k pool, k exps, v pool, v exps.  grid [KV, n].
+int launch_kv_append_blocks(const LaunchArgs& a)
+{
+    const uint32_t n_kv = a.groups[0], n = a.groups[1];
+    if (n_kv == 0 || n == 0) return fail_validation(a, "append_blocks: groups must be [kv heads, tokens]");
+    const size_t tile_row = (size_t)n_kv * TILE_BYTES, src = (size_t)n * n_kv * 256;
+    const size_t blocks = a.b[3].bytes / tile_row;
+    if (int r = need_bytes(a, 0, src, "k")) return r;
+    if (int r = need_bytes(a, 1, src, "v")) return r;
+    if (int r = need_bytes(a, 2, 4 * (size_t)n, "slots")) return r;
+    if (blocks == 0 || a.b[5].bytes / tile_row != blocks)
+        return fail_validation(a, "append_blocks: K and V pools must hold the same (non-zero) number of 16-token blocks");
+    if (blocks > NO_SLOT / TILE_TOK) return fail_validation(a, "append_blocks: a pool holds less than 2^32 rows");
+    if (int r = need_bytes(a, 4, blocks * n_kv, "k exponents")) return r;
+    if (int r = need_bytes(a, 6, blocks * n_kv, "v exponents")) return r;
+    if (int r = need_aligned(a, {16, 16, 4, 16, 1, 16, 1})) return r;
+    AppendArgs k{{(const __half*)a.b[0].ptr, (const __half*)a.b[1].ptr}, (const uint32_t*)a.b[2].ptr, {(uint8_t*)a.b[3].ptr, (uint8_t*)a.b[5].ptr},
+                 {(int8_t*)a.b[4].ptr, (int8_t*)a.b[6].ptr}, n, n_kv, (uint32_t)blocks, a.status};
+    const uint64_t units = 2ull * n_kv * n;
+    const unsigned ctas = (unsigned)((units + APPEND_THREADS / 32 - 1) / (APPEND_THREADS / 32));
+    const cudaError_t e = launch_dependent(append_blocks_kernel<1>, dim3(ctas), dim3(APPEND_THREADS), 0, a.stream, k);
+    ++*a.launches;
+    return check_cuda(a, e, "kv_append_blocks_e4m3_d128");
+}
+
+}  // namespace sgb

@@ -144,6 +144,12 @@ int launch_prefill_flash_f16_d128(const LaunchArgs&);
 int launch_prefill_sliding_ring_flash_d128(const LaunchArgs&);
 int launch_prefill_paged_q8kv_flash_d128(const LaunchArgs&);
 
+// kv_blocks.cu, attn_blocks.cu: a batch of requests over one 8-bit cache
+int launch_kv_block_tables(const LaunchArgs&);
+int launch_kv_append_blocks(const LaunchArgs&);
+int launch_attn_blocks(const LaunchArgs&);
+size_t attn_blocks_work_bytes(int sm_count, uint32_t n_kv, uint32_t group, uint32_t requests, uint32_t tokens, uint32_t max_q);
+
 // mma_probe.cu
 int launch_diag_mma_cycles(const LaunchArgs&);
 

@@ -170,6 +170,24 @@ const KernelEntry REGISTRY[] = {
     {"kv_dequant_paged_q8_d128", {256, 1, 1}, 5, 8,
      "scales f16, quants i8, page_table u32, dst f16[rows x row_len], step | push {row_len, page} | first step[2] tokens, gathered to linear f16; rows up to the next multiple of 64 zeroed",
      launch_kv_dequant_paged_q8_d128, W(3)},
+    // ---- a batch of requests over one 8-bit cache (no counterpart in the reference, which serves one sequence) -----------------
+    {"kv_block_tables", {1024, 1, 1}, 12, 8,
+     "ctx u32[R] (tokens cached), new u32[R] (tokens of this step), held u32[R] (pages in the request's table row), count u32 (pages on the free list), "
+     "free_list u32, table u32[R x stride], held_out u32[R], free_out u32[4] = pages left, requests refused, tokens placed, pages taken, starts u32[R+1], "
+     "lens u32[R], slots u32[N], positions u32[N] | push {page u32, stride u32} | grid [R, N]; row r ends with ceil((ctx+new)/page) pages: surplus ones go to "
+     "the end of the list, missing ones come from it, in the order of requests; a request that it no longer covers, or that does not fit the stride or N, is "
+     "refused: it keeps its pages, lens = 0, slots 0xffffffff; held_out and free_out may be held and count",
+     launch_kv_block_tables, W(4) | W(5) | W(6) | W(7) | W(8) | W(9) | W(10) | W(11)},
+    {"kv_append_blocks_e4m3_d128", {256, 1, 1}, 7, 0,
+     "k f16[n x KV x128], v, slots u32[n] (pool rows, 0xffffffff = none), k_pool e4m3[row/16 x KV x16x128], k_exps i8[row/16 x KV], v_pool, v_exps | "
+     "grid [KV, n]; value = e4m3 * 2^e, e the least >= -15 that holds the tile; a tile's tokens are consecutive in slots, a tile that does not begin with "
+     "them keeps its rows before them (rounded again where e grows); no tile twice in a call",
+     launch_kv_append_blocks, W(3) | W(4) | W(5) | W(6)},
+    {"attn_blocks_e4m3_d128", {128, 1, 1}, 10, 24,
+     "q f16[N x H x128], k_pool, k_exps, v_pool, v_exps, table u32[R x stride], lens u32[R], starts u32[R+1], out f16[N x H x128], work (sgb_attn_blocks_work_bytes) | "
+     "push {scale f32, page u32, stride u32, window u32 (0 = none), q_per_kv u32 (1, 2, 4, 8), max_q u32} | grid [KV, R, N]; request r's queries are its last "
+     "starts[r+1] - starts[r] <= max_q tokens, causal; rows that see no key are zero, rows behind starts[R] are left",
+     launch_attn_blocks, W(8) | W(9)},
     // ---- measurement aid -----------------------------------------------------------------------------------------
     {"diag_mma_cycles", {64, 1, 1}, 1, 8,
      "cycles u64[2 x SMs x groups[0]] (per CTA: cycles until n_mma back-to-back tcgen05.mma completed, cycles until they were issued) | "

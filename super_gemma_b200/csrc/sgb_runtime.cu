@@ -328,6 +328,11 @@ uint32_t sgb_decode_paged_splits_hint(const sgb_ctx* c, uint32_t n_kv_heads, uin
     return n ? n : 1u;
 }
 
+size_t sgb_attn_blocks_work_bytes(const sgb_ctx* c, uint32_t n_kv_heads, uint32_t q_per_kv, uint32_t requests, uint32_t n_tokens, uint32_t max_q)
+{
+    return attn_blocks_work_bytes(c && c->sm_count > 0 ? c->sm_count : 148, n_kv_heads, q_per_kv, requests, n_tokens, max_q);
+}
+
 int sgb_sync(sgb_ctx* c, uint32_t timeout_ms)
 {
     if (!c) return set_error(SGB_ERR_VALIDATION, "sgb_sync: ctx is NULL");

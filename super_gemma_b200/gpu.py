@@ -115,6 +115,7 @@ ABI = {
     "sgb_dispatch_blocking": (_int, [_vp, _vp, C.POINTER(_Binding), _u32, _vp, _sz, C.POINTER(_u32)]),
     "sgb_launch_count": (_u64, [_vp]),
     "sgb_decode_paged_splits_hint": (_u32, [_vp, _u32, _u32]),
+    "sgb_attn_blocks_work_bytes": (_sz, [_vp, _u32, _u32, _u32, _u32, _u32]),
     "sgb_graph_begin": (_int, [_vp]),
     "sgb_graph_end": (_int, [_vp, _PP]),
     "sgb_graph_launch": (_int, [_vp, _vp]),
@@ -358,6 +359,10 @@ class GpuContext:
     def decode_splits_hint(self, n_kv_heads: int, kv_len: int) -> int:
         """A split count for the paged decode / verify kernels that fills every SM evenly."""
         return lib().sgb_decode_paged_splits_hint(self._h, n_kv_heads, kv_len)
+
+    def attn_blocks_work_bytes(self, n_kv_heads: int, q_per_kv: int, requests: int, n_tokens: int, max_q: int) -> int:
+        """Bytes of the work binding of ``attn_blocks_e4m3_d128`` for a dispatch of that grid and push."""
+        return lib().sgb_attn_blocks_work_bytes(self._h, n_kv_heads, q_per_kv, requests, n_tokens, max_q)
 
     @property
     def launch_count(self) -> int:
