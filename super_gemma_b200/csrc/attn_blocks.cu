@@ -12,18 +12,8 @@ namespace sgb {
 
 namespace {
 
-struct AttnArgs {
-    Requests req;
-    const __half* q;
-    const uint8_t* pool[2];
-    const int8_t* exps[2];
-    __half* out;
-    uint32_t n_kv, group;
-    float scale;
-};
-
 // One CTA of four warps per (query token, query head); a warp takes every fourth tile, a lane four dims.
-__global__ void __launch_bounds__(128) attn_blocks_simple_kernel(const AttnArgs a)
+__global__ void __launch_bounds__(128) attn_blocks_simple_kernel(const BlocksAttn a)
 {
     __shared__ float part[4][130];
     pdl_wait();
@@ -35,7 +25,7 @@ __global__ void __launch_bounds__(128) attn_blocks_simple_kernel(const AttnArgs 
         if (ld_global(a.req.starts + mid) <= t) lo = mid; else hi = mid;
     }
     const Request rq = request_at(a.req, lo);
-    if (t - rq.first >= rq.n) return;
+    if (t - rq.first >= rq.n || rq.n * a.group <= FEW_ROWS) return;
     const int64_t pos = (int64_t)rq.len - rq.n + (t - rq.first);
     const int64_t from = a.req.window && pos + 1 > (int64_t)a.req.window ? pos + 1 - a.req.window : 0;
     const uint2 qw = ld_global(reinterpret_cast<const uint2*>(a.q + ((size_t)t * a.n_kv * a.group + qh) * 128 + 4 * lane));
@@ -89,7 +79,7 @@ struct PushAttnBlocks {
 
 size_t attn_blocks_work_bytes(int sm_count, uint32_t n_kv, uint32_t group, uint32_t requests, uint32_t tokens, uint32_t max_q)
 {
-    return 256;
+    return blocks_decode_work(sm_count, n_kv, group, requests, max_q);
 }
 
 // attn_blocks_e4m3_d128: q, k pool, k exps, v pool, v exps, table, lens, starts, out f16, work.
@@ -99,6 +89,7 @@ int launch_attn_blocks(const LaunchArgs& a)
     const PushAttnBlocks p = *(const PushAttnBlocks*)a.push;
     const uint32_t n_kv = a.groups[0], n = a.groups[1], tokens = a.groups[2];
     if (n_kv == 0 || n == 0 || tokens == 0) return fail_validation(a, "attn_blocks: groups must be [kv heads, requests, query tokens]");
+    if (n_kv > 1024) return fail_validation(a, "attn_blocks: at most 1024 kv heads");
     if (n > MOST_REQUESTS) return fail_validation(a, "attn_blocks: at most 65536 requests");
     if (p.group != 1 && p.group != 2 && p.group != 4 && p.group != 8) return fail_validation(a, "attn_blocks: query heads per kv head must be 1, 2, 4 or 8");
     if (p.page < (uint32_t)TILE_TOK || (p.page & (p.page - 1))) return fail_validation(a, "attn_blocks: page must be a power of two, at least 16 tokens");
@@ -109,6 +100,7 @@ int launch_attn_blocks(const LaunchArgs& a)
     if (blocks == 0 || a.b[3].bytes / tile_row != blocks)
         return fail_validation(a, "attn_blocks: K and V pools must hold the same (non-zero) number of 16-token blocks");
     if (blocks > NO_SLOT / TILE_TOK) return fail_validation(a, "attn_blocks: a pool holds less than 2^32 rows");
+    if (blocks * n_kv >= 0x80000000ull) return fail_validation(a, "attn_blocks: a pool holds less than 2^31 tiles");
     if (blocks * TILE_TOK < p.page) return fail_validation(a, "attn_blocks: the pools hold no whole page");
     if (int r = need_bytes(a, 0, rows * 256, "q")) return r;
     if (int r = need_bytes(a, 2, blocks * n_kv, "k exponents")) return r;
@@ -120,10 +112,12 @@ int launch_attn_blocks(const LaunchArgs& a)
     if (int r = need_bytes(a, 9, attn_blocks_work_bytes(a.sm_count, n_kv, p.group, n, tokens, p.max_q), "work")) return r;
     if (int r = need_aligned(a, {16, 16, 1, 16, 1, 4, 4, 4, 16, 16})) return r;
     const uint32_t shift = (uint32_t)__builtin_ctz(p.page);
-    AttnArgs k{{(const uint32_t*)a.b[5].ptr, (const uint32_t*)a.b[6].ptr, (const uint32_t*)a.b[7].ptr, n, p.stride, shift,
-                (uint32_t)(blocks >> (shift - 4)), tokens, p.max_q, p.window, a.status},
-               (const __half*)a.b[0].ptr, {(const uint8_t*)a.b[1].ptr, (const uint8_t*)a.b[3].ptr}, {(const int8_t*)a.b[2].ptr, (const int8_t*)a.b[4].ptr},
-               (__half*)a.b[8].ptr, n_kv, p.group, p.scale};
+    const BlocksAttn k{{(const uint32_t*)a.b[5].ptr, (const uint32_t*)a.b[6].ptr, (const uint32_t*)a.b[7].ptr, n, p.stride, shift,
+                        (uint32_t)(blocks >> (shift - 4)), tokens, p.max_q, p.window, a.status},
+                       (const __half*)a.b[0].ptr, {(const uint8_t*)a.b[1].ptr, (const uint8_t*)a.b[3].ptr}, {(const int8_t*)a.b[2].ptr, (const int8_t*)a.b[4].ptr},
+                       (__half*)a.b[8].ptr, (uint8_t*)a.b[9].ptr, n_kv, p.group, (uint32_t)(blocks * n_kv), p.scale};
+    if (int r = launch_blocks_decode(a, k)) return r;
+    if ((uint64_t)p.max_q * p.group <= FEW_ROWS) return 0;
     const cudaError_t e = launch_dependent(attn_blocks_simple_kernel, dim3(tokens, n_kv * p.group), dim3(128), 0, a.stream, k);
     ++*a.launches;
     return check_cuda(a, e, "attn_blocks_e4m3_d128");

@@ -1,0 +1,524 @@
+// Attention of many requests with few queries each over the 8-bit cache of blocks.cuh: decode, and the verification of short drafts.
+//
+// The work is the flat list of all requests' 16-token tiles, in their order, for every kv head.  The lengths are known on the device
+// only, so the list is cut there: every warp that fits the GPU at once takes an equal stretch of one head's list, whatever
+// the requests' lengths are, and walks it tile by tile through its own ring of TMA copies, which runs on across the ends of
+// requests.  A request that lies in one stretch is finished by its warp; of one that several warps share each leaves (O, m, l), and a
+// second kernel merges them in the list's order, so reruns give the same bits.  (The cut rests on all lengths, so a request's bits
+// depend on its neighbours' lengths.)
+//
+// One tile: S = K Q^T with the 16 tokens as M and the at most eight query rows as N of mma.sync m16n8k16 (far below tcgen05's 64
+// rows), e4m3 -> f16 exactly on the way from shared memory (ldmatrix, one conversion a pair), O^T += V^T P^T with 16 dims as M.
+// The powers of two never touch the elements: K's multiplies the scores, V's goes into the exponent, P' = 2^(s + e_v - m),
+// and out of the sum again, l += P' 2^-e_v.  Softmax in base 2 with a running maximum that is raised when it grows by more than 2^8.
+// Bound by the cache's bytes: 2 x 128 1/16 per token and kv head.
+#include <mutex>
+
+#include "blocks.cuh"
+#include "sgb_kernels.h"
+
+namespace sgb {
+
+namespace {
+
+constexpr int HD = 128;
+constexpr int WARPS = 4, CTAS_PER_SM = 4, STAGES = 3;
+constexpr uint32_t LEAST_TILES = 4;  // of a stretch: below that more warps only mean more to merge
+constexpr float RESCALE_T = 8.0f;
+constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES;
+
+struct __align__(1024) DecodeSmem {
+    uint8_t k[WARPS][STAGES][TILE_BYTES];  // 128-byte swizzled by TMA
+    uint8_t v[WARPS][STAGES][TILE_BYTES];
+    uint64_t full[WARPS][STAGES];
+    uint64_t sums[WARPS];
+    uint64_t from[WARPS];  // of each warp's stretch: tiles before it in its first request
+    uint32_t request[WARPS];
+};
+
+// What the merge needs of the cut, at the start of the work buffer: u64 tiles before each request, then their total and the
+// number of stretches.  Then (m, l) and O of [slot][kv head][row]: a stretch p has slot 2p for the request that it goes on with
+// and 2p + 1 for one that it begins and does not end.
+struct Work {
+    uint64_t* before;
+    float2* ml;
+    float4* acc;
+    uint32_t rows;
+};
+__host__ __device__ __forceinline__ uint32_t few_rows(uint32_t group, uint32_t max_q)
+{
+    const uint32_t tokens = FEW_ROWS / group;
+    return group * (max_q < tokens ? max_q : tokens);
+}
+__host__ __device__ __forceinline__ size_t header_bytes(uint32_t requests) { return ((size_t)(requests + 2) * 8 + 255) / 256 * 256; }
+__host__ __device__ __forceinline__ Work work_of(uint8_t* p, uint32_t requests, uint32_t n_kv, uint32_t stretches, uint32_t group, uint32_t max_q)
+{
+    Work w;
+    w.rows = few_rows(group, max_q);
+    w.before = reinterpret_cast<uint64_t*>(p);
+    const size_t slots = 2ull * stretches * n_kv * w.rows;
+    w.acc = reinterpret_cast<float4*>(p + header_bytes(requests));
+    w.ml = reinterpret_cast<float2*>(w.acc + slots * (HD / 4));
+    return w;
+}
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a)
+{
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+// Over the eight lanes that share lane % 4: the tokens of a tile.
+__device__ __forceinline__ float tok_max(float v)
+{
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+}
+__device__ __forceinline__ float tok_sum(float v)
+{
+    v += __shfl_xor_sync(0xffffffffu, v, 4);
+    v += __shfl_xor_sync(0xffffffffu, v, 8);
+    return v + __shfl_xor_sync(0xffffffffu, v, 16);
+}
+
+// The tiles of a request that any of its queries sees: [lo, lo + n).  None of a request that is prefilled.
+struct Tiles {
+    uint32_t lo, n;
+};
+__device__ __forceinline__ Tiles tiles_of(const BlocksAttn& a, const Request& q)
+{
+    if (q.n == 0 || q.n > FEW_ROWS / a.group || q.len == 0) return Tiles{0, 0};
+    const int64_t from = (int64_t)q.len - q.n + 1 - a.req.window;
+    const uint32_t lo = a.req.window != 0 && from > 0 ? (uint32_t)from / TILE_TOK : 0;
+    return Tiles{lo, (q.len + TILE_TOK - 1) / TILE_TOK - lo};
+}
+// Stretch p of `n` is [begin(p), begin(p + 1)) of `total` tiles.
+__device__ __forceinline__ uint64_t stretch_begin(uint64_t total, uint32_t n, uint32_t p) { return total * p / n; }
+__device__ __forceinline__ uint32_t stretch_of(uint64_t total, uint32_t n, uint64_t tile) { return (uint32_t)(((tile + 1) * n - 1) / total); }
+__device__ __forceinline__ uint32_t stretches_for(uint64_t total, uint32_t most)
+{
+    const uint64_t n = (total + LEAST_TILES - 1) / LEAST_TILES;
+    return n < most ? (uint32_t)n : most;
+}
+
+__global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
+    blocks_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const BlocksAttn a, const Work work, uint32_t most)
+{
+    extern __shared__ uint8_t smem_raw[];
+    DecodeSmem& sm = *reinterpret_cast<DecodeSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    if (lane == 0) {
+        tma_prefetch_desc(&tm_k);
+        tma_prefetch_desc(&tm_v);
+        for (int i = 0; i < STAGES; i++) mbar_init(&sm.full[warp][i], 1);
+        mbar_fence_init();
+    }
+    pdl_wait();  // lengths, tables, queries and the cache come from earlier kernels of the stream
+    pdl_launch_dependents();
+
+    // ---- cut the list: every CTA sums up all requests' tiles and finds where its own warps begin ---------------------------------
+    const uint32_t flat = blockIdx.x * WARPS + warp, head = flat % a.n_kv, part = flat / a.n_kv;
+    const uint32_t per_thread = (a.req.n + WARPS * 32 - 1) / (WARPS * 32);
+    const uint32_t r_begin = min(threadIdx.x * per_thread, a.req.n), r_end = min(r_begin + per_thread, a.req.n);
+    uint64_t mine = 0;
+    for (uint32_t r = r_begin; r < r_end; r++) mine += tiles_of(a, request_at(a.req, r)).n;
+    uint64_t up_to = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const uint64_t t = __shfl_up_sync(0xffffffffu, up_to, off);
+        if (lane >= (uint32_t)off) up_to += t;
+    }
+    if (lane == 31) sm.sums[warp] = up_to;
+    __syncthreads();
+    uint64_t total = 0, base = up_to - mine;
+#pragma unroll
+    for (int w = 0; w < WARPS; w++) {
+        if (w < (int)warp) base += sm.sums[w];
+        total += sm.sums[w];
+    }
+    const uint32_t n_parts = stretches_for(total, most);
+    if (total != 0) {
+        uint64_t want[WARPS];
+#pragma unroll
+        for (int w = 0; w < WARPS; w++) {
+            const uint32_t p = (blockIdx.x * WARPS + w) / a.n_kv;
+            want[w] = p < n_parts ? stretch_begin(total, n_parts, p) : ~0ull;
+        }
+        uint64_t at = base;
+        for (uint32_t r = r_begin; r < r_end; r++) {
+            const uint32_t n = per_thread == 1 ? (uint32_t)mine : tiles_of(a, request_at(a.req, r)).n;
+#pragma unroll
+            for (int w = 0; w < WARPS; w++)
+                if (want[w] >= at && want[w] < at + n) {
+                    sm.request[w] = r;
+                    sm.from[w] = want[w] - at;
+                }
+            if (blockIdx.x == 0) work.before[r] = at;
+            at += n;
+        }
+    } else if (blockIdx.x == 0) {
+        for (uint32_t r = r_begin; r < r_end; r++) work.before[r] = 0;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        work.before[a.req.n] = total;
+        work.before[a.req.n + 1] = n_parts;
+    }
+    __syncthreads();
+    if (part >= n_parts) return;
+    const uint32_t n_iter = (uint32_t)(stretch_begin(total, n_parts, part + 1) - stretch_begin(total, n_parts, part));
+
+    // ---- the copies' side: STAGES tiles ahead of the arithmetic -------------------------------------------------------------------
+    uint32_t to_r = sm.request[warp], to_tile, to_left;
+    {
+        const Tiles t = tiles_of(a, request_at(a.req, to_r));
+        to_tile = t.lo + (uint32_t)sm.from[warp];
+        to_left = t.n - (uint32_t)sm.from[warp];
+    }
+    uint32_t to_block = block_at(a.req, to_r, to_tile);
+    auto next_tile = [&]() {
+        to_tile++;
+        if (--to_left == 0) {
+            Tiles t{0, 0};
+            while (t.n == 0 && ++to_r < a.req.n) t = tiles_of(a, request_at(a.req, to_r));
+            to_tile = t.lo;
+            to_left = t.n;
+        }
+        if (to_r < a.req.n) to_block = block_at(a.req, to_r, to_tile);
+    };
+    // What is under way: request, tile, and (lanes 0 and 1) the exponents of K and V.
+    uint32_t way_r[STAGES], way_tile[STAGES];
+    int way_exp[STAGES];
+    const CUtensorMap* my_map = lane == 0 ? &tm_k : &tm_v;
+    const uint32_t my_dst = lane == 0 ? smem_u32(sm.k[warp][0]) : smem_u32(sm.v[warp][0]);
+    const int8_t* my_exps = a.exps[lane & 1];
+    const uint32_t bar0 = smem_u32(&sm.full[warp][0]);
+    auto issue = [&](uint32_t st, int& e) {
+        const uint32_t bar = bar0 + st * 8, tile = to_block * a.n_kv + head;
+        if (lane < 2) {
+            e = *(volatile const int8_t*)(my_exps + tile);
+            if (lane == 0) {
+                fence_proxy_async_smem();  // the slot's previous contents were read through the generic proxy
+                asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(STAGE_BYTES) : "memory");
+            }
+            asm volatile(
+                "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+                ::"r"(my_dst + st * TILE_BYTES), "l"(reinterpret_cast<uint64_t>(my_map)), "r"(bar), "r"(0), "r"(0), "r"((int)tile)
+                : "memory");
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES; i++) {
+        way_r[i] = way_tile[i] = 0;
+        way_exp[i] = 0;
+        if ((uint32_t)i < n_iter) {
+            way_r[i] = to_r;
+            way_tile[i] = to_tile;
+            issue(i, way_exp[i]);
+            if ((uint32_t)i + 1 < n_iter) next_tile();
+        }
+    }
+
+    // ---- the arithmetic's side ------------------------------------------------------------------------------------------------------
+    // A lane supplies Q for query row g (B operand) and owns the accumulators of rows 2 t4 and 2 t4 + 1.  Row = token * group + head.
+    const uint32_t heads = a.n_kv * a.group;
+    uint32_t qb[8][2];
+    float o[8][4], m_run[2], l_part[2];
+    uint32_t r_now = ~0u, rows = 0, first_tok = 0, tile_first = 0, tile_begin = 0, tile_end = 0;
+    int hi_row[2] = {0, 0}, lo_row[2] = {0, 0}, lo_all = 0, hi_all = 0, lo_any = 0, hi_any = 0;  // keys that a row, all rows, any row sees
+    auto begin_request = [&](uint32_t r, uint32_t tile) {
+        const Request rq = request_at(a.req, r);
+        const Tiles t = tiles_of(a, rq);
+        r_now = r;
+        rows = rq.n * a.group;
+        first_tok = rq.first;
+        tile_first = tile;
+        tile_begin = t.lo;
+        tile_end = t.lo + t.n;
+        const __half* qrow = a.q + ((size_t)(rq.first + g / a.group) * heads + head * a.group + g % a.group) * HD + 4 * t4;
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+            uint2 w = make_uint2(0u, 0u);
+            if (g < rows) w = ld_global(reinterpret_cast<const uint2*>(qrow + 16 * c));
+            qb[c][0] = w.x;
+            qb[c][1] = w.y;
+            o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.0f;
+        }
+        const int len = (int)rq.len, pos0 = len - (int)rq.n, window = a.req.window && a.req.window < MOST_KEYS ? (int)a.req.window : (int)MOST_KEYS;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            hi_row[e] = min(pos0 + (int)((2 * t4 + e) / a.group), len - 1);
+            lo_row[e] = max(hi_row[e] + 1 - window, 0);
+            m_run[e] = NEG_SENTINEL;
+            l_part[e] = 0.0f;
+        }
+        hi_all = pos0;
+        lo_all = max(len - window, 0);
+        hi_any = len - 1;
+        lo_any = max(pos0 + 1 - window, 0);
+    };
+    auto end_request = [&](uint32_t tile_last) {
+        const float l_row[2] = {tok_sum(l_part[0]), tok_sum(l_part[1])};
+        const bool began = tile_first == tile_begin, ended = tile_last + 1 == tile_end;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const uint32_t row = 2 * t4 + e;
+            if (row >= rows) continue;
+            if (began && ended) {
+                const float f = l_row[e] != 0.0f ? 1.0f / l_row[e] : 0.0f;
+                __half* dst = a.out + ((size_t)(first_tok + row / a.group) * heads + head * a.group + row % a.group) * HD + 2 * g;
+#pragma unroll
+                for (int c = 0; c < 8; c++) *reinterpret_cast<__half2*>(dst + 16 * c) = __floats2half2_rn(o[c][e] * f, o[c][2 + e] * f);
+            } else {
+                const size_t at = ((size_t)(2 * part + (began ? 1 : 0)) * a.n_kv + head) * work.rows + row;
+                float* dst = reinterpret_cast<float*>(work.acc + at * (HD / 4)) + 2 * g;
+#pragma unroll
+                for (int c = 0; c < 8; c++) *reinterpret_cast<float2*>(dst + 16 * c) = make_float2(o[c][e], o[c][2 + e]);
+                if (g == 0) work.ml[at] = make_float2(m_run[e], l_row[e]);
+            }
+        }
+    };
+
+    // Shared-memory offsets of a tile [16 tokens][128 B, swizzled]: one ldmatrix.x4 fetches 32 bytes of 16 tokens; lane l addresses row
+    // (l & 7) of matrix (l >> 3) = (token half (l >> 3) & 1, 16-byte chunk 2b + (l >> 4)).
+    const uint32_t lrow = lane & 7, lmat = lane >> 3;
+    uint32_t off[4];
+#pragma unroll
+    for (int b = 0; b < 4; b++) off[b] = (8 * (lmat & 1) + lrow) * 128 + (((2 * b + (lmat >> 1)) ^ lrow) << 4);
+    const float scale2 = a.scale * 1.4426950408889634f;
+    bool failed = false;
+    uint32_t tile_now = 0;
+
+    for (uint32_t it = 0; it < n_iter; ++it) {
+        const uint32_t st = it % STAGES;
+        if (way_r[0] != r_now) {
+            if (r_now != ~0u) end_request(tile_now);
+            begin_request(way_r[0], way_tile[0]);
+        }
+        tile_now = way_tile[0];
+        const int ek = __shfl_sync(0xffffffffu, way_exp[0], 0), ev = __shfl_sync(0xffffffffu, way_exp[0], 1);
+        mbar_wait_warp(&sm.full[warp][st], (it / STAGES) & 1, a.req.status, 631, failed);
+        if (failed) break;
+        const int tok0 = (int)(tile_now * TILE_TOK);
+        const uint32_t k_base = smem_u32(sm.k[warp][st]), v_base = smem_u32(sm.v[warp][st]);
+
+        // S: s[2 th + e] = score of token g + 8 th against row 2 t4 + e
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            uint32_t x[4];
+            ldsm_x4(k_base + off[b], x);
+#pragma unroll
+            for (int cc = 0; cc < 2; cc++) {
+                const uint32_t f[4] = {e4m3x2_to_f16x2(x[2 * cc] & 0xffffu), e4m3x2_to_f16x2(x[2 * cc + 1] & 0xffffu), e4m3x2_to_f16x2(x[2 * cc] >> 16),
+                                       e4m3x2_to_f16x2(x[2 * cc + 1] >> 16)};
+                mma16816(s, f, qb[2 * b + cc][0], qb[2 * b + cc][1]);
+            }
+        }
+        const float ks = scale2 * __int_as_float((127 + ek) << 23), shift = (float)ev;
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[i] = fmaf(s[i], ks, shift);
+        if (tok0 < lo_all || tok0 + TILE_TOK - 1 > hi_all) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int t = tok0 + (int)g + 8 * (i / 2);
+                if (t < lo_row[i % 2] || t > hi_row[i % 2]) s[i] = -INFINITY;
+            }
+        }
+        const float mx0 = tok_max(fmaxf(s[0], s[2])), mx1 = tok_max(fmaxf(s[1], s[3]));
+        const bool grow0 = mx0 > m_run[0] + RESCALE_T, grow1 = mx1 > m_run[1] + RESCALE_T;
+        if (__any_sync(0xffffffffu, grow0 || grow1)) {
+            const float n0 = grow0 ? mx0 : m_run[0], n1 = grow1 ? mx1 : m_run[1];
+            const float c0 = ex2(m_run[0] - n0), c1 = ex2(m_run[1] - n1);
+            m_run[0] = n0;
+            m_run[1] = n1;
+            l_part[0] *= c0;
+            l_part[1] *= c1;
+#pragma unroll
+            for (int c = 0; c < 8; c++) {
+                o[c][0] *= c0;
+                o[c][1] *= c1;
+                o[c][2] *= c0;
+                o[c][3] *= c1;
+            }
+        }
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) p[i] = ex2(s[i] - m_run[i % 2]);
+        const float back = __int_as_float((127 - ev) << 23);
+        l_part[0] = fmaf(p[0] + p[2], back, l_part[0]);
+        l_part[1] = fmaf(p[1] + p[3], back, l_part[1]);
+
+        // P (tokens x rows) -> P^T fragments: lane (g, t4) gets row g, tokens 2 t4, 2 t4 + 1 and 8 + those
+        const uint32_t pt0 = movmatrix_trans(pack_half2(p[0], p[1])), pt1 = movmatrix_trans(pack_half2(p[2], p[3]));
+        // Tokens that no row sees have P = 0, but 0 times a NaN that stands there would not be: they count as 0.
+        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+        if (tok0 < lo_any || tok0 + TILE_TOK - 1 > hi_any) {
+#pragma unroll
+            for (int th = 0; th < 2; th++) {
+                const int t = tok0 + 8 * th + 2 * (int)t4;
+                keep[th] = (t >= lo_any && t <= hi_any ? 0xffffu : 0u) | (t + 1 >= lo_any && t + 1 <= hi_any ? 0xffff0000u : 0u);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            uint32_t y[4];  // transposed: bytes V[8 th + 2 t4 (+1)][16c + 2g (+1)] for (th, c) = (0, 2b), (1, 2b), (0, 2b + 1), (1, 2b + 1)
+            ldsm_x4_trans(v_base + off[b], y);
+#pragma unroll
+            for (int cc = 0; cc < 2; cc++) {
+                const uint32_t y0 = __byte_perm(y[2 * cc] & keep[0], 0u, 0x3120), y1 = __byte_perm(y[2 * cc + 1] & keep[1], 0u, 0x3120);
+                const uint32_t f[4] = {e4m3x2_to_f16x2(y0 & 0xffffu), e4m3x2_to_f16x2(y0 >> 16), e4m3x2_to_f16x2(y1 & 0xffffu), e4m3x2_to_f16x2(y1 >> 16)};
+                mma16816(o[2 * b + cc], f, pt0, pt1);
+            }
+        }
+        __syncwarp();  // every lane has read the slot
+#pragma unroll
+        for (int i = 0; i + 1 < STAGES; i++) {
+            way_r[i] = way_r[i + 1];
+            way_tile[i] = way_tile[i + 1];
+            way_exp[i] = way_exp[i + 1];
+        }
+        if (it + STAGES < n_iter) {
+            way_r[STAGES - 1] = to_r;
+            way_tile[STAGES - 1] = to_tile;
+            issue(st, way_exp[STAGES - 1]);
+            if (it + STAGES + 1 < n_iter) next_tile();  // its page is looked up while a tile is worked on
+        }
+    }
+    if (failed) let_copies_land();
+    if (r_now != ~0u) end_request(tile_now);
+}
+
+// One CTA per request and kv head: nothing to do where one warp had all its tiles; zeros where it had none; else the warps' parts in
+// the order of the list, a warp per row and every SUB-th part.
+constexpr int MERGE_WARPS = 8;
+__global__ void __launch_bounds__(MERGE_WARPS * 32) blocks_merge_kernel(const BlocksAttn a, const Work work)
+{
+    __shared__ float4 left[MERGE_WARPS][32];
+    pdl_wait();
+    pdl_launch_dependents();
+    const uint32_t r = blockIdx.x, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint64_t at = ld_global(work.before + r), end = ld_global(work.before + r + 1), total = ld_global(work.before + a.req.n);
+    const uint32_t n_parts = (uint32_t)ld_global(work.before + a.req.n + 1);
+    const uint32_t first = ld_global(a.req.starts + r), last = ld_global(a.req.starts + r + 1);
+    uint32_t p0 = 0, n = 0;
+    if (end > at) {
+        p0 = stretch_of(total, n_parts, at);
+        n = stretch_of(total, n_parts, end - 1) - p0 + 1;
+        if (n == 1) return;
+    }
+    if (last <= first || last > a.req.tokens || last - first > FEW_ROWS / a.group || last - first > a.req.max_q) return;
+    const uint32_t rows = (last - first) * a.group, per_row = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;  // rows, up to a power of two
+    const uint32_t row = warp % per_row, sub = warp / per_row, subs = MERGE_WARPS / per_row;
+    __half* out = a.out + ((size_t)(first + row / a.group) * (a.n_kv * a.group) + head * a.group + row % a.group) * HD + 4 * lane;
+    if (n == 0) {
+        if (row < rows && sub == 0) *reinterpret_cast<uint2*>(out) = make_uint2(0u, 0u);
+        return;
+    }
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float den = 0.0f;
+    if (row < rows) {
+        const auto slot = [&](uint32_t j) { return ((size_t)(2 * (p0 + j) + (j == 0 ? 1 : 0)) * a.n_kv + head) * work.rows + row; };
+        float big = NEG_SENTINEL;
+        for (uint32_t j = lane; j < n; j += 32) big = fmaxf(big, ld_global(work.ml + slot(j)).x);
+#pragma unroll
+        for (int off = 16; off; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+        for (uint32_t j0 = 0; j0 < n; j0 += 32) {
+            const float2 ml = ld_global(work.ml + slot(min(j0 + lane, n - 1)));
+            const float w = j0 + lane < n ? ex2(ml.x - big) : 0.0f;
+            den = fmaf(w, ml.y, den);
+            for (uint32_t u0 = sub; u0 < 32 && j0 + u0 < n; u0 += 8 * subs) {
+                float4 v[8];
+#pragma unroll
+                for (int i = 0; i < 8; i++) v[i] = ld_global(work.acc + slot(min(j0 + u0 + i * subs, n - 1)) * (HD / 4) + lane);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const uint32_t u = u0 + i * subs;
+                    const float f = __shfl_sync(0xffffffffu, w, u & 31);
+                    if (u < 32 && j0 + u < n) {
+                        acc.x = fmaf(f, v[i].x, acc.x);
+                        acc.y = fmaf(f, v[i].y, acc.y);
+                        acc.z = fmaf(f, v[i].z, acc.z);
+                        acc.w = fmaf(f, v[i].w, acc.w);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int off = 16; off; off >>= 1) den += __shfl_xor_sync(0xffffffffu, den, off);
+    }
+    left[warp][lane] = acc;
+    __syncthreads();
+    if (row < rows && sub == 0) {
+        for (uint32_t s = 1; s < subs; s++) {
+            const float4 o = left[row + s * per_row][lane];
+            acc.x += o.x;
+            acc.y += o.y;
+            acc.z += o.z;
+            acc.w += o.w;
+        }
+        const float f = den != 0.0f ? 1.0f / den : 0.0f;
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack_half2(acc.x * f, acc.y * f), pack_half2(acc.z * f, acc.w * f));
+    }
+}
+
+// Warps that fit the GPU at once, and what every kv head gets of them.
+uint32_t grid_ctas(int sm_count, uint32_t n_kv)
+{
+    const uint32_t ctas = (uint32_t)sm_count * CTAS_PER_SM, least = (n_kv + WARPS - 1) / WARPS;
+    return ctas > least ? ctas : least;
+}
+uint32_t most_stretches(int sm_count, uint32_t n_kv) { return grid_ctas(sm_count, n_kv) * WARPS / n_kv; }
+
+}  // namespace
+
+size_t blocks_decode_work(int sm_count, uint32_t n_kv, uint32_t group, uint32_t requests, uint32_t max_q)
+{
+    if (n_kv == 0 || group == 0 || group > FEW_ROWS || max_q == 0) return 256;
+    return header_bytes(requests) + 2ull * most_stretches(sm_count, n_kv) * n_kv * few_rows(group, max_q) * (HD + 2) * 4;
+}
+
+int launch_blocks_decode(const LaunchArgs& a, const BlocksAttn& k)
+{
+    CUtensorMap tm[2];
+    for (int i = 0; i < 2; i++) {
+        const uint64_t dims[3] = {128, TILE_TOK, k.tiles}, strides[2] = {128, TILE_BYTES};
+        const uint32_t box[3] = {128, TILE_TOK, 1};
+        if (int r = encode_tensor_map(a, &tm[i], 0, 3, const_cast<uint8_t*>(k.pool[i]), dims, strides, box, 3)) return r;
+    }
+    const size_t smem = sizeof(DecodeSmem) + 1024;
+    {
+        static std::mutex attr_mutex;
+        static bool attr_set[64] = {};
+        std::lock_guard<std::mutex> lock(attr_mutex);
+        if (a.device < 0 || a.device >= 64 || !attr_set[a.device]) {
+            if (int r = check_cuda(a, cudaFuncSetAttribute(blocks_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "cudaFuncSetAttribute(blocks_decode)"))
+                return r;
+            if (a.device >= 0 && a.device < 64) attr_set[a.device] = true;
+        }
+    }
+    const uint32_t most = most_stretches(a.sm_count, k.n_kv);
+    const Work w = work_of(k.work, k.req.n, k.n_kv, most, k.group, k.req.max_q);
+    cudaError_t e = launch_dependent(blocks_decode_kernel, dim3(grid_ctas(a.sm_count, k.n_kv)), dim3(WARPS * 32), smem, a.stream, tm[0], tm[1], k, w, most);
+    ++*a.launches;
+    if (int r = check_cuda(a, e, "attn_blocks decode")) return r;
+    e = launch_dependent(blocks_merge_kernel, dim3(k.req.n, k.n_kv), dim3(MERGE_WARPS * 32), 0, a.stream, k, w);
+    ++*a.launches;
+    return check_cuda(a, e, "attn_blocks merge");
+}
+
+}  // namespace sgb

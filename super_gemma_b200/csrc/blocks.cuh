@@ -19,6 +19,8 @@ constexpr uint32_t TILE_BYTES = TILE_TOK * 128;
 constexpr uint32_t NO_SLOT = 0xffffffffu;
 constexpr int LOWEST_EXP = -15;
 constexpr uint32_t MOST_REQUESTS = 65536;
+constexpr uint32_t MOST_KEYS = 0x7fffff00u;  // of one request: positions are signed words
+constexpr uint32_t FEW_ROWS = 8;             // requests of at most so many rows (query tokens x heads of a group) are decoded, the others prefilled
 
 // What a dispatch over the cache knows of its requests.
 struct Requests {
@@ -43,7 +45,7 @@ __device__ __forceinline__ Request request_at(const Requests& a, uint32_t r)
         report_error(a.status, DEV_ERR_BOUNDS, 601, r, end);
         q.n = 0;
     }
-    const uint64_t most = (uint64_t)a.stride << a.page_shift;
+    const uint64_t most = min((uint64_t)a.stride << a.page_shift, (uint64_t)MOST_KEYS);
     if (q.len > most) {
         report_error(a.status, DEV_ERR_BOUNDS, 602, r, q.len);
         q.len = (uint32_t)most;
@@ -66,6 +68,22 @@ __device__ __forceinline__ uint32_t block_at(const Requests& a, uint32_t r, uint
     }
     return (page << shift) + (tile & ((1u << shift) - 1));
 }
+
+// A dispatch of attn_blocks_e4m3_d128.
+struct BlocksAttn {
+    Requests req;
+    const __half* q;
+    const uint8_t* pool[2];
+    const int8_t* exps[2];
+    __half* out;
+    uint8_t* work;
+    uint32_t n_kv, group, tiles;  // tiles of a pool: blocks x kv heads
+    float scale;
+};
+struct LaunchArgs;
+// attn_blocks_decode.cu
+size_t blocks_decode_work(int sm_count, uint32_t n_kv, uint32_t group, uint32_t requests, uint32_t max_q);
+int launch_blocks_decode(const LaunchArgs&, const BlocksAttn&);
 
 // Two e4m3 bytes as two f16, exactly (one instruction at the rate of an integer one: 64 a clock and SM).
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes)
