@@ -15,6 +15,7 @@
 #include <mutex>
 
 #include "blocks.cuh"
+#include "blocks_work.cuh"
 #include "sgb_kernels.h"
 
 namespace sgb {
@@ -36,11 +37,10 @@ struct __align__(1024) DecodeSmem {
     uint32_t request[WARPS];
 };
 
-// What the merge needs of the cut, at the start of the work buffer: u64 tiles before each request, then their total and the
-// number of stretches.  Then (m, l) and O of [slot][kv head][row]: a stretch p has slot 2p for the request that it goes on with
-// and 2p + 1 for one that it begins and does not end.
+// Parts: (m, l) and O of [slot][kv head][row].  A stretch p has slot 2p for the request that it goes on with and 2p + 1 for
+// one that it begins and does not end.
 struct Work {
-    uint64_t* before;
+    BlocksWork head;
     float2* ml;
     float4* acc;
     uint32_t rows;
@@ -49,17 +49,6 @@ __host__ __device__ __forceinline__ uint32_t few_rows(uint32_t group, uint32_t m
 {
     const uint32_t tokens = FEW_ROWS / group;
     return group * (max_q < tokens ? max_q : tokens);
-}
-__host__ __device__ __forceinline__ size_t header_bytes(uint32_t requests) { return ((size_t)(requests + 2) * 8 + 255) / 256 * 256; }
-__host__ __device__ __forceinline__ Work work_of(uint8_t* p, uint32_t requests, uint32_t n_kv, uint32_t stretches, uint32_t group, uint32_t max_q)
-{
-    Work w;
-    w.rows = few_rows(group, max_q);
-    w.before = reinterpret_cast<uint64_t*>(p);
-    const size_t slots = 2ull * stretches * n_kv * w.rows;
-    w.acc = reinterpret_cast<float4*>(p + header_bytes(requests));
-    w.ml = reinterpret_cast<float2*>(w.acc + slots * (HD / 4));
-    return w;
 }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
@@ -117,7 +106,7 @@ __device__ __forceinline__ uint32_t stretches_for(uint64_t total, uint32_t most)
 }
 
 __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
-    blocks_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const BlocksAttn a, const Work work, uint32_t most)
+    blocks_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ BlocksAttn a, const __grid_constant__ Work work, uint32_t most)
 {
     extern __shared__ uint8_t smem_raw[];
     DecodeSmem& sm = *reinterpret_cast<DecodeSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -168,15 +157,15 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
                     sm.request[w] = r;
                     sm.from[w] = want[w] - at;
                 }
-            if (blockIdx.x == 0) work.before[r] = at;
+            if (blockIdx.x == 0) work.head.before[r] = at;
             at += n;
         }
     } else if (blockIdx.x == 0) {
-        for (uint32_t r = r_begin; r < r_end; r++) work.before[r] = 0;
+        for (uint32_t r = r_begin; r < r_end; r++) work.head.before[r] = 0;
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) {
-        work.before[a.req.n] = total;
-        work.before[a.req.n + 1] = n_parts;
+        work.head.before[a.req.n] = total;
+        work.head.before[a.req.n + 1] = n_parts;
     }
     __syncthreads();
     if (part >= n_parts) return;
@@ -189,7 +178,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
         to_tile = t.lo + (uint32_t)sm.from[warp];
         to_left = t.n - (uint32_t)sm.from[warp];
     }
-    uint32_t to_block = block_at(a.req, to_r, to_tile);
+    uint32_t to_page = ld_global(page_at(a.req, to_r, to_tile));
     auto next_tile = [&]() {
         to_tile++;
         if (--to_left == 0) {
@@ -198,7 +187,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
             to_tile = t.lo;
             to_left = t.n;
         }
-        if (to_r < a.req.n) to_block = block_at(a.req, to_r, to_tile);
+        if (to_r < a.req.n) to_page = ld_global(page_at(a.req, to_r, to_tile));
     };
     // What is under way: request, tile, and (lanes 0 and 1) the exponents of K and V.
     uint32_t way_r[STAGES], way_tile[STAGES];
@@ -208,9 +197,9 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
     const int8_t* my_exps = a.exps[lane & 1];
     const uint32_t bar0 = smem_u32(&sm.full[warp][0]);
     auto issue = [&](uint32_t st, int& e) {
-        const uint32_t bar = bar0 + st * 8, tile = to_block * a.n_kv + head;
+        const uint32_t bar = bar0 + st * 8, tile = block_of_page(a.req, to_r, to_tile, to_page) * a.n_kv + head;
+        e = ld_global_if(lane < 2, my_exps + tile);
         if (lane < 2) {
-            e = *(volatile const int8_t*)(my_exps + tile);
             if (lane == 0) {
                 fence_proxy_async_smem();  // the slot's previous contents were read through the generic proxy
                 asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(STAGE_BYTES) : "memory");
@@ -406,14 +395,55 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
 // One CTA per request and kv head: nothing to do where one warp had all its tiles; zeros where it had none; else the warps' parts in
 // the order of the list, a warp per row and every SUB-th part.
 constexpr int MERGE_WARPS = 8;
-__global__ void __launch_bounds__(MERGE_WARPS * 32) blocks_merge_kernel(const BlocksAttn a, const Work work)
+// What the prefill kernel takes its units from: those before each request that it serves.  By one CTA.
+__device__ __forceinline__ void list_units(const BlocksAttn& a, const BlocksWork& w, uint32_t* sums)
+{
+    const uint32_t per_thread = (a.req.n + MERGE_WARPS * 32 - 1) / (MERGE_WARPS * 32);
+    const uint32_t r_begin = min(threadIdx.x * per_thread, a.req.n), r_end = min(r_begin + per_thread, a.req.n);
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const auto units = [&](uint32_t r) -> uint32_t {
+        const uint32_t n = request_at(a.req, r).n;
+        return n > FEW_ROWS / a.group ? (uint32_t)(((uint64_t)n * a.group + UNIT_ROWS - 1) / UNIT_ROWS) : 0;
+    };
+    uint32_t mine = 0;
+    for (uint32_t r = r_begin; r < r_end; r++) mine += units(r);
+    uint32_t up_to = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+        const uint32_t t = __shfl_up_sync(0xffffffffu, up_to, off);
+        if (lane >= (uint32_t)off) up_to += t;
+    }
+    if (lane == 31) sums[warp] = up_to;
+    __syncthreads();
+    uint32_t at = up_to - mine, total = 0;
+#pragma unroll
+    for (int i = 0; i < MERGE_WARPS; i++) {
+        if (i < (int)warp) at += sums[i];
+        total += sums[i];
+    }
+    for (uint32_t r = r_begin; r < r_end; r++) {
+        w.units_before[r] = at;
+        at += units(r);
+    }
+    if (threadIdx.x == 0) {
+        w.units_before[a.req.n] = total;
+        *w.queue = 0;
+    }
+    for (uint32_t i = threadIdx.x; i < 2 * w.places; i += MERGE_WARPS * 32) w.done[i] = 0;
+}
+
+__global__ void __launch_bounds__(MERGE_WARPS * 32) blocks_merge_kernel(const __grid_constant__ BlocksAttn a, const __grid_constant__ Work work)
 {
     __shared__ float4 left[MERGE_WARPS][32];
     pdl_wait();
     pdl_launch_dependents();
+    if (blockIdx.x == a.req.n) {  // there if a prefill follows
+        if (blockIdx.y == 0) list_units(a, work.head, reinterpret_cast<uint32_t*>(left));
+        return;
+    }
     const uint32_t r = blockIdx.x, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint64_t at = ld_global(work.before + r), end = ld_global(work.before + r + 1), total = ld_global(work.before + a.req.n);
-    const uint32_t n_parts = (uint32_t)ld_global(work.before + a.req.n + 1);
+    const uint64_t at = ld_global(work.head.before + r), end = ld_global(work.head.before + r + 1), total = ld_global(work.head.before + a.req.n);
+    const uint32_t n_parts = (uint32_t)ld_global(work.head.before + a.req.n + 1);
     const uint32_t first = ld_global(a.req.starts + r), last = ld_global(a.req.starts + r + 1);
     uint32_t p0 = 0, n = 0;
     if (end > at) {
@@ -486,13 +516,12 @@ uint32_t most_stretches(int sm_count, uint32_t n_kv) { return grid_ctas(sm_count
 
 }  // namespace
 
-size_t blocks_decode_work(int sm_count, uint32_t n_kv, uint32_t group, uint32_t requests, uint32_t max_q)
+size_t blocks_decode_work(int sm_count, uint32_t n_kv, uint32_t group, uint32_t max_q)
 {
-    if (n_kv == 0 || group == 0 || group > FEW_ROWS || max_q == 0) return 256;
-    return header_bytes(requests) + 2ull * most_stretches(sm_count, n_kv) * n_kv * few_rows(group, max_q) * (HD + 2) * 4;
+    return 2ull * most_stretches(sm_count, n_kv) * n_kv * few_rows(group, max_q) * (HD + 2) * 4;
 }
 
-int launch_blocks_decode(const LaunchArgs& a, const BlocksAttn& k)
+int launch_blocks_decode(const LaunchArgs& a, const BlocksAttn& k, const BlocksWork& head)
 {
     CUtensorMap tm[2];
     for (int i = 0; i < 2; i++) {
@@ -512,11 +541,12 @@ int launch_blocks_decode(const LaunchArgs& a, const BlocksAttn& k)
         }
     }
     const uint32_t most = most_stretches(a.sm_count, k.n_kv);
-    const Work w = work_of(k.work, k.req.n, k.n_kv, most, k.group, k.req.max_q);
+    Work w{head, nullptr, reinterpret_cast<float4*>(head.parts), few_rows(k.group, k.req.max_q)};
+    w.ml = reinterpret_cast<float2*>(w.acc + 2ull * most * k.n_kv * w.rows * (HD / 4));
     cudaError_t e = launch_dependent(blocks_decode_kernel, dim3(grid_ctas(a.sm_count, k.n_kv)), dim3(WARPS * 32), smem, a.stream, tm[0], tm[1], k, w, most);
     ++*a.launches;
     if (int r = check_cuda(a, e, "attn_blocks decode")) return r;
-    e = launch_dependent(blocks_merge_kernel, dim3(k.req.n, k.n_kv), dim3(MERGE_WARPS * 32), 0, a.stream, k, w);
+    e = launch_dependent(blocks_merge_kernel, dim3(k.req.n + (k.req.max_q > FEW_ROWS / k.group ? 1 : 0), k.n_kv), dim3(MERGE_WARPS * 32), 0, a.stream, k, w);
     ++*a.launches;
     return check_cuda(a, e, "attn_blocks merge");
 }

@@ -1,0 +1,623 @@
+// Attention of requests with many queries (prompts, chunks of them, long drafts) over the 8-bit cache of blocks.cuh, on tcgen05.
+//
+// A unit is 256 rows of one request and kv head: 256 / group query tokens x the group's heads, so that a key is fetched and converted
+// once for all of them.  They are two tiles of 128 rows, one softmax warpgroup each.  Per 64 keys and tile, as in the f16 flash
+// kernel: S = Q K^T into one of two tensor-memory buffers, one thread per row for the online softmax (base 2, the maximum raised when it
+// grows by more than 2^8, l from the unrounded weights), P back over S, O += P V.
+// What differs is where K and V come from.  One warp copies the cache's bytes, 16 tokens of one head at a time through the block
+// table, up to four tiles of keys ahead; four warps turn them into f16 in the swizzled operand tiles (16 bytes in, 32 out, one
+// conversion a pair), so the cache is read once per unit at one byte a value and no f16 copy of it exists.  The powers of two go to the
+// softmax, as in the decode: K's times the scores, V's into the exponent.
+//
+// One CTA per SM stays and takes units from a queue (the lengths are known on the device only); one warp fetches the next while the
+// others work.  What is left when every CTA has had its whole units is cut along the keys; the CTA that finishes the last piece of a unit
+// merges them, in their order, so reruns give the same bits.
+#include <mutex>
+
+#include "blocks.cuh"
+#include "blocks_work.cuh"
+#include "sgb_kernels.h"
+
+namespace sgb {
+
+namespace {
+
+constexpr int HD = 128;
+constexpr int ROWS = 128, KEYS = 64;              // of a tile of queries, of keys
+constexpr int THREADS = 512;                      // two softmax warpgroups, one that converts, one of single warps
+constexpr int CONVERT_WARP = 8, MMA_WARP = 12, COPY_WARP = 13, QUEUE_WARP = 14;
+constexpr int RAW = 4;                            // tiles of keys under way from the cache
+constexpr uint32_t HALF_TILE = 64 * 128;          // [64 rows][64 dims] f16
+constexpr uint32_t Q_BYTES = 4 * HALF_TILE;       // of one tile of queries
+constexpr uint32_t TMEM_COLS = 512, TMEM_O = 256; // S: [tile][buffer] of 64 columns, then O: [tile] of 128
+constexpr float RESCALE_T = 8.0f;
+constexpr int LEAST_TILES = 8;                    // of a piece
+// Registers: 512 threads are launched with 128 each; the warpgroups redistribute exactly those.
+constexpr uint32_t LAUNCH_REGS = 128, SOFTMAX_REGS = 160, CONVERT_REGS = 96, ISSUE_REGS = 96;
+static_assert(2 * SOFTMAX_REGS + CONVERT_REGS + ISSUE_REGS <= 4 * LAUNCH_REGS, "setmaxnreg draws on what the block was launched with");
+
+struct Item {
+    uint32_t valid, request, head, first_tok, toks, piece, pieces, slot, counter;
+    int first_pos, band_lo, tile0;  // position of the first query, first key that any row sees, first tile of 64 keys
+    int n_tiles[2];                 // of either tile of queries; the second has none, or as many as the unit
+    __device__ int unit_tiles() const { return max(n_tiles[0], n_tiles[1]); }
+    __device__ int last_pos() const { return first_pos + (int)toks - 1; }
+};
+
+struct PrefillSmem {
+    uint8_t q[2][2][2 * HALF_TILE];  // [tile][dim half][128 rows x 128 B]
+    uint8_t k[2][2][HALF_TILE];      // [stage][dim half][64 keys x 128 B]
+    uint8_t v[2][2][HALF_TILE];
+    uint8_t raw[RAW][2][4][TILE_BYTES];  // [stage][K, V][block]: as cached
+    uint64_t raw_full[RAW], raw_empty[RAW];
+    uint64_t full_k[2], full_v[2];   // converting warps: the tile is there
+    uint64_t s_ready[2][2];          // [tile][buffer] MMA commit: S holds Q K^T
+    uint64_t p_ready[2][2];          // softmax threads: P is in tensor memory
+    uint64_t pv_done[2][2];          // MMA commit: O += P V is complete
+    uint64_t q_bar;
+    float4 exps[2 * RAW][2];         // [tile of keys % 8]: the powers of two of K, and the exponents of V, of its four blocks
+    Item item[2];
+    uint32_t tmem_base, last[2];
+};
+static_assert(sizeof(PrefillSmem) <= 227 * 1024, "shared memory of a CTA");
+
+template <uint32_t N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <uint32_t N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// How the units go over the places: `whole` of them one by one, each of the others in `pieces`.
+struct Cut {
+    uint32_t units, whole, pieces;
+    __device__ uint32_t items() const { return whole + (units - whole) * pieces; }
+};
+__device__ __forceinline__ Cut cut_units(uint32_t units, uint32_t places, uint32_t most_slots)
+{
+    Cut c{units, units / places * places, 1};
+    const uint32_t rest = units - c.whole;
+    float best = 1.0f;
+    for (uint32_t p = 2; p <= 16 && rest * p <= most_slots; p++) {
+        const float cost = (float)((rest * p + places - 1) / places) / (float)p + 0.005f * (float)p;  // a piece's partial costs about a three-hundredth of a long unit
+        if (rest != 0 && cost < best) best = cost, c.pieces = p;
+    }
+    if (c.pieces == 1) c.whole = units;
+    return c;
+}
+
+// The queue's next item that has work; by a whole warp.
+__device__ __forceinline__ void fetch_item(const BlocksAttn& a, const PrefillWork& w, uint32_t total, const Cut& cut, Item* out)
+{
+    const uint32_t lane = threadIdx.x & 31;
+    Item it;
+    it.valid = 0;
+    for (;;) {
+        uint32_t i = 0;
+        if (lane == 0) i = atomicAdd(w.queue, 1u);
+        i = __shfl_sync(0xffffffffu, i, 0);
+        if (i >= cut.items()) break;
+        uint32_t unit = i;
+        it.piece = 0;
+        uint32_t pieces = 1;
+        it.slot = it.counter = 0;
+        if (i >= cut.whole) {
+            it.slot = i - cut.whole;
+            it.counter = it.slot / cut.pieces;
+            unit = cut.whole + it.counter;
+            it.piece = it.slot % cut.pieces;
+            pieces = cut.pieces;
+        }
+        it.head = unit / total;
+        const uint32_t u = total - 1 - unit % total;  // the last tile of a request has the most keys
+        uint32_t lo = 0, n = a.req.n;                 // the request: the last one with units_before <= u
+        while (n > 1) {
+            const uint32_t step = (n + 31) / 32, probe = lo + lane * step;
+            const bool at_or_before = lane * step < n && ld_global(w.units_before + probe) <= u;
+            const uint32_t k = 31 - __clz(__ballot_sync(0xffffffffu, at_or_before));  // lane 0 always is
+            lo += k * step;
+            n = min(step, n - k * step);
+        }
+        it.request = lo;
+        const Request rq = request_at(a.req, lo);
+        const uint32_t per = UNIT_ROWS / a.group, half = per / 2, tok0 = (u - ld_global(w.units_before + lo)) * per;
+        it.first_tok = rq.first + tok0;
+        it.toks = min(per, rq.n - tok0);
+        it.first_pos = (int)rq.len - (int)rq.n + (int)tok0;
+        const int last_pos = it.last_pos(), window = a.req.window && a.req.window < MOST_KEYS ? (int)a.req.window : (int)MOST_KEYS;
+        it.band_lo = max(it.first_pos + 1 - window, 0);
+        const int t_lo = it.band_lo / KEYS, n_tiles = last_pos >= 0 ? last_pos / KEYS - t_lo + 1 : 0;
+        it.pieces = min(pieces, (uint32_t)max(1, n_tiles / LEAST_TILES));
+        if (it.piece >= it.pieces) continue;
+        const int per_piece = (n_tiles + (int)it.pieces - 1) / (int)it.pieces, begin = min(n_tiles, (int)it.piece * per_piece);
+        it.tile0 = t_lo + begin;
+        const int mine = min(n_tiles, begin + per_piece) - begin;
+        it.n_tiles[0] = mine;
+        it.n_tiles[1] = 0;
+        if (it.toks > half) {  // the second tile of queries goes to the end, the first as far as its last query sees
+            const int last_first = it.first_pos + (int)half - 1;
+            it.n_tiles[1] = mine;
+            it.n_tiles[0] = last_first >= 0 ? min(mine, max(0, last_first / KEYS + 1 - it.tile0)) : 0;
+        }
+        it.valid = 1;
+        break;
+    }
+    if (lane == 0) *out = it;
+}
+
+// 16 cached bytes as 16 f16 numbers, into two 16-byte chunks of a row.
+__device__ __forceinline__ void put_converted(uint32_t chunk0, uint32_t chunk1, const uint4& raw)
+{
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    uint32_t f[8];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        f[2 * i] = e4m3x2_to_f16x2(w[i] & 0xffffu);
+        f[2 * i + 1] = e4m3x2_to_f16x2(w[i] >> 16);
+    }
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(chunk0), "r"(f[0]), "r"(f[1]), "r"(f[2]), "r"(f[3]) : "memory");
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(chunk1), "r"(f[4]), "r"(f[5]), "r"(f[6]), "r"(f[7]) : "memory");
+}
+
+__global__ void __launch_bounds__(THREADS, 1)
+    blocks_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ BlocksAttn a, const __grid_constant__ PrefillWork w)
+{
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    PrefillSmem& sm = *reinterpret_cast<PrefillSmem*>(smem_raw);
+    uint32_t* status = a.req.status;
+    if ((smem_u32(smem_raw) & 1023u) != 0u) {  // the swizzled tiles need it; never seen, but never assumed
+        if (threadIdx.x == 0) report_error(status, DEV_ERR_BOUNDS, 640, smem_u32(smem_raw), 0);
+        return;
+    }
+    const int tid = threadIdx.x, warp = warp_uniform(tid >> 5);
+    const uint32_t lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < RAW; i++) {
+            mbar_init(&sm.raw_full[i], 2);  // the copies, and the exponents
+            mbar_init(&sm.raw_empty[i], 4);
+        }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sm.full_k[i], 4);
+            mbar_init(&sm.full_v[i], 4);
+            for (int t = 0; t < 2; t++) {
+                mbar_init(&sm.s_ready[t][i], 1);
+                mbar_init(&sm.p_ready[t][i], 128);
+                mbar_init(&sm.pv_done[t][i], 1);
+            }
+        }
+        mbar_init(&sm.q_bar, 1);
+        mbar_fence_init();
+    }
+    pdl_wait();  // everything this kernel reads comes from earlier kernels of the stream, the cut of the units among it
+    pdl_launch_dependents();
+    if (warp == 0) {
+        tmem_alloc(&sm.tmem_base, TMEM_COLS);
+        tmem_relinquish();
+    }
+    const uint32_t total = ld_global(w.units_before + a.req.n);  // units of a kv head
+    const Cut cut = cut_units(total * a.n_kv, gridDim.x, w.slots);
+    if (warp == QUEUE_WARP) fetch_item(a, w, total, cut, &sm.item[0]);
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = sm.tmem_base;
+    bool failed = false;
+    uint32_t slot = 0;
+    // All roles leave an item together, through this.  False: a wait has run out somewhere.
+    auto leave = [&]() {
+        slot ^= 1;
+        tc_fence_before_sync();
+        const bool any = __syncthreads_or(failed) != 0;
+        tc_fence_after_sync();
+        return !any;
+    };
+    // A barrier's phases go on from item to item: tile j of an item is use `before + j / 2` of buffer j % 2.
+    struct Uses {
+        uint32_t before[2] = {0, 0};
+        __device__ uint32_t parity(int j) const { return (((j & 1) ? before[1] : before[0]) + (uint32_t)(j >> 1)) & 1u; }
+        __device__ void add(int n)
+        {
+            before[0] += (uint32_t)(n + 1) / 2;
+            before[1] += (uint32_t)n / 2;
+        }
+    };
+
+    if (warp >= MMA_WARP) {
+        regs_down<ISSUE_REGS>();
+        if (warp == MMA_WARP) {
+            // ======================= MMA issue (the whole warp runs the loop, one lane issues) =======================
+            // The tensor pipe runs ... PV_0(j) QK_0(j+2) PV_1(j) QK_1(j+2) ...: while one tile's softmax is at work the other's products run.
+            const uint32_t one = elect_one(), tm = warp_uniform(tmem);
+            constexpr uint32_t IDESC_QK = umma_idesc_f16(ROWS, KEYS, 0, 0), IDESC_PV = umma_idesc_f16(ROWS, HD, 0, 1);
+            const uint64_t dq = umma_desc_sw128(smem_u32(sm.q[0][0]), 16, 1024), dk = umma_desc_sw128(smem_u32(sm.k[0][0]), 16, 1024),
+                           dv = umma_desc_sw128(smem_u32(sm.v[0][0]), HALF_TILE, 1024);
+            constexpr uint64_t Q_TILE = Q_BYTES >> 4, Q_HALF = 2 * HALF_TILE >> 4, K_HALF = HALF_TILE >> 4, STAGE = 2 * HALF_TILE >> 4;
+            Uses keys, rows[2];
+            uint32_t q_phase = 0;
+            for (;;) {
+                const Item& it = sm.item[slot];
+                if (!it.valid) break;
+                const int n[2] = {warp_uniform(it.n_tiles[0]), warp_uniform(it.n_tiles[1])}, tiles = max(n[0], n[1]);
+                if (tiles > 0) {
+                    if (one) {
+                        mbar_arrive_expect_tx(&sm.q_bar, n[1] ? 2 * Q_BYTES : Q_BYTES);
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {
+                            if (t == 1 && !n[1]) break;
+                            const int row = (int)(it.first_tok + t * (ROWS / a.group));
+                            tma_load_3d(sm.q[t][0], &tm_q, &sm.q_bar, 0, (int)(it.head * a.group), row);
+                            tma_load_3d(sm.q[t][1], &tm_q, &sm.q_bar, 64, (int)(it.head * a.group), row);
+                        }
+                    }
+                    __syncwarp();
+                    auto issue_qk = [&](int t, int j) {
+                        const int b = j & 1;
+                        mbar_wait_warp(&sm.full_k[b], keys.parity(j), status, 641, failed);
+                        if (failed) return;
+                        tc_fence_after_sync();
+                        const uint64_t q0 = dq + t * Q_TILE, k0 = dk + b * STAGE;
+                        const uint32_t d = tm + (2 * t + b) * KEYS;
+#pragma unroll
+                        for (int kk = 0; kk < 4; kk++) umma_f16_ss(d, q0 + 2 * kk, k0 + 2 * kk, IDESC_QK, kk ? 1u : 0u, one);
+#pragma unroll
+                        for (int kk = 0; kk < 4; kk++) umma_f16_ss(d, q0 + Q_HALF + 2 * kk, k0 + K_HALF + 2 * kk, IDESC_QK, 1u, one);
+                        umma_commit(&sm.s_ready[t][b], one);
+                    };
+                    mbar_wait_warp(&sm.q_bar, q_phase & 1, status, 642, failed);
+                    q_phase++;
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+#pragma unroll
+                        for (int t = 0; t < 2; t++)
+                            if (j < n[t]) issue_qk(t, j);
+                    for (int j = 0; j < tiles && !failed; ++j) {
+                        const int b = j & 1;
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {
+                            if (j >= n[t]) continue;
+                            mbar_wait_warp(&sm.p_ready[t][b], rows[t].parity(j), status, 643, failed);
+                            mbar_wait_warp(&sm.full_v[b], keys.parity(j), status, 644, failed);
+                            if (failed) break;
+                            tc_fence_after_sync();
+                            const uint64_t v0 = dv + b * STAGE;
+                            const uint32_t pa = tm + (2 * t + b) * KEYS, d = tm + TMEM_O + t * HD;
+                            umma_f16_ts(d, pa, v0, IDESC_PV, j ? 1u : 0u, one);
+#pragma unroll
+                            for (int kk = 1; kk < 4; kk++) umma_f16_ts(d, pa + kk * 8, v0 + 128 * kk, IDESC_PV, 1u, one);
+                            umma_commit(&sm.pv_done[t][b], one);
+                            if (j + 2 < n[t]) issue_qk(t, j + 2);  // S was read before P(j) was made
+                        }
+                    }
+                }
+                keys.add(tiles);
+                rows[0].add(n[0]);
+                rows[1].add(n[1]);
+                if (!leave()) break;
+            }
+        } else if (warp == COPY_WARP) {
+            // ======================= bytes out of the cache =======================
+            // Lane l keeps what concerns one block of 16 tokens of a tile of keys, K's for l = 0..3, V's for l = 4..7: its page's number,
+            // asked for two tiles ahead, its exponent, one ahead, and its copy of 2048 bytes.  Blocks that no query sees are not copied.
+            const uint32_t side = (lane >> 2) & 1, blk = lane & 3;
+            uint32_t stage = 0, round = 0;  // of the raw ring, over all items
+            for (;;) {
+                const Item& it = sm.item[slot];
+                if (!it.valid) break;
+                const int tiles = it.unit_tiles(), tile0 = it.tile0, band_lo = it.band_lo, last_pos = it.last_pos();
+                const uint32_t request = it.request, head = it.head;
+                auto key_of = [&](int j) { return (tile0 + j) * KEYS + (int)blk * TILE_TOK; };
+                auto seen = [&](int j) { return lane < 8 && j < tiles && key_of(j) <= last_pos && key_of(j) + TILE_TOK > band_lo; };
+                auto look = [&](int j) { return ld_global_if(seen(j), page_at(a.req, request, (uint32_t)key_of(j) / TILE_TOK)); };
+                auto tile_of = [&](int j, uint32_t page) { return seen(j) ? block_of_page(a.req, request, (uint32_t)key_of(j) / TILE_TOK, page) * a.n_kv + head : NO_SLOT; };
+                uint32_t now = tile_of(0, look(0)), page = look(1);
+                int e = ld_global_if(now != NO_SLOT, a.exps[side] + now);
+                for (int j = 0; j < tiles; ++j) {
+                    const uint32_t next = tile_of(j + 1, page);
+                    page = look(j + 2);
+                    mbar_wait_warp(&sm.raw_empty[stage], (round & 1) ^ 1, status, 650, failed, 50);
+                    if (failed) break;
+                    const uint32_t copied = __popc(__ballot_sync(0xffffffffu, now != NO_SLOT));
+                    if (lane == 0) mbar_arrive_expect_tx(&sm.raw_full[stage], copied * TILE_BYTES);
+                    __syncwarp();
+                    if (now != NO_SLOT)
+                        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                                     ::"r"(smem_u32(sm.raw[stage][side][blk])), "l"(a.pool[side] + (size_t)now * TILE_BYTES), "r"(TILE_BYTES), "r"(smem_u32(&sm.raw_full[stage]))
+                                     : "memory");
+                    const int e_next = ld_global_if(next != NO_SLOT, a.exps[side] + next);
+                    if (lane < 8) reinterpret_cast<float*>(sm.exps[stage + RAW * (round & 1)])[lane] = side ? (float)e : __int_as_float((127 + e) << 23);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sm.raw_full[stage]);
+                    e = e_next;
+                    now = next;
+                    if (++stage == RAW) stage = 0, round++;
+                }
+                if (!leave()) break;
+            }
+        } else {
+            for (;;) {
+                if (!sm.item[slot].valid) break;
+                if (warp == QUEUE_WARP) fetch_item(a, w, total, cut, &sm.item[slot ^ 1]);
+                if (!leave()) break;
+            }
+        }
+    } else if (warp >= CONVERT_WARP) {
+        // ======================= bytes to f16 =======================
+        regs_down<CONVERT_REGS>();
+        // Its 16 bytes of every block: eight lanes read one half of a row and the other half of the next, so that neither their reads
+        // nor their writes (the swizzle puts the even chunks of an even row where the odd row has its odd ones) meet a bank twice.
+        const uint32_t cw = warp - CONVERT_WARP, odd = (lane >> 2) & 1, half = (cw & 1) ^ odd, tok = (cw >> 1) * 8 + (lane >> 2), c = 2 * (lane & 3);
+        const uint32_t from = tok * 128 + half * 64 + (lane & 3) * 16;
+        const uint32_t to = half * HALF_TILE + tok * 128, at0 = to + ((c ^ (tok & 7)) << 4), at1 = to + (((c + 1) ^ (tok & 7)) << 4);
+        uint32_t stage = 0, round = 0;
+        Uses rows[2];
+        for (;;) {
+            const Item& it = sm.item[slot];
+            if (!it.valid) break;
+            const int n0 = it.n_tiles[0], n1 = it.n_tiles[1], tiles = max(n0, n1), tile0 = it.tile0, band_lo = it.band_lo, last_pos = it.last_pos();
+            const int last = n1 ? 1 : 0;  // the tile of queries whose products come last
+            for (int j = 0; j < tiles; ++j) {
+                const int b = j & 1, key0 = (tile0 + j) * KEYS + (int)tok;
+                const bool edge = (tile0 + j + 1) * KEYS - 1 > last_pos || (tile0 + j) * KEYS < band_lo;
+                const uint32_t raw = smem_u32(sm.raw[stage][0][0]) + from;
+                const uint32_t parity = last ? rows[1].parity(j) : rows[0].parity(j);  // of tile j - 2: the other one
+                mbar_wait_warp(&sm.raw_full[stage], round & 1, status, 651, failed);
+                if (j >= 2) mbar_wait_warp(&sm.s_ready[last][b], parity ^ 1, status, 645, failed);  // Q K^T of tile j - 2 has read the stage
+                if (failed) break;
+#pragma unroll
+                for (int side = 0; side < 2; side++) {
+                    if (side == 1 && j >= 2) mbar_wait_warp(&sm.pv_done[last][b], parity ^ 1, status, 646, failed);
+                    if (failed) break;
+                    uint4 d[4];
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(d[x].x), "=r"(d[x].y), "=r"(d[x].z), "=r"(d[x].w)
+                                     : "r"(raw + (side * 4 + x) * TILE_BYTES)
+                                     : "memory");
+                        // what no query sees counts as 0: its weight is 0, but 0 times a NaN that stands there would not be
+                        if (edge && (key0 + 16 * x > last_pos || key0 + 16 * x < band_lo)) d[x] = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    const uint32_t out = smem_u32(side ? sm.v[b][0] : sm.k[b][0]);
+#pragma unroll
+                    for (int x = 0; x < 4; x++) put_converted(out + at0 + x * 2048, out + at1 + x * 2048, d[x]);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(side ? &sm.full_v[b] : &sm.full_k[b]);
+                }
+                if (failed) break;
+                if (lane == 0) mbar_arrive(&sm.raw_empty[stage]);
+                if (++stage == RAW) stage = 0, round++;
+            }
+            rows[0].add(n0);
+            rows[1].add(n1);
+            if (!leave()) break;
+        }
+    } else {
+        // ======================= softmax: row r of tile t <-> tensor-memory lane r <-> thread r of warpgroup t =======================
+        regs_up<SOFTMAX_REGS>();
+        const int r = tid & 127, t = warp >> 2;
+        const float scale2 = a.scale * 1.4426950408889634f;  // > 0 (checked on the host)
+        const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = lane_addr + 2 * t * KEYS, o_at = lane_addr + TMEM_O + t * HD;
+        const uint32_t tok = (uint32_t)t * (ROWS / a.group) + (uint32_t)r / a.group;
+        const int window = a.req.window && a.req.window < MOST_KEYS ? (int)a.req.window : (int)MOST_KEYS;
+        Uses rows;
+        uint32_t key_tile = 0;  // over all items, for the exponents' ring
+        for (;;) {
+            const Item& it = sm.item[slot];
+            if (!it.valid) break;
+            const int tiles = it.n_tiles[t], tile0 = it.tile0, pos = it.first_pos + (int)tok, row_lo = max(pos + 1 - window, 0);
+            const int first_pos = it.first_pos + t * (ROWS / (int)a.group), last_lo = max(it.last_pos() + 1 - window, 0);
+            float m_run = NEG_SENTINEL, l_run = 0.0f;
+            for (int j = 0; j < tiles; ++j) {
+                const int b = j & 1, key0 = (tile0 + j) * KEYS;
+                mbar_wait(&sm.s_ready[t][b], rows.parity(j), status, 647, failed);
+                tc_fence_after_sync();
+                float v[64];
+                {
+                    uint32_t a0[32], a1[32];
+                    tmem_ld_32x32b_x32(s_at + b * KEYS, a0);
+                    tmem_ld_32x32b_x32(s_at + b * KEYS + 32, a1);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int x = 0; x < 32; x++) {
+                        v[x] = __uint_as_float(a0[x]);
+                        v[32 + x] = __uint_as_float(a1[x]);
+                    }
+                }
+                if (key0 + KEYS - 1 > first_pos || key0 < last_lo) {  // the tile crosses an edge of the band: keys [lo, end) as a bit each
+                    const int lo = min(max(row_lo - key0, 0), KEYS), end = min(max(pos + 1 - key0, 0), KEYS);
+                    const uint64_t upto = end == KEYS ? ~0ull : (1ull << end) - 1, from = lo == KEYS ? 0ull : ~0ull << lo;
+                    const uint32_t seen[2] = {(uint32_t)(upto & from), (uint32_t)((upto & from) >> 32)};
+#pragma unroll
+                    for (int x = 0; x < 64; x++)
+                        if (((seen[x / 32] >> (x % 32)) & 1u) == 0) v[x] = -INFINITY;
+                }
+                // Block by block of 16 keys: scores times K's power of two, plus V's exponent (the weights carry V's scale, l does not).
+                const float4 k4 = sm.exps[(key_tile + j) & (2 * RAW - 1)][0], v4 = sm.exps[(key_tile + j) & (2 * RAW - 1)][1];
+                const float ks[4] = {k4.x * scale2, k4.y * scale2, k4.z * scale2, k4.w * scale2}, ve[4] = {v4.x, v4.y, v4.z, v4.w};
+                float mx = -INFINITY;
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    float m0 = max3(v[16 * x], v[16 * x + 1], v[16 * x + 2]), m1 = max3(v[16 * x + 3], v[16 * x + 4], v[16 * x + 5]);
+#pragma unroll
+                    for (int y = 6; y < 16; y += 5) {
+                        m0 = max3(m0, v[16 * x + y], v[16 * x + y + 1]);
+                        m1 = max3(m1, v[16 * x + y + 2], v[16 * x + y + 3]);
+                        m0 = fmaxf(m0, v[16 * x + y + 4]);
+                    }
+                    mx = fmaxf(mx, fmaf(fmaxf(m0, m1), ks[x], ve[x]));
+                }
+                const bool grow = mx > m_run + RESCALE_T;
+                float corr = 1.0f;
+                if (grow) {
+                    corr = ex2(m_run - mx);
+                    m_run = mx;
+                    l_run *= corr;
+                }
+                uint32_t pk[32];
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    const float2 sc2 = make_float2(ks[x], ks[x]), neg_m = make_float2(ve[x] - m_run, ve[x] - m_run);
+                    float2 ls[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+                    for (int y = 8 * x; y < 8 * x + 8; y++) {
+                        const float2 z = __ffma2_rn(make_float2(v[2 * y], v[2 * y + 1]), sc2, neg_m);
+                        const float2 pp = make_float2(ex2(z.x), ex2(z.y));
+                        ls[y & 1] = __fadd2_rn(ls[y & 1], pp);  // l from the unrounded weights
+                        pk[y] = pack_half2(pp.x, pp.y);
+                    }
+                    l_run = fmaf((ls[0].x + ls[0].y) + (ls[1].x + ls[1].y), __int_as_float((127 - (int)ve[x]) << 23), l_run);
+                }
+                // O is scaled anew where a row's maximum moved, once P V of the tile before is complete.
+                if (j > 0 && __any_sync(0xffffffffu, grow)) {
+                    mbar_wait(&sm.pv_done[t][b ^ 1], rows.parity(j - 1), status, 648, failed);
+                    tc_fence_after_sync();
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t o[32];
+                        tmem_ld_32x32b_x32(o_at + 32 * c, o);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int x = 0; x < 32; x++) o[x] = __float_as_uint(__uint_as_float(o[x]) * corr);
+                        tmem_st_32x32b_x32(o_at + 32 * c, o);
+                    }
+                }
+                tmem_st_32x32b_x32(s_at + b * KEYS, pk);
+                tc_wait_st();
+                tc_fence_before_sync();
+                mbar_arrive(&sm.p_ready[t][b]);
+            }
+            if (tiles > 0) mbar_wait(&sm.pv_done[t][(tiles - 1) & 1], rows.parity(tiles - 1), status, 649, failed);  // the last P V: all of them
+            tc_fence_after_sync();
+
+            // ---- out = O / l, or this piece's part ----
+            const bool live = tok < it.toks, whole = it.pieces == 1;
+            __half* orow = a.out + ((size_t)(it.first_tok + tok) * (a.n_kv * a.group) + it.head * a.group + (uint32_t)r % a.group) * HD;
+            float4* prow = w.acc + ((size_t)it.slot * UNIT_ROWS + t * ROWS + r) * (HD / 4);
+            const float mul = l_run != 0.0f ? 1.0f / l_run : 0.0f;
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                uint32_t o[32];
+                if (tiles > 0) {  // the same for all
+                    tmem_ld_32x32b_x32(o_at + 32 * c, o);
+                    tc_wait_ld();
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 32; x++) o[x] = 0u;
+                }
+                if (!live) continue;
+                if (whole) {
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        uint4 h;
+                        uint32_t* hw = reinterpret_cast<uint32_t*>(&h);
+#pragma unroll
+                        for (int y = 0; y < 4; y++)  // a row that saw nothing is 0, whatever stands in V
+                            hw[y] = l_run != 0.0f ? pack_half2(__uint_as_float(o[8 * x + 2 * y]) * mul, __uint_as_float(o[8 * x + 2 * y + 1]) * mul) : 0u;
+                        *reinterpret_cast<uint4*>(orow + 32 * c + 8 * x) = h;
+                    }
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 8; x++)
+                        prow[8 * c + x] = make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]), __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
+                }
+            }
+            if (!whole) {
+                if (live) w.ml[(size_t)it.slot * UNIT_ROWS + t * ROWS + r] = make_float2(m_run, l_run);
+                __threadfence();
+                named_barrier_sync(1 + t, 128);
+                if (r == 0) {
+                    const uint32_t before = atomicAdd(w.done + 2 * it.counter + t, 1u);
+                    sm.last[t] = before + 1 == it.pieces;
+                    __threadfence();
+                }
+                named_barrier_sync(1 + t, 128);
+                if (sm.last[t] && live) {  // all pieces are written: merge them in their order
+                    const size_t first = ((size_t)(it.slot - it.piece)) * UNIT_ROWS + t * ROWS + r;
+                    float big = NEG_SENTINEL, den = 0.0f;
+                    for (uint32_t p = 0; p < it.pieces; p++) big = fmaxf(big, __ldcg(w.ml + first + (size_t)p * UNIT_ROWS).x);
+                    for (uint32_t p = 0; p < it.pieces; p++) {
+                        const float2 ml = __ldcg(w.ml + first + (size_t)p * UNIT_ROWS);
+                        den = fmaf(ex2(ml.x - big), ml.y, den);
+                    }
+                    const float inv = den != 0.0f ? 1.0f / den : 0.0f;
+#pragma unroll 1
+                    for (int c = 0; c < 8; c++) {
+                        float4 acc[4] = {};
+                        for (uint32_t p = 0; p < it.pieces; p++) {
+                            const float f = ex2(__ldcg(w.ml + first + (size_t)p * UNIT_ROWS).x - big) * inv;
+#pragma unroll
+                            for (int x = 0; x < 4; x++) {
+                                const float4 o = __ldcg(w.acc + (first + (size_t)p * UNIT_ROWS) * (HD / 4) + 4 * c + x);
+                                acc[x].x = fmaf(f, o.x, acc[x].x);
+                                acc[x].y = fmaf(f, o.y, acc[x].y);
+                                acc[x].z = fmaf(f, o.z, acc[x].z);
+                                acc[x].w = fmaf(f, o.w, acc[x].w);
+                            }
+                        }
+#pragma unroll
+                        for (int x = 0; x < 2; x++)
+                            *reinterpret_cast<uint4*>(orow + 16 * c + 8 * x) =
+                                make_uint4(pack_half2(acc[2 * x].x, acc[2 * x].y), pack_half2(acc[2 * x].z, acc[2 * x].w), pack_half2(acc[2 * x + 1].x, acc[2 * x + 1].y),
+                                           pack_half2(acc[2 * x + 1].z, acc[2 * x + 1].w));
+                    }
+                }
+            }
+            key_tile += (uint32_t)it.unit_tiles();
+            rows.add(tiles);
+            if (!leave()) break;
+        }
+    }
+    // A wait that ran out leaves MMAs (and Q's copy) in flight that nobody waits for: they get a bounded time to land.
+    if (__syncthreads_or(failed)) {
+        let_copies_land();
+        __syncthreads();
+    }
+    if (warp == 0) tmem_dealloc(tmem, TMEM_COLS);
+}
+
+// Pieces that can be under way: four for every place, and no more than sixteen of every unit there can be.
+uint32_t most_slots(int sm_count, uint32_t n_kv, uint32_t group, uint32_t requests, uint32_t tokens)
+{
+    const uint64_t by_units = ((uint64_t)tokens * group / UNIT_ROWS + requests) * n_kv * 16, by_places = 4ull * sm_count;
+    return (uint32_t)(by_units < by_places ? by_units : by_places);
+}
+
+}  // namespace
+
+size_t blocks_prefill_work(int sm_count, uint32_t n_kv, uint32_t group, uint32_t requests, uint32_t tokens)
+{
+    return (size_t)most_slots(sm_count, n_kv, group, requests, tokens) * UNIT_ROWS * (HD + 2) * 4;
+}
+
+int launch_blocks_prefill(const LaunchArgs& a, const BlocksAttn& k, const BlocksWork& work)
+{
+    CUtensorMap tm_q;
+    {
+        const uint64_t heads = (uint64_t)k.n_kv * k.group;
+        const uint64_t dims[3] = {HD, heads, k.req.tokens}, strides[2] = {HD * 2, heads * HD * 2};
+        const uint32_t box[3] = {64, k.group, ROWS / k.group};
+        if (int r = encode_tensor_map(a, &tm_q, 1, 3, const_cast<__half*>(k.q), dims, strides, box, 3)) return r;
+    }
+    const size_t smem = sizeof(PrefillSmem);
+    {
+        static std::mutex attr_mutex;
+        static bool attr_set[64] = {};
+        std::lock_guard<std::mutex> lock(attr_mutex);
+        if (a.device < 0 || a.device >= 64 || !attr_set[a.device]) {
+            if (int r = check_cuda(a, cudaFuncSetAttribute(blocks_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "cudaFuncSetAttribute(blocks_prefill)"))
+                return r;
+            cudaFuncAttributes at;
+            if (int r = check_cuda(a, cudaFuncGetAttributes(&at, blocks_prefill_kernel), "cudaFuncGetAttributes(blocks_prefill)")) return r;
+            if (at.numRegs < (int)LAUNCH_REGS) {  // setmaxnreg.inc would wait for registers that the block does not have
+                if (a.err) *a.err = "blocks_prefill_kernel was built with fewer registers than it redistributes";
+                return 4;
+            }
+            if (a.device >= 0 && a.device < 64) attr_set[a.device] = true;
+        }
+    }
+    PrefillWork w{work.units_before, work.queue, work.done, nullptr, nullptr, most_slots(a.sm_count, k.n_kv, k.group, k.req.n, k.req.tokens)};
+    w.acc = reinterpret_cast<float4*>(work.parts);
+    w.ml = reinterpret_cast<float2*>(w.acc + (size_t)w.slots * UNIT_ROWS * (HD / 4));
+    const cudaError_t e = launch_dependent(blocks_prefill_kernel, dim3(a.sm_count), dim3(THREADS), smem, a.stream, tm_q, k, w);
+    ++*a.launches;
+    return check_cuda(a, e, "attn_blocks prefill");
+}
+
+}  // namespace sgb

@@ -52,22 +52,19 @@ __device__ __forceinline__ Request request_at(const Requests& a, uint32_t r)
     }
     return q;
 }
-// The pool's block that holds tokens 16 * tile .. of request r; a page that the pool does not have is reported and read as page 0.
-__device__ __forceinline__ uint32_t block_at(const Requests& a, uint32_t r, uint32_t tile)
+// The pool's block that holds tokens 16 * tile .. of request r, in two steps, so that nothing waits for the table in between: its
+// page's number, then the block.  A page that the pool does not have is reported and read as page 0.
+__device__ __forceinline__ uint32_t block_of_page(const Requests& a, uint32_t r, uint32_t tile, uint32_t page)
 {
-    const uint32_t shift = a.page_shift - 4, lp = tile >> shift;
-    uint32_t page = 0;
-    if (lp < a.stride) {
-        page = ld_global(a.table + (size_t)r * a.stride + lp);
-    } else {
-        report_error(a.status, DEV_ERR_BOUNDS, 603, r, lp);
-    }
+    const uint32_t shift = a.page_shift - 4;
     if (page >= a.pool_pages) {
         report_error(a.status, DEV_ERR_BOUNDS, 604, r, page);
         page = 0;
     }
     return (page << shift) + (tile & ((1u << shift) - 1));
 }
+// `tile` lies within the request's keys, and those within its row of the table (request_at cuts them).
+__device__ __forceinline__ const uint32_t* page_at(const Requests& a, uint32_t r, uint32_t tile) { return a.table + (size_t)r * a.stride + (tile >> (a.page_shift - 4)); }
 
 // A dispatch of attn_blocks_e4m3_d128.
 struct BlocksAttn {
@@ -76,14 +73,34 @@ struct BlocksAttn {
     const uint8_t* pool[2];
     const int8_t* exps[2];
     __half* out;
-    uint8_t* work;
     uint32_t n_kv, group, tiles;  // tiles of a pool: blocks x kv heads
     float scale;
 };
 struct LaunchArgs;
-// attn_blocks_decode.cu
-size_t blocks_decode_work(int sm_count, uint32_t n_kv, uint32_t group, uint32_t requests, uint32_t max_q);
-int launch_blocks_decode(const LaunchArgs&, const BlocksAttn&);
+
+// Loads that may be left out, as one instruction: a branch around the load would have its result moved behind it, and so waited for.
+__device__ __forceinline__ uint4 ld_global_if(bool p, const uint4* at)
+{
+    uint4 v;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %5, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+        "@p ld.global.v4.b32 {%0, %1, %2, %3}, [%4];\n\t}"
+        : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+        : "l"(at), "r"((uint32_t)p));
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_global_if(bool p, const uint32_t* at)
+{
+    uint32_t v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.b32 %0, [%1];\n\t}" : "=&r"(v) : "l"(at), "r"((uint32_t)p));
+    return v;
+}
+__device__ __forceinline__ int ld_global_if(bool p, const int8_t* at)
+{
+    int v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.s8 %0, [%1];\n\t}" : "=&r"(v) : "l"(at), "r"((uint32_t)p));
+    return v;
+}
 
 // Two e4m3 bytes as two f16, exactly (one instruction at the rate of an integer one: 64 a clock and SM).
 __device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two_bytes)

@@ -71,7 +71,7 @@ __device__ __forceinline__ void place_token(const PlanArgs& a, uint32_t t)
     a.at[t] = pos;
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) block_tables_kernel(const PlanArgs a)
+__global__ void __launch_bounds__(PLAN_THREADS) block_tables_kernel(const __grid_constant__ PlanArgs a)
 {
     __shared__ uint64_t sums[PLAN_WARPS];
     const int lane = threadIdx.x & 31;
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_tables_kernel(const PlanAr
     }
 }
 
-__global__ void __launch_bounds__(256) place_tokens_kernel(const PlanArgs a)
+__global__ void __launch_bounds__(256) place_tokens_kernel(const __grid_constant__ PlanArgs a)
 {
     pdl_wait();
     pdl_launch_dependents();
@@ -269,7 +269,7 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int side, uint32
 
 // SPAN tokens of the slot map per warp, kv head and side.
 template <int SPAN>
-__global__ void __launch_bounds__(APPEND_THREADS) append_blocks_kernel(const AppendArgs a)
+__global__ void __launch_bounds__(APPEND_THREADS) append_blocks_kernel(const __grid_constant__ AppendArgs a)
 {
     pdl_wait();
     pdl_launch_dependents();
