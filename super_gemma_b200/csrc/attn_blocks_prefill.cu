@@ -344,46 +344,52 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t cw = warp - CONVERT_WARP, odd = (lane >> 2) & 1, half = (cw & 1) ^ odd, tok = (cw >> 1) * 8 + (lane >> 2), c = 2 * (lane & 3);
         const uint32_t from = tok * 128 + half * 64 + (lane & 3) * 16;
         const uint32_t to = half * HALF_TILE + tok * 128, at0 = to + ((c ^ (tok & 7)) << 4), at1 = to + (((c + 1) ^ (tok & 7)) << 4);
-        uint32_t stage = 0, round = 0;
+        // Keys go two tiles ahead of values: Q K^T(j + 2) is issued right behind P V(j), so the order is K(0) K(1) V(0) K(2) V(1) K(3) ...
+        // (in step, a tile's K behind the V before it, the tensor pipe waited 540 cycles a tile for K; a chunk of 2048 tokens 2055 us).
+        uint32_t ring = 0;  // tiles through the raw ring before this item
         Uses rows[2];
         for (;;) {
             const Item& it = sm.item[slot];
             if (!it.valid) break;
             const int n0 = it.n_tiles[0], n1 = it.n_tiles[1], tiles = max(n0, n1), tile0 = it.tile0, band_lo = it.band_lo, last_pos = it.last_pos();
             const int last = n1 ? 1 : 0;  // the tile of queries whose products come last
-            for (int j = 0; j < tiles; ++j) {
-                const int b = j & 1, key0 = (tile0 + j) * KEYS + (int)tok;
+            auto convert = [&](int side, int j) {
+                const int key0 = (tile0 + j) * KEYS + (int)tok;
                 const bool edge = (tile0 + j + 1) * KEYS - 1 > last_pos || (tile0 + j) * KEYS < band_lo;
-                const uint32_t raw = smem_u32(sm.raw[stage][0][0]) + from;
-                const uint32_t parity = last ? rows[1].parity(j) : rows[0].parity(j);  // of tile j - 2: the other one
-                mbar_wait_warp(&sm.raw_full[stage], round & 1, status, 651, failed);
-                if (j >= 2) mbar_wait_warp(&sm.s_ready[last][b], parity ^ 1, status, 645, failed);  // Q K^T of tile j - 2 has read the stage
-                if (failed) break;
+                const uint32_t raw = smem_u32(sm.raw[(ring + j) % RAW][side][0]) + from;
+                uint4 d[4];
 #pragma unroll
-                for (int side = 0; side < 2; side++) {
-                    if (side == 1 && j >= 2) mbar_wait_warp(&sm.pv_done[last][b], parity ^ 1, status, 646, failed);
-                    if (failed) break;
-                    uint4 d[4];
-#pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                     : "=r"(d[x].x), "=r"(d[x].y), "=r"(d[x].z), "=r"(d[x].w)
-                                     : "r"(raw + (side * 4 + x) * TILE_BYTES)
-                                     : "memory");
-                        // what no query sees counts as 0: its weight is 0, but 0 times a NaN that stands there would not be
-                        if (edge && (key0 + 16 * x > last_pos || key0 + 16 * x < band_lo)) d[x] = make_uint4(0u, 0u, 0u, 0u);
-                    }
-                    const uint32_t out = smem_u32(side ? sm.v[b][0] : sm.k[b][0]);
-#pragma unroll
-                    for (int x = 0; x < 4; x++) put_converted(out + at0 + x * 2048, out + at1 + x * 2048, d[x]);
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(side ? &sm.full_v[b] : &sm.full_k[b]);
+                for (int x = 0; x < 4; x++) {
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(d[x].x), "=r"(d[x].y), "=r"(d[x].z), "=r"(d[x].w)
+                                 : "r"(raw + x * TILE_BYTES)
+                                 : "memory");
+                    // what no query sees counts as 0: its weight is 0, but 0 times a NaN that stands there would not be
+                    if (edge && (key0 + 16 * x > last_pos || key0 + 16 * x < band_lo)) d[x] = make_uint4(0u, 0u, 0u, 0u);
                 }
+                const uint32_t out = smem_u32(side ? sm.v[j & 1][0] : sm.k[j & 1][0]);
+#pragma unroll
+                for (int x = 0; x < 4; x++) put_converted(out + at0 + x * 2048, out + at1 + x * 2048, d[x]);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(side ? &sm.full_v[j & 1] : &sm.full_k[j & 1]);
+            };
+            auto keys = [&](int j) {
+                mbar_wait_warp(&sm.raw_full[(ring + j) % RAW], ((ring + j) / RAW) & 1, status, 651, failed);
+                // Q K^T of tile j - 2 has read the stage
+                if (j >= 2) mbar_wait_warp(&sm.s_ready[last][j & 1], (last ? rows[1].parity(j) : rows[0].parity(j)) ^ 1, status, 645, failed);
+                if (!failed) convert(0, j);
+            };
+            if (tiles > 0) keys(0);
+            if (tiles > 1 && !failed) keys(1);
+            for (int j = 0; j < tiles && !failed; ++j) {
+                if (j >= 2) mbar_wait_warp(&sm.pv_done[last][j & 1], (last ? rows[1].parity(j) : rows[0].parity(j)) ^ 1, status, 646, failed);
                 if (failed) break;
-                if (lane == 0) mbar_arrive(&sm.raw_empty[stage]);
-                if (++stage == RAW) stage = 0, round++;
+                convert(1, j);
+                if (lane == 0) mbar_arrive(&sm.raw_empty[(ring + j) % RAW]);
+                if (j + 2 < tiles) keys(j + 2);
             }
+            ring += (uint32_t)tiles;
             rows[0].add(n0);
             rows[1].add(n1);
             if (!leave()) break;
