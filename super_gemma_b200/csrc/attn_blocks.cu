@@ -27,8 +27,8 @@ size_t attn_blocks_work_bytes(int sm_count, uint32_t n_kv, uint32_t group, uint3
 {
     if (n_kv == 0 || group == 0 || group > FEW_ROWS || requests == 0 || tokens == 0 || max_q == 0) return 0;
     const size_t few = blocks_decode_work(sm_count, n_kv, group, max_q);
-    const size_t many = (uint64_t)max_q * group > FEW_ROWS ? blocks_prefill_work(sm_count, n_kv, group, requests, tokens) : 0;
-    return blocks_work_header(requests, (uint32_t)sm_count) + (few > many ? few : many);
+    const size_t many = (uint64_t)max_q * group > FEW_ROWS ? blocks_prefill_work(sm_count) : 0;
+    return blocks_work_header(requests, blocks_places(sm_count)) + (few > many ? few : many);
 }
 
 // attn_blocks_e4m3_d128: q, k pool, k exps, v pool, v exps, table, lens, starts, out f16, work.
@@ -64,8 +64,8 @@ int launch_attn_blocks(const LaunchArgs& a)
     const BlocksAttn k{{(const uint32_t*)a.b[5].ptr, (const uint32_t*)a.b[6].ptr, (const uint32_t*)a.b[7].ptr, n, p.stride, shift,
                         (uint32_t)(blocks >> (shift - 4)), tokens, p.max_q, p.window, a.status},
                        (const __half*)a.b[0].ptr, {(const uint8_t*)a.b[1].ptr, (const uint8_t*)a.b[3].ptr}, {(const int8_t*)a.b[2].ptr, (const int8_t*)a.b[4].ptr},
-                       (__half*)a.b[8].ptr, n_kv, p.group, (uint32_t)(blocks * n_kv), p.scale};
-    const BlocksWork work = blocks_work_at((uint8_t*)a.b[9].ptr, n, (uint32_t)a.sm_count);
+                       (__half*)a.b[8].ptr, n_kv, p.group, (uint32_t)__builtin_ctz(p.group), (uint32_t)(blocks * n_kv), p.scale};
+    const BlocksWork work = blocks_work_at((uint8_t*)a.b[9].ptr, n, blocks_places(a.sm_count));
     if (int r = launch_blocks_decode(a, k, work)) return r;
     return (uint64_t)p.max_q * p.group > FEW_ROWS ? launch_blocks_prefill(a, k, work) : 0;
 }

@@ -10,8 +10,8 @@
 // softmax, as in the decode: K's times the scores, V's into the exponent.
 //
 // One CTA per SM stays and takes units from a queue (the lengths are known on the device only); one warp fetches the next while the
-// others work.  What is left when every CTA has had its whole units is cut along the keys; the CTA that finishes the last piece of a unit
-// merges them, in their order, so reruns give the same bits.
+// others work.  The units that are left when every CTA has had its whole ones are laid end to end and cut into equal stretches; the CTA
+// that finishes the last piece of a unit merges them, in their order, so reruns give the same bits.
 #include <mutex>
 
 #include "blocks.cuh"
@@ -25,19 +25,20 @@ namespace {
 constexpr int HD = 128;
 constexpr int ROWS = 128, KEYS = 64;              // of a tile of queries, of keys
 constexpr int THREADS = 512;                      // two softmax warpgroups, one that converts, one of single warps
-constexpr int CONVERT_WARP = 8, MMA_WARP = 12, COPY_WARP = 13, QUEUE_WARP = 14;
+constexpr int CONVERT_WARP = 8, MMA_WARP = 12, COPY_WARP = 13, QUEUE_WARP = 14, QUERY_WARP = 15;
 constexpr int RAW = 4;                            // tiles of keys under way from the cache
+constexpr int ITEMS = 2;                          // the item at work and the next: what a CTA takes early no other can take
+constexpr int ITEM_READERS = 8 + 4 + 3;           // warps that give an item's place back
 constexpr uint32_t HALF_TILE = 64 * 128;          // [64 rows][64 dims] f16
 constexpr uint32_t Q_BYTES = 4 * HALF_TILE;       // of one tile of queries
 constexpr uint32_t TMEM_COLS = 512, TMEM_O = 256; // S: [tile][buffer] of 64 columns, then O: [tile] of 128
 constexpr float RESCALE_T = 8.0f;
-constexpr int LEAST_TILES = 8;                    // of a piece
 // Registers: 512 threads are launched with 128 each; the warpgroups redistribute exactly those.
 constexpr uint32_t LAUNCH_REGS = 128, SOFTMAX_REGS = 160, CONVERT_REGS = 96, ISSUE_REGS = 96;
 static_assert(2 * SOFTMAX_REGS + CONVERT_REGS + ISSUE_REGS <= 4 * LAUNCH_REGS, "setmaxnreg draws on what the block was launched with");
 
 struct Item {
-    uint32_t valid, request, head, first_tok, toks, piece, pieces, slot, counter;
+    uint32_t valid, request, head, first_tok, toks, piece, pieces, slot, slot0, counter;  // slot, slot0: of this piece's part and of piece 0's
     int first_pos, band_lo, tile0;  // position of the first query, first key that any row sees, first tile of 64 keys
     int n_tiles[2];                 // of either tile of queries; the second has none, or as many as the unit
     __device__ int unit_tiles() const { return max(n_tiles[0], n_tiles[1]); }
@@ -49,94 +50,115 @@ struct PrefillSmem {
     uint8_t k[2][2][HALF_TILE];      // [stage][dim half][64 keys x 128 B]
     uint8_t v[2][2][HALF_TILE];
     uint8_t raw[RAW][2][4][TILE_BYTES];  // [stage][K, V][block]: as cached
+    uint64_t item_full[ITEMS], item_empty[ITEMS];
     uint64_t raw_full[RAW], raw_empty[RAW];
     uint64_t full_k[2], full_v[2];   // converting warps: the tile is there
+    uint64_t k_free[2], v_free[2];   // MMA commit: both tiles of queries are done with it
     uint64_t s_ready[2][2];          // [tile][buffer] MMA commit: S holds Q K^T
     uint64_t p_ready[2][2];          // softmax threads: P is in tensor memory
     uint64_t pv_done[2][2];          // MMA commit: O += P V is complete
-    uint64_t q_bar;
+    uint64_t q_full, o_free[2];      // Q's copies; softmax threads: O of the last item has been read
     float4 exps[2 * RAW][2];         // [tile of keys % 8]: the powers of two of K, and the exponents of V, of its four blocks
-    Item item[2];
+    Item item[ITEMS];
     uint32_t tmem_base, last[2];
+    uint4 rows[8][32][5];            // of each softmax warp: 32 dims of its 32 rows in f16 on their way out, 80 bytes a row
 };
 static_assert(sizeof(PrefillSmem) <= 227 * 1024, "shared memory of a CTA");
 
 template <uint32_t N> __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <uint32_t N> __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// How the units go over the places: `whole` of them one by one, each of the others in `pieces`.
-struct Cut {
-    uint32_t units, whole, pieces;
-    __device__ uint32_t items() const { return whole + (units - whole) * pieces; }
+// Takes items from the queue; by a whole warp, which keeps what is left of its stretch.
+struct Feed {
+    uint32_t total, items, whole, stretches, rest_tiles;
+    bool by_head, sorted;
+    uint32_t at = 0, end = 0, stretch = 0, next_unit = 0;  // of the stretch: tiles of the cut units that are still to do, the unit that they begin in
 };
-__device__ __forceinline__ Cut cut_units(uint32_t units, uint32_t places, uint32_t most_slots)
+__device__ __forceinline__ uint32_t stretch_of_tile(const Feed& f, uint32_t tile) { return (uint32_t)((((uint64_t)tile + 1) * f.stretches - 1) / f.rest_tiles); }
+__device__ __forceinline__ Feed open_feed(const BlocksAttn& a, const BlocksWork& w)
 {
-    Cut c{units, units / places * places, 1};
-    const uint32_t rest = units - c.whole;
-    float best = 1.0f;
-    for (uint32_t p = 2; p <= 16 && rest * p <= most_slots; p++) {
-        const float cost = (float)((rest * p + places - 1) / places) / (float)p + 0.005f * (float)p;  // a piece's partial costs about a three-hundredth of a long unit
-        if (rest != 0 && cost < best) best = cost, c.pieces = p;
-    }
-    if (c.pieces == 1) c.whole = units;
-    return c;
+    Feed f;
+    f.total = ld_global(w.units_before + a.req.n);  // units of a kv head
+    f.items = f.total * a.n_kv;
+    f.whole = whole_items(f.items, w.places);
+    f.rest_tiles = ld_global(w.rest + w.places);
+    f.stretches = rest_stretches(f.rest_tiles, w.places);
+    f.by_head = ld_global(w.by_head) != 0;
+    f.sorted = f.total <= MOST_SORTED;
+    return f;
 }
-
-// The queue's next item that has work; by a whole warp.
-__device__ __forceinline__ void fetch_item(const BlocksAttn& a, const PrefillWork& w, uint32_t total, const Cut& cut, Item* out)
+__device__ __forceinline__ void fetch_item(const BlocksAttn& a, const BlocksWork& w, Feed& f, Item* out)
 {
     const uint32_t lane = threadIdx.x & 31;
     Item it;
     it.valid = 0;
+    uint32_t i = 0, rest = 0, begin = 0, n = 0;  // the item; of one that is cut: its number among those, its first tile and its tiles
+    it.piece = it.slot = it.slot0 = it.counter = 0;
+    it.pieces = 1;
+    const uint32_t cut = f.items - f.whole;
     for (;;) {
-        uint32_t i = 0;
+        if (f.at < f.end) {  // on with the stretch
+            rest = f.next_unit;
+            const uint32_t before = ld_global(w.rest + rest), after = rest + 1 < cut ? ld_global(w.rest + rest + 1) : f.rest_tiles;
+            f.next_unit++;
+            begin = f.at - before;
+            n = min(after, f.end) - f.at;
+            f.at += n;
+            i = f.whole + rest;
+            const uint32_t s0 = stretch_of_tile(f, before), s1 = stretch_of_tile(f, after - 1);
+            it.pieces = s1 - s0 + 1;
+            it.piece = f.stretch - s0;
+            it.slot0 = 2 * s0 + 1;
+            it.slot = it.piece ? 2 * f.stretch : it.slot0;
+            it.counter = rest;
+            break;
+        }
         if (lane == 0) i = atomicAdd(w.queue, 1u);
         i = __shfl_sync(0xffffffffu, i, 0);
-        if (i >= cut.items()) break;
-        uint32_t unit = i;
-        it.piece = 0;
-        uint32_t pieces = 1;
-        it.slot = it.counter = 0;
-        if (i >= cut.whole) {
-            it.slot = i - cut.whole;
-            it.counter = it.slot / cut.pieces;
-            unit = cut.whole + it.counter;
-            it.piece = it.slot % cut.pieces;
-            pieces = cut.pieces;
+        if (i < f.whole) break;
+        i -= f.whole;
+        if (i >= f.stretches) {
+            if (lane == 0) *out = it;
+            return;
         }
-        it.head = unit / total;
-        const uint32_t u = total - 1 - unit % total;  // the last tile of a request has the most keys
-        uint32_t lo = 0, n = a.req.n;                 // the request: the last one with units_before <= u
-        while (n > 1) {
-            const uint32_t step = (n + 31) / 32, probe = lo + lane * step;
-            const bool at_or_before = lane * step < n && ld_global(w.units_before + probe) <= u;
-            const uint32_t k = 31 - __clz(__ballot_sync(0xffffffffu, at_or_before));  // lane 0 always is
-            lo += k * step;
-            n = min(step, n - k * step);
+        f.stretch = i;
+        f.at = (uint32_t)((uint64_t)f.rest_tiles * i / f.stretches);
+        f.end = (uint32_t)((uint64_t)f.rest_tiles * (i + 1) / f.stretches);
+        // the unit that tile `at` is of: the last one with rest <= at
+        uint32_t lo = 0;
+        for (uint32_t base = 0; base < cut; base += 32) {
+            const bool le = base + lane < cut && ld_global(w.rest + base + lane) <= f.at;
+            lo += __popc(__ballot_sync(0xffffffffu, le));
         }
-        it.request = lo;
-        const Request rq = request_at(a.req, lo);
-        const uint32_t per = UNIT_ROWS / a.group, half = per / 2, tok0 = (u - ld_global(w.units_before + lo)) * per;
-        it.first_tok = rq.first + tok0;
-        it.toks = min(per, rq.n - tok0);
-        it.first_pos = (int)rq.len - (int)rq.n + (int)tok0;
-        const int last_pos = it.last_pos(), window = a.req.window && a.req.window < MOST_KEYS ? (int)a.req.window : (int)MOST_KEYS;
-        it.band_lo = max(it.first_pos + 1 - window, 0);
-        const int t_lo = it.band_lo / KEYS, n_tiles = last_pos >= 0 ? last_pos / KEYS - t_lo + 1 : 0;
-        it.pieces = min(pieces, (uint32_t)max(1, n_tiles / LEAST_TILES));
-        if (it.piece >= it.pieces) continue;
-        const int per_piece = (n_tiles + (int)it.pieces - 1) / (int)it.pieces, begin = min(n_tiles, (int)it.piece * per_piece);
-        it.tile0 = t_lo + begin;
-        const int mine = min(n_tiles, begin + per_piece) - begin;
-        it.n_tiles[0] = mine;
-        it.n_tiles[1] = 0;
-        if (it.toks > half) {  // the second tile of queries goes to the end, the first as far as its last query sees
-            const int last_first = it.first_pos + (int)half - 1;
-            it.n_tiles[1] = mine;
-            it.n_tiles[0] = last_first >= 0 ? min(mine, max(0, last_first / KEYS + 1 - it.tile0)) : 0;
-        }
-        it.valid = 1;
-        break;
+        f.next_unit = lo - 1;
+    }
+    uint32_t head, rank;
+    split_item(i, f.total, a.n_kv, f.by_head, head, rank);
+    const uint32_t u = f.sorted ? ld_global(w.order + rank) : f.total - 1 - rank;
+    uint32_t lo = 0, left = a.req.n;  // the request: the last one with units_before <= u
+    while (left > 1) {
+        const uint32_t step = (left + 31) / 32, probe = lo + lane * step;
+        const bool at_or_before = lane * step < left && ld_global(w.units_before + probe) <= u;
+        const uint32_t k = 31 - __clz(__ballot_sync(0xffffffffu, at_or_before));  // lane 0 always is
+        lo += k * step;
+        left = min(step, left - k * step);
+    }
+    const Unit unit = unit_at(a, lo, u - ld_global(w.units_before + lo));
+    it.valid = 1;
+    it.request = lo;
+    it.head = head;
+    it.first_tok = unit.first_tok;
+    it.toks = unit.toks;
+    it.first_pos = unit.first_pos;
+    it.band_lo = unit.band_lo;
+    const int mine = i < f.whole ? unit.n_tiles : min((int)n, unit.n_tiles), half = (ROWS >> (int)a.group_shift);
+    it.tile0 = unit.tile0 + (int)begin;
+    it.n_tiles[0] = mine;
+    it.n_tiles[1] = 0;
+    if ((int)it.toks > half) {  // the second tile of queries goes to the end, the first as far as its last query sees
+        const int last_first = it.first_pos + half - 1;
+        it.n_tiles[1] = mine;
+        it.n_tiles[0] = last_first >= 0 ? min(mine, max(0, last_first / KEYS + 1 - it.tile0)) : 0;
     }
     if (lane == 0) *out = it;
 }
@@ -156,7 +178,7 @@ __device__ __forceinline__ void put_converted(uint32_t chunk0, uint32_t chunk1, 
 }
 
 __global__ void __launch_bounds__(THREADS, 1)
-    blocks_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ BlocksAttn a, const __grid_constant__ PrefillWork w)
+    blocks_prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ BlocksAttn a, const __grid_constant__ BlocksWork w, float4* acc_parts, float2* ml_parts)
 {
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     PrefillSmem& sm = *reinterpret_cast<PrefillSmem*>(smem_raw);
@@ -168,6 +190,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int tid = threadIdx.x, warp = warp_uniform(tid >> 5);
     const uint32_t lane = tid & 31;
     if (tid == 0) {
+        for (int i = 0; i < ITEMS; i++) {
+            mbar_init(&sm.item_full[i], 1);
+            mbar_init(&sm.item_empty[i], ITEM_READERS);
+        }
         for (int i = 0; i < RAW; i++) {
             mbar_init(&sm.raw_full[i], 2);  // the copies, and the exponents
             mbar_init(&sm.raw_empty[i], 4);
@@ -175,13 +201,16 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int i = 0; i < 2; i++) {
             mbar_init(&sm.full_k[i], 4);
             mbar_init(&sm.full_v[i], 4);
+            mbar_init(&sm.k_free[i], 1);
+            mbar_init(&sm.v_free[i], 1);
             for (int t = 0; t < 2; t++) {
                 mbar_init(&sm.s_ready[t][i], 1);
                 mbar_init(&sm.p_ready[t][i], 128);
                 mbar_init(&sm.pv_done[t][i], 1);
             }
+            mbar_init(&sm.o_free[i], 128);
         }
-        mbar_init(&sm.q_bar, 1);
+        mbar_init(&sm.q_full, 1);
         mbar_fence_init();
     }
     pdl_wait();  // everything this kernel reads comes from earlier kernels of the stream, the cut of the units among it
@@ -190,33 +219,26 @@ __global__ void __launch_bounds__(THREADS, 1)
         tmem_alloc(&sm.tmem_base, TMEM_COLS);
         tmem_relinquish();
     }
-    const uint32_t total = ld_global(w.units_before + a.req.n);  // units of a kv head
-    const Cut cut = cut_units(total * a.n_kv, gridDim.x, w.slots);
-    if (warp == QUEUE_WARP) fetch_item(a, w, total, cut, &sm.item[0]);
     tc_fence_before_sync();
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = sm.tmem_base;
     bool failed = false;
-    uint32_t slot = 0;
-    // All roles leave an item together, through this.  False: a wait has run out somewhere.
-    auto leave = [&]() {
-        slot ^= 1;
-        tc_fence_before_sync();
-        const bool any = __syncthreads_or(failed) != 0;
-        tc_fence_after_sync();
-        return !any;
+    // The roles go through the items each at its own pace, the copies and conversions of the next one beside the end of this one.
+    // Buffers are counted through: use u of a buffer of two is tile u of all, a barrier's phase u / 2.  Every wait is bounded, and a
+    // role that has waited in vain leaves; the others then run into their own bounds.
+    uint32_t nth = 0;
+    auto next_item = [&]() -> const Item* {  // by whole warps; null at the end
+        const Item& it = sm.item[nth % ITEMS];
+        mbar_wait_warp(&sm.item_full[nth % ITEMS], (nth / ITEMS) & 1, status, 652, failed, 20);
+        return !failed && it.valid ? &it : nullptr;
     };
-    // A barrier's phases go on from item to item: tile j of an item is use `before + j / 2` of buffer j % 2.
-    struct Uses {
-        uint32_t before[2] = {0, 0};
-        __device__ uint32_t parity(int j) const { return (((j & 1) ? before[1] : before[0]) + (uint32_t)(j >> 1)) & 1u; }
-        __device__ void add(int n)
-        {
-            before[0] += (uint32_t)(n + 1) / 2;
-            before[1] += (uint32_t)n / 2;
-        }
+    auto done_item = [&]() {  // what it said has been read
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.item_empty[nth % ITEMS]);
+        nth++;
     };
+    auto phase = [](uint32_t use) { return (use >> 1) & 1u; };
 
     if (warp >= MMA_WARP) {
         regs_down<ISSUE_REGS>();
@@ -228,67 +250,63 @@ __global__ void __launch_bounds__(THREADS, 1)
             const uint64_t dq = umma_desc_sw128(smem_u32(sm.q[0][0]), 16, 1024), dk = umma_desc_sw128(smem_u32(sm.k[0][0]), 16, 1024),
                            dv = umma_desc_sw128(smem_u32(sm.v[0][0]), HALF_TILE, 1024);
             constexpr uint64_t Q_TILE = Q_BYTES >> 4, Q_HALF = 2 * HALF_TILE >> 4, K_HALF = HALF_TILE >> 4, STAGE = 2 * HALF_TILE >> 4;
-            Uses keys, rows[2];
-            uint32_t q_phase = 0;
-            for (;;) {
-                const Item& it = sm.item[slot];
-                if (!it.valid) break;
-                const int n[2] = {warp_uniform(it.n_tiles[0]), warp_uniform(it.n_tiles[1])}, tiles = max(n[0], n[1]);
-                if (tiles > 0) {
-                    if (one) {
-                        mbar_arrive_expect_tx(&sm.q_bar, n[1] ? 2 * Q_BYTES : Q_BYTES);
+            uint32_t nth_q = 0, items[2] = {0, 0};
+            uint32_t key = 0, row[2] = {0, 0};  // tiles of keys, and of either tile of queries, before this item
+            for (; const Item* it = next_item();) {
+                const int n[2] = {warp_uniform(it->n_tiles[0]), warp_uniform(it->n_tiles[1])}, tiles = max(n[0], n[1]);
+                done_item();
+                if (tiles == 0) continue;
+                const int last = n[1] ? 1 : 0;  // the tile of queries whose products come last
+                auto issue_qk = [&](int t, int j) {
+                    const uint32_t kb = (key + j) & 1, sb = (row[t] + j) & 1;
+                    const uint64_t q0 = dq + t * Q_TILE, k0 = dk + kb * STAGE;
+                    const uint32_t d = tm + (2 * t + sb) * KEYS;
 #pragma unroll
-                        for (int t = 0; t < 2; t++) {
-                            if (t == 1 && !n[1]) break;
-                            const int row = (int)(it.first_tok + t * (ROWS / a.group));
-                            tma_load_3d(sm.q[t][0], &tm_q, &sm.q_bar, 0, (int)(it.head * a.group), row);
-                            tma_load_3d(sm.q[t][1], &tm_q, &sm.q_bar, 64, (int)(it.head * a.group), row);
-                        }
-                    }
-                    __syncwarp();
-                    auto issue_qk = [&](int t, int j) {
-                        const int b = j & 1;
-                        mbar_wait_warp(&sm.full_k[b], keys.parity(j), status, 641, failed);
-                        if (failed) return;
+                    for (int kk = 0; kk < 4; kk++) umma_f16_ss(d, q0 + 2 * kk, k0 + 2 * kk, IDESC_QK, kk ? 1u : 0u, one);
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++) umma_f16_ss(d, q0 + Q_HALF + 2 * kk, k0 + K_HALF + 2 * kk, IDESC_QK, 1u, one);
+                    umma_commit(&sm.s_ready[t][sb], one);
+                    if (t == last) umma_commit(&sm.k_free[kb], one);
+                };
+                auto keys = [&](int j) {  // waited for once, by the first tile that multiplies with them
+                    mbar_wait_warp(&sm.full_k[(key + j) & 1], phase(key + j), status, 641, failed);
+                    tc_fence_after_sync();
+                };
+                mbar_wait_warp(&sm.q_full, (nth_q++) & 1, status, 642, failed);
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    if (j < tiles) keys(j);
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+                        if (j < n[t] && !failed) issue_qk(t, j);
+                }
+                for (int j = 0; j < tiles && !failed; ++j) {
+#pragma unroll
+                    for (int t = 0; t < 2; t++) {
+                        if (j >= n[t]) continue;
+                        const uint32_t vb = (key + j) & 1, sb = (row[t] + j) & 1;
+                        if (j == 0) mbar_wait_warp(&sm.o_free[t], (items[t]++ & 1) ^ 1, status, 653, failed);
+                        mbar_wait_warp(&sm.p_ready[t][sb], phase(row[t] + j), status, 643, failed);
+                        if (t == 0 || j >= n[0]) mbar_wait_warp(&sm.full_v[vb], phase(key + j), status, 644, failed);
+                        if (failed) break;
                         tc_fence_after_sync();
-                        const uint64_t q0 = dq + t * Q_TILE, k0 = dk + b * STAGE;
-                        const uint32_t d = tm + (2 * t + b) * KEYS;
+                        const uint64_t v0 = dv + vb * STAGE;
+                        const uint32_t pa = tm + (2 * t + sb) * KEYS, d = tm + TMEM_O + t * HD;
+                        umma_f16_ts(d, pa, v0, IDESC_PV, j ? 1u : 0u, one);
 #pragma unroll
-                        for (int kk = 0; kk < 4; kk++) umma_f16_ss(d, q0 + 2 * kk, k0 + 2 * kk, IDESC_QK, kk ? 1u : 0u, one);
-#pragma unroll
-                        for (int kk = 0; kk < 4; kk++) umma_f16_ss(d, q0 + Q_HALF + 2 * kk, k0 + K_HALF + 2 * kk, IDESC_QK, 1u, one);
-                        umma_commit(&sm.s_ready[t][b], one);
-                    };
-                    mbar_wait_warp(&sm.q_bar, q_phase & 1, status, 642, failed);
-                    q_phase++;
-#pragma unroll
-                    for (int j = 0; j < 2; j++)
-#pragma unroll
-                        for (int t = 0; t < 2; t++)
-                            if (j < n[t]) issue_qk(t, j);
-                    for (int j = 0; j < tiles && !failed; ++j) {
-                        const int b = j & 1;
-#pragma unroll
-                        for (int t = 0; t < 2; t++) {
-                            if (j >= n[t]) continue;
-                            mbar_wait_warp(&sm.p_ready[t][b], rows[t].parity(j), status, 643, failed);
-                            mbar_wait_warp(&sm.full_v[b], keys.parity(j), status, 644, failed);
+                        for (int kk = 1; kk < 4; kk++) umma_f16_ts(d, pa + kk * 8, v0 + 128 * kk, IDESC_PV, 1u, one);
+                        umma_commit(&sm.pv_done[t][sb], one);
+                        if (t == last) umma_commit(&sm.v_free[vb], one);
+                        if (j + 2 < n[t]) {  // S was read before P(j) was made
+                            if (t == 0 || j + 2 >= n[0]) keys(j + 2);
                             if (failed) break;
-                            tc_fence_after_sync();
-                            const uint64_t v0 = dv + b * STAGE;
-                            const uint32_t pa = tm + (2 * t + b) * KEYS, d = tm + TMEM_O + t * HD;
-                            umma_f16_ts(d, pa, v0, IDESC_PV, j ? 1u : 0u, one);
-#pragma unroll
-                            for (int kk = 1; kk < 4; kk++) umma_f16_ts(d, pa + kk * 8, v0 + 128 * kk, IDESC_PV, 1u, one);
-                            umma_commit(&sm.pv_done[t][b], one);
-                            if (j + 2 < n[t]) issue_qk(t, j + 2);  // S was read before P(j) was made
+                            issue_qk(t, j + 2);
                         }
                     }
                 }
-                keys.add(tiles);
-                rows[0].add(n[0]);
-                rows[1].add(n[1]);
-                if (!leave()) break;
+                key += (uint32_t)tiles;
+                row[0] += (uint32_t)n[0];
+                row[1] += (uint32_t)n[1];
             }
         } else if (warp == COPY_WARP) {
             // ======================= bytes out of the cache =======================
@@ -296,11 +314,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             // asked for two tiles ahead, its exponent, one ahead, and its copy of 2048 bytes.  Blocks that no query sees are not copied.
             const uint32_t side = (lane >> 2) & 1, blk = lane & 3;
             uint32_t stage = 0, round = 0;  // of the raw ring, over all items
-            for (;;) {
-                const Item& it = sm.item[slot];
-                if (!it.valid) break;
-                const int tiles = it.unit_tiles(), tile0 = it.tile0, band_lo = it.band_lo, last_pos = it.last_pos();
-                const uint32_t request = it.request, head = it.head;
+            for (; const Item* it = next_item();) {
+                const int tiles = it->unit_tiles(), tile0 = it->tile0, band_lo = it->band_lo, last_pos = it->last_pos();
+                const uint32_t request = it->request, head = it->head;
+                done_item();
                 auto key_of = [&](int j) { return (tile0 + j) * KEYS + (int)blk * TILE_TOK; };
                 auto seen = [&](int j) { return lane < 8 && j < tiles && key_of(j) <= last_pos && key_of(j) + TILE_TOK > band_lo; };
                 auto look = [&](int j) { return ld_global_if(seen(j), page_at(a.req, request, (uint32_t)key_of(j) / TILE_TOK)); };
@@ -327,13 +344,36 @@ __global__ void __launch_bounds__(THREADS, 1)
                     now = next;
                     if (++stage == RAW) stage = 0, round++;
                 }
-                if (!leave()) break;
             }
-        } else {
-            for (;;) {
-                if (!sm.item[slot].valid) break;
-                if (warp == QUEUE_WARP) fetch_item(a, w, total, cut, &sm.item[slot ^ 1]);
-                if (!leave()) break;
+        } else if (warp == QUEUE_WARP) {
+            Feed feed = open_feed(a, w);
+            for (;; nth++) {
+                mbar_wait_warp(&sm.item_empty[nth % ITEMS], ((nth / ITEMS) & 1) ^ 1, status, 654, failed, 200);
+                if (failed) break;
+                fetch_item(a, w, feed, &sm.item[nth % ITEMS]);
+                __syncwarp();
+                const bool valid = sm.item[nth % ITEMS].valid;
+                if (lane == 0) mbar_arrive(&sm.item_full[nth % ITEMS]);
+                if (!valid) break;
+            }
+        } else if (warp == QUERY_WARP) {
+            // ======================= queries: once the item before has multiplied with its own for the last time =======================
+            uint32_t key = 0;
+            for (; const Item* it = next_item();) {
+                const int tiles = it->unit_tiles(), column = (int)(it->head * a.group), row = (int)it->first_tok;
+                const bool both = it->n_tiles[1] != 0;
+                done_item();
+                if (tiles == 0) continue;
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&sm.q_full, both ? 2 * Q_BYTES : Q_BYTES);
+                    for (int t = 0; t < (both ? 2 : 1); t++) {
+                        tma_load_3d(sm.q[t][0], &tm_q, &sm.q_full, 0, column, row + t * (ROWS >> a.group_shift));
+                        tma_load_3d(sm.q[t][1], &tm_q, &sm.q_full, 64, column, row + t * (ROWS >> a.group_shift));
+                    }
+                }
+                __syncwarp();
+                // phase after phase: a parity tells the awaited one from the one before it, and from no other
+                for (int j = 0; j < tiles && !failed; j++, key++) mbar_wait_warp(&sm.k_free[key & 1], phase(key), status, 655, failed, 100);
             }
         }
     } else if (warp >= CONVERT_WARP) {
@@ -346,17 +386,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t to = half * HALF_TILE + tok * 128, at0 = to + ((c ^ (tok & 7)) << 4), at1 = to + (((c + 1) ^ (tok & 7)) << 4);
         // Keys go two tiles ahead of values: Q K^T(j + 2) is issued right behind P V(j), so the order is K(0) K(1) V(0) K(2) V(1) K(3) ...
         // (in step, a tile's K behind the V before it, the tensor pipe waited 540 cycles a tile for K; a chunk of 2048 tokens 2055 us).
-        uint32_t ring = 0;  // tiles through the raw ring before this item
-        Uses rows[2];
-        for (;;) {
-            const Item& it = sm.item[slot];
-            if (!it.valid) break;
-            const int n0 = it.n_tiles[0], n1 = it.n_tiles[1], tiles = max(n0, n1), tile0 = it.tile0, band_lo = it.band_lo, last_pos = it.last_pos();
-            const int last = n1 ? 1 : 0;  // the tile of queries whose products come last
+        uint32_t key = 0;  // tiles of keys before this item
+        for (; const Item* it = next_item();) {
+            const int tiles = it->unit_tiles(), tile0 = it->tile0, band_lo = it->band_lo, last_pos = it->last_pos();
+            done_item();
             auto convert = [&](int side, int j) {
                 const int key0 = (tile0 + j) * KEYS + (int)tok;
                 const bool edge = (tile0 + j + 1) * KEYS - 1 > last_pos || (tile0 + j) * KEYS < band_lo;
-                const uint32_t raw = smem_u32(sm.raw[(ring + j) % RAW][side][0]) + from;
+                const uint32_t raw = smem_u32(sm.raw[(key + j) % RAW][side][0]) + from;
                 uint4 d[4];
 #pragma unroll
                 for (int x = 0; x < 4; x++) {
@@ -367,32 +404,28 @@ __global__ void __launch_bounds__(THREADS, 1)
                     // what no query sees counts as 0: its weight is 0, but 0 times a NaN that stands there would not be
                     if (edge && (key0 + 16 * x > last_pos || key0 + 16 * x < band_lo)) d[x] = make_uint4(0u, 0u, 0u, 0u);
                 }
-                const uint32_t out = smem_u32(side ? sm.v[j & 1][0] : sm.k[j & 1][0]);
+                const uint32_t out = smem_u32(side ? sm.v[(key + j) & 1][0] : sm.k[(key + j) & 1][0]);
 #pragma unroll
                 for (int x = 0; x < 4; x++) put_converted(out + at0 + x * 2048, out + at1 + x * 2048, d[x]);
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(side ? &sm.full_v[j & 1] : &sm.full_k[j & 1]);
+                if (lane == 0) mbar_arrive(side ? &sm.full_v[(key + j) & 1] : &sm.full_k[(key + j) & 1]);
             };
             auto keys = [&](int j) {
-                mbar_wait_warp(&sm.raw_full[(ring + j) % RAW], ((ring + j) / RAW) & 1, status, 651, failed);
-                // Q K^T of tile j - 2 has read the stage
-                if (j >= 2) mbar_wait_warp(&sm.s_ready[last][j & 1], (last ? rows[1].parity(j) : rows[0].parity(j)) ^ 1, status, 645, failed);
+                mbar_wait_warp(&sm.raw_full[(key + j) % RAW], ((key + j) / RAW) & 1, status, 651, failed);
+                if (key + j >= 2) mbar_wait_warp(&sm.k_free[(key + j) & 1], phase(key + j - 2), status, 645, failed, 20);
                 if (!failed) convert(0, j);
             };
             if (tiles > 0) keys(0);
             if (tiles > 1 && !failed) keys(1);
             for (int j = 0; j < tiles && !failed; ++j) {
-                if (j >= 2) mbar_wait_warp(&sm.pv_done[last][j & 1], (last ? rows[1].parity(j) : rows[0].parity(j)) ^ 1, status, 646, failed);
+                if (key + j >= 2) mbar_wait_warp(&sm.v_free[(key + j) & 1], phase(key + j - 2), status, 646, failed, 20);
                 if (failed) break;
                 convert(1, j);
-                if (lane == 0) mbar_arrive(&sm.raw_empty[(ring + j) % RAW]);
+                if (lane == 0) mbar_arrive(&sm.raw_empty[(key + j) % RAW]);
                 if (j + 2 < tiles) keys(j + 2);
             }
-            ring += (uint32_t)tiles;
-            rows[0].add(n0);
-            rows[1].add(n1);
-            if (!leave()) break;
+            key += (uint32_t)tiles;
         }
     } else {
         // ======================= softmax: row r of tile t <-> tensor-memory lane r <-> thread r of warpgroup t =======================
@@ -400,19 +433,27 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int r = tid & 127, t = warp >> 2;
         const float scale2 = a.scale * 1.4426950408889634f;  // > 0 (checked on the host)
         const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16), s_at = lane_addr + 2 * t * KEYS, o_at = lane_addr + TMEM_O + t * HD;
-        const uint32_t tok = (uint32_t)t * (ROWS / a.group) + (uint32_t)r / a.group;
+        const uint32_t tok = (uint32_t)t * (ROWS >> a.group_shift) + ((uint32_t)r >> a.group_shift);
         const int window = a.req.window && a.req.window < MOST_KEYS ? (int)a.req.window : (int)MOST_KEYS;
-        Uses rows;
-        uint32_t key_tile = 0;  // over all items, for the exponents' ring
+        uint32_t row = 0, key = 0;  // tiles of this warpgroup's, and of keys (for the exponents' ring), before this item
         for (;;) {
-            const Item& it = sm.item[slot];
-            if (!it.valid) break;
-            const int tiles = it.n_tiles[t], tile0 = it.tile0, pos = it.first_pos + (int)tok, row_lo = max(pos + 1 - window, 0);
-            const int first_pos = it.first_pos + t * (ROWS / (int)a.group), last_lo = max(it.last_pos() + 1 - window, 0);
+            const Item* at = next_item();
+            if (named_barrier_or(1 + t, 128, failed)) {  // its warps leave together: they meet at barriers without a limit
+                failed = true;
+                break;
+            }
+            if (!at) break;
+            const int tiles = at->n_tiles[t], unit_tiles = at->unit_tiles();
+            const struct {
+                uint32_t head, first_tok, toks, pieces, slot, slot0, counter;
+                int first_pos, tile0, last_pos;
+            } it = {at->head, at->first_tok, at->toks, at->pieces, at->slot, at->slot0, at->counter, at->first_pos, at->tile0, at->last_pos()};
+            const int tile0 = it.tile0, pos = it.first_pos + (int)tok, row_lo = max(pos + 1 - window, 0);
+            const int first_pos = it.first_pos + t * (ROWS >> a.group_shift), last_lo = max(it.last_pos + 1 - window, 0);
             float m_run = NEG_SENTINEL, l_run = 0.0f;
             for (int j = 0; j < tiles; ++j) {
-                const int b = j & 1, key0 = (tile0 + j) * KEYS;
-                mbar_wait(&sm.s_ready[t][b], rows.parity(j), status, 647, failed);
+                const int b = (int)((row + j) & 1), key0 = (tile0 + j) * KEYS;
+                mbar_wait(&sm.s_ready[t][b], phase(row + j), status, 647, failed);
                 tc_fence_after_sync();
                 float v[64];
                 {
@@ -435,7 +476,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         if (((seen[x / 32] >> (x % 32)) & 1u) == 0) v[x] = -INFINITY;
                 }
                 // Block by block of 16 keys: scores times K's power of two, plus V's exponent (the weights carry V's scale, l does not).
-                const float4 k4 = sm.exps[(key_tile + j) & (2 * RAW - 1)][0], v4 = sm.exps[(key_tile + j) & (2 * RAW - 1)][1];
+                const float4 k4 = sm.exps[(key + j) & (2 * RAW - 1)][0], v4 = sm.exps[(key + j) & (2 * RAW - 1)][1];
                 const float ks[4] = {k4.x * scale2, k4.y * scale2, k4.z * scale2, k4.w * scale2}, ve[4] = {v4.x, v4.y, v4.z, v4.w};
                 float mx = -INFINITY;
 #pragma unroll
@@ -472,9 +513,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 // O is scaled anew where a row's maximum moved, once P V of the tile before is complete.
                 if (j > 0 && __any_sync(0xffffffffu, grow)) {
-                    mbar_wait(&sm.pv_done[t][b ^ 1], rows.parity(j - 1), status, 648, failed);
+                    mbar_wait(&sm.pv_done[t][b ^ 1], phase(row + j - 1), status, 648, failed);
                     tc_fence_after_sync();
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < 4; c++) {
                         uint32_t o[32];
                         tmem_ld_32x32b_x32(o_at + 32 * c, o);
@@ -489,15 +530,26 @@ __global__ void __launch_bounds__(THREADS, 1)
                 tc_fence_before_sync();
                 mbar_arrive(&sm.p_ready[t][b]);
             }
-            if (tiles > 0) mbar_wait(&sm.pv_done[t][(tiles - 1) & 1], rows.parity(tiles - 1), status, 649, failed);  // the last P V: all of them
+            if (tiles > 0) mbar_wait(&sm.pv_done[t][(row + tiles - 1) & 1], phase(row + tiles - 1), status, 649, failed);  // the last P V: all of them
             tc_fence_after_sync();
 
             // ---- out = O / l, or this piece's part ----
             const bool live = tok < it.toks, whole = it.pieces == 1;
-            __half* orow = a.out + ((size_t)(it.first_tok + tok) * (a.n_kv * a.group) + it.head * a.group + (uint32_t)r % a.group) * HD;
-            float4* prow = w.acc + ((size_t)it.slot * UNIT_ROWS + t * ROWS + r) * (HD / 4);
+            __half* orow = a.out + ((size_t)(it.first_tok + tok) * (a.n_kv * a.group) + it.head * a.group + ((uint32_t)r & (a.group - 1))) * HD;
+            // A part is [32 groups of four dims][128 rows] and (m, l) of the rows: neighbouring threads write neighbouring 16 bytes.
+            const auto part = [&](uint32_t s) { return acc_parts + (size_t)(2 * s + t) * (HD / 4) * ROWS + r; };
+            const auto part_ml = [&](uint32_t s) { return ml_parts + (size_t)(2 * s + t) * ROWS + r; };
             const float mul = l_run != 0.0f ? 1.0f / l_run : 0.0f;
+            const bool blank = __any_sync(0xffffffffu, l_run == 0.0f);
+            __half* row_out[4];  // where this thread stores its sixteen bytes of other threads' rows
+            bool row_live[4];
 #pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const uint32_t other = (uint32_t)(warp & 3) * 32 + 8 * x + (lane >> 2), tk = (uint32_t)t * (ROWS >> a.group_shift) + (other >> a.group_shift);
+                row_live[x] = tk < it.toks;
+                row_out[x] = a.out + ((size_t)(it.first_tok + tk) * (a.n_kv * a.group) + it.head * a.group + (other & (a.group - 1))) * HD + 8 * (lane & 3);
+            }
+#pragma unroll 1
             for (int c = 0; c < 4; c++) {
                 uint32_t o[32];
                 if (tiles > 0) {  // the same for all
@@ -507,25 +559,37 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                     for (int x = 0; x < 32; x++) o[x] = 0u;
                 }
-                if (!live) continue;
+                if (c == 3 && tiles > 0) {  // O may be overwritten
+                    tc_fence_before_sync();
+                    mbar_arrive(&sm.o_free[t]);
+                }
                 if (whole) {
 #pragma unroll
                     for (int x = 0; x < 4; x++) {
                         uint4 h;
                         uint32_t* hw = reinterpret_cast<uint32_t*>(&h);
 #pragma unroll
-                        for (int y = 0; y < 4; y++)  // a row that saw nothing is 0, whatever stands in V
-                            hw[y] = l_run != 0.0f ? pack_half2(__uint_as_float(o[8 * x + 2 * y]) * mul, __uint_as_float(o[8 * x + 2 * y + 1]) * mul) : 0u;
-                        *reinterpret_cast<uint4*>(orow + 32 * c + 8 * x) = h;
+                        for (int y = 0; y < 4; y++) {
+                            const float2 z = __fmul2_rn(make_float2(__uint_as_float(o[8 * x + 2 * y]), __uint_as_float(o[8 * x + 2 * y + 1])), make_float2(mul, mul));
+                            hw[y] = pack_half2(z.x, z.y);
+                        }
+                        if (blank && l_run == 0.0f) h = make_uint4(0u, 0u, 0u, 0u);  // a row that saw nothing is 0, whatever stands in V
+                        sm.rows[warp][lane][x] = h;
                     }
-                } else {
+                    // 64 bytes of each of eight rows go out together (a thread's own row by itself met a line a thread: 4700 cycles a unit)
+                    __syncwarp();
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        if (row_live[x]) *reinterpret_cast<uint4*>(row_out[x] + 32 * c) = sm.rows[warp][8 * x + (lane >> 2)][lane & 3];
+                    __syncwarp();
+                } else if (live) {
 #pragma unroll
                     for (int x = 0; x < 8; x++)
-                        prow[8 * c + x] = make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]), __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
+                        part(it.slot)[(8 * c + x) * ROWS] = make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]), __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
                 }
             }
             if (!whole) {
-                if (live) w.ml[(size_t)it.slot * UNIT_ROWS + t * ROWS + r] = make_float2(m_run, l_run);
+                if (live) *part_ml(it.slot) = make_float2(m_run, l_run);
                 __threadfence();
                 named_barrier_sync(1 + t, 128);
                 if (r == 0) {
@@ -535,11 +599,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 named_barrier_sync(1 + t, 128);
                 if (sm.last[t] && live) {  // all pieces are written: merge them in their order
-                    const size_t first = ((size_t)(it.slot - it.piece)) * UNIT_ROWS + t * ROWS + r;
+                    const auto slot = [&](uint32_t p) { return p ? it.slot0 - 1 + 2 * p : it.slot0; };
                     float big = NEG_SENTINEL, den = 0.0f;
-                    for (uint32_t p = 0; p < it.pieces; p++) big = fmaxf(big, __ldcg(w.ml + first + (size_t)p * UNIT_ROWS).x);
+                    for (uint32_t p = 0; p < it.pieces; p++) big = fmaxf(big, __ldcg(part_ml(slot(p))).x);
                     for (uint32_t p = 0; p < it.pieces; p++) {
-                        const float2 ml = __ldcg(w.ml + first + (size_t)p * UNIT_ROWS);
+                        const float2 ml = __ldcg(part_ml(slot(p)));
                         den = fmaf(ex2(ml.x - big), ml.y, den);
                     }
                     const float inv = den != 0.0f ? 1.0f / den : 0.0f;
@@ -547,10 +611,10 @@ __global__ void __launch_bounds__(THREADS, 1)
                     for (int c = 0; c < 8; c++) {
                         float4 acc[4] = {};
                         for (uint32_t p = 0; p < it.pieces; p++) {
-                            const float f = ex2(__ldcg(w.ml + first + (size_t)p * UNIT_ROWS).x - big) * inv;
+                            const float f = ex2(__ldcg(part_ml(slot(p))).x - big) * inv;
 #pragma unroll
                             for (int x = 0; x < 4; x++) {
-                                const float4 o = __ldcg(w.acc + (first + (size_t)p * UNIT_ROWS) * (HD / 4) + 4 * c + x);
+                                const float4 o = __ldcg(part(slot(p)) + (4 * c + x) * ROWS);
                                 acc[x].x = fmaf(f, o.x, acc[x].x);
                                 acc[x].y = fmaf(f, o.y, acc[x].y);
                                 acc[x].z = fmaf(f, o.z, acc[x].z);
@@ -565,9 +629,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                     }
                 }
             }
-            key_tile += (uint32_t)it.unit_tiles();
-            rows.add(tiles);
-            if (!leave()) break;
+            key += (uint32_t)unit_tiles;
+            row += (uint32_t)tiles;
+            done_item();  // only now: the queue gives out the next but one behind it
         }
     }
     // A wait that ran out leaves MMAs (and Q's copy) in flight that nobody waits for: they get a bounded time to land.
@@ -578,19 +642,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (warp == 0) tmem_dealloc(tmem, TMEM_COLS);
 }
 
-// Pieces that can be under way: four for every place, and no more than sixteen of every unit there can be.
-uint32_t most_slots(int sm_count, uint32_t n_kv, uint32_t group, uint32_t requests, uint32_t tokens)
-{
-    const uint64_t by_units = ((uint64_t)tokens * group / UNIT_ROWS + requests) * n_kv * 16, by_places = 4ull * sm_count;
-    return (uint32_t)(by_units < by_places ? by_units : by_places);
-}
-
 }  // namespace
 
-size_t blocks_prefill_work(int sm_count, uint32_t n_kv, uint32_t group, uint32_t requests, uint32_t tokens)
-{
-    return (size_t)most_slots(sm_count, n_kv, group, requests, tokens) * UNIT_ROWS * (HD + 2) * 4;
-}
+// Two parts for every stretch: of the unit that it goes on with, and of the one that it begins and does not end.
+size_t blocks_prefill_work(int sm_count) { return 2ull * blocks_places(sm_count) * UNIT_ROWS * (HD + 2) * 4; }
 
 int launch_blocks_prefill(const LaunchArgs& a, const BlocksAttn& k, const BlocksWork& work)
 {
@@ -618,10 +673,9 @@ int launch_blocks_prefill(const LaunchArgs& a, const BlocksAttn& k, const Blocks
             if (a.device >= 0 && a.device < 64) attr_set[a.device] = true;
         }
     }
-    PrefillWork w{work.units_before, work.queue, work.done, nullptr, nullptr, most_slots(a.sm_count, k.n_kv, k.group, k.req.n, k.req.tokens)};
-    w.acc = reinterpret_cast<float4*>(work.parts);
-    w.ml = reinterpret_cast<float2*>(w.acc + (size_t)w.slots * UNIT_ROWS * (HD / 4));
-    const cudaError_t e = launch_dependent(blocks_prefill_kernel, dim3(a.sm_count), dim3(THREADS), smem, a.stream, tm_q, k, w);
+    float4* acc = reinterpret_cast<float4*>(work.parts);
+    float2* ml = reinterpret_cast<float2*>(acc + 2ull * work.places * UNIT_ROWS * (HD / 4));
+    const cudaError_t e = launch_dependent(blocks_prefill_kernel, dim3(work.places), dim3(THREADS), smem, a.stream, tm_q, k, work, acc, ml);
     ++*a.launches;
     return check_cuda(a, e, "attn_blocks prefill");
 }

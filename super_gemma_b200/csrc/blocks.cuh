@@ -19,7 +19,7 @@ constexpr uint32_t TILE_BYTES = TILE_TOK * 128;
 constexpr uint32_t NO_SLOT = 0xffffffffu;
 constexpr int LOWEST_EXP = -15;
 constexpr uint32_t MOST_REQUESTS = 65536;
-constexpr uint32_t MOST_KEYS = 0x7fffff00u;  // of one request: positions are signed words
+constexpr uint32_t MOST_KEYS = 0x3fffff00u;  // of one request: positions are signed words, and 256 requests' tiles of 64 keys fit one
 constexpr uint32_t FEW_ROWS = 8;             // requests of at most so many rows (query tokens x heads of a group) are decoded, the others prefilled
 
 // What a dispatch over the cache knows of its requests.
@@ -73,7 +73,7 @@ struct BlocksAttn {
     const uint8_t* pool[2];
     const int8_t* exps[2];
     __half* out;
-    uint32_t n_kv, group, tiles;  // tiles of a pool: blocks x kv heads
+    uint32_t n_kv, group, group_shift, tiles;  // tiles of a pool: blocks x kv heads
     float scale;
 };
 struct LaunchArgs;
