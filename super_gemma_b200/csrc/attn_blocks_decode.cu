@@ -28,13 +28,20 @@ constexpr uint32_t LEAST_TILES = 4;  // of a stretch: below that more warps only
 constexpr float RESCALE_T = 8.0f;
 constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES;
 
+// What the arithmetic needs of a request, left for it by the side that copies, which comes to it up to STAGES tiles earlier.
+struct Met {
+    uint32_t request, first, n, len, lo, tiles;
+};
+constexpr int MET = 4;  // STAGES tiles under way are of three requests at most
+static_assert(MET > STAGES, "a request is not overwritten before its last tile");
+
 struct __align__(1024) DecodeSmem {
     uint8_t k[WARPS][STAGES][TILE_BYTES];  // 128-byte swizzled by TMA
     uint8_t v[WARPS][STAGES][TILE_BYTES];
     uint64_t full[WARPS][STAGES];
     uint64_t sums[WARPS];
-    uint64_t from[WARPS];  // of each warp's stretch: tiles before it in its first request
-    uint32_t request[WARPS];
+    Met met[WARPS][MET];  // the last requests that a warp's copies have come to
+    uint32_t from[WARPS]; // tiles of a stretch's first request that lie before it
 };
 
 // Parts: (m, l) and O of [slot][kv head][row].  A stretch p has slot 2p for the request that it goes on with and 2p + 1 for
@@ -91,14 +98,18 @@ struct Tiles {
 };
 __device__ __forceinline__ Tiles tiles_of(const BlocksAttn& a, const Request& q)
 {
-    if (q.n == 0 || q.n > FEW_ROWS / a.group || q.len == 0) return Tiles{0, 0};
+    if (q.n == 0 || q.n > (FEW_ROWS >> a.group_shift) || q.len == 0) return Tiles{0, 0};
     const int64_t from = (int64_t)q.len - q.n + 1 - a.req.window;
     const uint32_t lo = a.req.window != 0 && from > 0 ? (uint32_t)from / TILE_TOK : 0;
     return Tiles{lo, (q.len + TILE_TOK - 1) / TILE_TOK - lo};
 }
 // Stretch p of `n` is [begin(p), begin(p + 1)) of `total` tiles.
 __device__ __forceinline__ uint64_t stretch_begin(uint64_t total, uint32_t n, uint32_t p) { return total * p / n; }
-__device__ __forceinline__ uint32_t stretch_of(uint64_t total, uint32_t n, uint64_t tile) { return (uint32_t)(((tile + 1) * n - 1) / total); }
+__device__ __forceinline__ uint32_t stretch_of(uint64_t total, uint32_t n, uint64_t tile)
+{
+    const uint64_t x = (tile + 1) * n - 1;
+    return x >> 32 ? (uint32_t)(x / total) : (uint32_t)x / (uint32_t)total;
+}
 __device__ __forceinline__ uint32_t stretches_for(uint64_t total, uint32_t most)
 {
     const uint64_t n = (total + LEAST_TILES - 1) / LEAST_TILES;
@@ -124,8 +135,14 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
     const uint32_t flat = blockIdx.x * WARPS + warp, head = flat % a.n_kv, part = flat / a.n_kv;
     const uint32_t per_thread = (a.req.n + WARPS * 32 - 1) / (WARPS * 32);
     const uint32_t r_begin = min(threadIdx.x * per_thread, a.req.n), r_end = min(r_begin + per_thread, a.req.n);
+    Request rq{0, 0, 0};
+    Tiles tl{0, 0};
     uint64_t mine = 0;
-    for (uint32_t r = r_begin; r < r_end; r++) mine += tiles_of(a, request_at(a.req, r)).n;
+    for (uint32_t r = r_begin; r < r_end; r++) {
+        rq = request_at(a.req, r);
+        tl = tiles_of(a, rq);
+        mine += tl.n;
+    }
     uint64_t up_to = mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -150,15 +167,18 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
         }
         uint64_t at = base;
         for (uint32_t r = r_begin; r < r_end; r++) {
-            const uint32_t n = per_thread == 1 ? (uint32_t)mine : tiles_of(a, request_at(a.req, r)).n;
+            if (per_thread != 1) {
+                rq = request_at(a.req, r);
+                tl = tiles_of(a, rq);
+            }
 #pragma unroll
             for (int w = 0; w < WARPS; w++)
-                if (want[w] >= at && want[w] < at + n) {
-                    sm.request[w] = r;
-                    sm.from[w] = want[w] - at;
+                if (want[w] >= at && want[w] < at + tl.n) {
+                    sm.met[w][0] = Met{r, rq.first, rq.n, rq.len, tl.lo, tl.n};
+                    sm.from[w] = (uint32_t)(want[w] - at);
                 }
             if (blockIdx.x == 0) work.head.before[r] = at;
-            at += n;
+            at += tl.n;
         }
     } else if (blockIdx.x == 0) {
         for (uint32_t r = r_begin; r < r_end; r++) work.head.before[r] = 0;
@@ -172,24 +192,28 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
     const uint32_t n_iter = (uint32_t)(stretch_begin(total, n_parts, part + 1) - stretch_begin(total, n_parts, part));
 
     // ---- the copies' side: STAGES tiles ahead of the arithmetic -------------------------------------------------------------------
-    uint32_t to_r = sm.request[warp], to_tile, to_left;
-    {
-        const Tiles t = tiles_of(a, request_at(a.req, to_r));
-        to_tile = t.lo + (uint32_t)sm.from[warp];
-        to_left = t.n - (uint32_t)sm.from[warp];
-    }
-    uint32_t to_page = ld_global(page_at(a.req, to_r, to_tile));
+    uint32_t to_r = sm.met[warp][0].request, to_nth = 0, to_tile = sm.met[warp][0].lo + sm.from[warp], to_left = sm.met[warp][0].tiles - sm.from[warp];
+    // The first pages are asked for side by side, by a lane each.
+    const uint32_t tile0 = to_tile, left0 = to_left;
+    const uint32_t first_pages = ld_global_if(lane < STAGES && lane < left0 && lane < n_iter, page_at(a.req, to_r, to_tile + lane));
     auto next_tile = [&]() {
         to_tile++;
         if (--to_left == 0) {
             Tiles t{0, 0};
-            while (t.n == 0 && ++to_r < a.req.n) t = tiles_of(a, request_at(a.req, to_r));
+            Request q{0, 0, 0};
+            while (t.n == 0 && ++to_r < a.req.n) {
+                q = request_at(a.req, to_r);
+                t = tiles_of(a, q);
+            }
             to_tile = t.lo;
             to_left = t.n;
+            to_nth++;
+            if (lane == 0) sm.met[warp][to_nth % MET] = Met{to_r, q.first, q.n, q.len, t.lo, t.n};
         }
-        if (to_r < a.req.n) to_page = ld_global(page_at(a.req, to_r, to_tile));
     };
-    // What is under way: request, tile, and (lanes 0 and 1) the exponents of K and V.
+    uint32_t to_page = 0;
+    auto look = [&]() { to_page = ld_global(page_at(a.req, to_r, to_tile)); };
+    // What is under way: which of the warp's requests, tile, and (lanes 0 and 1) the exponents of K and V.
     uint32_t way_r[STAGES], way_tile[STAGES];
     int way_exp[STAGES];
     const CUtensorMap* my_map = lane == 0 ? &tm_k : &tm_v;
@@ -210,35 +234,23 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
                 : "memory");
         }
     };
-#pragma unroll
-    for (int i = 0; i < STAGES; i++) {
-        way_r[i] = way_tile[i] = 0;
-        way_exp[i] = 0;
-        if ((uint32_t)i < n_iter) {
-            way_r[i] = to_r;
-            way_tile[i] = to_tile;
-            issue(i, way_exp[i]);
-            if ((uint32_t)i + 1 < n_iter) next_tile();
-        }
-    }
-
     // ---- the arithmetic's side ------------------------------------------------------------------------------------------------------
     // A lane supplies Q for query row g (B operand) and owns the accumulators of rows 2 t4 and 2 t4 + 1.  Row = token * group + head.
     const uint32_t heads = a.n_kv * a.group;
     uint32_t qb[8][2];
     float o[8][4], m_run[2], l_part[2];
-    uint32_t r_now = ~0u, rows = 0, first_tok = 0, tile_first = 0, tile_begin = 0, tile_end = 0;
+    uint32_t r_now = 0, rows = 0, first_tok = 0, tile_first = 0, tile_begin = 0, tile_end = 0;
     int hi_row[2] = {0, 0}, lo_row[2] = {0, 0}, lo_all = 0, hi_all = 0, lo_any = 0, hi_any = 0;  // keys that a row, all rows, any row sees
-    auto begin_request = [&](uint32_t r, uint32_t tile) {
-        const Request rq = request_at(a.req, r);
-        const Tiles t = tiles_of(a, rq);
-        r_now = r;
+    auto begin_request = [&](uint32_t nth, uint32_t tile) {
+        __syncwarp();  // lane 0 left it there
+        const Met rq = sm.met[warp][nth % MET];
+        r_now = nth;
         rows = rq.n * a.group;
         first_tok = rq.first;
         tile_first = tile;
-        tile_begin = t.lo;
-        tile_end = t.lo + t.n;
-        const __half* qrow = a.q + ((size_t)(rq.first + g / a.group) * heads + head * a.group + g % a.group) * HD + 4 * t4;
+        tile_begin = rq.lo;
+        tile_end = rq.lo + rq.tiles;
+        const __half* qrow = a.q + ((size_t)(rq.first + (g >> a.group_shift)) * heads + head * a.group + (g & (a.group - 1))) * HD + 4 * t4;
 #pragma unroll
         for (int c = 0; c < 8; c++) {
             uint2 w = make_uint2(0u, 0u);
@@ -250,7 +262,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
         const int len = (int)rq.len, pos0 = len - (int)rq.n, window = a.req.window && a.req.window < MOST_KEYS ? (int)a.req.window : (int)MOST_KEYS;
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-            hi_row[e] = min(pos0 + (int)((2 * t4 + e) / a.group), len - 1);
+            hi_row[e] = min(pos0 + (int)((2 * t4 + e) >> a.group_shift), len - 1);
             lo_row[e] = max(hi_row[e] + 1 - window, 0);
             m_run[e] = NEG_SENTINEL;
             l_part[e] = 0.0f;
@@ -269,7 +281,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
             if (row >= rows) continue;
             if (began && ended) {
                 const float f = l_row[e] != 0.0f ? 1.0f / l_row[e] : 0.0f;
-                __half* dst = a.out + ((size_t)(first_tok + row / a.group) * heads + head * a.group + row % a.group) * HD + 2 * g;
+                __half* dst = a.out + ((size_t)(first_tok + (row >> a.group_shift)) * heads + head * a.group + (row & (a.group - 1))) * HD + 2 * g;
 #pragma unroll
                 for (int c = 0; c < 8; c++) *reinterpret_cast<__half2*>(dst + 16 * c) = __floats2half2_rn(o[c][e] * f, o[c][2 + e] * f);
             } else {
@@ -290,12 +302,29 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
     for (int b = 0; b < 4; b++) off[b] = (8 * (lmat & 1) + lrow) * 128 + (((2 * b + (lmat >> 1)) ^ lrow) << 4);
     const float scale2 = a.scale * 1.4426950408889634f;
     bool failed = false;
-    uint32_t tile_now = 0;
+    uint32_t tile_now = tile0;
+    begin_request(0, tile0);  // its queries are on their way while the first pages are
+#pragma unroll
+    for (int i = 0; i < STAGES; i++) {
+        way_r[i] = way_tile[i] = 0;
+        way_exp[i] = 0;
+        if ((uint32_t)i < n_iter) {
+            if (i > 0) next_tile();
+            if ((uint32_t)i < left0) to_page = __shfl_sync(0xffffffffu, first_pages, i); else look();
+            way_r[i] = to_nth;
+            way_tile[i] = to_tile;
+            issue(i, way_exp[i]);
+        }
+    }
+    if (STAGES < n_iter) {
+        next_tile();
+        look();
+    }
 
     for (uint32_t it = 0; it < n_iter; ++it) {
         const uint32_t st = it % STAGES;
         if (way_r[0] != r_now) {
-            if (r_now != ~0u) end_request(tile_now);
+            end_request(tile_now);
             begin_request(way_r[0], way_tile[0]);
         }
         tile_now = way_tile[0];
@@ -382,19 +411,20 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
             way_exp[i] = way_exp[i + 1];
         }
         if (it + STAGES < n_iter) {
-            way_r[STAGES - 1] = to_r;
+            way_r[STAGES - 1] = to_nth;
             way_tile[STAGES - 1] = to_tile;
             issue(st, way_exp[STAGES - 1]);
-            if (it + STAGES + 1 < n_iter) next_tile();  // its page is looked up while a tile is worked on
+            if (it + STAGES + 1 < n_iter) {  // its page is looked up while a tile is worked on
+                next_tile();
+                look();
+            }
         }
     }
     if (failed) let_copies_land();
-    if (r_now != ~0u) end_request(tile_now);
+    end_request(tile_now);
 }
 
-// One CTA per request and kv head: nothing to do where one warp had all its tiles; zeros where it had none; else the warps' parts in
-// the order of the list, a warp per row and every SUB-th part.
-constexpr int MERGE_WARPS = 8;
+constexpr int MERGE_WARPS = 4;
 // What the prefill kernel takes its items from; by one CTA of the merge.  Units go out with the most keys first, so that what is left at
 // the end is short (24 requests, three of them prompts of 841 to 1281 tokens: 110 us in the requests' order).  All heads of a unit
 // follow each other while the keys and values of all prompts stay in about three quarters of the 126 MB L2; else a head's units do.
@@ -476,23 +506,28 @@ __device__ __forceinline__ void list_units(const BlocksAttn& a, const BlocksWork
         __syncthreads();
     }
     const uint32_t items = total * a.n_kv, whole = whole_items(items, w.places);
-    uint32_t tiles = 0;
-    if (whole + tid < items) {  // fewer than places, which are at most the CTA's threads
-        uint32_t head, rank;
-        split_item(whole + tid, total, a.n_kv, by_head, head, rank);
-        tiles = (uint32_t)max(1, locate(sorted ? ld_global(w.order + rank) : total - 1 - rank).n_tiles);  // one without a key counts for its rows
+    uint32_t all_tiles = 0;
+    for (uint32_t base = 0; base < w.places; base += N) {  // fewer than places are left
+        uint32_t tiles = 0, more;
+        if (whole + base + tid < items) {
+            uint32_t head, rank;
+            split_item(whole + base + tid, total, a.n_kv, by_head, head, rank);
+            tiles = (uint32_t)max(1, locate(sorted ? ld_global(w.order + rank) : total - 1 - rank).n_tiles);  // one without a key counts for its rows
+        }
+        const uint32_t before = all_tiles + scan(tiles, more);
+        if (base + tid < w.places) w.rest[base + tid] = before;
+        all_tiles += more;
     }
-    static_assert(MOST_PLACES <= N, "a thread per unit that is cut");
-    uint32_t all_tiles;
-    const uint32_t before = scan(tiles, all_tiles);
-    if (tid < w.places) w.rest[tid] = before;
     if (tid == 0) w.rest[w.places] = all_tiles;
 }
 
+// One CTA per request and kv head: nothing to do where one warp had all its tiles; zeros where it had none; else the warps' parts,
+// every fourth of all rows a warp, each in the order of the list.  The first parts are asked for together with the maxima.
+template <int ROWS>
 __global__ void __launch_bounds__(MERGE_WARPS * 32) blocks_merge_kernel(const __grid_constant__ BlocksAttn a, const __grid_constant__ Work work)
 {
     __shared__ union {
-        float4 left[MERGE_WARPS][32];
+        float4 left[MERGE_WARPS - 1][ROWS][32];
         uint32_t sort[MOST_SORTED];
     } sm;
     pdl_wait();
@@ -511,58 +546,81 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) blocks_merge_kernel(const __
         n = stretch_of(total, n_parts, end - 1) - p0 + 1;
         if (n == 1) return;
     }
-    if (last <= first || last > a.req.tokens || last - first > FEW_ROWS / a.group || last - first > a.req.max_q) return;
-    const uint32_t rows = (last - first) * a.group, per_row = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;  // rows, up to a power of two
-    const uint32_t row = warp % per_row, sub = warp / per_row, subs = MERGE_WARPS / per_row;
-    __half* out = a.out + ((size_t)(first + row / a.group) * (a.n_kv * a.group) + head * a.group + row % a.group) * HD + 4 * lane;
+    if (last <= first || last > a.req.tokens || last - first > (FEW_ROWS >> a.group_shift) || last - first > a.req.max_q) return;
+    const uint32_t rows = (last - first) * a.group;
+    const auto out = [&](uint32_t row) {
+        return reinterpret_cast<uint2*>(a.out + ((size_t)(first + (row >> a.group_shift)) * (a.n_kv * a.group) + head * a.group + (row & (a.group - 1))) * HD + 4 * lane);
+    };
     if (n == 0) {
-        if (row < rows && sub == 0) *reinterpret_cast<uint2*>(out) = make_uint2(0u, 0u);
+        for (uint32_t row = warp; row < rows; row += MERGE_WARPS) *out(row) = make_uint2(0u, 0u);
         return;
     }
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float den = 0.0f;
-    if (row < rows) {
-        const auto slot = [&](uint32_t j) { return ((size_t)(2 * (p0 + j) + (j == 0 ? 1 : 0)) * a.n_kv + head) * work.rows + row; };
-        float big = NEG_SENTINEL;
-        for (uint32_t j = lane; j < n; j += 32) big = fmaxf(big, ld_global(work.ml + slot(j)).x);
+    const auto slot = [&](uint32_t j) { return ((size_t)(2 * (p0 + j) + (j == 0 ? 1 : 0)) * a.n_kv + head) * work.rows; };
+    float4 v[ROWS], acc[ROWS];
+    float big[ROWS], den[ROWS];
+    const auto fetch = [&](uint32_t j) {
+        const size_t s = slot(min(j, n - 1));
 #pragma unroll
-        for (int off = 16; off; off >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
-        for (uint32_t j0 = 0; j0 < n; j0 += 32) {
-            const float2 ml = ld_global(work.ml + slot(min(j0 + lane, n - 1)));
-            const float w = j0 + lane < n ? ex2(ml.x - big) : 0.0f;
-            den = fmaf(w, ml.y, den);
-            for (uint32_t u0 = sub; u0 < 32 && j0 + u0 < n; u0 += 8 * subs) {
-                float4 v[8];
+        for (int i = 0; i < ROWS; i++) v[i] = ld_global(work.acc + (s + min((uint32_t)i, rows - 1)) * (HD / 4) + lane);
+    };
+    fetch(warp);
+    // (m, l) of part lane, lane + 32, ... of every row: the first 32 stay, more are read again
+    float2 ml[ROWS];
 #pragma unroll
-                for (int i = 0; i < 8; i++) v[i] = ld_global(work.acc + slot(min(j0 + u0 + i * subs, n - 1)) * (HD / 4) + lane);
+    for (int i = 0; i < ROWS; i++) ml[i] = ld_global(work.ml + slot(min(lane, n - 1)) + min((uint32_t)i, rows - 1));
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const uint32_t u = u0 + i * subs;
-                    const float f = __shfl_sync(0xffffffffu, w, u & 31);
-                    if (u < 32 && j0 + u < n) {
-                        acc.x = fmaf(f, v[i].x, acc.x);
-                        acc.y = fmaf(f, v[i].y, acc.y);
-                        acc.z = fmaf(f, v[i].z, acc.z);
-                        acc.w = fmaf(f, v[i].w, acc.w);
-                    }
-                }
+    for (int i = 0; i < ROWS; i++) {
+        big[i] = ml[i].x;
+        for (uint32_t j = lane + 32; j < n; j += 32) big[i] = fmaxf(big[i], ld_global(work.ml + slot(j) + min((uint32_t)i, rows - 1)).x);
+#pragma unroll
+        for (int off = 16; off; off >>= 1) big[i] = fmaxf(big[i], __shfl_xor_sync(0xffffffffu, big[i], off));
+        den[i] = 0.0f;
+        acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    for (uint32_t j0 = 0; j0 < n; j0 += 32) {
+        float w[ROWS];
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) {
+            if (j0) ml[i] = ld_global(work.ml + slot(min(j0 + lane, n - 1)) + min((uint32_t)i, rows - 1));
+            w[i] = j0 + lane < n ? ex2(ml[i].x - big[i]) : 0.0f;
+            den[i] = fmaf(w[i], ml[i].y, den[i]);
+        }
+        for (uint32_t u = warp; u < 32 && j0 + u < n; u += MERGE_WARPS) {
+            float4 now[ROWS];
+#pragma unroll
+            for (int i = 0; i < ROWS; i++) now[i] = v[i];
+            if (j0 + u + MERGE_WARPS < n) fetch(j0 + u + MERGE_WARPS);
+#pragma unroll
+            for (int i = 0; i < ROWS; i++) {
+                const float f = __shfl_sync(0xffffffffu, w[i], u);
+                acc[i].x = fmaf(f, now[i].x, acc[i].x);
+                acc[i].y = fmaf(f, now[i].y, acc[i].y);
+                acc[i].z = fmaf(f, now[i].z, acc[i].z);
+                acc[i].w = fmaf(f, now[i].w, acc[i].w);
             }
         }
-#pragma unroll
-        for (int off = 16; off; off >>= 1) den += __shfl_xor_sync(0xffffffffu, den, off);
     }
-    sm.left[warp][lane] = acc;
+    const uint32_t used = min(n, (uint32_t)MERGE_WARPS);  // warps that had a part
+    if (warp != 0) {
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) sm.left[warp - 1][i][lane] = acc[i];
+    }
     __syncthreads();
-    if (row < rows && sub == 0) {
-        for (uint32_t s = 1; s < subs; s++) {
-            const float4 o = sm.left[row + s * per_row][lane];
-            acc.x += o.x;
-            acc.y += o.y;
-            acc.z += o.z;
-            acc.w += o.w;
+    if (warp != 0) return;
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+        if ((uint32_t)i >= rows) break;
+        for (uint32_t s = 1; s < used; s++) {
+            const float4 o = sm.left[s - 1][i][lane];
+            acc[i].x += o.x;
+            acc[i].y += o.y;
+            acc[i].z += o.z;
+            acc[i].w += o.w;
         }
-        const float f = den != 0.0f ? 1.0f / den : 0.0f;
-        *reinterpret_cast<uint2*>(out) = make_uint2(pack_half2(acc.x * f, acc.y * f), pack_half2(acc.z * f, acc.w * f));
+#pragma unroll
+        for (int off = 16; off; off >>= 1) den[i] += __shfl_xor_sync(0xffffffffu, den[i], off);
+        const float f = den[i] != 0.0f ? 1.0f / den[i] : 0.0f;
+        *out(i) = make_uint2(pack_half2(acc[i].x * f, acc[i].y * f), pack_half2(acc[i].z * f, acc[i].w * f));
     }
 }
 
@@ -606,7 +664,8 @@ int launch_blocks_decode(const LaunchArgs& a, const BlocksAttn& k, const BlocksW
     cudaError_t e = launch_dependent(blocks_decode_kernel, dim3(grid_ctas(a.sm_count, k.n_kv)), dim3(WARPS * 32), smem, a.stream, tm[0], tm[1], k, w, most);
     ++*a.launches;
     if (int r = check_cuda(a, e, "attn_blocks decode")) return r;
-    e = launch_dependent(blocks_merge_kernel, dim3(k.req.n + (k.req.max_q > FEW_ROWS / k.group ? 1 : 0), k.n_kv), dim3(MERGE_WARPS * 32), 0, a.stream, k, w);
+    const auto merge = w.rows <= 1 ? blocks_merge_kernel<1> : w.rows <= 2 ? blocks_merge_kernel<2> : w.rows <= 4 ? blocks_merge_kernel<4> : blocks_merge_kernel<8>;
+    e = launch_dependent(merge, dim3(k.req.n + (k.req.max_q > FEW_ROWS / k.group ? 1 : 0), k.n_kv), dim3(MERGE_WARPS * 32), 0, a.stream, k, w);
     ++*a.launches;
     return check_cuda(a, e, "attn_blocks merge");
 }
