@@ -13,6 +13,7 @@
 // and out of the sum again, l += P' 2^-e_v.  Softmax in base 2 with a running maximum that is raised when it grows by more than 2^8.
 // Bound by the cache's bytes: 2 x 128 1/16 per token and kv head.
 #include <mutex>
+#include <type_traits>
 
 #include "blocks.cuh"
 #include "blocks_work.cuh"
@@ -424,10 +425,13 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
     end_request(tile_now);
 }
 
-constexpr int MERGE_WARPS = 4;
+constexpr int MANY_CTAS_WARPS = 4;                                          // of the merge
+constexpr int few_ctas_warps(int rows) { return rows == 8 ? 8 : 16; }
+
 // What the prefill kernel takes its items from; by one CTA of the merge.  Units go out with the most keys first, so that what is left at
 // the end is short (24 requests, three of them prompts of 841 to 1281 tokens: 110 us in the requests' order).  All heads of a unit
 // follow each other while the keys and values of all prompts stay in about three quarters of the 126 MB L2; else a head's units do.
+template <int MERGE_WARPS>
 __device__ __forceinline__ void list_units(const BlocksAttn& a, const BlocksWork& w, uint32_t* shared)
 {
     constexpr uint32_t N = MERGE_WARPS * 32;
@@ -521,19 +525,23 @@ __device__ __forceinline__ void list_units(const BlocksAttn& a, const BlocksWork
     if (tid == 0) w.rest[w.places] = all_tiles;
 }
 
-// One CTA per request and kv head: nothing to do where one warp had all its tiles; zeros where it had none; else the warps' parts,
-// every fourth of all rows a warp, each in the order of the list.  The first parts are asked for together with the maxima.
-template <int ROWS>
-__global__ void __launch_bounds__(MERGE_WARPS * 32) blocks_merge_kernel(const __grid_constant__ BlocksAttn a, const __grid_constant__ Work work)
+// One CTA per request and kv head: nothing to do where one warp had all its tiles; zeros where it had none; else the warps' parts.
+// Warp x of W takes parts x, x + W, ... of all rows, lane k the (m, l) of its k-th part, so that those and the first parts come in one
+// round of loads; maxima and sums of the warps meet in shared memory, in the warps' order.
+template <int ROWS, int W>
+__global__ void __launch_bounds__(W * 32, W != MANY_CTAS_WARPS ? 1 : ROWS == 8 ? 4 : 8) blocks_merge_kernel(const __grid_constant__ BlocksAttn a, const __grid_constant__ Work work)
 {
     __shared__ union {
-        float4 left[MERGE_WARPS - 1][ROWS][32];
+        struct {
+            float4 acc[W][ROWS][32];
+            float big[W][ROWS], den[W][ROWS];
+        } of;
         uint32_t sort[MOST_SORTED];
     } sm;
     pdl_wait();
     pdl_launch_dependents();
     if (blockIdx.x == a.req.n) {  // there if a prefill follows
-        if (blockIdx.y == 0) list_units(a, work.head, sm.sort);
+        if (blockIdx.y == 0) list_units<W>(a, work.head, sm.sort);
         return;
     }
     const uint32_t r = blockIdx.x, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -552,75 +560,97 @@ __global__ void __launch_bounds__(MERGE_WARPS * 32) blocks_merge_kernel(const __
         return reinterpret_cast<uint2*>(a.out + ((size_t)(first + (row >> a.group_shift)) * (a.n_kv * a.group) + head * a.group + (row & (a.group - 1))) * HD + 4 * lane);
     };
     if (n == 0) {
-        for (uint32_t row = warp; row < rows; row += MERGE_WARPS) *out(row) = make_uint2(0u, 0u);
+        for (uint32_t row = warp; row < rows; row += W) *out(row) = make_uint2(0u, 0u);
         return;
     }
     const auto slot = [&](uint32_t j) { return ((size_t)(2 * (p0 + j) + (j == 0 ? 1 : 0)) * a.n_kv + head) * work.rows; };
-    float4 v[ROWS], acc[ROWS];
-    float big[ROWS], den[ROWS];
-    const auto fetch = [&](uint32_t j) {
-        const size_t s = slot(min(j, n - 1));
-#pragma unroll
-        for (int i = 0; i < ROWS; i++) v[i] = ld_global(work.acc + (s + min((uint32_t)i, rows - 1)) * (HD / 4) + lane);
-    };
-    fetch(warp);
-    // (m, l) of part lane, lane + 32, ... of every row: the first 32 stay, more are read again
+    constexpr int BATCH = W == MANY_CTAS_WARPS ? (ROWS <= 2 ? 4 / ROWS : 1) : 8 / ROWS;  // parts asked for at a time
+    float4 v[BATCH][ROWS], acc[ROWS];
     float2 ml[ROWS];
+    float big[ROWS], den[ROWS];
+    const auto fetch = [&](uint32_t k) {  // this warp's parts k ..
 #pragma unroll
-    for (int i = 0; i < ROWS; i++) ml[i] = ld_global(work.ml + slot(min(lane, n - 1)) + min((uint32_t)i, rows - 1));
+        for (int x = 0; x < BATCH; x++) {
+            const size_t s = slot(min(warp + (k + x) * W, n - 1));
+#pragma unroll
+            for (int i = 0; i < ROWS; i++) v[x][i] = ld_global(work.acc + (s + min((uint32_t)i, rows - 1)) * (HD / 4) + lane);
+        }
+    };
+    const auto fetch_ml = [&](uint32_t k) {
+        const size_t s = slot(min(warp + (k + lane) * W, n - 1));
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) ml[i] = ld_global(work.ml + s + min((uint32_t)i, rows - 1));
+    };
+    fetch_ml(0);
+    fetch(0);
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
-        big[i] = ml[i].x;
-        for (uint32_t j = lane + 32; j < n; j += 32) big[i] = fmaxf(big[i], ld_global(work.ml + slot(j) + min((uint32_t)i, rows - 1)).x);
-#pragma unroll
-        for (int off = 16; off; off >>= 1) big[i] = fmaxf(big[i], __shfl_xor_sync(0xffffffffu, big[i], off));
+        big[i] = ml[i].x;  // (parts past the end are the last one again)
         den[i] = 0.0f;
         acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    for (uint32_t j0 = 0; j0 < n; j0 += 32) {
+    for (uint32_t k = 32; warp + k * W < n; k += 32) {
+        fetch_ml(k);
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) big[i] = fmaxf(big[i], ml[i].x);
+    }
+    if (32 * W < n) fetch_ml(0);
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+#pragma unroll
+        for (int off = 16; off; off >>= 1) big[i] = fmaxf(big[i], __shfl_xor_sync(0xffffffffu, big[i], off));
+        if (lane == 0) sm.of.big[warp][i] = big[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ROWS; i++)
+#pragma unroll
+        for (int x = 0; x < W; x++) big[i] = fmaxf(big[i], sm.of.big[x][i]);
+    for (uint32_t k0 = 0; warp + k0 * W < n; k0 += 32) {
+        if (k0) fetch_ml(k0), fetch(k0);
         float w[ROWS];
 #pragma unroll
         for (int i = 0; i < ROWS; i++) {
-            if (j0) ml[i] = ld_global(work.ml + slot(min(j0 + lane, n - 1)) + min((uint32_t)i, rows - 1));
-            w[i] = j0 + lane < n ? ex2(ml[i].x - big[i]) : 0.0f;
+            w[i] = warp + (k0 + lane) * W < n ? ex2(ml[i].x - big[i]) : 0.0f;
             den[i] = fmaf(w[i], ml[i].y, den[i]);
         }
-        for (uint32_t u = warp; u < 32 && j0 + u < n; u += MERGE_WARPS) {
-            float4 now[ROWS];
+        for (uint32_t k = 0;; k += BATCH) {
 #pragma unroll
-            for (int i = 0; i < ROWS; i++) now[i] = v[i];
-            if (j0 + u + MERGE_WARPS < n) fetch(j0 + u + MERGE_WARPS);
+            for (int x = 0; x < BATCH; x++)
 #pragma unroll
-            for (int i = 0; i < ROWS; i++) {
-                const float f = __shfl_sync(0xffffffffu, w[i], u);
-                acc[i].x = fmaf(f, now[i].x, acc[i].x);
-                acc[i].y = fmaf(f, now[i].y, acc[i].y);
-                acc[i].z = fmaf(f, now[i].z, acc[i].z);
-                acc[i].w = fmaf(f, now[i].w, acc[i].w);
-            }
+                for (int i = 0; i < ROWS; i++) {
+                    const float f = __shfl_sync(0xffffffffu, w[i], k + x);  // 0 past the end
+                    acc[i].x = fmaf(f, v[x][i].x, acc[i].x);
+                    acc[i].y = fmaf(f, v[x][i].y, acc[i].y);
+                    acc[i].z = fmaf(f, v[x][i].z, acc[i].z);
+                    acc[i].w = fmaf(f, v[x][i].w, acc[i].w);
+                }
+            if (k + BATCH >= 32 || warp + (k0 + k + BATCH) * W >= n) break;
+            fetch(k0 + k + BATCH);
         }
     }
-    const uint32_t used = min(n, (uint32_t)MERGE_WARPS);  // warps that had a part
-    if (warp != 0) {
-#pragma unroll
-        for (int i = 0; i < ROWS; i++) sm.left[warp - 1][i][lane] = acc[i];
-    }
-    __syncthreads();
-    if (warp != 0) return;
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
-        if ((uint32_t)i >= rows) break;
-        for (uint32_t s = 1; s < used; s++) {
-            const float4 o = sm.left[s - 1][i][lane];
-            acc[i].x += o.x;
-            acc[i].y += o.y;
-            acc[i].z += o.z;
-            acc[i].w += o.w;
-        }
 #pragma unroll
         for (int off = 16; off; off >>= 1) den[i] += __shfl_xor_sync(0xffffffffu, den[i], off);
-        const float f = den[i] != 0.0f ? 1.0f / den[i] : 0.0f;
-        *out(i) = make_uint2(pack_half2(acc[i].x * f, acc[i].y * f), pack_half2(acc[i].z * f, acc[i].w * f));
+        sm.of.acc[warp][i][lane] = acc[i];
+        if (lane == 0) sm.of.den[warp][i] = den[i];
+    }
+    __syncthreads();
+    for (uint32_t row = warp; row < rows; row += W) {
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float l = 0.0f;
+#pragma unroll
+        for (int x = 0; x < W; x++) {
+            const float4 o = sm.of.acc[x][row][lane];
+            sum.x += o.x;
+            sum.y += o.y;
+            sum.z += o.z;
+            sum.w += o.w;
+            l += sm.of.den[x][row];
+        }
+        const float f = l != 0.0f ? 1.0f / l : 0.0f;
+        *out(row) = make_uint2(pack_half2(sum.x * f, sum.y * f), pack_half2(sum.z * f, sum.w * f));
     }
 }
 
@@ -664,8 +694,16 @@ int launch_blocks_decode(const LaunchArgs& a, const BlocksAttn& k, const BlocksW
     cudaError_t e = launch_dependent(blocks_decode_kernel, dim3(grid_ctas(a.sm_count, k.n_kv)), dim3(WARPS * 32), smem, a.stream, tm[0], tm[1], k, w, most);
     ++*a.launches;
     if (int r = check_cuda(a, e, "attn_blocks decode")) return r;
-    const auto merge = w.rows <= 1 ? blocks_merge_kernel<1> : w.rows <= 2 ? blocks_merge_kernel<2> : w.rows <= 4 ? blocks_merge_kernel<4> : blocks_merge_kernel<8>;
-    e = launch_dependent(merge, dim3(k.req.n + (k.req.max_q > FEW_ROWS / k.group ? 1 : 0), k.n_kv), dim3(MERGE_WARPS * 32), 0, a.stream, k, w);
+    // Few CTAs have many parts each (one request of 131072 keys: 148 of every head; 9.4 us with four warps a CTA).
+    const bool few = (uint64_t)k.req.n * k.n_kv <= 2u * (uint32_t)a.sm_count;
+    const dim3 grid(k.req.n + (k.req.max_q > FEW_ROWS / k.group ? 1 : 0), k.n_kv);
+    const auto merge = [&](auto rows) {
+        constexpr int ROWS = decltype(rows)::value, FEW = few_ctas_warps(ROWS);
+        return few ? launch_dependent(blocks_merge_kernel<ROWS, FEW>, grid, dim3(FEW * 32), 0, a.stream, k, w)
+                   : launch_dependent(blocks_merge_kernel<ROWS, MANY_CTAS_WARPS>, grid, dim3(MANY_CTAS_WARPS * 32), 0, a.stream, k, w);
+    };
+    e = w.rows <= 1 ? merge(std::integral_constant<int, 1>()) : w.rows <= 2 ? merge(std::integral_constant<int, 2>())
+        : w.rows <= 4 ? merge(std::integral_constant<int, 4>()) : merge(std::integral_constant<int, 8>());
     ++*a.launches;
     return check_cuda(a, e, "attn_blocks merge");
 }
