@@ -26,6 +26,9 @@ namespace {
 constexpr int HD = 128;
 constexpr int WARPS = 4, CTAS_PER_SM = 4, STAGES = 3;
 constexpr uint32_t LEAST_TILES = 2;  // of a stretch: fewer would only mean more to merge (one request of 1000 keys: 12.3 us with 4, 10.3 with 2 and with 1)
+// A request weighs a tile more than it has: its queries to fetch, its result to write.  (256 requests of 17 to 2048 keys: a warp whose
+// stretch was of many short ones ended 11 of 52 us after the median one.)
+constexpr uint32_t REQUEST_WEIGHT = 1;
 constexpr float RESCALE_T = 8.0f;
 constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES;
 
@@ -34,6 +37,7 @@ struct Met {
     uint32_t request, first, n, len, lo, tiles;
 };
 constexpr int MET = 4;  // STAGES tiles under way are of three requests at most
+static_assert(REQUEST_WEIGHT == 1, "a stretch that begins within a request's own weight begins with it");
 static_assert(MET > STAGES, "a request is not overwritten before its last tile");
 
 struct __align__(1024) DecodeSmem {
@@ -42,7 +46,8 @@ struct __align__(1024) DecodeSmem {
     uint64_t full[WARPS][STAGES];
     uint64_t sums[WARPS];
     Met met[WARPS][MET];  // the last requests that a warp's copies have come to
-    uint32_t from[WARPS]; // tiles of a stretch's first request that lie before it
+    uint32_t from[WARPS]; // weight of a stretch's first request that lies before it
+    uint32_t begun[WARPS][2];  // requests that begin before a stretch, before its end
 };
 
 // Parts: (m, l) and O of [slot][kv head][row].  A stretch p has slot 2p for the request that it goes on with and 2p + 1 for
@@ -96,6 +101,7 @@ __device__ __forceinline__ float tok_sum(float v)
 // The tiles of a request that any of its queries sees: [lo, lo + n).  None of a request that is prefilled.
 struct Tiles {
     uint32_t lo, n;
+    __device__ uint32_t weight() const { return n ? n + REQUEST_WEIGHT : 0; }
 };
 __device__ __forceinline__ Tiles tiles_of(const BlocksAttn& a, const Request& q)
 {
@@ -149,11 +155,12 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
     const uint32_t r_begin = min(threadIdx.x * per_thread, a.req.n), r_end = min(r_begin + per_thread, a.req.n);
     Request rq{0, 0, 0};
     Tiles tl{0, 0};
+    constexpr int COUNT_BITS = 17;  // of the sums: requests with tiles (at most MOST_REQUESTS) below, weights above
     uint64_t mine = 0;
     for (uint32_t r = r_begin; r < r_end; r++) {
         rq = request_at(a.req, r);
         tl = tiles_of(a, rq);
-        mine += tl.n;
+        mine += (uint64_t)tl.weight() << COUNT_BITS | (tl.n ? 1 : 0);
     }
     uint64_t up_to = mine;
 #pragma unroll
@@ -163,34 +170,43 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
     }
     if (lane == 31) sm.sums[warp] = up_to;
     __syncthreads();
-    uint64_t total = 0, base = up_to - mine;
+    uint64_t all = 0, base = up_to - mine;
 #pragma unroll
     for (int w = 0; w < WARPS; w++) {
         if (w < (int)warp) base += sm.sums[w];
-        total += sm.sums[w];
+        all += sm.sums[w];
     }
+    const uint64_t total = all >> COUNT_BITS;
     const Stretches cut = stretches_for(total, most);
     if (total != 0) {
-        uint64_t want[WARPS];
+        uint64_t want[WARPS][2];  // where the warps' stretches begin and end
 #pragma unroll
         for (int w = 0; w < WARPS; w++) {
             const uint32_t p = (blockIdx.x * WARPS + w) / a.n_kv;
-            want[w] = p < cut.n ? cut.begin(p) : ~0ull;
+            want[w][0] = p < cut.n ? cut.begin(p) : ~0ull;
+            want[w][1] = p < cut.n ? cut.begin(p + 1) : ~0ull;
         }
-        uint64_t at = base;
+        uint64_t at = base >> COUNT_BITS;
+        uint32_t nth = (uint32_t)base & ((1u << COUNT_BITS) - 1);
         for (uint32_t r = r_begin; r < r_end; r++) {
             if (per_thread != 1) {
                 rq = request_at(a.req, r);
                 tl = tiles_of(a, rq);
             }
+            const uint64_t end = at + tl.weight();
 #pragma unroll
-            for (int w = 0; w < WARPS; w++)
-                if (want[w] >= at && want[w] < at + tl.n) {
+            for (int w = 0; w < WARPS; w++) {
+                if (want[w][0] >= at && want[w][0] < end) {
                     sm.met[w][0] = Met{r, rq.first, rq.n, rq.len, tl.lo, tl.n};
-                    sm.from[w] = (uint32_t)(want[w] - at);
+                    sm.from[w] = (uint32_t)(want[w][0] - at);
                 }
+#pragma unroll
+                for (int i = 0; i < 2; i++)
+                    if (want[w][i] >= at && want[w][i] < end) sm.begun[w][i] = nth + (want[w][i] > at ? 1 : 0);
+            }
             if (blockIdx.x == 0) work.head.before[r] = at;
-            at += tl.n;
+            at = end;
+            nth += tl.n ? 1 : 0;
         }
     } else if (blockIdx.x == 0) {
         for (uint32_t r = r_begin; r < r_end; r++) work.head.before[r] = 0;
@@ -201,10 +217,15 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
     }
     __syncthreads();
     if (part >= cut.n) return;
-    const uint32_t n_iter = (uint32_t)(cut.begin(part + 1) - cut.begin(part));
+    // The tiles of the stretch are its weights less those of the requests that begin in it.
+    const uint64_t part_end = cut.begin(part + 1);
+    const uint32_t begun_end = part_end == total ? (uint32_t)all & ((1u << COUNT_BITS) - 1) : sm.begun[warp][1];
+    const uint32_t n_iter = (uint32_t)(part_end - cut.begin(part)) - REQUEST_WEIGHT * (begun_end - sm.begun[warp][0]);
+    if (n_iter == 0) return;
+    const uint32_t passed = sm.from[warp] > REQUEST_WEIGHT ? sm.from[warp] - REQUEST_WEIGHT : 0;  // tiles of the first request that lie before
 
     // ---- the copies' side: STAGES tiles ahead of the arithmetic -------------------------------------------------------------------
-    uint32_t to_r = sm.met[warp][0].request, to_nth = 0, to_tile = sm.met[warp][0].lo + sm.from[warp], to_left = sm.met[warp][0].tiles - sm.from[warp];
+    uint32_t to_r = sm.met[warp][0].request, to_nth = 0, to_tile = sm.met[warp][0].lo + passed, to_left = sm.met[warp][0].tiles - passed;
     // The first pages are asked for side by side, by a lane each.
     const uint32_t tile0 = to_tile, left0 = to_left;
     const uint32_t first_pages = ld_global_if(lane < STAGES && lane < left0 && lane < n_iter, page_at(a.req, to_r, to_tile + lane));
@@ -562,7 +583,7 @@ __global__ void __launch_bounds__(W * 32, W != MANY_CTAS_WARPS ? 1 : ROWS == 8 ?
     uint32_t p0 = 0, n = 0;
     if (end > at) {
         const Stretches cut = stretches_for(total, most);
-        p0 = cut.of(at);
+        p0 = cut.of(at + REQUEST_WEIGHT);
         n = cut.of(end - 1) - p0 + 1;
         if (n == 1) return;
     }

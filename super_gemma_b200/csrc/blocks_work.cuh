@@ -1,5 +1,5 @@
 // The work buffer of attn_blocks_e4m3_d128: what the first of its kernels leaves the others, and partial results.
-//   u64 before[n + 2]        16-token tiles of the decoded requests before each, their total, the most stretches of a kv head
+//   u64 before[n + 2]        weight of the decoded requests before each (its 16-token tiles and one more), their total, the most stretches of a kv head
 //   u32 units_before[n + 1]  units (256 rows) of the prefilled requests before each, their total
 //   u32 order[2048]          the units of a kv head, those with the most keys first (only if there are no more than that)
 //   u32 rest[places + 1]     tiles of 64 keys before each of the units that are cut, their total
