@@ -209,6 +209,30 @@ __device__ __forceinline__ int exponent_for(float a)
 // 2^e as f16 pair, e in [-24, 15].
 __device__ __forceinline__ __half2 power_of_two(int e) { return __float2half2_rn(__int_as_float((e + 127) << 23)); }
 
+// Eight f16 numbers as e4m3(x * f); 16 cached ones as e4m3(q * f).
+__device__ __forceinline__ uint2 quantise(const uint4& x, __half2 f)
+{
+    const __half2 top = __float2half2_rn(61440.0f), low = __float2half2_rn(-61440.0f);
+    const auto pair = [&](uint32_t w) { return f16x2_to_e4m3x2(as_u32(__hmul2(__hmax2_nan(__hmin2_nan(as_half2(w), top), low), f))); };
+    return make_uint2(pair(x.x) | (pair(x.y) << 16), pair(x.z) | (pair(x.w) << 16));
+}
+__device__ __forceinline__ uint4 round_again(uint4 v, __half2 f)
+{
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const uint32_t lo = f16x2_to_e4m3x2(as_u32(__hmul2(as_half2(e4m3x2_to_f16x2(w[k] & 0xffffu)), f)));
+        const uint32_t hi = f16x2_to_e4m3x2(as_u32(__hmul2(as_half2(e4m3x2_to_f16x2(w[k] >> 16)), f)));
+        w[k] = lo | (hi << 16);
+    }
+    return v;
+}
+__device__ __forceinline__ __half2 largest(__half2 m, const uint4& x)  // a NaN loses against a number
+{
+    m = __hmax2(__hmax2(m, __habs2(as_half2(x.x))), __habs2(as_half2(x.y)));
+    return __hmax2(__hmax2(m, __habs2(as_half2(x.z))), __habs2(as_half2(x.w)));
+}
+
 __device__ __forceinline__ void append_run(const AppendArgs& a, int side, uint32_t head, uint32_t t, uint32_t slot, uint32_t run)
 {
     const uint32_t lane = threadIdx.x & 31, half = lane >> 4, c = lane & 15;
@@ -227,12 +251,7 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int side, uint32
     if (at != 0) old = *(volatile const int8_t*)(a.exps[side] + tile);
     __half2 m = __float2half2_rn(0.0f);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        m = __hmax2(m, __habs2(as_half2(x[i].x)));  // a NaN loses against a number
-        m = __hmax2(m, __habs2(as_half2(x[i].y)));
-        m = __hmax2(m, __habs2(as_half2(x[i].z)));
-        m = __hmax2(m, __habs2(as_half2(x[i].w)));
-    }
+    for (int i = 0; i < 8; i++) m = largest(m, x[i]);
 #pragma unroll
     for (int off = 16; off; off >>= 1) m = __hmax2(m, as_half2(__shfl_xor_sync(0xffffffffu, as_u32(m), off)));
     const float most = fminf(fmaxf(__low2float(m), __high2float(m)), 61440.0f);
@@ -243,34 +262,72 @@ __device__ __forceinline__ void append_run(const AppendArgs& a, int side, uint32
         for (int i = 0; i < 4; i++) {
             if (4 * i + lane / 8 < at) {
                 uint4* p = reinterpret_cast<uint4*>(out + i * 512 + lane * 16);
-                uint4 v = ld_global(p);
-                uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const uint32_t lo = f16x2_to_e4m3x2(as_u32(__hmul2(as_half2(e4m3x2_to_f16x2(w[k] & 0xffffu)), f)));
-                    const uint32_t hi = f16x2_to_e4m3x2(as_u32(__hmul2(as_half2(e4m3x2_to_f16x2(w[k] >> 16)), f)));
-                    w[k] = lo | (hi << 16);
-                }
-                *p = v;
+                *p = round_again(ld_global(p), f);
             }
         }
     }
-    const __half2 f = power_of_two(-e), top = __float2half2_rn(61440.0f), low = __float2half2_rn(-61440.0f);
-    auto quantise = [&](uint32_t w) { return f16x2_to_e4m3x2(as_u32(__hmul2(__hmax2_nan(__hmin2_nan(as_half2(w), top), low), f))); };
+    const __half2 f = power_of_two(-e);
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const uint32_t j = 2 * i + half;
         if (j < run)
             *reinterpret_cast<uint2*>(out + (at + j) * 128 + c * 8) =
-                make_uint2(quantise(x[i].x) | (quantise(x[i].y) << 16), quantise(x[i].z) | (quantise(x[i].w) << 16));
+                quantise(x[i], f);
     }
     if (lane == 0) a.exps[side][tile] = (int8_t)e;
 }
 
-// SPAN tokens of the slot map per warp, kv head and side.
+// Runs of one token (a decode step's), up to 2 N of them at a time: half a warp for each, all their loads on their way together.
+template <int N>
+__device__ __forceinline__ void append_singles(const AppendArgs& a, int side, uint32_t head, uint32_t t0, uint32_t my_slot, uint32_t& todo)
+{
+    const uint32_t lane = threadIdx.x & 31, half = lane >> 4, c = lane & 15;
+    uint4 x[N];
+    uint32_t slot[N];
+    int old[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int first = todo ? __ffs(todo) - 1 : 0;
+        const bool has_first = todo != 0;
+        todo &= todo - 1;
+        const int second = todo ? __ffs(todo) - 1 : 0;
+        const bool has_second = todo != 0;
+        todo &= todo - 1;
+        const uint32_t src = half ? second : first;
+        const uint32_t s = __shfl_sync(0xffffffffu, my_slot, src);
+        slot[i] = (half ? has_second : has_first) ? s : NO_SLOT;
+        const bool on = slot[i] != NO_SLOT;
+        x[i] = ld_global_if(on, reinterpret_cast<const uint4*>(a.src[side] + ((size_t)(t0 + src) * a.n_kv + head) * 128 + c * 8));
+        old[i] = ld_global_if(on && slot[i] % TILE_TOK != 0, a.exps[side] + (size_t)(slot[i] / TILE_TOK) * a.n_kv + head);
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        __half2 m = largest(__float2half2_rn(0.0f), x[i]);
+#pragma unroll
+        for (int off = 8; off; off >>= 1) m = __hmax2(m, as_half2(__shfl_xor_sync(0xffffffffu, as_u32(m), off)));
+        if (slot[i] == NO_SLOT) continue;
+        const uint32_t at = slot[i] % TILE_TOK;
+        const size_t tile = (size_t)(slot[i] / TILE_TOK) * a.n_kv + head;
+        uint8_t* out = a.pool[side] + tile * TILE_BYTES;
+        const int least = at ? old[i] : LOWEST_EXP, e = max(exponent_for(fminf(fmaxf(__low2float(m), __high2float(m)), 61440.0f)), least);
+        if (at != 0 && e > least) {
+            const __half2 f = power_of_two(max(least - e, -24));
+            for (uint32_t j = c / 8; j < at; j += 2) {
+                uint4* p = reinterpret_cast<uint4*>(out + j * 128 + (c & 7) * 16);
+                *p = round_again(ld_global(p), f);
+            }
+        }
+        *reinterpret_cast<uint2*>(out + at * 128 + c * 8) = quantise(x[i], power_of_two(-e));
+        if (c == 0) a.exps[side][tile] = (int8_t)e;
+    }
+}
+
+// SPAN tokens of the slot map per warp, kv head and side.  A lane looks at one slot, of the SPAN tokens and of those that a run which one of
+// them leads can go on with, so that the runs are known after one load.
 template <int SPAN>
 __global__ void __launch_bounds__(APPEND_THREADS) append_blocks_kernel(const __grid_constant__ AppendArgs a)
 {
+    static_assert(SPAN + TILE_TOK - 1 <= 32, "a lane a slot");
     pdl_wait();
     pdl_launch_dependents();
     const uint32_t lane = threadIdx.x & 31;
@@ -279,28 +336,30 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_blocks_kernel(const __g
     const uint32_t head = (uint32_t)((unit >> 1) % a.n_kv);
     const uint64_t t0 = (unit >> 1) / a.n_kv * SPAN;
     if (t0 >= a.n) return;
-    uint32_t mine = NO_SLOT, before = NO_SLOT;
-    if (lane < SPAN && t0 + lane < a.n) {
-        mine = ld_global(a.slots + t0 + lane);
-        if (t0 + lane > 0) before = ld_global(a.slots + t0 + lane - 1);
-    }
+    uint32_t slot = NO_SLOT, first_before = NO_SLOT;
+    if (t0 + lane < a.n) slot = ld_global(a.slots + t0 + lane);
+    if (lane == 0 && t0 > 0) first_before = ld_global(a.slots + t0 - 1);
+    uint32_t before = __shfl_up_sync(0xffffffffu, slot, 1);
+    if (lane == 0) before = first_before;
+    const bool follows = slot != NO_SLOT && before != NO_SLOT && before + 1 == slot && slot % TILE_TOK != 0;
     bool leads = false;
-    if (mine != NO_SLOT) {
-        if (mine / TILE_TOK >= a.blocks) {
-            report_error(a.status, DEV_ERR_BOUNDS, 621, mine, a.blocks);
-        } else if (before != NO_SLOT && before / TILE_TOK == mine / TILE_TOK && before + 1 != mine) {
-            report_error(a.status, DEV_ERR_BOUNDS, 622, before, mine);  // a tile's tokens stand in its order
+    if (lane < SPAN && slot != NO_SLOT) {
+        if (slot / TILE_TOK >= a.blocks) {
+            report_error(a.status, DEV_ERR_BOUNDS, 621, slot, a.blocks);
+        } else if (before != NO_SLOT && before / TILE_TOK == slot / TILE_TOK && before + 1 != slot) {
+            report_error(a.status, DEV_ERR_BOUNDS, 622, before, slot);  // a tile's tokens stand in its order
         } else {
-            leads = !(before != NO_SLOT && before + 1 == mine && mine % TILE_TOK != 0);
+            leads = !follows;
         }
     }
-    for (uint32_t todo = __ballot_sync(0xffffffffu, leads); todo; todo &= todo - 1) {
+    const uint32_t chain = __ballot_sync(0xffffffffu, follows), leaders = __ballot_sync(0xffffffffu, leads);
+    uint32_t singles = leaders & ~(chain >> 1);
+    const uint32_t longer = leaders & ~singles;
+    while (singles) append_singles<SPAN >= 8 ? 4 : SPAN / 2>(a, side, head, (uint32_t)t0, slot, singles);
+    for (uint32_t todo = longer; todo; todo &= todo - 1) {
         const int src = __ffs(todo) - 1;
-        const uint32_t slot = __shfl_sync(0xffffffffu, mine, src), t = (uint32_t)t0 + src;
-        bool follows = false;
-        if (lane < TILE_TOK - slot % TILE_TOK && (uint64_t)t + lane < a.n) follows = ld_global(a.slots + t + lane) == slot + lane;
-        const uint32_t run = __ffs(~__ballot_sync(0xffffffffu, follows)) - 1;
-        append_run(a, side, head, t, slot, run);
+        const uint32_t more = src == 31 ? 0 : chain >> (src + 1);
+        append_run(a, side, head, (uint32_t)t0 + src, __shfl_sync(0xffffffffu, slot, src), (uint32_t)__ffs(~more));
     }
 }
 
@@ -356,9 +415,13 @@ int launch_kv_append_blocks(const LaunchArgs& a)
     if (int r = need_aligned(a, {16, 16, 4, 16, 1, 16, 1})) return r;
     AppendArgs k{{(const __half*)a.b[0].ptr, (const __half*)a.b[1].ptr}, (const uint32_t*)a.b[2].ptr, {(uint8_t*)a.b[3].ptr, (uint8_t*)a.b[5].ptr},
                  {(int8_t*)a.b[4].ptr, (int8_t*)a.b[6].ptr}, n, n_kv, (uint32_t)blocks, a.status};
-    const uint64_t units = 2ull * n_kv * n;
-    const unsigned ctas = (unsigned)((units + APPEND_THREADS / 32 - 1) / (APPEND_THREADS / 32));
-    const cudaError_t e = launch_dependent(append_blocks_kernel<1>, dim3(ctas), dim3(APPEND_THREADS), 0, a.stream, k);
+    // Four tokens a warp while all warps are on the GPU at once, else sixteen (us, 16 kv heads, with 4 | with 16: 64 requests of one token 4.2 |
+    // 6.2, 300 4.2 | 6.2, 1100 6.7 | 6.4, 4000 20.6 | 18.6; 17 prompts, 20300 tokens, 60.0 | 45.9; with one token a warp the last took 181).
+    const uint64_t per_token = 2ull * n_kv;
+    const bool few = per_token * ((n + 3ull) / 4) <= 64ull * a.sm_count;
+    const uint64_t warps = per_token * (few ? (n + 3ull) / 4 : (n + 15ull) / 16);
+    const unsigned ctas = (unsigned)((warps + APPEND_THREADS / 32 - 1) / (APPEND_THREADS / 32));
+    const cudaError_t e = launch_dependent(few ? append_blocks_kernel<4> : append_blocks_kernel<16>, dim3(ctas), dim3(APPEND_THREADS), 0, a.stream, k);
     ++*a.launches;
     return check_cuda(a, e, "kv_append_blocks_e4m3_d128");
 }

@@ -187,6 +187,24 @@ def test_append_token_by_token_and_large(ctx):
     assert all(np.array_equal(g, w) for g, w in zip(got, pools))
 
 
+@pytest.mark.parametrize("requests,kv", [(5, 3), (64, 16), (700, 2), (2500, 5)])
+def test_append_of_decode_steps(ctx, requests, kv):
+    """One token of each of few and many requests, some with a draft of a few, at every place of a tile, over tiles that have to grow and some that have not."""
+    rng = np.random.default_rng(requests)
+    run = np.where(rng.random(requests) < 0.1, rng.integers(2, 6, requests), 1)
+    first = rng.integers(0, TILE, requests)
+    block = rng.permutation(2 * requests)  # two blocks for each: a draft may go on in the second
+    slots = np.concatenate([[block[2 * r + (first[r] + i) // TILE] * TILE + (first[r] + i) % TILE for i in range(run[r])] for r in range(requests)])
+    if requests == 700:
+        slots[np.isin(np.repeat(np.arange(requests), run), np.arange(0, requests, 9))] = NONE  # requests that were refused
+    k, v = _hard_values(rng, (len(slots), kv, D)), _hard_values(rng, (len(slots), kv, D))
+    pools = [*_pool(1, 2 * requests, kv), *_pool(2, 2 * requests, kv)]
+    got = _run_append(ctx, k, v, slots, pools, kv)
+    ref.append(k, slots, *pools[:2])
+    ref.append(v, slots, *pools[2:])
+    assert all(np.array_equal(g, w) for g, w in zip(got, pools))
+
+
 def test_append_keeps_nan_and_cuts_infinity(ctx):
     k = np.ones((2, 1, D), np.float16)
     k[0, 0, :4] = [np.nan, np.inf, -np.inf, 65504]
