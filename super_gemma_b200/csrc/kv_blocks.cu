@@ -15,9 +15,12 @@ namespace {
 // end, in the same order, by every request whose wants the list still covers when all before it are counted.  The others are
 // refused: they keep what they hold, their length is 0 and their tokens have no slot.
 //
-// Prefix sums over the requests and little else: bound by its own latency.  One CTA does the sums (1024 requests at a time); a
-// page's number is moved by one lane, a request's pages by one warp.
-constexpr int PLAN_THREADS = 1024, PLAN_WARPS = PLAN_THREADS / 32;
+// Prefix sums over the requests and little else: bound by its own latency.  One CTA does the sums, of up to 1024 requests at a time; a
+// request's pages are moved by one warp, and the tokens are placed by the same CTA while there are few of them.
+constexpr uint32_t PLAN_THREADS = 1024, PLAN_WARPS = PLAN_THREADS / 32;
+constexpr uint32_t PLACE_THREADS = 256;
+constexpr uint32_t SEARCHED = 1024;      // requests whose first tokens a CTA keeps at hand
+constexpr uint32_t PLACED_HERE = 4096;   // tokens that the first CTA places itself (64 requests of one token: 8.2 us with a second kernel)
 
 struct PlanArgs {
     const uint32_t *ctx, *add, *held, *count;
@@ -26,42 +29,55 @@ struct PlanArgs {
     uint32_t* status;
 };
 
-// Exclusive prefix sum over the CTA; `total` is everybody's.
-__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t* warp_sums, uint64_t& total)
+// Exclusive prefix sums of N values over the CTA; `total` is everybody's.
+template <int N>
+__device__ __forceinline__ void block_scan(uint64_t (&v)[N], uint64_t (*warp_sums)[N], uint64_t (&total)[N])
 {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint64_t x = v;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x / 32;
+    uint64_t x[N];
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const uint64_t t = __shfl_up_sync(0xffffffffu, x, off);
-        if (lane >= off) x += t;
+    for (int i = 0; i < N; i++) {
+        x[i] = v[i];
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const uint64_t t = __shfl_up_sync(0xffffffffu, x[i], off);
+            if (lane >= (uint32_t)off) x[i] += t;
+        }
     }
     __syncthreads();  // the last use of warp_sums is over
-    if (lane == 31) warp_sums[warp] = x;
-    __syncthreads();
-    uint64_t s = warp_sums[lane];
-    const uint64_t mine = s;
+    if (lane == 31) {
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        const uint64_t t = __shfl_up_sync(0xffffffffu, s, off);
-        if (lane >= off) s += t;
+        for (int i = 0; i < N; i++) warp_sums[warp][i] = x[i];
     }
-    total = __shfl_sync(0xffffffffu, s, 31);
-    return __shfl_sync(0xffffffffu, s - mine, warp) + x - v;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const uint64_t mine = lane < warps ? warp_sums[lane][i] : 0;
+        uint64_t s = mine;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+            const uint64_t t = __shfl_up_sync(0xffffffffu, s, off);
+            if (lane >= (uint32_t)off) s += t;
+        }
+        total[i] = __shfl_sync(0xffffffffu, s, 31);
+        v[i] = __shfl_sync(0xffffffffu, s - mine, warp) + x[i] - v[i];
+    }
 }
 
-// Slot and position of token t of the step.
-__device__ __forceinline__ void place_token(const PlanArgs& a, uint32_t t)
+// Slot and position of token t of the step; `starts` is the requests' first tokens, at hand or in memory.
+template <typename First>
+__device__ __forceinline__ void place_token(const PlanArgs& a, uint32_t t, const First& starts)
 {
-    uint32_t lo = 0, hi = a.n;  // the request whose tokens t is among: the last one with starts[r] <= t
+    uint32_t lo = 0, hi = a.n;  // the request whose tokens t is among: the last one with starts <= t
     while (hi - lo > 1) {
         const uint32_t mid = (lo + hi) >> 1;
-        if (ld_global(a.starts + mid) <= t) lo = mid; else hi = mid;
+        if (starts(mid) <= t) lo = mid; else hi = mid;
     }
     uint32_t slot = NO_SLOT, pos = 0;
-    if (t < ld_global(a.starts + a.n)) {
-        pos = ld_global(a.ctx + lo) + (t - ld_global(a.starts + lo));
-        if (ld_global(a.lens + lo) != 0) {
+    if (t < starts(a.n)) {
+        const uint32_t ctx = ld_global(a.ctx + lo), len = ld_global(a.lens + lo);
+        pos = ctx + (t - starts(lo));
+        if (len != 0) {
             const uint64_t row = ((uint64_t)ld_global(a.table + (size_t)lo * a.stride + (pos >> a.page_shift)) << a.page_shift) +
                                  (pos & ((1u << a.page_shift) - 1));
             if (row < NO_SLOT) slot = (uint32_t)row;
@@ -71,115 +87,161 @@ __device__ __forceinline__ void place_token(const PlanArgs& a, uint32_t t)
     a.at[t] = pos;
 }
 
-__global__ void __launch_bounds__(PLAN_THREADS) block_tables_kernel(const __grid_constant__ PlanArgs a)
+// n words by a warp, four of each lane on their way at a time.
+template <typename From, typename To>
+__device__ __forceinline__ void move_words(uint32_t n, const From& from, const To& to)
 {
-    __shared__ uint64_t sums[PLAN_WARPS];
-    const int lane = threadIdx.x & 31;
+    for (uint32_t j0 = threadIdx.x & 31; j0 < n; j0 += 128) {
+        uint32_t w[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) w[k] = ld_global_if(j0 + 32 * k < n, from(j0 + 32 * k));
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++)
+            if (j0 + 32 * k < n) to(j0 + 32 * k, w[k]);
+    }
+}
+
+__global__ void __launch_bounds__(PLAN_THREADS) block_tables_kernel(const __grid_constant__ PlanArgs a, bool place_here)
+{
+    __shared__ uint64_t sums[PLAN_WARPS][2];
+    __shared__ uint32_t firsts[SEARCHED + 1];
+    __shared__ unsigned long long counted[3];  // pages taken, requests refused, tokens placed
+    const uint32_t threads = blockDim.x;
+    if (threadIdx.x < 3) counted[threadIdx.x] = 0;
     pdl_wait();
     pdl_launch_dependents();
     uint32_t count = ld_global(a.count);
-    if (count > a.capacity) {
-        if (threadIdx.x == 0) report_error(a.status, DEV_ERR_BOUNDS, 611, count, a.capacity);
-        count = a.capacity;
-    }
     struct Mine {
         uint32_t held, need, add, len;
         uint64_t end;
         bool fits;
+        __device__ uint32_t back() const { return fits && held > need ? held - need : 0; }
+        __device__ uint32_t want() const { return fits && need > held ? need - held : 0; }
     };
     auto look = [&](uint32_t r, uint64_t& carry) {
         Mine m{0, 0, 0, 0, 0, false};
         uint64_t need = 0, len = 0;
         if (r < a.n) {
             m.add = ld_global(a.add + r);
-            len = (uint64_t)ld_global(a.ctx + r) + m.add;
-            need = (len + (1u << a.page_shift) - 1) >> a.page_shift;
+            const uint32_t ctx = ld_global(a.ctx + r);
             m.held = ld_global(a.held + r);
+            len = (uint64_t)ctx + m.add;
+            need = (len + (1u << a.page_shift) - 1) >> a.page_shift;
             if (m.held > a.stride) {
                 report_error(a.status, DEV_ERR_BOUNDS, 612, r, m.held);
                 m.held = a.stride;
             }
         }
-        uint64_t total;
-        m.end = carry + block_scan(m.add, sums, total) + m.add;
-        carry += total;
+        uint64_t before[1] = {m.add}, total[1];
+        block_scan<1>(before, reinterpret_cast<uint64_t(*)[1]>(sums), total);
+        m.end = carry + before[0] + m.add;
+        carry += total[0];
         m.fits = r < a.n && need <= a.stride && m.end <= a.tokens && len < NO_SLOT;
         m.need = m.fits ? (uint32_t)need : 0;
         m.len = (uint32_t)len;
         return m;
     };
+    const bool once = a.n <= threads;  // all requests at a time: what has been looked at stays
+    Mine m;
 
     // Pages given back, and where every request's tokens start.
-    uint64_t ends = 0, given = 0;
-    for (uint32_t base = 0; base < a.n; base += PLAN_THREADS) {
+    uint64_t ends = 0, given = 0, wanted = 0, mine_before = 0;
+    if (count > a.capacity) {
+        if (threadIdx.x == 0) report_error(a.status, DEV_ERR_BOUNDS, 611, count, a.capacity);
+        count = a.capacity;
+    }
+    for (uint32_t base = 0; base < a.n; base += threads) {
         const uint32_t r = base + threadIdx.x;
-        const Mine m = look(r, ends);
-        const uint32_t back = m.fits && m.held > m.need ? m.held - m.need : 0;
-        uint64_t total;
-        const uint64_t to = count + given + block_scan(back, sums, total);
-        given += total;
+        m = look(r, ends);
+        uint64_t before[2] = {m.back(), m.want()}, total[2];
+        block_scan<2>(before, sums, total);
+        const uint64_t to = count + given + before[0];
+        mine_before = before[1];
+        given += total[0];
         if (r < a.n) {
-            a.starts[r + 1] = (uint32_t)min(m.end, (uint64_t)a.tokens);
-            if (r == 0) a.starts[0] = 0;
+            const uint32_t first = (uint32_t)min(m.end, (uint64_t)a.tokens);
+            a.starts[r + 1] = first;
+            if (r < SEARCHED) firsts[r + 1] = first;
+            if (r == 0) a.starts[0] = firsts[0] = 0;
         }
-        for (uint32_t todo = __ballot_sync(0xffffffffu, back != 0); todo; todo &= todo - 1) {
+        for (uint32_t todo = __ballot_sync(0xffffffffu, m.back() != 0); todo; todo &= todo - 1) {
             const int src = __ffs(todo) - 1;
-            const uint32_t n = __shfl_sync(0xffffffffu, back, src), from = __shfl_sync(0xffffffffu, m.need, src);
+            const uint32_t n = __shfl_sync(0xffffffffu, m.back(), src), from = __shfl_sync(0xffffffffu, m.need, src);
             const uint64_t at = __shfl_sync(0xffffffffu, to, src);
-            const uint32_t* row = a.table + (size_t)(base + (threadIdx.x & ~31) + src) * a.stride + from;
-            for (uint32_t j = lane; j < n; j += 32) {
-                if (at + j < a.capacity) a.free_list[at + j] = ld_global(row + j);
-                else report_error(a.status, DEV_ERR_BOUNDS, 613, (uint32_t)(at + j), a.capacity);
-            }
+            const uint32_t* row = a.table + (size_t)(base + (threadIdx.x & ~31u) + src) * a.stride + from;
+            move_words(n, [&](uint32_t j) { return row + j; },
+                       [&](uint32_t j, uint32_t page) {
+                           if (at + j < a.capacity) a.free_list[at + j] = page;
+                           else report_error(a.status, DEV_ERR_BOUNDS, 613, (uint32_t)(at + j), a.capacity);
+                       });
         }
     }
     const uint64_t have = min(count + given, (uint64_t)a.capacity);
-    __syncthreads();  // the list is read from here on
+    if (given != 0) __syncthreads();  // the list is read from here on
 
     // Pages taken.
-    uint64_t wanted = 0, used = 0, refused = 0, placed = 0;
+    uint64_t used = 0, placed = 0;
+    uint32_t refused = 0;
     ends = 0;
-    for (uint32_t base = 0; base < a.n; base += PLAN_THREADS) {
+    for (uint32_t base = 0; base < a.n; base += threads) {
         const uint32_t r = base + threadIdx.x;
-        const Mine m = look(r, ends);
-        const uint32_t want = m.fits && m.need > m.held ? m.need - m.held : 0;
-        uint64_t total;
-        const uint64_t before = wanted + block_scan(want, sums, total);
-        wanted += total;
-        const bool granted = m.fits && (want == 0 || before + want <= have);
+        if (!once) {
+            m = look(r, ends);
+            uint64_t before[1] = {m.want()}, total[1];
+            block_scan<1>(before, reinterpret_cast<uint64_t(*)[1]>(sums), total);
+            mine_before = wanted + before[0];
+            wanted += total[0];
+        }
+        const uint32_t want = m.want();
+        const bool granted = m.fits && (want == 0 || mine_before + want <= have);
         if (r < a.n) {
             a.held_out[r] = granted ? m.need : m.held;
             a.lens[r] = granted ? m.len : 0;
+            if (granted) used += want, placed += m.add; else refused++;
         }
         for (uint32_t todo = __ballot_sync(0xffffffffu, granted && want != 0); todo; todo &= todo - 1) {
             const int src = __ffs(todo) - 1;
             const uint32_t n = __shfl_sync(0xffffffffu, want, src), to = __shfl_sync(0xffffffffu, m.held, src);
-            const uint64_t at = have - 1 - __shfl_sync(0xffffffffu, before, src);
-            uint32_t* row = a.table + (size_t)(base + (threadIdx.x & ~31) + src) * a.stride + to;
-            for (uint32_t j = lane; j < n; j += 32) row[j] = ld_global(a.free_list + (at - j));
+            const uint32_t* last = a.free_list + (have - 1 - __shfl_sync(0xffffffffu, mine_before, src));
+            uint32_t* row = a.table + (size_t)(base + (threadIdx.x & ~31u) + src) * a.stride + to;
+            move_words(n, [&](uint32_t j) { return last - j; }, [&](uint32_t j, uint32_t page) { row[j] = page; });
         }
-        uint64_t sum;
-        block_scan(granted ? want : 0, sums, sum);
-        used += sum;
-        block_scan(r < a.n && !granted, sums, sum);
-        refused += sum;
-        block_scan(granted ? m.add : 0, sums, sum);
-        placed += sum;
     }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) {
+        used += __shfl_xor_sync(0xffffffffu, used, off);
+        placed += __shfl_xor_sync(0xffffffffu, placed, off);
+        refused += __shfl_xor_sync(0xffffffffu, refused, off);
+    }
+    if ((threadIdx.x & 31) == 0) {
+        atomicAdd(&counted[0], (unsigned long long)used);
+        atomicAdd(&counted[1], (unsigned long long)refused);
+        atomicAdd(&counted[2], (unsigned long long)placed);
+    }
+    __syncthreads();  // tables, lengths and starts are read from here on
     if (threadIdx.x == 0) {
-        a.free_out[0] = (uint32_t)(have - used);
-        a.free_out[1] = (uint32_t)refused;
-        a.free_out[2] = (uint32_t)placed;
-        a.free_out[3] = (uint32_t)used;
+        a.free_out[0] = (uint32_t)(have - counted[0]);
+        a.free_out[1] = (uint32_t)counted[1];
+        a.free_out[2] = (uint32_t)counted[2];
+        a.free_out[3] = (uint32_t)counted[0];
     }
+    if (!place_here) return;
+    for (uint32_t t = threadIdx.x; t < a.tokens; t += threads) place_token(a, t, [&](uint32_t r) { return firsts[r]; });
 }
 
-__global__ void __launch_bounds__(256) place_tokens_kernel(const __grid_constant__ PlanArgs a)
+__global__ void __launch_bounds__(PLACE_THREADS) place_tokens_kernel(const __grid_constant__ PlanArgs a)
 {
+    __shared__ uint32_t firsts[SEARCHED + 1];
     pdl_wait();
     pdl_launch_dependents();
-    const uint32_t t = blockIdx.x * 256 + threadIdx.x;
-    if (t < a.tokens) place_token(a, t);
+    const uint32_t t = blockIdx.x * PLACE_THREADS + threadIdx.x;
+    if (a.n <= SEARCHED) {
+        for (uint32_t r = threadIdx.x; r <= a.n; r += PLACE_THREADS) firsts[r] = ld_global(a.starts + r);
+        __syncthreads();
+        if (t < a.tokens) place_token(a, t, [&](uint32_t r) { return firsts[r]; });
+    } else if (t < a.tokens) {
+        place_token(a, t, [&](uint32_t r) { return ld_global(a.starts + r); });
+    }
 }
 
 // ---- append --------------------------------------------------------------------------------------------------------------------
@@ -389,10 +451,13 @@ int launch_kv_block_tables(const LaunchArgs& a)
     const size_t capacity = a.b[4].bytes / 4;
     PlanArgs k{u(0), u(1), u(2), u(3), u(4), u(5), u(6), u(7), u(8), u(9), u(10), u(11), n, tokens, (uint32_t)__builtin_ctz(p.page), p.stride,
                (uint32_t)(capacity < NO_SLOT ? capacity : NO_SLOT), a.status};
-    cudaError_t e = launch_dependent(block_tables_kernel, dim3(1), dim3(PLAN_THREADS), 0, a.stream, k);
+    const bool place_here = n <= SEARCHED && tokens <= PLACED_HERE;
+    const uint32_t work = place_here && tokens > n ? tokens : n, threads = work < PLAN_THREADS ? (work + 31) / 32 * 32 : PLAN_THREADS;
+    cudaError_t e = launch_dependent(block_tables_kernel, dim3(1), dim3(threads), 0, a.stream, k, place_here);
     ++*a.launches;
     if (int r = check_cuda(a, e, "kv_block_tables")) return r;
-    e = launch_dependent(place_tokens_kernel, dim3((unsigned)((tokens + 255ull) / 256)), dim3(256), 0, a.stream, k);
+    if (place_here) return 0;
+    e = launch_dependent(place_tokens_kernel, dim3((unsigned)((tokens + PLACE_THREADS - 1ull) / PLACE_THREADS)), dim3(PLACE_THREADS), 0, a.stream, k);
     ++*a.launches;
     return check_cuda(a, e, "kv_block_tables tokens");
 }
