@@ -154,13 +154,17 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
     const uint32_t per_thread = (a.req.n + WARPS * 32 - 1) / (WARPS * 32);
     const uint32_t r_begin = min(threadIdx.x * per_thread, a.req.n), r_end = min(r_begin + per_thread, a.req.n);
     Request rq{0, 0, 0};
-    Tiles tl{0, 0};
     constexpr int COUNT_BITS = 17;  // of the sums: requests with tiles (at most MOST_REQUESTS) below, weights above
     uint64_t mine = 0;
-    for (uint32_t r = r_begin; r < r_end; r++) {
-        rq = request_at(a.req, r);
-        tl = tiles_of(a, rq);
+    const auto add = [&](uint32_t, const Request& q) {
+        rq = q;
+        const Tiles tl = tiles_of(a, q);
         mine += (uint64_t)tl.weight() << COUNT_BITS | (tl.n ? 1 : 0);
+    };
+    if (per_thread == 1) {
+        if (r_begin < r_end) add(r_begin, request_at(a.req, r_begin));
+    } else {
+        for_requests(a.req, r_begin, r_end, add);
     }
     uint64_t up_to = mine;
 #pragma unroll
@@ -188,16 +192,13 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
         }
         uint64_t at = base >> COUNT_BITS;
         uint32_t nth = (uint32_t)base & ((1u << COUNT_BITS) - 1);
-        for (uint32_t r = r_begin; r < r_end; r++) {
-            if (per_thread != 1) {
-                rq = request_at(a.req, r);
-                tl = tiles_of(a, rq);
-            }
-            const uint64_t end = at + tl.weight();
+        const auto find = [&](uint32_t r, const Request& q) {
+            const Tiles tiles = tiles_of(a, q);
+            const uint64_t end = at + tiles.weight();
 #pragma unroll
             for (int w = 0; w < WARPS; w++) {
                 if (want[w][0] >= at && want[w][0] < end) {
-                    sm.met[w][0] = Met{r, rq.first, rq.n, rq.len, tl.lo, tl.n};
+                    sm.met[w][0] = Met{r, q.first, q.n, q.len, tiles.lo, tiles.n};
                     sm.from[w] = (uint32_t)(want[w][0] - at);
                 }
 #pragma unroll
@@ -206,7 +207,12 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
             }
             if (blockIdx.x == 0) work.head.before[r] = at;
             at = end;
-            nth += tl.n ? 1 : 0;
+            nth += tiles.n ? 1 : 0;
+        };
+        if (per_thread == 1) {
+            if (r_begin < r_end) find(r_begin, rq);
+        } else {
+            for_requests(a.req, r_begin, r_end, find);
         }
     } else if (blockIdx.x == 0) {
         for (uint32_t r = r_begin; r < r_end; r++) work.head.before[r] = 0;
@@ -492,19 +498,17 @@ __device__ __forceinline__ void list_units(const BlocksAttn& a, const BlocksWork
     const uint32_t per_thread = (a.req.n + N - 1) / N, r_begin = min(tid * per_thread, a.req.n), r_end = min(r_begin + per_thread, a.req.n);
     const auto units = [&](const Request& q) -> uint32_t { return q.n > FEW_ROWS / a.group ? (uint32_t)(((uint64_t)q.n * a.group + UNIT_ROWS - 1) / UNIT_ROWS) : 0; };
     uint32_t mine = 0, kilokeys = 0, total, all_kilokeys;
-    for (uint32_t r = r_begin; r < r_end; r++) {
-        const Request q = request_at(a.req, r);
+    for_requests(a.req, r_begin, r_end, [&](uint32_t, const Request& q) {
         const uint32_t n = units(q);
         mine += n;
-        if (n) kilokeys += q.len / 1024;  // (at most 2^21 a request; what is past the sum's end says no more than that it is much)
-        kilokeys = min(kilokeys, 1u << 22);
-    }
+        if (n) kilokeys = min(kilokeys + q.len / 1024, 1u << 22);  // (no more than that it is much)
+    });
     uint32_t at = scan(mine, total);
     scan(kilokeys, all_kilokeys);
-    for (uint32_t r = r_begin; r < r_end; r++) {
+    for_requests(a.req, r_begin, r_end, [&](uint32_t r, const Request& q) {
         w.units_before[r] = at;
-        at += units(request_at(a.req, r));
-    }
+        at += units(q);
+    });
     const bool by_head = (uint64_t)all_kilokeys * 1024 * a.n_kv * 2 * HD > ((uint64_t)96 << 20);
     if (tid == 0) {
         w.units_before[a.req.n] = total;
@@ -699,7 +703,7 @@ uint32_t most_stretches(int sm_count, uint32_t n_kv) { return grid_ctas(sm_count
 
 size_t blocks_decode_work(int sm_count, uint32_t n_kv, uint32_t group, uint32_t max_q)
 {
-    return 2ull * most_stretches(sm_count, n_kv) * n_kv * few_rows(group, max_q) * (HD + 2) * 4;
+    return 2ull * grid_ctas(sm_count, n_kv) * WARPS * few_rows(group, max_q) * (HD + 2) * 4;  // (no less for fewer heads)
 }
 
 int launch_blocks_decode(const LaunchArgs& a, const BlocksAttn& k, const BlocksWork& head)

@@ -28,6 +28,7 @@ constexpr int THREADS = 512;                      // two softmax warpgroups, one
 constexpr int CONVERT_WARP = 8, MMA_WARP = 12, COPY_WARP = 13, QUEUE_WARP = 14, QUERY_WARP = 15;
 constexpr int RAW = 4;                            // tiles of keys under way from the cache
 constexpr int ITEMS = 2;                          // the item at work and the next: what a CTA takes early no other can take
+constexpr int TILES_A_WAIT = 100000;              // fewer tiles of keys than go through in the time that a wait is bounded to (2000 cycles each)
 constexpr int ITEM_READERS = 8 + 4 + 3;           // warps that give an item's place back
 constexpr uint32_t HALF_TILE = 64 * 128;          // [64 rows][64 dims] f16
 constexpr uint32_t Q_BYTES = 4 * HALF_TILE;       // of one tile of queries
@@ -61,6 +62,7 @@ struct PrefillSmem {
     float4 exps[2 * RAW][2];         // [tile of keys % 8]: the powers of two of K, and the exponents of V, of its four blocks
     Item item[ITEMS];
     uint32_t tmem_base, last[2];
+    uint32_t gave_up;                // a role has waited in vain
     uint4 rows[8][32][5];            // of each softmax warp: 32 dims of its 32 rows in f16 on their way out, 80 bytes a row
 };
 static_assert(sizeof(PrefillSmem) <= 227 * 1024, "shared memory of a CTA");
@@ -211,6 +213,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             mbar_init(&sm.o_free[i], 128);
         }
         mbar_init(&sm.q_full, 1);
+        sm.gave_up = 0;
         mbar_fence_init();
     }
     pdl_wait();  // everything this kernel reads comes from earlier kernels of the stream, the cut of the units among it
@@ -348,7 +351,14 @@ __global__ void __launch_bounds__(THREADS, 1)
         } else if (warp == QUEUE_WARP) {
             Feed feed = open_feed(a, w);
             for (;; nth++) {
-                mbar_wait_warp(&sm.item_empty[nth % ITEMS], ((nth / ITEMS) & 1) ^ 1, status, 654, failed, 200);
+                // An item lasts as long as its keys: the bound here grows with the tiles of the one that is waited for.
+                const int tiles = nth < ITEMS ? 0 : sm.item[nth % ITEMS].unit_tiles();
+                for (int waited = 0; waited <= tiles; waited += TILES_A_WAIT) {
+                    bool late = false;
+                    mbar_wait_warp(&sm.item_empty[nth % ITEMS], ((nth / ITEMS) & 1) ^ 1, waited + TILES_A_WAIT <= tiles ? nullptr : status, 654, late, 200);
+                    failed = late;
+                    if (!late || *(volatile uint32_t*)&sm.gave_up) break;
+                }
                 if (failed) break;
                 fetch_item(a, w, feed, &sm.item[nth % ITEMS]);
                 __syncwarp();
@@ -634,6 +644,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             done_item();  // only now: the queue gives out the next but one behind it
         }
     }
+    if (failed) sm.gave_up = 1;
     // A wait that ran out leaves MMAs (and Q's copy) in flight that nobody waits for: they get a bounded time to land.
     if (__syncthreads_or(failed)) {
         let_copies_land();

@@ -34,14 +34,10 @@ struct Request {
     uint32_t first, n, len;  // its query tokens, its keys
 };
 // Lengths come from the device: what does not fit the buffers is reported and taken as nothing (queries) or cut (keys).
-__device__ __forceinline__ Request request_at(const Requests& a, uint32_t r)
+__device__ __forceinline__ Request checked_request(const Requests& a, uint32_t r, uint32_t first, uint32_t end, uint32_t len)
 {
-    Request q;
-    q.first = ld_global(a.starts + r);
-    const uint32_t end = ld_global(a.starts + r + 1);
-    q.len = ld_global(a.lens + r);
-    q.n = end - q.first;
-    if (end < q.first || end > a.tokens || q.n > a.max_q) {
+    Request q{first, end - first, len};
+    if (end < first || end > a.tokens || q.n > a.max_q) {
         report_error(a.status, DEV_ERR_BOUNDS, 601, r, end);
         q.n = 0;
     }
@@ -51,6 +47,11 @@ __device__ __forceinline__ Request request_at(const Requests& a, uint32_t r)
         q.len = (uint32_t)most;
     }
     return q;
+}
+__device__ __forceinline__ Request request_at(const Requests& a, uint32_t r)
+{
+    const uint32_t first = ld_global(a.starts + r), end = ld_global(a.starts + r + 1), len = ld_global(a.lens + r);
+    return checked_request(a, r, first, end, len);
 }
 // The pool's block that holds tokens 16 * tile .. of request r, in two steps, so that nothing waits for the table in between: its
 // page's number, then the block.  A page that the pool does not have is reported and read as page 0.
@@ -100,6 +101,22 @@ __device__ __forceinline__ int ld_global_if(bool p, const int8_t* at)
     int v;
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.b32 %0, 0;\n\t@p ld.global.s8 %0, [%1];\n\t}" : "=&r"(v) : "l"(at), "r"((uint32_t)p));
     return v;
+}
+
+// f(r, request) for r in [begin, end), four requests' words on their way at a time.
+template <typename F>
+__device__ __forceinline__ void for_requests(const Requests& a, uint32_t begin, uint32_t end, const F& f)
+{
+    for (uint32_t r0 = begin; r0 < end; r0 += 4) {
+        uint32_t first[5], len[4];
+#pragma unroll
+        for (uint32_t k = 0; k < 5; k++) first[k] = ld_global_if(r0 + k <= end, a.starts + r0 + k);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) len[k] = ld_global_if(r0 + k < end, a.lens + r0 + k);
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++)
+            if (r0 + k < end) f(r0 + k, checked_request(a, r0 + k, first[k], first[k + 1], len[k]));
+    }
 }
 
 // Two e4m3 bytes as two f16, exactly (one instruction at the rate of an integer one: 64 a clock and SM).

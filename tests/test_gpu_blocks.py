@@ -396,6 +396,113 @@ def test_lengths_that_no_buffer_holds_are_reported(ctx):
         ctx.sync()
 
 
+def test_many_parts_of_one_request_among_many(ctx):
+    """One kv head: every warp of the GPU has a stretch of it, and one long request's parts are merged by a CTA of few warps."""
+    rng = np.random.default_rng(8)
+    lens = rng.integers(1, 40, 400)
+    lens[137] = 30000
+    Batch(8, lens, np.ones(400, int), 1, 2, 16).run(ctx)
+    Batch(9, lens[:300], rng.integers(0, 9, 300).clip(0, lens[:300]), 1, 1, 32).run(ctx)
+
+
+@pytest.mark.parametrize("requests", [127, 128, 129, 513, 1100])
+def test_more_requests_than_threads(ctx, requests):
+    rng = np.random.default_rng(requests)
+    lens = rng.integers(0, 50, requests)
+    new = np.minimum(rng.integers(0, 4, requests), np.maximum(lens, 1))
+    new[::37] = rng.integers(5, 30, len(new[::37]))
+    Batch(requests, np.maximum(lens, new), new, 1, 4, 16, dead=set(range(5, requests, 50))).run(ctx)
+
+
+def test_offsets_beyond_32_bits(ctx):
+    """Pools of more than 4 GiB each: tokens go into their last pages and are read from there."""
+    import super_gemma_b200 as sg
+
+    kv, page, keys = 16, 512, 700
+    pages = (1 << 32) // (page * kv * D) + 3
+    blocks = pages * page // TILE
+    pools = [ctx.new_buffer(blocks * kv * TILE * D, np.uint8) for _ in range(2)]
+    exps = [ctx.new_buffer(blocks * kv, np.int8) for _ in range(2)]
+    assert pools[0].nbytes > 1 << 32
+    table = _u32([[pages - 1, pages - 2, 0]])
+    rng = np.random.default_rng(3)
+    x = {n: rng.standard_normal((keys, kv * (2 if n == "q" else 1), D)).astype(np.float16) for n in "qkv"}
+    slots = ref.rows_of(table[0], keys, page)
+    assert slots.max() * kv * D > 1 << 32
+    up = ctx.buffer_from_iter
+    b = {n: up(x[n]) for n in "qkv"}
+    ctx.dispatch_blocking(ctx.load_kernel("kv_append_blocks_e4m3_d128"), bind(b["k"], b["v"], up(_u32(slots)), pools[0], exps[0], pools[1], exps[1]), None, [kv, keys, 1])
+    first = (pages - 2) * page // TILE  # the last two pages, as a pool of their own
+    host = [np.zeros((2 * page // TILE, kv, TILE, D), np.uint8), np.zeros((2 * page // TILE, kv), np.int8)]
+    host += [h.copy() for h in host]
+    ref.append(x["k"], slots - first * TILE, *host[:2])
+    ref.append(x["v"], slots - first * TILE, *host[2:])
+    for p, e, hp, he in ((pools[0], exps[0], host[0], host[1]), (pools[1], exps[1], host[2], host[3])):
+        assert np.array_equal(p.read(hp.size, first * kv * TILE * D).reshape(hp.shape), hp) and np.array_equal(e.read(he.size, first * kv).reshape(he.shape), he)
+    for m in (1, 3, 300):
+        q, out = up(x["q"][:m]), ctx.new_buffer(m * kv * 2 * D, np.uint16)
+        work = ctx.new_buffer(ctx.attn_blocks_work_bytes(kv, 2, 1, m, m), np.uint8)
+        ctx.dispatch_blocking(ctx.load_kernel("attn_blocks_e4m3_d128"),
+                              bind(q, pools[0], exps[0], pools[1], exps[1], up(table.reshape(-1)), up(_u32([keys])), up(_u32([0, m])), out, work),
+                              (SCALE, page, 3, 0, 2, m), [kv, 1, m])
+        want, bound = ref.attend(x["q"][:m], *host, table - (pages - 2), [keys], [0, m], page, 0, 2, SCALE)
+        got = out.read().view(np.float16).reshape(want.shape)
+        assert (np.abs(got - want) <= bound).all(), m
+    with pytest.raises(sg.Validation):  # a slice that is no whole number of heads' tiles is no pool
+        ctx.dispatch(ctx.load_kernel("attn_blocks_e4m3_d128"), bind(q, pools[0].slice(0, 4096), exps[0], pools[1], exps[1], up(table.reshape(-1)), up(_u32([keys])),
+                                                                    up(_u32([0, m])), out, work), (SCALE, page, 3, 0, 2, m), [kv, 1, m])
+
+
+def test_contexts_side_by_side(ctx):
+    """Two contexts, a stream and a work buffer each, with dispatches of both under way at a time, decode and prompts."""
+    import super_gemma_b200 as sg
+
+    other = sg.GpuContext(0)
+    a, b = Batch(1, [3000, 50, 700], [1, 1, 300], 4, 2, 64), Batch(2, [900, 2000, 40], [200, 1, 40], 4, 2, 64)
+    ba, bb = a.buffers(ctx), b.buffers(other)
+    ka, kb = ctx.load_kernel("attn_blocks_e4m3_d128"), other.load_kernel("attn_blocks_e4m3_d128")
+    for _ in range(20):
+        ctx.dispatch(ka, ba, *a.call(0))
+        other.dispatch(kb, bb, *b.call(0))
+    ctx.sync()
+    other.sync()
+    a.check(a.out.read(), 0)
+    b.check(b.out.read(), 0)
+
+
+def test_graphs_that_share_a_work_buffer(ctx):
+    """Two recorded dispatches over one work buffer, in one graph and in two, replayed in turn."""
+    a, b = Batch(3, [1000, 50], [1, 100], 2, 2, 32), Batch(4, [600, 333], [90, 1], 2, 2, 32)
+    ba, bb = a.buffers(ctx), b.buffers(ctx)
+    work = a.work if a.work.nbytes >= b.work.nbytes else b.work
+    ba[9].buf = bb[9].buf = work
+    k = ctx.load_kernel("attn_blocks_e4m3_d128")
+    ctx.dispatch(k, ba, *a.call(0))
+    ctx.dispatch(k, bb, *b.call(0))
+    ctx.sync()
+    want = a.out.read(), b.out.read()
+    a.check(want[0], 0)
+    b.check(want[1], 0)
+
+    def both(at):
+        for _ in range(4):
+            at.dispatch(k, ba, *a.call(0))
+            at.dispatch(k, bb, *b.call(0))
+
+    graphs = [ctx.record_graph(both), ctx.record_graph(lambda at: at.dispatch(k, ba, *a.call(0))), ctx.record_graph(lambda at: at.dispatch(k, bb, *b.call(0)))]
+    a.out.zero()
+    b.out.zero()
+    for g in graphs + graphs[::-1]:
+        ctx.submit(g)
+    ctx.sync()
+    assert np.array_equal(a.out.read(), want[0]) and np.array_equal(b.out.read(), want[1])
+
+
+def test_work_of_a_larger_grid_serves_a_smaller_one(ctx):
+    sizes = [ctx.attn_blocks_work_bytes(kv, 2, r, n, q) for kv, r, n, q in ((1, 1, 1, 1), (16, 1, 1, 1), (1000, 1, 1, 1), (1000, 64, 1, 1), (1000, 64, 64, 1), (1000, 64, 640, 10), (1000, 64, 6400, 100))]
+    assert sizes == sorted(sizes) and sizes[0] > 0
+
+
 # ---- together ------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("recorded", [False, True])
 def test_a_server_plans_appends_and_attends(ctx, recorded):
