@@ -15,11 +15,12 @@ namespace {
 // end, in the same order, by every request whose wants the list still covers when all before it are counted.  The others are
 // refused: they keep what they hold, their length is 0 and their tokens have no slot.
 //
-// Prefix sums over the requests and little else: bound by its own latency.  One CTA does the sums, of up to 1024 requests at a time; a
-// request's pages are moved by one warp, and the tokens are placed by the same CTA while there are few of them.
+// Prefix sums over the requests and little else: bound by its own latency.  One CTA does the sums, of up to 1024 requests at a time, and
+// moves the pages; it places the tokens too while there are few of them.
 constexpr uint32_t PLAN_THREADS = 1024, PLAN_WARPS = PLAN_THREADS / 32;
 constexpr uint32_t PLACE_THREADS = 256;
-constexpr uint32_t SEARCHED = 1024;      // requests whose first tokens a CTA keeps at hand
+constexpr uint32_t MOST_STRIDE = 1u << 21;
+constexpr uint32_t SEARCHED = 4096;      // requests whose first tokens a CTA keeps at hand (16 KB)
 constexpr uint32_t PLACED_HERE = 4096;   // tokens that the first CTA places itself (64 requests of one token: 8.2 us with a second kernel)
 
 struct PlanArgs {
@@ -87,24 +88,47 @@ __device__ __forceinline__ void place_token(const PlanArgs& a, uint32_t t, const
     a.at[t] = pos;
 }
 
-// n words by a warp, four of each lane on their way at a time.
+// Moves of up to PLAN_THREADS requests: request r's words [0, n_r) by whichever thread comes to them, four of each on their way at a time.
+// (A request's pages by one warp: a prompt of 32768 tokens in pages of 16 took 6 us of its own.)
+struct Moves {
+    uint32_t before[PLAN_THREADS + 1];  // words of the requests before each
+    uint32_t first[PLAN_THREADS];       // where its words start in its row
+};
 template <typename From, typename To>
-__device__ __forceinline__ void move_words(uint32_t n, const From& from, const To& to)
+__device__ __forceinline__ void move_words(const Moves& mv, uint32_t requests, const From& from, const To& to)
 {
-    for (uint32_t j0 = threadIdx.x & 31; j0 < n; j0 += 128) {
-        uint32_t w[4];
+    const uint32_t total = mv.before[requests];
+    for (uint32_t j0 = threadIdx.x; j0 < total; j0 += 4 * blockDim.x) {
+        uint32_t w[4], r[4];
 #pragma unroll
-        for (uint32_t k = 0; k < 4; k++) w[k] = ld_global_if(j0 + 32 * k < n, from(j0 + 32 * k));
+        for (uint32_t k = 0; k < 4; k++) {
+            const uint32_t j = j0 + k * blockDim.x;
+            uint32_t lo = 0, hi = requests;  // the last request with before <= j
+            while (j < total && hi - lo > 1) {
+                const uint32_t mid = (lo + hi) >> 1;
+                if (mv.before[mid] <= j) lo = mid; else hi = mid;
+            }
+            r[k] = lo;
+            w[k] = ld_global_if(j < total, from(lo, j - mv.before[lo], j));
+        }
 #pragma unroll
-        for (uint32_t k = 0; k < 4; k++)
-            if (j0 + 32 * k < n) to(j0 + 32 * k, w[k]);
+        for (uint32_t k = 0; k < 4; k++) {
+            const uint32_t j = j0 + k * blockDim.x;
+            if (j < total) to(r[k], j - mv.before[r[k]], j, w[k]);
+        }
     }
 }
 
+// KEPT: all requests fit four rounds of the CTA's threads; what has been looked at stays in registers for the second pass.
+constexpr uint32_t KEPT_ROUNDS = 4;
+template <bool KEPT>
 __global__ void __launch_bounds__(PLAN_THREADS) block_tables_kernel(const __grid_constant__ PlanArgs a, bool place_here)
 {
-    __shared__ uint64_t sums[PLAN_WARPS][2];
-    __shared__ uint32_t firsts[SEARCHED + 1];
+    __shared__ uint64_t sums[PLAN_WARPS][1];
+    __shared__ union {
+        Moves moves;
+        uint32_t firsts[SEARCHED + 1];
+    } sm;
     __shared__ unsigned long long counted[3];  // pages taken, requests refused, tokens placed
     const uint32_t threads = blockDim.x;
     if (threadIdx.x < 3) counted[threadIdx.x] = 0;
@@ -112,99 +136,131 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_tables_kernel(const __grid
     pdl_launch_dependents();
     uint32_t count = ld_global(a.count);
     struct Mine {
-        uint32_t held, need, add, len;
-        uint64_t end;
+        uint32_t held, add, ctx, need;
         bool fits;
         __device__ uint32_t back() const { return fits && held > need ? held - need : 0; }
         __device__ uint32_t want() const { return fits && need > held ? need - held : 0; }
     };
-    auto look = [&](uint32_t r, uint64_t& carry) {
-        Mine m{0, 0, 0, 0, 0, false};
-        uint64_t need = 0, len = 0;
-        if (r < a.n) {
-            m.add = ld_global(a.add + r);
-            const uint32_t ctx = ld_global(a.ctx + r);
-            m.held = ld_global(a.held + r);
-            len = (uint64_t)ctx + m.add;
-            need = (len + (1u << a.page_shift) - 1) >> a.page_shift;
-            if (m.held > a.stride) {
-                report_error(a.status, DEV_ERR_BOUNDS, 612, r, m.held);
-                m.held = a.stride;
-            }
-        }
-        uint64_t before[1] = {m.add}, total[1];
-        block_scan<1>(before, reinterpret_cast<uint64_t(*)[1]>(sums), total);
-        m.end = carry + before[0] + m.add;
-        carry += total[0];
-        m.fits = r < a.n && need <= a.stride && m.end <= a.tokens && len < NO_SLOT;
-        m.need = m.fits ? (uint32_t)need : 0;
-        m.len = (uint32_t)len;
+    auto load = [&](uint32_t r) {
+        Mine m{0, 0, 0, 0, false};
+        m.add = ld_global_if(r < a.n, a.add + r);
+        m.ctx = ld_global_if(r < a.n, a.ctx + r);
+        m.held = ld_global_if(r < a.n, a.held + r);
         return m;
     };
-    const bool once = a.n <= threads;  // all requests at a time: what has been looked at stays
-    Mine m;
-
-    // Pages given back, and where every request's tokens start.
-    uint64_t ends = 0, given = 0, wanted = 0, mine_before = 0;
+    // Where the request's tokens end, whether it takes part, how many pages it needs.
+    auto look = [&](Mine& m, uint32_t r, uint64_t& carry) -> uint64_t {
+        if (m.held > a.stride) {
+            report_error(a.status, DEV_ERR_BOUNDS, 612, r, m.held);
+            m.held = a.stride;
+        }
+        const uint64_t len = (uint64_t)m.ctx + m.add, need = (len + (1u << a.page_shift) - 1) >> a.page_shift;
+        uint64_t before[1] = {m.add}, total[1];
+        block_scan<1>(before, sums, total);
+        const uint64_t end = carry + before[0] + m.add;
+        carry += total[0];
+        m.fits = r < a.n && need <= a.stride && end <= a.tokens && len < NO_SLOT;
+        m.need = m.fits ? (uint32_t)need : 0;
+        return end;
+    };
+    constexpr uint32_t ROUNDS = KEPT ? KEPT_ROUNDS : 1;
+    Mine kept[ROUNDS];
+    uint32_t kept_first[ROUNDS];
+    uint64_t kept_before[ROUNDS], kept_total[ROUNDS];
+    if (KEPT) {
+#pragma unroll
+        for (uint32_t k = 0; k < ROUNDS; k++) kept[k] = load(k * threads + threadIdx.x);
+    }
     if (count > a.capacity) {
         if (threadIdx.x == 0) report_error(a.status, DEV_ERR_BOUNDS, 611, count, a.capacity);
         count = a.capacity;
     }
-    for (uint32_t base = 0; base < a.n; base += threads) {
-        const uint32_t r = base + threadIdx.x;
-        m = look(r, ends);
-        uint64_t before[2] = {m.back(), m.want()}, total[2];
-        block_scan<2>(before, sums, total);
-        const uint64_t to = count + given + before[0];
-        mine_before = before[1];
-        given += total[0];
-        if (r < a.n) {
-            const uint32_t first = (uint32_t)min(m.end, (uint64_t)a.tokens);
-            a.starts[r + 1] = first;
-            if (r < SEARCHED) firsts[r + 1] = first;
-            if (r == 0) a.starts[0] = firsts[0] = 0;
-        }
-        for (uint32_t todo = __ballot_sync(0xffffffffu, m.back() != 0); todo; todo &= todo - 1) {
-            const int src = __ffs(todo) - 1;
-            const uint32_t n = __shfl_sync(0xffffffffu, m.back(), src), from = __shfl_sync(0xffffffffu, m.need, src);
-            const uint64_t at = __shfl_sync(0xffffffffu, to, src);
-            const uint32_t* row = a.table + (size_t)(base + (threadIdx.x & ~31u) + src) * a.stride + from;
-            move_words(n, [&](uint32_t j) { return row + j; },
-                       [&](uint32_t j, uint32_t page) {
-                           if (at + j < a.capacity) a.free_list[at + j] = page;
-                           else report_error(a.status, DEV_ERR_BOUNDS, 613, (uint32_t)(at + j), a.capacity);
-                       });
-        }
-    }
-    const uint64_t have = min(count + given, (uint64_t)a.capacity);
-    if (given != 0) __syncthreads();  // the list is read from here on
 
-    // Pages taken.
-    uint64_t used = 0, placed = 0;
-    uint32_t refused = 0;
-    ends = 0;
-    for (uint32_t base = 0; base < a.n; base += threads) {
+    // Pages given back, and where every request's tokens start.
+    uint64_t ends = 0, given = 0;
+    // Pages back (low half) and wanted (high half) before a request and of all of the round: 1024 rows of at most MOST_STRIDE fit a word.
+    auto sum_up = [&](const Mine& m, uint64_t& total) -> uint64_t {
+        uint64_t before[1] = {(uint64_t)m.want() << 32 | m.back()}, all[1];
+        block_scan<1>(before, sums, all);
+        total = all[0];
+        return before[0];
+    };
+    auto first_pass = [&](Mine& m, uint32_t base, uint64_t& before, uint64_t& total) -> uint32_t {
         const uint32_t r = base + threadIdx.x;
-        if (!once) {
-            m = look(r, ends);
-            uint64_t before[1] = {m.want()}, total[1];
-            block_scan<1>(before, reinterpret_cast<uint64_t(*)[1]>(sums), total);
-            mine_before = wanted + before[0];
-            wanted += total[0];
+        const uint32_t first = (uint32_t)min(look(m, r, ends), (uint64_t)a.tokens);
+        before = sum_up(m, total);
+        const uint32_t back_total = (uint32_t)total;
+        if (r < a.n) {
+            a.starts[r + 1] = first;
+            if (r == 0) a.starts[0] = 0;
         }
-        const uint32_t want = m.want();
-        const bool granted = m.fits && (want == 0 || mine_before + want <= have);
+        if (back_total != 0) {
+            sm.moves.before[threadIdx.x] = (uint32_t)before;
+            sm.moves.first[threadIdx.x] = m.need;
+            if (threadIdx.x == 0) sm.moves.before[threads] = back_total;
+            __syncthreads();
+            const uint64_t to = count + given;
+            move_words(sm.moves, threads, [&](uint32_t q, uint32_t j, uint32_t) { return a.table + (size_t)(base + q) * a.stride + sm.moves.first[q] + j; },
+                       [&](uint32_t, uint32_t, uint32_t j, uint32_t page) {
+                           if (to + j < a.capacity) a.free_list[to + j] = page;
+                           else report_error(a.status, DEV_ERR_BOUNDS, 613, (uint32_t)(to + j), a.capacity);
+                       });
+            given += back_total;
+            __syncthreads();
+        }
+        return first;
+    };
+    // Pages taken.
+    uint64_t wanted = 0, used = 0, placed = 0, have = 0;
+    uint32_t refused = 0;
+    auto second_pass = [&](const Mine& m, uint32_t base, uint64_t both_before, uint64_t both_total) {
+        const uint32_t r = base + threadIdx.x, want = m.want(), before = (uint32_t)(both_before >> 32), total = (uint32_t)(both_total >> 32);
+        const bool granted = m.fits && (want == 0 || wanted + before + want <= have);
         if (r < a.n) {
             a.held_out[r] = granted ? m.need : m.held;
-            a.lens[r] = granted ? m.len : 0;
+            a.lens[r] = granted ? m.ctx + m.add : 0;
             if (granted) used += want, placed += m.add; else refused++;
         }
-        for (uint32_t todo = __ballot_sync(0xffffffffu, granted && want != 0); todo; todo &= todo - 1) {
-            const int src = __ffs(todo) - 1;
-            const uint32_t n = __shfl_sync(0xffffffffu, want, src), to = __shfl_sync(0xffffffffu, m.held, src);
-            const uint32_t* last = a.free_list + (have - 1 - __shfl_sync(0xffffffffu, mine_before, src));
-            uint32_t* row = a.table + (size_t)(base + (threadIdx.x & ~31u) + src) * a.stride + to;
-            move_words(n, [&](uint32_t j) { return last - j; }, [&](uint32_t j, uint32_t page) { row[j] = page; });
+        if (total != 0) {
+            sm.moves.before[threadIdx.x] = before;
+            sm.moves.first[threadIdx.x] = m.held;
+            // those that are granted are the first of those that want any: the words up to the first one that is not
+            const bool all = wanted + total <= have;
+            if (threadIdx.x == 0) sm.moves.before[threads] = all ? total : 0;
+            __syncthreads();
+            if (!all) {
+                if (granted && want) atomicMax(&sm.moves.before[threads], before + want);
+                __syncthreads();
+            }
+            const uint32_t* last = a.free_list + (have - 1 - wanted);
+            move_words(sm.moves, threads, [&](uint32_t, uint32_t, uint32_t j) { return last - j; },
+                       [&](uint32_t q, uint32_t j, uint32_t, uint32_t page) { a.table[(size_t)(base + q) * a.stride + sm.moves.first[q] + j] = page; });
+            __syncthreads();
+        }
+        wanted += total;
+    };
+    if (KEPT) {
+#pragma unroll
+        for (uint32_t k = 0; k < ROUNDS; k++)
+            if (k * threads < a.n) kept_first[k] = first_pass(kept[k], k * threads, kept_before[k], kept_total[k]);
+        have = min(count + given, (uint64_t)a.capacity);
+#pragma unroll
+        for (uint32_t k = 0; k < ROUNDS; k++)
+            if (k * threads < a.n) second_pass(kept[k], k * threads, kept_before[k], kept_total[k]);
+    } else {
+        for (uint32_t base = 0; base < a.n; base += threads) {
+            Mine m = load(base + threadIdx.x);
+            uint64_t before, total;
+            first_pass(m, base, before, total);
+        }
+        have = min(count + given, (uint64_t)a.capacity);
+        ends = 0;
+        for (uint32_t base = 0; base < a.n; base += threads) {
+            Mine m = load(base + threadIdx.x);
+            look(m, base + threadIdx.x, ends);
+            uint64_t total;
+            const uint64_t before = sum_up(m, total);
+            second_pass(m, base, before, total);
         }
     }
 #pragma unroll
@@ -218,6 +274,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_tables_kernel(const __grid
         atomicAdd(&counted[1], (unsigned long long)refused);
         atomicAdd(&counted[2], (unsigned long long)placed);
     }
+    if (KEPT && place_here) {
+#pragma unroll
+        for (uint32_t k = 0; k < ROUNDS; k++)
+            if (k * threads + threadIdx.x < a.n) sm.firsts[k * threads + threadIdx.x + 1] = kept_first[k];
+        if (threadIdx.x == 0) sm.firsts[0] = 0;
+    }
     __syncthreads();  // tables, lengths and starts are read from here on
     if (threadIdx.x == 0) {
         a.free_out[0] = (uint32_t)(have - counted[0]);
@@ -226,7 +288,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) block_tables_kernel(const __grid
         a.free_out[3] = (uint32_t)counted[0];
     }
     if (!place_here) return;
-    for (uint32_t t = threadIdx.x; t < a.tokens; t += threads) place_token(a, t, [&](uint32_t r) { return firsts[r]; });
+    for (uint32_t t = threadIdx.x; t < a.tokens; t += threads) place_token(a, t, [&](uint32_t r) { return sm.firsts[r]; });
 }
 
 __global__ void __launch_bounds__(PLACE_THREADS) place_tokens_kernel(const __grid_constant__ PlanArgs a)
@@ -440,7 +502,7 @@ int launch_kv_block_tables(const LaunchArgs& a)
     if (n == 0 || n > MOST_REQUESTS) return fail_validation(a, "block_tables: groups[0] (requests) must be 1..65536");
     if (tokens == 0) return fail_validation(a, "block_tables: groups[1] (tokens of the step) must be > 0");
     if (p.page < (uint32_t)TILE_TOK || (p.page & (p.page - 1))) return fail_validation(a, "block_tables: page must be a power of two, at least 16 tokens");
-    if (p.stride == 0) return fail_validation(a, "block_tables: the table's stride must be > 0");
+    if (p.stride == 0 || p.stride > MOST_STRIDE) return fail_validation(a, "block_tables: the table's stride must be 1..2097152 pages");
     if (int r = need_aligned(a, {4, 4, 4, 4, 4, 4, 4, 4, 4, 4, 4, 4})) return r;
     const size_t per = 4 * (size_t)n;
     const char* names[12] = {"ctx", "new", "held", "count", "free list", "table", "held out", "free out", "starts", "lens", "slots", "positions"};
@@ -452,8 +514,8 @@ int launch_kv_block_tables(const LaunchArgs& a)
     PlanArgs k{u(0), u(1), u(2), u(3), u(4), u(5), u(6), u(7), u(8), u(9), u(10), u(11), n, tokens, (uint32_t)__builtin_ctz(p.page), p.stride,
                (uint32_t)(capacity < NO_SLOT ? capacity : NO_SLOT), a.status};
     const bool place_here = n <= SEARCHED && tokens <= PLACED_HERE;
-    const uint32_t work = place_here && tokens > n ? tokens : n, threads = work < PLAN_THREADS ? (work + 31) / 32 * 32 : PLAN_THREADS;
-    cudaError_t e = launch_dependent(block_tables_kernel, dim3(1), dim3(threads), 0, a.stream, k, place_here);
+    const uint32_t work = !place_here && n < 256 ? 256 : place_here && tokens > n ? tokens : n, threads = work < PLAN_THREADS ? (work + 31) / 32 * 32 : PLAN_THREADS;
+    cudaError_t e = launch_dependent(n <= KEPT_ROUNDS * threads ? block_tables_kernel<true> : block_tables_kernel<false>, dim3(1), dim3(threads), 0, a.stream, k, place_here);
     ++*a.launches;
     if (int r = check_cuda(a, e, "kv_block_tables")) return r;
     if (place_here) return 0;

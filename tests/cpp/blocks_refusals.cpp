@@ -54,7 +54,8 @@ int main()
         with(plan, [=](Call& c) { c.b[i].ptr = (char*)c.b[i].ptr + 2; }).expect("misaligned", "aligned");
     }
     with(plan, [](Call& c) { c.b[4].bytes = 0; }).expect("empty list", "holds");
-    with(plan, [](Call& c) { c.groups[0] = 65536; c.push[1] = 0xffffffffu; }).expect("table beyond 2^32 bytes", "holds");
+    with(plan, [](Call& c) { c.groups[0] = 65536; c.push[1] = 1u << 21; c.b[0].bytes = c.b[1].bytes = c.b[2].bytes = 1 << 18; }).expect("table beyond 2^32 bytes", "holds");
+    with(plan, [](Call& c) { c.push[1] = (1u << 21) + 1; }).expect("stride", "stride");
 
     // 3 kv heads, 5 tokens, 4 blocks
     const size_t pool = 4 * 3 * 2048;

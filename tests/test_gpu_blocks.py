@@ -75,7 +75,8 @@ def _run_plan(ctx, state, page, tokens, in_place=False):
 
 @pytest.mark.parametrize("requests,page,stride,tokens,in_place", [
     (1, 16, 1, 1, False), (1, 256, 4, 1100, True), (3, 16, 5, 7, False), (33, 32, 9, 400, True), (64, 256, 4, 64, False), (64, 256, 4, 65, True), (1023, 16, 3, 9000, False),
-    (1024, 64, 2, 20000, True), (1025, 16, 7, 30001, True), (3000, 512, 2, 5000, False)])
+    (1024, 64, 2, 20000, True), (1025, 16, 7, 30001, True), (3000, 512, 2, 5000, False),
+    (4096, 16, 3, 4097, True), (4097, 16, 4, 9000, False), (9001, 64, 2, 20000, True)])
 def test_block_tables_match_the_plain_statement(ctx, requests, page, stride, tokens, in_place):
     for seed in range(4):
         state = _plan_state(seed, requests, page, stride, tokens, busy=(0.0, 0.4, 0.9, 1.0)[seed], most_new=min(stride * page, 3 * tokens // requests + 1))
