@@ -155,6 +155,11 @@ public:
     {
         submit_(sgb_dispatch_blocking, k, bindings, push, push ? sizeof(P) : 0, groups);
     }
+    // Bytes of the work binding of attn_blocks_e4m3_d128 for a dispatch of that grid and push.
+    size_t attn_blocks_work_bytes(uint32_t n_kv_heads, uint32_t q_per_kv, uint32_t requests, uint32_t n_tokens, uint32_t max_q) const
+    {
+        return sgb_attn_blocks_work_bytes(c_, n_kv_heads, q_per_kv, requests, n_tokens, max_q);
+    }
     void sync(uint32_t timeout_ms = 0) { check(sgb_sync(c_, timeout_ms)); }
 
     // record_graph (graph.rs:523-528): dispatches made inside `record` are captured, not run.

@@ -131,8 +131,11 @@ uint64_t sgb_launch_count(const sgb_ctx *ctx);
  * (sgb_decode_paged_q8kv_d128_noalloc caps m_q * q_heads * n_splits at 2048: 64 splits for 32 q heads.) */
 uint32_t sgb_decode_paged_splits_hint(const sgb_ctx *ctx, uint32_t n_kv_heads, uint32_t kv_len);
 
-/* Bytes of the `work` binding of attn_blocks_e4m3_d128 for a dispatch of that grid and push (partial results of requests that
- * several warps share; its contents mean nothing between dispatches).  Enough for every smaller grid and max_q as well. */
+/* A batch of requests over one 8-bit cache: kv_block_tables, kv_append_blocks_e4m3_d128 and attn_blocks_e4m3_d128 (no counterpart in
+ * the reference, which serves one sequence).  All lengths are read on the device, so that one recorded step serves every mix of requests
+ * that its buffers hold.  This gives the bytes of the attention's `work` binding for a dispatch of that grid and push: partial
+ * results of requests that several warps or CTAs share.  Its contents mean nothing between dispatches, and one dispatch uses it at
+ * a time.  Enough for every smaller grid and max_q as well.  0 for arguments that the dispatch would refuse. */
 size_t sgb_attn_blocks_work_bytes(const sgb_ctx *ctx, uint32_t n_kv_heads, uint32_t q_per_kv, uint32_t requests, uint32_t n_tokens,
                                   uint32_t max_q);
 

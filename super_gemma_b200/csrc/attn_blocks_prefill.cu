@@ -12,6 +12,11 @@
 // One CTA per SM stays and takes units from a queue (the lengths are known on the device only); one warp fetches the next while the
 // others work.  The units that are left when every CTA has had its whole ones are laid end to end and cut into equal stretches; the CTA
 // that finishes the last piece of a unit merges them, in their order, so reruns give the same bits.
+//
+// Bound by shared memory's port, 192 KB = 1536 cycles per 64 keys and 256 rows (raw bytes in and out 32, f16 tiles 32, operands of Q K^T 96, of
+// P V 32), of the 2000 or so that a tile takes; in long runs by the board's power.  1740 tokens of 65536 keys, 16 kv heads of two query heads:
+// 1840 us, 1.0 PFLOP/s (the f16 kernel reaches 1.05 to 1.1 on cached f16 keys).  128 rows a CTA and two CTAs an SM would convert every key twice
+// as often and need 256 KB of the port.
 #include <mutex>
 
 #include "blocks.cuh"

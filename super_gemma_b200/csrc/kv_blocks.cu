@@ -16,7 +16,8 @@ namespace {
 // refused: they keep what they hold, their length is 0 and their tokens have no slot.
 //
 // Prefix sums over the requests and little else: bound by its own latency.  One CTA does the sums, of up to 1024 requests at a time, and
-// moves the pages; it places the tokens too while there are few of them.
+// moves the pages; it places the tokens too while there are few of them.  64 requests of one token take 4.1 us, 1024 of which an
+// eighth ends and an eighth begins 12, 4000 with prompts 24 (one after the other in a stream).
 constexpr uint32_t PLAN_THREADS = 1024, PLAN_WARPS = PLAN_THREADS / 32;
 constexpr uint32_t PLACE_THREADS = 256;
 constexpr uint32_t MOST_STRIDE = 1u << 21;
@@ -311,7 +312,8 @@ __global__ void __launch_bounds__(PLACE_THREADS) place_tokens_kernel(const __gri
 // warp: A = max |x| over the run's rows, e = the least e >= -15 with A <= 448 * 2^e, no less than the tile's own exponent if
 // the run does not begin the tile; if that grows, the rows before the run are rounded again (q * 2^(old - e)); then the run's rows
 // are written as e4m3(x * 2^-e).  All products are by powers of two and exact in f16 wherever e4m3 does not round them to 0.
-// Two bytes read and one written per value: bound by bytes.
+// Two bytes read and one written per value: bound by bytes.  17 prompts, 21078 tokens of 16 heads, take 47 us (5.5 TB/s), 64 single tokens
+// 4.1, which is a launch and two loads one after the other.
 constexpr int APPEND_THREADS = 256;
 
 struct AppendArgs {
