@@ -321,10 +321,11 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
             const uint32_t row = 2 * t4 + e;
             if (row >= rows) continue;
             if (began && ended) {
-                const float f = l_row[e] != 0.0f ? 1.0f / l_row[e] : 0.0f;
+                const bool saw = l_row[e] != 0.0f;  // a row that saw nothing is 0, whatever stands in V
+                const float f = 1.0f / l_row[e];
                 __half* dst = a.out + ((size_t)(first_tok + (row >> a.group_shift)) * heads + head * a.group + (row & (a.group - 1))) * HD + 2 * g;
 #pragma unroll
-                for (int c = 0; c < 8; c++) *reinterpret_cast<__half2*>(dst + 16 * c) = __floats2half2_rn(o[c][e] * f, o[c][2 + e] * f);
+                for (int c = 0; c < 8; c++) *reinterpret_cast<__half2*>(dst + 16 * c) = saw ? __floats2half2_rn(o[c][e] * f, o[c][2 + e] * f) : __float2half2_rn(0.0f);
             } else {
                 const size_t at = ((size_t)(2 * part + (began ? 1 : 0)) * a.n_kv + head) * work.rows + row;
                 float* dst = reinterpret_cast<float*>(work.acc + at * (HD / 4)) + 2 * g;
@@ -465,8 +466,9 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
     end_request(tile_now);
 }
 
+constexpr uint32_t LISTED = 1024;  // requests whose first units the listing CTA keeps at hand
 constexpr int MANY_CTAS_WARPS = 4;                                          // of the merge
-constexpr int few_ctas_warps(int rows) { return rows == 8 ? 8 : 16; }
+constexpr int FEW_CTAS_WARPS = 16;
 
 // What the prefill kernel takes its items from; by one CTA of the merge.  Units go out with the most keys first, so that what is left at
 // the end is short (24 requests, three of them prompts of 841 to 1281 tokens: 110 us in the requests' order).  All heads of a unit
@@ -485,16 +487,16 @@ __device__ __forceinline__ void list_units(const BlocksAttn& a, const BlocksWork
             if (lane >= (uint32_t)off) up_to += t;
         }
         __syncthreads();
-        if (lane == 31) shared[warp] = up_to;
+        uint32_t* sums = shared + MOST_SORTED + LISTED;
+        if (lane == 31) sums[warp] = up_to;
         __syncthreads();
         uint32_t at = up_to - mine;
         total = 0;
 #pragma unroll
         for (int i = 0; i < MERGE_WARPS; i++) {
-            if (i < (int)warp) at += shared[i];
-            total += shared[i];
+            if (i < (int)warp) at += sums[i];
+            total += sums[i];
         }
-        __syncthreads();
         return at;
     };
     const uint32_t per_thread = (a.req.n + N - 1) / N, r_begin = min(tid * per_thread, a.req.n), r_end = min(r_begin + per_thread, a.req.n);
@@ -519,19 +521,30 @@ __device__ __forceinline__ void list_units(const BlocksAttn& a, const BlocksWork
     }
     for (uint32_t i = tid; i < 2 * w.places; i += N) w.done[i] = 0;
     __syncthreads();
-    const auto locate = [&](uint32_t u) {  // the last request with units_before <= u
+    // The request of a unit: the last one with units_before <= u.  At hand where the requests fit.
+    uint32_t* firsts = shared + MOST_SORTED;
+    const bool at_hand = a.req.n <= LISTED;
+    if (at_hand) {
+        for (uint32_t r = tid; r < a.req.n; r += N) firsts[r] = ld_global(w.units_before + r);
+        __syncthreads();
+    }
+    const auto locate = [&](uint32_t u) -> uint2 {
         uint32_t lo = 0, hi = a.req.n;
+        const auto before = [&](uint32_t r) { return at_hand ? firsts[r] : ld_global(w.units_before + r); };
         while (hi - lo > 1) {
             const uint32_t mid = (lo + hi) >> 1;
-            if (ld_global(w.units_before + mid) <= u) lo = mid; else hi = mid;
+            if (before(mid) <= u) lo = mid; else hi = mid;
         }
-        return unit_at(a, lo, u - ld_global(w.units_before + lo));
+        return make_uint2(lo, u - before(lo));
     };
     const bool sorted = total <= MOST_SORTED;
     if (sorted) {  // bitonic, by tiles of keys and then by number: the same order every time
         uint32_t n = 1;
         while (n < total) n <<= 1;
-        for (uint32_t u = tid; u < n; u += N) shared[u] = u < total ? (min((uint32_t)locate(u).n_tiles, (1u << 20) - 1) + 1) << 11 | u : 0;
+        for (uint32_t u = tid; u < n; u += N) {
+            const uint2 at = u < total ? locate(u) : make_uint2(0, 0);
+            shared[u] = u < total ? (min((uint32_t)unit_at(a, at.x, at.y).n_tiles, (1u << 20) - 1) + 1) << 11 | u : 0;
+        }
         for (uint32_t k = 2; k <= n; k <<= 1)
             for (uint32_t j = k >> 1; j > 0; j >>= 1) {
                 __syncthreads();
@@ -544,17 +557,22 @@ __device__ __forceinline__ void list_units(const BlocksAttn& a, const BlocksWork
                 }
             }
         __syncthreads();
-        for (uint32_t i = tid; i < total; i += N) w.order[i] = shared[i] & (MOST_SORTED - 1);
-        __syncthreads();
+        for (uint32_t i = tid; i < total; i += N) w.order[i] = locate(shared[i] & (MOST_SORTED - 1));
     }
     const uint32_t items = total * a.n_kv, whole = whole_items(items, w.places);
     uint32_t all_tiles = 0;
     for (uint32_t base = 0; base < w.places; base += N) {  // fewer than places are left
         uint32_t tiles = 0, more;
         if (whole + base + tid < items) {
-            uint32_t head, rank;
+            uint32_t head, rank, u;
             split_item(whole + base + tid, total, a.n_kv, by_head, head, rank);
-            tiles = (uint32_t)max(1, locate(sorted ? ld_global(w.order + rank) : total - 1 - rank).n_tiles);  // one without a key counts for its rows
+            u = total - 1 - rank;
+            if (sorted) u = shared[rank] & (MOST_SORTED - 1), tiles = (shared[rank] >> 11) - 1;
+            if (!sorted || tiles == (1u << 20) - 1) {
+                const uint2 at = locate(u);
+                tiles = (uint32_t)unit_at(a, at.x, at.y).n_tiles;
+            }
+            tiles = max(tiles, 1u);  // one without a key counts for its rows
         }
         const uint32_t before = all_tiles + scan(tiles, more);
         if (base + tid < w.places) w.rest[base + tid] = before;
@@ -564,17 +582,19 @@ __device__ __forceinline__ void list_units(const BlocksAttn& a, const BlocksWork
 }
 
 // One CTA per request and kv head: nothing to do where one warp had all its tiles; zeros where it had none; else the warps' parts.
-// Warp x of W takes parts x, x + W, ... of all rows, lane k the (m, l) of its k-th part, so that those and the first parts come in one
-// round of loads; maxima and sums of the warps meet in shared memory, in the warps' order.
-template <int ROWS, int W>
-__global__ void __launch_bounds__(W * 32, W != MANY_CTAS_WARPS ? 1 : ROWS == 8 ? 4 : 8) blocks_merge_kernel(const __grid_constant__ BlocksAttn a, const __grid_constant__ Work work)
+// Warp x of W takes parts x, x + W, ...  Row and part are spread over its lanes for (m, l), and over the E sums of four dims that a lane keeps
+// for O, so that few rows go through several parts at a time; maxima and sums of the warps meet in shared memory, in a fixed order.
+// SHIFT: rows up to this power of two in all requests, or -1: each request's own (a dispatch that has prompts as well knows no more than eight).
+template <int E, int W, int SHIFT>
+__global__ void __launch_bounds__(W * 32, W == MANY_CTAS_WARPS ? (E == 8 ? 4 : 8) : SHIFT < 0 ? 2 : 1) blocks_merge_kernel(const __grid_constant__ BlocksAttn a, const __grid_constant__ Work work)
 {
+    constexpr int LEFT = SHIFT >= 0 ? 1 << SHIFT : E;  // sums that a lane leaves: one a row, where the rows are known beforehand
     __shared__ union {
         struct {
-            float4 acc[W][ROWS][32];
-            float big[W][ROWS], den[W][ROWS];
+            float4 acc[W][LEFT][32];
+            float big[W][8], den[W][8];
         } of;
-        uint32_t sort[MOST_SORTED];
+        uint32_t sort[MOST_SORTED + LISTED + W];
     } sm;
     pdl_wait();
     pdl_launch_dependents();
@@ -602,94 +622,75 @@ __global__ void __launch_bounds__(W * 32, W != MANY_CTAS_WARPS ? 1 : ROWS == 8 ?
         for (uint32_t row = warp; row < rows; row += W) *out(row) = make_uint2(0u, 0u);
         return;
     }
+    const uint32_t shift = SHIFT >= 0 ? SHIFT : rows <= 1 ? 0 : rows <= 2 ? 1 : rows <= 4 ? 2 : 3, mask = (1u << shift) - 1;  // rows up to a power of two
     const auto slot = [&](uint32_t j) { return ((size_t)(2 * (p0 + j) + (j == 0 ? 1 : 0)) * a.n_kv + head) * work.rows; };
-    constexpr int BATCH = W == MANY_CTAS_WARPS ? (ROWS <= 2 ? 4 / ROWS : 1) : 8 / ROWS;  // parts asked for at a time
-    float4 v[BATCH][ROWS], acc[ROWS];
-    float2 ml[ROWS];
-    float big[ROWS], den[ROWS];
+    const uint32_t batch = E >> shift, chunk = 32 >> shift;  // parts that a lane's sums go through at a time, parts whose (m, l) the lanes hold
+    float4 v[E], acc[E];
     const auto fetch = [&](uint32_t k) {  // this warp's parts k ..
 #pragma unroll
-        for (int x = 0; x < BATCH; x++) {
-            const size_t s = slot(min(warp + (k + x) * W, n - 1));
-#pragma unroll
-            for (int i = 0; i < ROWS; i++) v[x][i] = ld_global(work.acc + (s + min((uint32_t)i, rows - 1)) * (HD / 4) + lane);
-        }
+        for (int e = 0; e < E; e++) v[e] = ld_global(work.acc + (slot(min(warp + (k + (e >> shift)) * W, n - 1)) + min(e & mask, rows - 1)) * (HD / 4) + lane);
     };
-    const auto fetch_ml = [&](uint32_t k) {
-        const size_t s = slot(min(warp + (k + lane) * W, n - 1));
-#pragma unroll
-        for (int i = 0; i < ROWS; i++) ml[i] = ld_global(work.ml + s + min((uint32_t)i, rows - 1));
-    };
-    fetch_ml(0);
+    const auto fetch_ml = [&](uint32_t k) { return ld_global(work.ml + slot(min(warp + (k + (lane >> shift)) * W, n - 1)) + min(lane & mask, rows - 1)); };
+    float2 ml = fetch_ml(0);  // (parts past the end are the last one again)
     fetch(0);
+    float big = ml.x, den = 0.0f;
+    for (uint32_t k = chunk; warp + k * W < n; k += chunk) big = fmaxf(big, fetch_ml(k).x);
 #pragma unroll
-    for (int i = 0; i < ROWS; i++) {
-        big[i] = ml[i].x;  // (parts past the end are the last one again)
-        den[i] = 0.0f;
-        acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    }
-    for (uint32_t k = 32; warp + k * W < n; k += 32) {
-        fetch_ml(k);
-#pragma unroll
-        for (int i = 0; i < ROWS; i++) big[i] = fmaxf(big[i], ml[i].x);
-    }
-    if (32 * W < n) fetch_ml(0);
-#pragma unroll
-    for (int i = 0; i < ROWS; i++) {
-#pragma unroll
-        for (int off = 16; off; off >>= 1) big[i] = fmaxf(big[i], __shfl_xor_sync(0xffffffffu, big[i], off));
-        if (lane == 0) sm.of.big[warp][i] = big[i];
-    }
+    for (uint32_t off = 16; off; off >>= 1)
+        if (off > mask) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, off));
+    if (lane <= mask) sm.of.big[warp][lane] = big;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < ROWS; i++)
+    for (int x = 0; x < W; x++) big = fmaxf(big, sm.of.big[x][lane & mask]);
 #pragma unroll
-        for (int x = 0; x < W; x++) big[i] = fmaxf(big[i], sm.of.big[x][i]);
-    for (uint32_t k0 = 0; warp + k0 * W < n; k0 += 32) {
-        if (k0) fetch_ml(k0), fetch(k0);
-        float w[ROWS];
+    for (int e = 0; e < E; e++) acc[e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (uint32_t k0 = 0; warp + k0 * W < n; k0 += chunk) {
+        if (k0) ml = fetch_ml(k0), fetch(k0);
+        const float w = warp + (k0 + (lane >> shift)) * W < n ? ex2(ml.x - big) : 0.0f;
+        den = fmaf(w, ml.y, den);
+        for (uint32_t k = 0;; k += batch) {
 #pragma unroll
-        for (int i = 0; i < ROWS; i++) {
-            w[i] = warp + (k0 + lane) * W < n ? ex2(ml[i].x - big[i]) : 0.0f;
-            den[i] = fmaf(w[i], ml[i].y, den[i]);
-        }
-        for (uint32_t k = 0;; k += BATCH) {
-#pragma unroll
-            for (int x = 0; x < BATCH; x++)
-#pragma unroll
-                for (int i = 0; i < ROWS; i++) {
-                    const float f = __shfl_sync(0xffffffffu, w[i], k + x);  // 0 past the end
-                    acc[i].x = fmaf(f, v[x][i].x, acc[i].x);
-                    acc[i].y = fmaf(f, v[x][i].y, acc[i].y);
-                    acc[i].z = fmaf(f, v[x][i].z, acc[i].z);
-                    acc[i].w = fmaf(f, v[x][i].w, acc[i].w);
-                }
-            if (k + BATCH >= 32 || warp + (k0 + k + BATCH) * W >= n) break;
-            fetch(k0 + k + BATCH);
+            for (int e = 0; e < E; e++) {
+                const float f = __shfl_sync(0xffffffffu, w, ((k + (e >> shift)) << shift) + (e & mask));  // 0 past the end
+                acc[e].x = fmaf(f, v[e].x, acc[e].x);
+                acc[e].y = fmaf(f, v[e].y, acc[e].y);
+                acc[e].z = fmaf(f, v[e].z, acc[e].z);
+                acc[e].w = fmaf(f, v[e].w, acc[e].w);
+            }
+            if (k + batch >= chunk || warp + (k0 + k + batch) * W >= n) break;
+            fetch(k0 + k + batch);
         }
     }
 #pragma unroll
-    for (int i = 0; i < ROWS; i++) {
+    for (uint32_t off = 16; off; off >>= 1)
+        if (off > mask) den += __shfl_xor_sync(0xffffffffu, den, off);
+    if (lane <= mask) sm.of.den[warp][lane] = den;
 #pragma unroll
-        for (int off = 16; off; off >>= 1) den[i] += __shfl_xor_sync(0xffffffffu, den[i], off);
-        sm.of.acc[warp][i][lane] = acc[i];
-        if (lane == 0) sm.of.den[warp][i] = den[i];
+    for (int e = LEFT; e < E; e++) {
+        float4& to = acc[e % LEFT];
+        to.x += acc[e].x;
+        to.y += acc[e].y;
+        to.z += acc[e].z;
+        to.w += acc[e].w;
     }
+#pragma unroll
+    for (int e = 0; e < LEFT; e++) sm.of.acc[warp][e][lane] = acc[e];
     __syncthreads();
     for (uint32_t row = warp; row < rows; row += W) {
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         float l = 0.0f;
-#pragma unroll
         for (int x = 0; x < W; x++) {
-            const float4 o = sm.of.acc[x][row][lane];
-            sum.x += o.x;
-            sum.y += o.y;
-            sum.z += o.z;
-            sum.w += o.w;
             l += sm.of.den[x][row];
+            for (uint32_t e = row; e < LEFT; e += mask + 1) {
+                const float4 o = sm.of.acc[x][e][lane];
+                sum.x += o.x;
+                sum.y += o.y;
+                sum.z += o.z;
+                sum.w += o.w;
+            }
         }
-        const float f = l != 0.0f ? 1.0f / l : 0.0f;
-        *out(row) = make_uint2(pack_half2(sum.x * f, sum.y * f), pack_half2(sum.z * f, sum.w * f));
+        const float f = 1.0f / l;  // a row that saw nothing is 0, whatever stands in V
+        *out(row) = l != 0.0f ? make_uint2(pack_half2(sum.x * f, sum.y * f), pack_half2(sum.z * f, sum.w * f)) : make_uint2(0u, 0u);
     }
 }
 
@@ -736,13 +737,13 @@ int launch_blocks_decode(const LaunchArgs& a, const BlocksAttn& k, const BlocksW
     // Few CTAs have many parts each (one request of 131072 keys: 148 of every head; 9.4 us with four warps a CTA).
     const bool few = (uint64_t)k.req.n * k.n_kv <= 2u * (uint32_t)a.sm_count;
     const dim3 grid(k.req.n + (k.req.max_q > FEW_ROWS / k.group ? 1 : 0), k.n_kv);
-    const auto merge = [&](auto rows) {
-        constexpr int ROWS = decltype(rows)::value, FEW = few_ctas_warps(ROWS);
-        return few ? launch_dependent(blocks_merge_kernel<ROWS, FEW>, grid, dim3(FEW * 32), 0, a.stream, k, w)
-                   : launch_dependent(blocks_merge_kernel<ROWS, MANY_CTAS_WARPS>, grid, dim3(MANY_CTAS_WARPS * 32), 0, a.stream, k, w);
+    const auto merge = [&](auto shift) {
+        constexpr int SHIFT = decltype(shift)::value, WARPS_IF_FEW = SHIFT < 0 ? FEW_CTAS_WARPS / 2 : FEW_CTAS_WARPS;
+        return few ? launch_dependent(blocks_merge_kernel<8, WARPS_IF_FEW, SHIFT>, grid, dim3(WARPS_IF_FEW * 32), 0, a.stream, k, w)
+                   : launch_dependent(blocks_merge_kernel<SHIFT < 0 ? 8 : 4, MANY_CTAS_WARPS, SHIFT>, grid, dim3(MANY_CTAS_WARPS * 32), 0, a.stream, k, w);
     };
-    e = w.rows <= 1 ? merge(std::integral_constant<int, 1>()) : w.rows <= 2 ? merge(std::integral_constant<int, 2>())
-        : w.rows <= 4 ? merge(std::integral_constant<int, 4>()) : merge(std::integral_constant<int, 8>());
+    e = w.rows <= 1 ? merge(std::integral_constant<int, 0>()) : w.rows <= 2 ? merge(std::integral_constant<int, 1>())
+        : w.rows <= 4 ? merge(std::integral_constant<int, 2>()) : merge(std::integral_constant<int, -1>());
     ++*a.launches;
     return check_cuda(a, e, "attn_blocks merge");
 }

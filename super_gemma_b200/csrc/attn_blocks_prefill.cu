@@ -78,7 +78,7 @@ template <uint32_t N> __device__ __forceinline__ void regs_down() { asm volatile
 // Takes items from the queue; by a whole warp, which keeps what is left of its stretch.
 struct Feed {
     uint32_t total, items, whole, stretches, rest_tiles;
-    bool by_head, sorted;
+    bool by_head, sorted, opened = false;
     uint32_t at = 0, end = 0, stretch = 0, next_unit = 0;  // of the stretch: tiles of the cut units that are still to do, the unit that they begin in
 };
 __device__ __forceinline__ uint32_t stretch_of_tile(const Feed& f, uint32_t tile) { return (uint32_t)((((uint64_t)tile + 1) * f.stretches - 1) / f.rest_tiles); }
@@ -120,8 +120,13 @@ __device__ __forceinline__ void fetch_item(const BlocksAttn& a, const BlocksWork
             it.counter = rest;
             break;
         }
-        if (lane == 0) i = atomicAdd(w.queue, 1u);
-        i = __shfl_sync(0xffffffffu, i, 0);
+        if (f.opened) {
+            if (lane == 0) i = gridDim.x + atomicAdd(w.queue, 1u);
+            i = __shfl_sync(0xffffffffu, i, 0);
+        } else {  // every CTA's first is its own
+            i = blockIdx.x;
+            f.opened = true;
+        }
         if (i < f.whole) break;
         i -= f.whole;
         if (i >= f.stretches) {
@@ -141,18 +146,24 @@ __device__ __forceinline__ void fetch_item(const BlocksAttn& a, const BlocksWork
     }
     uint32_t head, rank;
     split_item(i, f.total, a.n_kv, f.by_head, head, rank);
-    const uint32_t u = f.sorted ? ld_global(w.order + rank) : f.total - 1 - rank;
-    uint32_t lo = 0, left = a.req.n;  // the request: the last one with units_before <= u
-    while (left > 1) {
-        const uint32_t step = (left + 31) / 32, probe = lo + lane * step;
-        const bool at_or_before = lane * step < left && ld_global(w.units_before + probe) <= u;
-        const uint32_t k = 31 - __clz(__ballot_sync(0xffffffffu, at_or_before));  // lane 0 always is
-        lo += k * step;
-        left = min(step, left - k * step);
+    uint2 place;
+    if (f.sorted) {
+        place = ld_global(w.order + rank);
+    } else {  // the request of a unit: the last one with units_before <= u
+        const uint32_t u = f.total - 1 - rank;
+        uint32_t lo = 0, left = a.req.n;
+        while (left > 1) {
+            const uint32_t step = (left + 31) / 32, probe = lo + lane * step;
+            const bool at_or_before = lane * step < left && ld_global(w.units_before + probe) <= u;
+            const uint32_t k = 31 - __clz(__ballot_sync(0xffffffffu, at_or_before));  // lane 0 always is
+            lo += k * step;
+            left = min(step, left - k * step);
+        }
+        place = make_uint2(lo, u - ld_global(w.units_before + lo));
     }
-    const Unit unit = unit_at(a, lo, u - ld_global(w.units_before + lo));
+    const Unit unit = unit_at(a, place.x, place.y);
     it.valid = 1;
-    it.request = lo;
+    it.request = place.x;
     it.head = head;
     it.first_tok = unit.first_tok;
     it.toks = unit.toks;
@@ -638,7 +649,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         }
 #pragma unroll
                         for (int x = 0; x < 2; x++)
-                            *reinterpret_cast<uint4*>(orow + 16 * c + 8 * x) =
+                            *reinterpret_cast<uint4*>(orow + 16 * c + 8 * x) = den == 0.0f ? make_uint4(0u, 0u, 0u, 0u) :
                                 make_uint4(pack_half2(acc[2 * x].x, acc[2 * x].y), pack_half2(acc[2 * x].z, acc[2 * x].w), pack_half2(acc[2 * x + 1].x, acc[2 * x + 1].y),
                                            pack_half2(acc[2 * x + 1].z, acc[2 * x + 1].w));
                     }

@@ -1,7 +1,7 @@
 // The work buffer of attn_blocks_e4m3_d128: what the first of its kernels leaves the others, and partial results.
 //   u64 before[n + 2]        weight of the decoded requests before each (its 16-token tiles and one more), their total, the most stretches of a kv head
+//   u32 order[2048][2]       the units of a kv head, request and number in it, those with the most keys first (only if there are no more than that)
 //   u32 units_before[n + 1]  units (256 rows) of the prefilled requests before each, their total
-//   u32 order[2048]          the units of a kv head, those with the most keys first (only if there are no more than that)
 //   u32 rest[places + 1]     tiles of 64 keys before each of the units that are cut, their total
 //   u32 done[2 * places]     finished pieces of each unit that is cut, of either half of it
 //   u32 queue, by_head       the prefill's next item; whether a head's units stand together
@@ -17,7 +17,9 @@ constexpr uint32_t MOST_SORTED = 2048, MOST_PLACES = 256;
 
 struct BlocksWork {
     uint64_t* before;
-    uint32_t *units_before, *order, *rest, *done, *queue, *by_head;
+    uint32_t *units_before;
+    uint2* order;
+    uint32_t *rest, *done, *queue, *by_head;
     uint32_t places;
     uint8_t* parts;
 };
@@ -56,15 +58,15 @@ __device__ __forceinline__ uint32_t rest_stretches(uint32_t tiles, uint32_t plac
 inline uint32_t blocks_places(int sm_count) { return (uint32_t)sm_count < MOST_PLACES ? (uint32_t)sm_count : MOST_PLACES; }
 inline size_t blocks_work_header(uint32_t requests, uint32_t places)
 {
-    return ((size_t)(requests + 2) * 8 + ((size_t)requests + 1 + MOST_SORTED + 3 * places + 3) * 4 + 255) / 256 * 256;
+    return ((size_t)(requests + 2) * 8 + ((size_t)requests + 1 + 2 * MOST_SORTED + 3 * places + 3) * 4 + 255) / 256 * 256;
 }
 inline BlocksWork blocks_work_at(uint8_t* p, uint32_t requests, uint32_t places)
 {
     BlocksWork w;
     w.before = reinterpret_cast<uint64_t*>(p);
-    w.units_before = reinterpret_cast<uint32_t*>(w.before + requests + 2);
-    w.order = w.units_before + requests + 1;
-    w.rest = w.order + MOST_SORTED;
+    w.order = reinterpret_cast<uint2*>(w.before + requests + 2);
+    w.units_before = reinterpret_cast<uint32_t*>(w.order + MOST_SORTED);
+    w.rest = w.units_before + requests + 1;
     w.done = w.rest + places + 1;
     w.queue = w.done + 2 * places;
     w.by_head = w.queue + 1;
