@@ -89,7 +89,7 @@ __device__ __forceinline__ Feed open_feed(const BlocksAttn& a, const BlocksWork&
     f.items = f.total * a.n_kv;
     f.whole = whole_items(f.items, w.places);
     f.rest_tiles = ld_global(w.rest + w.places);
-    f.stretches = rest_stretches(f.rest_tiles, w.places);
+    f.stretches = rest_stretches(f.rest_tiles, f.items - f.whole, w.places);
     f.by_head = ld_global(w.by_head) != 0;
     f.sorted = f.total <= MOST_SORTED;
     return f;

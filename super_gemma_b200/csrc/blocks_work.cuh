@@ -51,9 +51,10 @@ __device__ __forceinline__ void split_item(uint32_t i, uint32_t total, uint32_t 
     rank = by_head ? i % total : i / n_kv;
 }
 // The first `whole` items go to the places one by one.  Those left over, fewer than there are places, are laid end to end and cut
-// into equal stretches, one per place, of eight tiles at least.
+// into equal stretches, one per place, of eight tiles at least unless that were fewer stretches than units: a unit has its start and its end to
+// pay for (four units of two tiles in one stretch: the last CTA ended 6 us after the others).
 __device__ __forceinline__ uint32_t whole_items(uint32_t items, uint32_t places) { return items / places * places; }
-__device__ __forceinline__ uint32_t rest_stretches(uint32_t tiles, uint32_t places) { return min((tiles + 7) / 8, places); }
+__device__ __forceinline__ uint32_t rest_stretches(uint32_t tiles, uint32_t units, uint32_t places) { return min(max((tiles + 7) / 8, units), places); }
 
 inline uint32_t blocks_places(int sm_count) { return (uint32_t)sm_count < MOST_PLACES ? (uint32_t)sm_count : MOST_PLACES; }
 inline size_t blocks_work_header(uint32_t requests, uint32_t places)
