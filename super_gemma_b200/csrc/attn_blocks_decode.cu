@@ -509,10 +509,19 @@ __device__ __forceinline__ void list_units(const BlocksAttn& a, const BlocksWork
     });
     uint32_t at = scan(mine, total);
     scan(kilokeys, all_kilokeys);
-    for_requests(a.req, r_begin, r_end, [&](uint32_t r, const Request& q) {
+    // At hand where the requests fit: what a unit's request is looked up in.
+    uint32_t* firsts = shared + MOST_SORTED;
+    const bool at_hand = a.req.n <= LISTED;
+    const auto note = [&](uint32_t r, uint32_t n) {
+        if (at_hand) firsts[r] = at;
         w.units_before[r] = at;
-        at += units(q);
-    });
+        at += n;
+    };
+    if (per_thread == 1) {
+        if (r_begin < r_end) note(r_begin, mine);
+    } else {
+        for_requests(a.req, r_begin, r_end, [&](uint32_t r, const Request& q) { note(r, units(q)); });
+    }
     const bool by_head = (uint64_t)all_kilokeys * 1024 * a.n_kv * 2 * HD > ((uint64_t)96 << 20);
     if (tid == 0) {
         w.units_before[a.req.n] = total;
@@ -521,13 +530,7 @@ __device__ __forceinline__ void list_units(const BlocksAttn& a, const BlocksWork
     }
     for (uint32_t i = tid; i < 2 * w.places; i += N) w.done[i] = 0;
     __syncthreads();
-    // The request of a unit: the last one with units_before <= u.  At hand where the requests fit.
-    uint32_t* firsts = shared + MOST_SORTED;
-    const bool at_hand = a.req.n <= LISTED;
-    if (at_hand) {
-        for (uint32_t r = tid; r < a.req.n; r += N) firsts[r] = ld_global(w.units_before + r);
-        __syncthreads();
-    }
+    // The request of a unit, the last one with units_before <= u, and its number there.
     const auto locate = [&](uint32_t u) -> uint2 {
         uint32_t lo = 0, hi = a.req.n;
         const auto before = [&](uint32_t r) { return at_hand ? firsts[r] : ld_global(w.units_before + r); };
