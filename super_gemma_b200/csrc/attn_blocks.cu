@@ -4,8 +4,8 @@
 // position lens[r] - n_r + i and sees the keys up to its own position, of those the last `window` if there is one.  A row that
 // sees nothing (a request that was refused: its length is 0) is zero.  Output f16.
 //
-// Requests of at most eight rows (query tokens x heads of a group) are decoded (attn_blocks_decode.cu), the others prefilled
-// (attn_blocks_prefill.cu); a dispatch that names no request as long as that launches the decode alone.
+// Requests of few rows (query tokens x heads of a group) are decoded (attn_blocks_decode.cu), the others prefilled
+// (attn_blocks_prefill.cu); a dispatch that names no request of more than 16 rows launches the decode alone.
 #include <cmath>
 
 #include "blocks.cuh"
@@ -21,11 +21,19 @@ struct PushAttnBlocks {
     uint32_t page, stride, window, group, max_q;
 };
 
+// Rows up to which a request is decoded: 8 or 16, as the most that the dispatch names need, and 8 beside prompts, for the single tokens' sake.
+// (16 drafts of 2 to 4 tokens, four heads a group, up to 32768 keys: 98 us, as prompts 160; of two heads, 4 to 8 tokens 186 and 256.)
+uint32_t rows_decoded(uint32_t group, uint32_t max_q)
+{
+    const uint64_t rows = (uint64_t)group * max_q;
+    return rows <= 8 || rows > FEW_ROWS ? 8 : 16;
+}
+
 }  // namespace
 
 size_t attn_blocks_work_bytes(int sm_count, uint32_t n_kv, uint32_t group, uint32_t requests, uint32_t tokens, uint32_t max_q)
 {
-    if (n_kv == 0 || group == 0 || group > FEW_ROWS || requests == 0 || tokens == 0 || max_q == 0) return 0;
+    if (n_kv == 0 || group == 0 || group > 8 || requests == 0 || tokens == 0 || max_q == 0) return 0;
     const size_t few = blocks_decode_work(sm_count, n_kv, group, max_q);
     const size_t many = (uint64_t)max_q * group > FEW_ROWS ? blocks_prefill_work(sm_count) : 0;
     return blocks_work_header(requests, blocks_places(sm_count)) + (few > many ? few : many);
@@ -64,7 +72,7 @@ int launch_attn_blocks(const LaunchArgs& a)
     const BlocksAttn k{{(const uint32_t*)a.b[5].ptr, (const uint32_t*)a.b[6].ptr, (const uint32_t*)a.b[7].ptr, n, p.stride, shift,
                         (uint32_t)(blocks >> (shift - 4)), tokens, p.max_q, p.window, a.status},
                        (const __half*)a.b[0].ptr, {(const uint8_t*)a.b[1].ptr, (const uint8_t*)a.b[3].ptr}, {(const int8_t*)a.b[2].ptr, (const int8_t*)a.b[4].ptr},
-                       (__half*)a.b[8].ptr, n_kv, p.group, (uint32_t)__builtin_ctz(p.group), (uint32_t)(blocks * n_kv), p.scale};
+                       (__half*)a.b[8].ptr, n_kv, p.group, (uint32_t)__builtin_ctz(p.group), (uint32_t)(blocks * n_kv), rows_decoded(p.group, p.max_q) / p.group, p.scale};
     const BlocksWork work = blocks_work_at((uint8_t*)a.b[9].ptr, n, blocks_places(a.sm_count));
     if (int r = launch_blocks_decode(a, k, work)) return r;
     return (uint64_t)p.max_q * p.group > FEW_ROWS ? launch_blocks_prefill(a, k, work) : 0;

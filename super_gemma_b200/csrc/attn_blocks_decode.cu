@@ -26,7 +26,7 @@ namespace sgb {
 namespace {
 
 constexpr int HD = 128;
-constexpr int WARPS = 4, CTAS_PER_SM = 4, STAGES = 3;
+constexpr int WARPS = 4;
 constexpr uint32_t LEAST_TILES = 2;  // of a stretch: fewer would only mean more to merge (one request of 1000 keys: 12.3 us with 4, 10.3 with 2 and with 1)
 // A request weighs a tile more than it has: its queries to fetch, its result to write.  (256 requests of 17 to 2048 keys: a warp whose
 // stretch was of many short ones ended 11 of 52 us after the median one.)
@@ -38,11 +38,20 @@ constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES;
 struct Met {
     uint32_t request, first, n, len, lo, tiles;
 };
-constexpr int MET = 4;  // STAGES tiles under way are of three requests at most
 static_assert(REQUEST_WEIGHT == 1, "a stretch that begins within a request's own weight begins with it");
-static_assert(MET > STAGES, "a request is not overwritten before its last tile");
 
+// What NB blocks of eight query rows take: O alone is 32 NB registers a thread, so three CTAs of 168 registers stand on an SM for two blocks.
+// Their queries, another 32, are kept in shared memory, every lane's own beside each other.  (Four blocks: eight warps on an SM cannot hide
+// their own latency; 16 drafts of 2 to 4 tokens of eight heads a group 187 us, as prompts 97.)
+template <int NB> struct Shape {
+    static constexpr int CTAS_PER_SM = NB == 1 ? 4 : 3, STAGES = 3;
+    static constexpr int MET = 4;  // STAGES tiles under way are of three requests at most
+    static constexpr bool Q_SHARED = NB > 1;
+    static_assert(MET > STAGES, "a request is not overwritten before its last tile");
+};
+template <int NB>
 struct __align__(1024) DecodeSmem {
+    static constexpr int STAGES = Shape<NB>::STAGES, MET = Shape<NB>::MET;
     uint8_t k[WARPS][STAGES][TILE_BYTES];  // 128-byte swizzled by TMA
     uint8_t v[WARPS][STAGES][TILE_BYTES];
     uint64_t full[WARPS][STAGES];
@@ -50,6 +59,7 @@ struct __align__(1024) DecodeSmem {
     Met met[WARPS][MET];  // the last requests that a warp's copies have come to
     uint32_t from[WARPS]; // weight of a stretch's first request that lies before it
     uint32_t begun[WARPS][2];  // requests that begin before a stretch, before its end
+    uint2 q[Shape<NB>::Q_SHARED ? WARPS : 1][Shape<NB>::Q_SHARED ? 8 * NB : 1][32];
 };
 
 // Parts: (m, l) and O of [slot][kv head][row].  A stretch p has slot 2p for the request that it goes on with and 2p + 1 for
@@ -60,9 +70,9 @@ struct Work {
     float4* acc;
     uint32_t rows;
 };
-__host__ __device__ __forceinline__ uint32_t few_rows(uint32_t group, uint32_t max_q)
+inline uint32_t part_rows(uint32_t most_rows, uint32_t group, uint32_t max_q)
 {
-    const uint32_t tokens = FEW_ROWS / group;
+    const uint32_t tokens = most_rows / group;
     return group * (max_q < tokens ? max_q : tokens);
 }
 
@@ -107,7 +117,7 @@ struct Tiles {
 };
 __device__ __forceinline__ Tiles tiles_of(const BlocksAttn& a, const Request& q)
 {
-    if (q.n == 0 || q.n > (FEW_ROWS >> a.group_shift) || q.len == 0) return Tiles{0, 0};
+    if (q.n == 0 || q.n > a.few || q.len == 0) return Tiles{0, 0};
     const int64_t from = (int64_t)q.len - q.n + 1 - a.req.window;
     const uint32_t lo = a.req.window != 0 && from > 0 ? (uint32_t)from / TILE_TOK : 0;
     return Tiles{lo, (q.len + TILE_TOK - 1) / TILE_TOK - lo};
@@ -136,11 +146,14 @@ __device__ __forceinline__ Stretches stretches_for(uint64_t total, uint32_t most
     return s;
 }
 
-__global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
+template <int NB>
+__global__ void __launch_bounds__(WARPS * 32, Shape<NB>::CTAS_PER_SM)
     blocks_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ BlocksAttn a, const __grid_constant__ Work work, uint32_t most)
 {
+    constexpr int STAGES = Shape<NB>::STAGES, MET = Shape<NB>::MET;
+    constexpr bool Q_SHARED = Shape<NB>::Q_SHARED;
     extern __shared__ uint8_t smem_raw[];
-    DecodeSmem& sm = *reinterpret_cast<DecodeSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    DecodeSmem<NB>& sm = *reinterpret_cast<DecodeSmem<NB>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     if (lane == 0) {
         tma_prefetch_desc(&tm_k);
@@ -276,12 +289,14 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
         }
     };
     // ---- the arithmetic's side ------------------------------------------------------------------------------------------------------
-    // A lane supplies Q for query row g (B operand) and owns the accumulators of rows 2 t4 and 2 t4 + 1.  Row = token * group + head.
+    // Of every block of eight rows a lane supplies Q for row g (B operand) and owns the accumulators of rows 2 t4 and 2 t4 + 1.
+    // Row = token * group + head.
     const uint32_t heads = a.n_kv * a.group;
-    uint32_t qb[8][2];
-    float o[8][4], m_run[2], l_part[2];
+    uint2 qb[Q_SHARED ? 1 : NB][8];
+    float o[NB][8][4], m_run[NB][2], l_part[NB][2];
     uint32_t r_now = 0, rows = 0, first_tok = 0, tile_first = 0, tile_begin = 0, tile_end = 0;
-    int hi_row[2] = {0, 0}, lo_row[2] = {0, 0}, lo_all = 0, hi_all = 0, lo_any = 0, hi_any = 0;  // keys that a row, all rows, any row sees
+    int pos0 = 0, len = 0, lo_all = 0, lo_any = 0;  // position of the first query; the first keys that all rows, that any row sees
+    const int window = a.req.window && a.req.window < MOST_KEYS ? (int)a.req.window : (int)MOST_KEYS;
     auto begin_request = [&](uint32_t nth, uint32_t tile) {
         __syncwarp();  // lane 0 left it there
         const Met rq = sm.met[warp][nth % MET];
@@ -291,47 +306,53 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
         tile_first = tile;
         tile_begin = rq.lo;
         tile_end = rq.lo + rq.tiles;
-        const __half* qrow = a.q + ((size_t)(rq.first + (g >> a.group_shift)) * heads + head * a.group + (g & (a.group - 1))) * HD + 4 * t4;
 #pragma unroll
-        for (int c = 0; c < 8; c++) {
-            uint2 w = make_uint2(0u, 0u);
-            if (g < rows) w = ld_global(reinterpret_cast<const uint2*>(qrow + 16 * c));
-            qb[c][0] = w.x;
-            qb[c][1] = w.y;
-            o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.0f;
-        }
-        const int len = (int)rq.len, pos0 = len - (int)rq.n, window = a.req.window && a.req.window < MOST_KEYS ? (int)a.req.window : (int)MOST_KEYS;
+        for (int n = 0; n < NB; n++) {
+            const uint32_t row = 8 * n + g;
+            const bool on = row < rows;
+            const __half* qrow = a.q + ((size_t)(rq.first + (on ? row >> a.group_shift : 0)) * heads + head * a.group + (row & (a.group - 1))) * HD + 4 * t4;
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            hi_row[e] = min(pos0 + (int)((2 * t4 + e) >> a.group_shift), len - 1);
-            lo_row[e] = max(hi_row[e] + 1 - window, 0);
-            m_run[e] = NEG_SENTINEL;
-            l_part[e] = 0.0f;
+            for (int c = 0; c < 8; c++) {
+                if constexpr (Q_SHARED) {
+                    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(&sm.q[warp][8 * n + c][lane])), "l"(qrow + 16 * c), "r"(on ? 8u : 0u) : "memory");
+                } else {
+                    qb[n][c] = make_uint2(0u, 0u);
+                    if (on) qb[n][c] = ld_global(reinterpret_cast<const uint2*>(qrow + 16 * c));
+                }
+                o[n][c][0] = o[n][c][1] = o[n][c][2] = o[n][c][3] = 0.0f;
+            }
+            m_run[n][0] = m_run[n][1] = NEG_SENTINEL;
+            l_part[n][0] = l_part[n][1] = 0.0f;
         }
-        hi_all = pos0;
+        len = (int)rq.len;
+        pos0 = len - (int)rq.n;
         lo_all = max(len - window, 0);
-        hi_any = len - 1;
         lo_any = max(pos0 + 1 - window, 0);
     };
     auto end_request = [&](uint32_t tile_last) {
-        const float l_row[2] = {tok_sum(l_part[0]), tok_sum(l_part[1])};
         const bool began = tile_first == tile_begin, ended = tile_last + 1 == tile_end;
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const uint32_t row = 2 * t4 + e;
-            if (row >= rows) continue;
-            if (began && ended) {
-                const bool saw = l_row[e] != 0.0f;  // a row that saw nothing is 0, whatever stands in V
-                const float f = 1.0f / l_row[e];
-                __half* dst = a.out + ((size_t)(first_tok + (row >> a.group_shift)) * heads + head * a.group + (row & (a.group - 1))) * HD + 2 * g;
+        for (int n = 0; n < NB; n++) {
+            if (NB > 1 && 8 * (uint32_t)n >= rows) break;
+            const float l_row[2] = {tok_sum(l_part[n][0]), tok_sum(l_part[n][1])};
 #pragma unroll
-                for (int c = 0; c < 8; c++) *reinterpret_cast<__half2*>(dst + 16 * c) = saw ? __floats2half2_rn(o[c][e] * f, o[c][2 + e] * f) : __float2half2_rn(0.0f);
-            } else {
-                const size_t at = ((size_t)(2 * part + (began ? 1 : 0)) * a.n_kv + head) * work.rows + row;
-                float* dst = reinterpret_cast<float*>(work.acc + at * (HD / 4)) + 2 * g;
+            for (int e = 0; e < 2; e++) {
+                const uint32_t row = 8 * n + 2 * t4 + e;
+                if (row >= rows) continue;
+                if (began && ended) {
+                    const bool saw = l_row[e] != 0.0f;  // a row that saw nothing is 0, whatever stands in V
+                    const float f = 1.0f / l_row[e];
+                    __half* dst = a.out + ((size_t)(first_tok + (row >> a.group_shift)) * heads + head * a.group + (row & (a.group - 1))) * HD + 2 * g;
 #pragma unroll
-                for (int c = 0; c < 8; c++) *reinterpret_cast<float2*>(dst + 16 * c) = make_float2(o[c][e], o[c][2 + e]);
-                if (g == 0) work.ml[at] = make_float2(m_run[e], l_row[e]);
+                    for (int c = 0; c < 8; c++)
+                        *reinterpret_cast<__half2*>(dst + 16 * c) = saw ? __floats2half2_rn(o[n][c][e] * f, o[n][c][2 + e] * f) : __float2half2_rn(0.0f);
+                } else {
+                    const size_t at = ((size_t)(2 * part + (began ? 1 : 0)) * a.n_kv + head) * work.rows + row;
+                    float* dst = reinterpret_cast<float*>(work.acc + at * (HD / 4)) + 2 * g;
+#pragma unroll
+                    for (int c = 0; c < 8; c++) *reinterpret_cast<float2*>(dst + 16 * c) = make_float2(o[n][c][e], o[n][c][2 + e]);
+                    if (g == 0) work.ml[at] = make_float2(m_run[n][e], l_row[e]);
+                }
             }
         }
     };
@@ -376,8 +397,9 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
         const int tok0 = (int)(tile_now * TILE_TOK);
         const uint32_t k_base = smem_u32(sm.k[warp][st]), v_base = smem_u32(sm.v[warp][st]);
 
-        // S: s[2 th + e] = score of token g + 8 th against row 2 t4 + e
-        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f}, s1[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // two chains of four products
+        if (Q_SHARED) asm volatile("cp.async.wait_all;" ::: "memory");  // (of a lane's own queries)
+        // S: s[n][2 th + e] = score of token g + 8 th against row 8 n + 2 t4 + e, of one block in two chains of four products
+        float s[NB][4] = {}, s1[4] = {};
 #pragma unroll
         for (int b = 0; b < 4; b++) {
             uint32_t x[4];
@@ -386,53 +408,67 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
             for (int cc = 0; cc < 2; cc++) {
                 const uint32_t f[4] = {e4m3x2_to_f16x2(x[2 * cc] & 0xffffu), e4m3x2_to_f16x2(x[2 * cc + 1] & 0xffffu), e4m3x2_to_f16x2(x[2 * cc] >> 16),
                                        e4m3x2_to_f16x2(x[2 * cc + 1] >> 16)};
-                mma16816(cc ? s1 : s, f, qb[2 * b + cc][0], qb[2 * b + cc][1]);
+#pragma unroll
+                for (int n = 0; n < NB; n++) {
+                    const uint2 q = Q_SHARED ? sm.q[Q_SHARED ? warp : 0][Q_SHARED ? 8 * n + 2 * b + cc : 0][lane] : qb[Q_SHARED ? 0 : n][2 * b + cc];
+                    mma16816(NB == 1 && cc ? s1 : s[n], f, q.x, q.y);
+                }
             }
         }
         const float ks = scale2 * __int_as_float((127 + ek) << 23), shift = (float)ev;
 #pragma unroll
-        for (int i = 0; i < 4; i++) s[i] = fmaf(s[i] + s1[i], ks, shift);
-        if (tok0 < lo_all || tok0 + TILE_TOK - 1 > hi_all) {
+        for (int n = 0; n < NB; n++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int t = tok0 + (int)g + 8 * (i / 2);
-                if (t < lo_row[i % 2] || t > hi_row[i % 2]) s[i] = -INFINITY;
-            }
+            for (int i = 0; i < 4; i++) s[n][i] = fmaf(NB == 1 ? s[n][i] + s1[i] : s[n][i], ks, shift);
+        if (tok0 < lo_all || tok0 + TILE_TOK - 1 > pos0) {
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int t = tok0 + (int)g + 8 * (i / 2), hi = min(pos0 + (int)((8 * n + 2 * t4 + i % 2) >> a.group_shift), len - 1);
+                    if (t < max(hi + 1 - window, 0) || t > hi) s[n][i] = -INFINITY;
+                }
         }
-        const float mx0 = tok_max(fmaxf(s[0], s[2])), mx1 = tok_max(fmaxf(s[1], s[3]));
-        const bool grow0 = mx0 > m_run[0] + RESCALE_T, grow1 = mx1 > m_run[1] + RESCALE_T;
-        if (__any_sync(0xffffffffu, grow0 || grow1)) {
-            const float n0 = grow0 ? mx0 : m_run[0], n1 = grow1 ? mx1 : m_run[1];
-            const float c0 = ex2(m_run[0] - n0), c1 = ex2(m_run[1] - n1);
-            m_run[0] = n0;
-            m_run[1] = n1;
-            l_part[0] *= c0;
-            l_part[1] *= c1;
+        bool grows = false;  // any row: a lane looks at its own scores, the rows' maxima are found only where one counts
 #pragma unroll
-            for (int c = 0; c < 8; c++) {
-                o[c][0] *= c0;
-                o[c][1] *= c1;
-                o[c][2] *= c0;
-                o[c][3] *= c1;
-            }
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) grows |= fmaxf(s[n][e], s[n][2 + e]) > m_run[n][e] + RESCALE_T;
+        if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const float mx = tok_max(fmaxf(s[n][e], s[n][2 + e])), m = mx > m_run[n][e] + RESCALE_T ? mx : m_run[n][e], corr = ex2(m_run[n][e] - m);
+                    m_run[n][e] = m;
+                    l_part[n][e] *= corr;
+#pragma unroll
+                    for (int c = 0; c < 8; c++) {
+                        o[n][c][e] *= corr;
+                        o[n][c][2 + e] *= corr;
+                    }
+                }
         }
-        float p[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) p[i] = ex2(s[i] - m_run[i % 2]);
         const float back = __int_as_float((127 - ev) << 23);
-        l_part[0] = fmaf(p[0] + p[2], back, l_part[0]);
-        l_part[1] = fmaf(p[1] + p[3], back, l_part[1]);
-
-        // P (tokens x rows) -> P^T fragments: lane (g, t4) gets row g, tokens 2 t4, 2 t4 + 1 and 8 + those
-        const uint32_t pt0 = movmatrix_trans(pack_half2(p[0], p[1])), pt1 = movmatrix_trans(pack_half2(p[2], p[3]));
-        // Tokens that no row sees have P = 0, but 0 times a NaN that stands there would not be: they count as 0.
-        uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-        if (tok0 < lo_any || tok0 + TILE_TOK - 1 > hi_any) {
+        uint32_t pt[NB][2];
 #pragma unroll
-            for (int th = 0; th < 2; th++) {
-                const int t = tok0 + 8 * th + 2 * (int)t4;
-                keep[th] = (t >= lo_any && t <= hi_any ? 0xffffu : 0u) | (t + 1 >= lo_any && t + 1 <= hi_any ? 0xffff0000u : 0u);
-            }
+        for (int n = 0; n < NB; n++) {
+            float p[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[i] = ex2(s[n][i] - m_run[n][i % 2]);
+            l_part[n][0] = fmaf(p[0] + p[2], back, l_part[n][0]);
+            l_part[n][1] = fmaf(p[1] + p[3], back, l_part[n][1]);
+            // P (tokens x rows) -> P^T fragments: lane (g, t4) gets row g, tokens 2 t4, 2 t4 + 1 and 8 + those
+            pt[n][0] = movmatrix_trans(pack_half2(p[0], p[1]));
+            pt[n][1] = movmatrix_trans(pack_half2(p[2], p[3]));
+        }
+        // Tokens that no row sees have P = 0, but 0 times a NaN that stands there would not be: they count as 0.
+        if (tok0 < lo_any || tok0 + TILE_TOK > len) {
+#pragma unroll 1
+            for (int t = 0; t < TILE_TOK; t++)
+                if (tok0 + t < lo_any || tok0 + t >= len) asm volatile("st.shared.u32 [%0], %1;" ::"r"(v_base + t * 128 + lane * 4), "r"(0) : "memory");
+            fence_proxy_async_smem();  // the slot's next copy comes behind these
+            __syncwarp();
         }
 #pragma unroll
         for (int b = 0; b < 4; b++) {
@@ -440,12 +476,13 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS_PER_SM)
             ldsm_x4_trans(v_base + off[b], y);
 #pragma unroll
             for (int cc = 0; cc < 2; cc++) {
-                const uint32_t y0 = __byte_perm(y[2 * cc] & keep[0], 0u, 0x3120), y1 = __byte_perm(y[2 * cc + 1] & keep[1], 0u, 0x3120);
+                const uint32_t y0 = __byte_perm(y[2 * cc], 0u, 0x3120), y1 = __byte_perm(y[2 * cc + 1], 0u, 0x3120);
                 const uint32_t f[4] = {e4m3x2_to_f16x2(y0 & 0xffffu), e4m3x2_to_f16x2(y0 >> 16), e4m3x2_to_f16x2(y1 & 0xffffu), e4m3x2_to_f16x2(y1 >> 16)};
-                mma16816(o[2 * b + cc], f, pt0, pt1);
+#pragma unroll
+                for (int n = 0; n < NB; n++) mma16816(o[n][2 * b + cc], f, pt[n][0], pt[n][1]);
             }
         }
-        __syncwarp();  // every lane has read the slot
+        __syncwarp();  // every lane is done with the slot
 #pragma unroll
         for (int i = 0; i + 1 < STAGES; i++) {
             way_r[i] = way_r[i + 1];
@@ -500,7 +537,7 @@ __device__ __forceinline__ void list_units(const BlocksAttn& a, const BlocksWork
         return at;
     };
     const uint32_t per_thread = (a.req.n + N - 1) / N, r_begin = min(tid * per_thread, a.req.n), r_end = min(r_begin + per_thread, a.req.n);
-    const auto units = [&](const Request& q) -> uint32_t { return q.n > FEW_ROWS / a.group ? (uint32_t)(((uint64_t)q.n * a.group + UNIT_ROWS - 1) / UNIT_ROWS) : 0; };
+    const auto units = [&](const Request& q) -> uint32_t { return q.n > a.few ? (uint32_t)(((uint64_t)q.n * a.group + UNIT_ROWS - 1) / UNIT_ROWS) : 0; };
     uint32_t mine = 0, kilokeys = 0, total, all_kilokeys;
     for_requests(a.req, r_begin, r_end, [&](uint32_t, const Request& q) {
         const uint32_t n = units(q);
@@ -584,7 +621,7 @@ __device__ __forceinline__ void list_units(const BlocksAttn& a, const BlocksWork
     if (tid == 0) w.rest[w.places] = all_tiles;
 }
 
-// One CTA per request and kv head: nothing to do where one warp had all its tiles; zeros where it had none; else the warps' parts.
+// One CTA per request, kv head and eight rows: nothing to do where one warp had all its tiles; zeros where it had none; else the warps' parts.
 // Warp x of W takes parts x, x + W, ...  Row and part are spread over its lanes for (m, l), and over the E sums of four dims that a lane keeps
 // for O, so that few rows go through several parts at a time; maxima and sums of the warps meet in shared memory, in a fixed order.
 // SHIFT: rows up to this power of two in all requests, or -1: each request's own (a dispatch that has prompts as well knows no more than eight).
@@ -602,7 +639,7 @@ __global__ void __launch_bounds__(W * 32, W == MANY_CTAS_WARPS ? (E == 8 ? 4 : 8
     pdl_wait();
     pdl_launch_dependents();
     if (blockIdx.x == a.req.n) {  // there if a prefill follows
-        if (blockIdx.y == 0) list_units<W>(a, work.head, sm.sort);
+        if (blockIdx.y + blockIdx.z == 0) list_units<W>(a, work.head, sm.sort);
         return;
     }
     const uint32_t r = blockIdx.x, head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -616,9 +653,12 @@ __global__ void __launch_bounds__(W * 32, W == MANY_CTAS_WARPS ? (E == 8 ? 4 : 8
         n = cut.of(end - 1) - p0 + 1;
         if (n == 1) return;
     }
-    if (last <= first || last > a.req.tokens || last - first > (FEW_ROWS >> a.group_shift) || last - first > a.req.max_q) return;
-    const uint32_t rows = (last - first) * a.group;
+    if (last <= first || last > a.req.tokens || last - first > a.few || last - first > a.req.max_q) return;
+    const uint32_t row0 = SHIFT < 0 ? 8 * blockIdx.z : 0, all_rows = (last - first) * a.group;
+    if (SHIFT < 0 && row0 >= all_rows) return;
+    const uint32_t rows = SHIFT < 0 ? min(all_rows - row0, 8u) : all_rows;  // of this CTA
     const auto out = [&](uint32_t row) {
+        row += row0;
         return reinterpret_cast<uint2*>(a.out + ((size_t)(first + (row >> a.group_shift)) * (a.n_kv * a.group) + head * a.group + (row & (a.group - 1))) * HD + 4 * lane);
     };
     if (n == 0) {
@@ -626,7 +666,7 @@ __global__ void __launch_bounds__(W * 32, W == MANY_CTAS_WARPS ? (E == 8 ? 4 : 8
         return;
     }
     const uint32_t shift = SHIFT >= 0 ? SHIFT : rows <= 1 ? 0 : rows <= 2 ? 1 : rows <= 4 ? 2 : 3, mask = (1u << shift) - 1;  // rows up to a power of two
-    const auto slot = [&](uint32_t j) { return ((size_t)(2 * (p0 + j) + (j == 0 ? 1 : 0)) * a.n_kv + head) * work.rows; };
+    const auto slot = [&](uint32_t j) { return ((size_t)(2 * (p0 + j) + (j == 0 ? 1 : 0)) * a.n_kv + head) * work.rows + row0; };
     const uint32_t batch = E >> shift, chunk = 32 >> shift;  // parts that a lane's sums go through at a time, parts whose (m, l) the lanes hold
     float4 v[E], acc[E];
     const auto fetch = [&](uint32_t k) {  // this warp's parts k ..
@@ -698,18 +738,46 @@ __global__ void __launch_bounds__(W * 32, W == MANY_CTAS_WARPS ? (E == 8 ? 4 : 8
 }
 
 // Warps that fit the GPU at once, and what every kv head gets of them.
-uint32_t grid_ctas(int sm_count, uint32_t n_kv)
+uint32_t grid_ctas(int sm_count, uint32_t n_kv, int ctas_per_sm)
 {
-    const uint32_t ctas = (uint32_t)sm_count * CTAS_PER_SM, least = (n_kv + WARPS - 1) / WARPS;
+    const uint32_t ctas = (uint32_t)(sm_count * ctas_per_sm), least = (n_kv + WARPS - 1) / WARPS;
     return ctas > least ? ctas : least;
 }
-uint32_t most_stretches(int sm_count, uint32_t n_kv) { return grid_ctas(sm_count, n_kv) * WARPS / n_kv; }
+
+template <int NB>
+int launch_decode(const LaunchArgs& a, const BlocksAttn& k, const CUtensorMap (&tm)[2], const Work& w, uint32_t ctas, uint32_t most)
+{
+    const size_t smem = sizeof(DecodeSmem<NB>) + 1024;
+    static_assert((sizeof(DecodeSmem<NB>) + 2048) * Shape<NB>::CTAS_PER_SM <= 228 * 1024, "shared memory of an SM");
+    {
+        static std::mutex attr_mutex;
+        static bool attr_set[64] = {};
+        std::lock_guard<std::mutex> lock(attr_mutex);
+        if (a.device < 0 || a.device >= 64 || !attr_set[a.device]) {
+            if (int r = check_cuda(a, cudaFuncSetAttribute(blocks_decode_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+                                   "cudaFuncSetAttribute(blocks_decode)"))
+                return r;
+            if (a.device >= 0 && a.device < 64) attr_set[a.device] = true;
+        }
+    }
+    const cudaError_t e = launch_dependent(blocks_decode_kernel<NB>, dim3(ctas), dim3(WARPS * 32), smem, a.stream, tm[0], tm[1], k, w, most);
+    ++*a.launches;
+    return check_cuda(a, e, "attn_blocks decode");
+}
+int ctas_per_sm(uint32_t most_rows) { return most_rows <= 8 ? Shape<1>::CTAS_PER_SM : Shape<2>::CTAS_PER_SM; }
 
 }  // namespace
 
+// (no less for fewer heads, nor for more query tokens of a request)
 size_t blocks_decode_work(int sm_count, uint32_t n_kv, uint32_t group, uint32_t max_q)
 {
-    return 2ull * grid_ctas(sm_count, n_kv) * WARPS * few_rows(group, max_q) * (HD + 2) * 4;  // (no less for fewer heads)
+    size_t parts = 0;
+    for (uint32_t rows = 8; rows <= FEW_ROWS; rows *= 2) {
+        if (rows > 8 && (uint64_t)group * max_q <= rows / 2) break;
+        const size_t n = 2ull * grid_ctas(sm_count, n_kv, ctas_per_sm(rows)) * WARPS * part_rows(rows, group, max_q);
+        parts = n > parts ? n : parts;
+    }
+    return parts * (HD + 2) * 4;
 }
 
 int launch_blocks_decode(const LaunchArgs& a, const BlocksAttn& k, const BlocksWork& head)
@@ -720,32 +788,20 @@ int launch_blocks_decode(const LaunchArgs& a, const BlocksAttn& k, const BlocksW
         const uint32_t box[3] = {128, TILE_TOK, 1};
         if (int r = encode_tensor_map(a, &tm[i], 0, 3, const_cast<uint8_t*>(k.pool[i]), dims, strides, box, 3)) return r;
     }
-    const size_t smem = sizeof(DecodeSmem) + 1024;
-    {
-        static std::mutex attr_mutex;
-        static bool attr_set[64] = {};
-        std::lock_guard<std::mutex> lock(attr_mutex);
-        if (a.device < 0 || a.device >= 64 || !attr_set[a.device]) {
-            if (int r = check_cuda(a, cudaFuncSetAttribute(blocks_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), "cudaFuncSetAttribute(blocks_decode)"))
-                return r;
-            if (a.device >= 0 && a.device < 64) attr_set[a.device] = true;
-        }
-    }
-    const uint32_t most = most_stretches(a.sm_count, k.n_kv);
-    Work w{head, nullptr, reinterpret_cast<float4*>(head.parts), few_rows(k.group, k.req.max_q)};
+    const uint32_t most_rows = k.few * k.group, ctas = grid_ctas(a.sm_count, k.n_kv, ctas_per_sm(most_rows)), most = ctas * WARPS / k.n_kv;
+    Work w{head, nullptr, reinterpret_cast<float4*>(head.parts), part_rows(most_rows, k.group, k.req.max_q)};
     w.ml = reinterpret_cast<float2*>(w.acc + 2ull * most * k.n_kv * w.rows * (HD / 4));
-    cudaError_t e = launch_dependent(blocks_decode_kernel, dim3(grid_ctas(a.sm_count, k.n_kv)), dim3(WARPS * 32), smem, a.stream, tm[0], tm[1], k, w, most);
-    ++*a.launches;
-    if (int r = check_cuda(a, e, "attn_blocks decode")) return r;
+    if (int r = most_rows <= 8 ? launch_decode<1>(a, k, tm, w, ctas, most) : launch_decode<2>(a, k, tm, w, ctas, most)) return r;
     // Few CTAs have many parts each (one request of 131072 keys: 148 of every head; 9.4 us with four warps a CTA).
-    const bool few = (uint64_t)k.req.n * k.n_kv <= 2u * (uint32_t)a.sm_count;
-    const dim3 grid(k.req.n + (k.req.max_q > FEW_ROWS / k.group ? 1 : 0), k.n_kv);
+    const uint32_t row_blocks = (w.rows + 7) / 8;
+    const bool few = (uint64_t)k.req.n * k.n_kv * row_blocks <= 2u * (uint32_t)a.sm_count;
+    const dim3 grid(k.req.n + (k.req.max_q > k.few ? 1 : 0), k.n_kv, row_blocks);
     const auto merge = [&](auto shift) {
         constexpr int SHIFT = decltype(shift)::value, WARPS_IF_FEW = SHIFT < 0 ? FEW_CTAS_WARPS / 2 : FEW_CTAS_WARPS;
         return few ? launch_dependent(blocks_merge_kernel<8, WARPS_IF_FEW, SHIFT>, grid, dim3(WARPS_IF_FEW * 32), 0, a.stream, k, w)
                    : launch_dependent(blocks_merge_kernel<SHIFT < 0 ? 8 : 4, MANY_CTAS_WARPS, SHIFT>, grid, dim3(MANY_CTAS_WARPS * 32), 0, a.stream, k, w);
     };
-    e = w.rows <= 1 ? merge(std::integral_constant<int, 0>()) : w.rows <= 2 ? merge(std::integral_constant<int, 1>())
+    const cudaError_t e = w.rows <= 1 ? merge(std::integral_constant<int, 0>()) : w.rows <= 2 ? merge(std::integral_constant<int, 1>())
         : w.rows <= 4 ? merge(std::integral_constant<int, 2>()) : merge(std::integral_constant<int, -1>());
     ++*a.launches;
     return check_cuda(a, e, "attn_blocks merge");

@@ -20,7 +20,7 @@ constexpr uint32_t NO_SLOT = 0xffffffffu;
 constexpr int LOWEST_EXP = -15;
 constexpr uint32_t MOST_REQUESTS = 65536;
 constexpr uint32_t MOST_KEYS = 0x3fffff00u;  // of one request: positions are signed words, and 256 requests' tiles of 64 keys fit one
-constexpr uint32_t FEW_ROWS = 8;             // requests of at most so many rows (query tokens x heads of a group) are decoded, the others prefilled
+constexpr uint32_t FEW_ROWS = 16;            // requests of at most so many rows (query tokens x heads of a group) can be decoded, the others are prefilled
 
 // What a dispatch over the cache knows of its requests.
 struct Requests {
@@ -75,6 +75,7 @@ struct BlocksAttn {
     const int8_t* exps[2];
     __half* out;
     uint32_t n_kv, group, group_shift, tiles;  // tiles of a pool: blocks x kv heads
+    uint32_t few;                              // requests of at most so many query tokens are decoded
     float scale;
 };
 struct LaunchArgs;

@@ -32,7 +32,9 @@ struct Unit {
 __device__ __forceinline__ Unit unit_at(const BlocksAttn& a, uint32_t request, uint32_t nth)
 {
     const Request rq = request_at(a.req, request);
-    const uint32_t per = UNIT_ROWS / a.group, tok0 = nth * per;
+    const uint32_t per = UNIT_ROWS / a.group;
+    uint32_t tok0 = nth * per;
+    if (tok0 >= rq.n) tok0 = 0;  // only if starts that go back and forth, which are reported, made more units than a word counts
     Unit u;
     u.request = request;
     u.first_tok = rq.first + tok0;

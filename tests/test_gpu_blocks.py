@@ -314,6 +314,42 @@ def test_verify_is_causal_among_the_new_tokens(ctx, m, group):
     Batch(m * group, lens, [m, m, 1, m, 0, m, m - 1, m], 3, group, 16).run(ctx)
 
 
+WIDE = [(9, 1), (16, 1), (17, 1), (32, 1), (5, 2), (8, 2), (9, 2), (16, 2), (3, 4), (4, 4), (5, 4), (8, 4), (2, 8), (3, 8), (4, 8)]
+
+
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("m,group", WIDE)
+def test_drafts_of_more_than_eight_rows(ctx, m, group, window):
+    """Up to 32 rows, beside requests of fewer rows and of none; two requests that many warps share, two refused."""
+    lens = [max(n, m) for n in (m, m + 1, 15, 16, 17, 50, 200, 1037, 5003, 64, 33)]
+    Batch(m * group, lens, [m, m, 1, m, 0, m, m - 1, m, m, (m + 1) // 2, m], 3, group, 16, spare_rows=2, dead=(4, 10)).run(ctx, window)
+
+
+@pytest.mark.parametrize("m,group", [(16, 1), (8, 4), (4, 8)])
+def test_wide_drafts_over_one_head_and_large_scores(ctx, m, group):
+    rng = np.random.default_rng(m)
+    lens = rng.integers(m, 90, 70)
+    lens[41] = 12000
+    Batch(m, lens, rng.integers(0, m + 1, 70), 1, group, 16).run(ctx)
+    Batch(m, [500, 2000, 35], [m, m, 1], 2, group, 32, spread=8.0).run(ctx)
+    b = Batch(m, [3, 40, 9], [m, m, min(m, 9)], 2, group, 16)  # more queries than keys
+    b.run(ctx)
+
+
+@pytest.mark.parametrize("m,group", [(16, 1), (16, 2)])
+def test_wide_drafts_again_give_the_same_bits(ctx, m, group):
+    b = Batch(5, [4000, 17, 900, 333], [m, 1, m, m - 1], 4, group, 64)
+    push, grid = b.call(0)
+    k, bound = ctx.load_kernel("attn_blocks_e4m3_d128"), b.buffers(ctx)
+    ctx.dispatch_blocking(k, bound, push, grid)
+    first = b.out.read()
+    b.check(first, 0)
+    for _ in range(3):
+        ctx.dispatch(k, bound, push, grid)
+    ctx.sync()
+    assert np.array_equal(b.out.read(), first)
+
+
 @pytest.mark.parametrize("window", [1, 2, 16, 17, 100, 1024])
 def test_window_over_few_and_many_queries(ctx, window):
     Batch(window, [1, 16, 40, 130, 1500, 3000], [1, 1, 4, 2, 1, 3], 2, 2, 32).run(ctx, window)
