@@ -7,13 +7,15 @@
 // second kernel merges them in the list's order, so reruns give the same bits.  (The cut rests on all lengths, so a request's bits
 // depend on its neighbours' lengths.)
 //
-// One tile: S = K Q^T with the 16 tokens as M and the at most eight query rows as N of mma.sync m16n8k16 (far below tcgen05's 64
+// One tile: S = K Q^T with the 16 tokens as M and eight query rows (or twice eight) as N of mma.sync m16n8k16 (far below tcgen05's 64
 // rows), e4m3 -> f16 exactly on the way from shared memory (ldmatrix, one conversion a pair), O^T += V^T P^T with 16 dims as M.
 // The powers of two never touch the elements: K's multiplies the scores, V's goes into the exponent, P' = 2^(s + e_v - m),
-// and out of the sum again, l += P' 2^-e_v.  Softmax in base 2 with a running maximum that is raised when it grows by more than 2^8.
-// Bound by the cache's bytes: 2 x 128 1/16 per token and kv head.  16 kv heads, two query heads each: 64 requests of 256 to 8192 keys 115 us
-// (5.2 TB/s, of which the merge is 5 us), one of 131072 102 us, drafts of 2 to 4 tokens over up to 32768 keys in 16 requests 146 us
-// (5.3 TB/s), one of 1000 keys 10.3 us.
+// and out of the sum again, l += P' 2^-e_v.  Softmax in base 2 with a running maximum that is raised when it grows by more than 2^8:
+// every lane compares its own scores with it, a row's maximum over the lanes is found only where one is that much larger (three shuffles
+// a tile and row, and the wait for them: 64 requests 114 us, 107 without).
+// Bound by the cache's bytes: 2 x 128 1/16 per token and kv head.  16 kv heads, two query heads each: 64 requests of 256 to 8192 keys 107 us
+// (5.6 TB/s; 6.2 in this kernel, the merge is 6 us), one of 131072 96 us, drafts of 2 to 4 tokens over up to 32768 keys in 16 requests 138 us
+// (5.6 TB/s), one of 1000 keys 10.3 us.  Two blocks of rows are bound by their warps' own latency: drafts of 4 to 8 tokens 180 us (4.3 TB/s).
 #include <mutex>
 #include <type_traits>
 
