@@ -561,7 +561,6 @@ __global__ void __launch_bounds__(THREADS, 1)
 
             // ---- out = O / l, or this piece's part ----
             const bool live = tok < it.toks, whole = it.pieces == 1;
-            __half* orow = a.out + ((size_t)(it.first_tok + tok) * (a.n_kv * a.group) + it.head * a.group + ((uint32_t)r & (a.group - 1))) * HD;
             // A part is [32 groups of four dims][128 rows] and (m, l) of the rows: neighbouring threads write neighbouring 16 bytes.
             const auto part = [&](uint32_t s) { return acc_parts + (size_t)(2 * s + t) * (HD / 4) * ROWS + r; };
             const auto part_ml = [&](uint32_t s) { return ml_parts + (size_t)(2 * s + t) * ROWS + r; };
@@ -624,34 +623,57 @@ __global__ void __launch_bounds__(THREADS, 1)
                     __threadfence();
                 }
                 named_barrier_sync(1 + t, 128);
-                if (sm.last[t] && live) {  // all pieces are written: merge them in their order
-                    const auto slot = [&](uint32_t p) { return p ? it.slot0 - 1 + 2 * p : it.slot0; };
-                    float big = NEG_SENTINEL, den = 0.0f;
-                    for (uint32_t p = 0; p < it.pieces; p++) big = fmaxf(big, __ldcg(part_ml(slot(p))).x);
-                    for (uint32_t p = 0; p < it.pieces; p++) {
-                        const float2 ml = __ldcg(part_ml(slot(p)));
-                        den = fmaf(ex2(ml.x - big), ml.y, den);
-                    }
-                    const float inv = den != 0.0f ? 1.0f / den : 0.0f;
-#pragma unroll 1
-                    for (int c = 0; c < 8; c++) {
-                        float4 acc[4] = {};
+                if (sm.last[t]) {  // all pieces are written: merge them in their order
+                    // Few rows are spread over all threads, every thread with a part of a row's dims; sixteen dims of four pieces are on their way at a time
+                    // (a piece after another, a row a thread: 16 pieces of 32 rows took 25 us).
+                    const uint32_t in_tile = (uint32_t)t * (ROWS >> a.group_shift), rows = it.toks > in_tile ? min((it.toks - in_tile) << a.group_shift, (uint32_t)ROWS) : 0;
+                    const uint32_t shares = rows <= ROWS / 4 ? 4 : rows <= ROWS / 2 ? 2 : 1, share_rows = ROWS / shares, at_row = (uint32_t)r & (share_rows - 1), share = (uint32_t)r / share_rows;
+                    const float4* acc_at = acc_parts + (size_t)t * (HD / 4) * ROWS + at_row;
+                    const float2* ml_at = ml_parts + (size_t)t * ROWS + at_row;
+                    const auto slot = [&](uint32_t p) { return 2 * (size_t)(p ? it.slot0 - 1 + 2 * p : it.slot0); };
+                    if (at_row < rows) {
+                        float big = NEG_SENTINEL, den = 0.0f;
+#pragma unroll 4
+                        for (uint32_t p = 0; p < it.pieces; p++) big = fmaxf(big, __ldcg(ml_at + slot(p) * ROWS).x);
+#pragma unroll 4
                         for (uint32_t p = 0; p < it.pieces; p++) {
-                            const float f = ex2(__ldcg(part_ml(slot(p))).x - big) * inv;
-#pragma unroll
-                            for (int x = 0; x < 4; x++) {
-                                const float4 o = __ldcg(part(slot(p)) + (4 * c + x) * ROWS);
-                                acc[x].x = fmaf(f, o.x, acc[x].x);
-                                acc[x].y = fmaf(f, o.y, acc[x].y);
-                                acc[x].z = fmaf(f, o.z, acc[x].z);
-                                acc[x].w = fmaf(f, o.w, acc[x].w);
-                            }
+                            const float2 ml = __ldcg(ml_at + slot(p) * ROWS);
+                            den = fmaf(ex2(ml.x - big), ml.y, den);
                         }
+                        const float inv = den != 0.0f ? 1.0f / den : 0.0f;
+                        __half* to = a.out + ((size_t)(it.first_tok + in_tile + (at_row >> a.group_shift)) * (a.n_kv * a.group) + it.head * a.group + (at_row & (a.group - 1))) * HD;
+#pragma unroll 1
+                        for (uint32_t c = share; c < 8; c += shares) {
+                            float4 acc[4] = {};
+#pragma unroll 1
+                            for (uint32_t p0 = 0; p0 < it.pieces; p0 += 4) {
+                                float4 o[4][4];
+                                float f[4];
 #pragma unroll
-                        for (int x = 0; x < 2; x++)
-                            *reinterpret_cast<uint4*>(orow + 16 * c + 8 * x) = den == 0.0f ? make_uint4(0u, 0u, 0u, 0u) :
-                                make_uint4(pack_half2(acc[2 * x].x, acc[2 * x].y), pack_half2(acc[2 * x].z, acc[2 * x].w), pack_half2(acc[2 * x + 1].x, acc[2 * x + 1].y),
-                                           pack_half2(acc[2 * x + 1].z, acc[2 * x + 1].w));
+                                for (uint32_t y = 0; y < 4; y++) {
+                                    const size_t from = slot(min(p0 + y, it.pieces - 1));  // (those past the end are the last one again, and count nothing)
+                                    f[y] = __ldcg(ml_at + from * ROWS).x;
+#pragma unroll
+                                    for (int x = 0; x < 4; x++) o[y][x] = __ldcg(acc_at + from * (HD / 4) * ROWS + (4 * c + x) * ROWS);
+                                }
+#pragma unroll
+                                for (uint32_t y = 0; y < 4; y++) {
+                                    const float w = p0 + y < it.pieces ? ex2(f[y] - big) * inv : 0.0f;
+#pragma unroll
+                                    for (int x = 0; x < 4; x++) {
+                                        acc[x].x = fmaf(w, o[y][x].x, acc[x].x);
+                                        acc[x].y = fmaf(w, o[y][x].y, acc[x].y);
+                                        acc[x].z = fmaf(w, o[y][x].z, acc[x].z);
+                                        acc[x].w = fmaf(w, o[y][x].w, acc[x].w);
+                                    }
+                                }
+                            }
+#pragma unroll
+                            for (int x = 0; x < 2; x++)
+                                *reinterpret_cast<uint4*>(to + 16 * c + 8 * x) = den == 0.0f ? make_uint4(0u, 0u, 0u, 0u) :
+                                    make_uint4(pack_half2(acc[2 * x].x, acc[2 * x].y), pack_half2(acc[2 * x].z, acc[2 * x].w), pack_half2(acc[2 * x + 1].x, acc[2 * x + 1].y),
+                                               pack_half2(acc[2 * x + 1].z, acc[2 * x + 1].w));
+                        }
                     }
                 }
             }
