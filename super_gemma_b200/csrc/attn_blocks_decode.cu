@@ -44,7 +44,7 @@ static_assert(REQUEST_WEIGHT == 1, "a stretch that begins within a request's own
 
 // What NB blocks of eight query rows take: O alone is 32 NB registers a thread, so three CTAs of 168 registers stand on an SM for two blocks.
 // Their queries, another 32, are kept in shared memory, every lane's own beside each other.  (Four blocks: eight warps on an SM cannot hide
-// their own latency; 16 drafts of 2 to 4 tokens of eight heads a group 187 us, as prompts 97.)
+// their own latency; 16 drafts of 2 to 4 tokens of eight heads a group 187 us, as prompts 88.)
 template <int NB> struct Shape {
     static constexpr int CTAS_PER_SM = NB == 1 ? 4 : 3, STAGES = 3;
     static constexpr int MET = 4;  // STAGES tiles under way are of three requests at most

@@ -15,7 +15,7 @@
 //
 // Bound by shared memory's port, 192 KB = 1536 cycles per 64 keys and 256 rows (raw bytes in and out 32, f16 tiles 32, operands of Q K^T 96, of
 // P V 32), of the 2000 or so that a tile takes; in long runs by the board's power.  1740 tokens of 65536 keys, 16 kv heads of two query heads:
-// 1840 us, 1.0 PFLOP/s (the f16 kernel reaches 1.05 to 1.1 on cached f16 keys).  128 rows a CTA and two CTAs an SM would convert every key twice
+// 1835 us, 1.0 PFLOP/s (the f16 kernel reaches 1.05 to 1.1 on cached f16 keys).  128 rows a CTA and two CTAs an SM would convert every key twice
 // as often and need 256 KB of the port.
 #include <mutex>
 
@@ -625,7 +625,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 named_barrier_sync(1 + t, 128);
                 if (sm.last[t]) {  // all pieces are written: merge them in their order
                     // Few rows are spread over all threads, every thread with a part of a row's dims; sixteen dims of four pieces are on their way at a time
-                    // (a piece after another, a row a thread: 16 pieces of 32 rows took 25 us).
+                    // (a piece after another and a row a thread: 16 pieces of 32 rows took 13 us more).
                     const uint32_t in_tile = (uint32_t)t * (ROWS >> a.group_shift), rows = it.toks > in_tile ? min((it.toks - in_tile) << a.group_shift, (uint32_t)ROWS) : 0;
                     const uint32_t shares = rows <= ROWS / 4 ? 4 : rows <= ROWS / 2 ? 2 : 1, share_rows = ROWS / shares, at_row = (uint32_t)r & (share_rows - 1), share = (uint32_t)r / share_rows;
                     const float4* acc_at = acc_parts + (size_t)t * (HD / 4) * ROWS + at_row;
