@@ -451,6 +451,17 @@ def test_more_requests_than_threads(ctx, requests):
     Batch(requests, np.maximum(lens, new), new, 1, 4, 16, dead=set(range(5, requests, 50))).run(ctx)
 
 
+@pytest.mark.parametrize("group", [1, 2, 4, 8])
+def test_a_work_buffer_for_longer_drafts_does_for_shorter_ones(ctx, group):
+    for kv in (1, 5, 16, 1024):
+        sizes = [ctx.attn_blocks_work_bytes(kv, group, 20, 200, m) for m in range(1, 41)]
+        assert sizes[0] > 0 and sizes == sorted(sizes)
+    m = 16 // group
+    b = Batch(group, [90, 40, 700], [m, 1, m], 2, group, 16)
+    b.max_q = m + 30  # the prompts' kernel is launched too, and the drafts are its work
+    b.run(ctx)
+
+
 def test_offsets_beyond_32_bits(ctx):
     """Pools of more than 4 GiB each: tokens go into their last pages and are read from there."""
     import super_gemma_b200 as sg
