@@ -33,7 +33,6 @@ constexpr uint32_t LEAST_TILES = 2;  // of a stretch: fewer would only mean more
 // A request weighs a tile more than it has: its queries to fetch, its result to write.  (256 requests of 17 to 2048 keys: a warp whose
 // stretch was of many short ones ended 11 of 52 us after the median one.)
 constexpr uint32_t REQUEST_WEIGHT = 1;
-constexpr float RESCALE_T = 8.0f;
 constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES;
 
 // What the arithmetic needs of a request, left for it by the side that copies, which comes to it up to STAGES tiles earlier.
@@ -435,13 +434,13 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<NB>::CTAS_PER_SM)
 #pragma unroll
         for (int n = 0; n < NB; n++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) grows |= fmaxf(s[n][e], s[n][2 + e]) > m_run[n][e] + RESCALE_T;
+            for (int e = 0; e < 2; e++) grows |= fmaxf(s[n][e], s[n][2 + e]) > m_run[n][e] + GROWTH_T;
         if (__any_sync(0xffffffffu, grows)) {
 #pragma unroll
             for (int n = 0; n < NB; n++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    const float mx = tok_max(fmaxf(s[n][e], s[n][2 + e])), m = mx > m_run[n][e] + RESCALE_T ? mx : m_run[n][e], corr = ex2(m_run[n][e] - m);
+                    const float mx = tok_max(fmaxf(s[n][e], s[n][2 + e])), m = mx > m_run[n][e] + GROWTH_T ? mx - LIFT : m_run[n][e], corr = ex2(m_run[n][e] - m);
                     m_run[n][e] = m;
                     l_part[n][e] *= corr;
 #pragma unroll

@@ -38,7 +38,6 @@ constexpr int ITEM_READERS = 8 + 4 + 3;           // warps that give an item's p
 constexpr uint32_t HALF_TILE = 64 * 128;          // [64 rows][64 dims] f16
 constexpr uint32_t Q_BYTES = 4 * HALF_TILE;       // of one tile of queries
 constexpr uint32_t TMEM_COLS = 512, TMEM_O = 256; // S: [tile][buffer] of 64 columns, then O: [tile] of 128
-constexpr float RESCALE_T = 8.0f;
 // Registers: 512 threads are launched with 128 each; the warpgroups redistribute exactly those.
 constexpr uint32_t LAUNCH_REGS = 128, SOFTMAX_REGS = 160, CONVERT_REGS = 96, ISSUE_REGS = 96;
 static_assert(2 * SOFTMAX_REGS + CONVERT_REGS + ISSUE_REGS <= 4 * LAUNCH_REGS, "setmaxnreg draws on what the block was launched with");
@@ -516,11 +515,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                     }
                     mx = fmaxf(mx, fmaf(fmaxf(m0, m1), ks[x], ve[x]));
                 }
-                const bool grow = mx > m_run + RESCALE_T;
+                const bool grow = mx > m_run + GROWTH_T;
                 float corr = 1.0f;
                 if (grow) {
-                    corr = ex2(m_run - mx);
-                    m_run = mx;
+                    const float m = mx - LIFT;
+                    corr = ex2(m_run - m);
+                    m_run = m;
                     l_run *= corr;
                 }
                 uint32_t pk[32];
