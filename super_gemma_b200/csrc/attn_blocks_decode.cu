@@ -147,7 +147,8 @@ __device__ __forceinline__ Stretches stretches_for(uint64_t total, uint32_t most
     return s;
 }
 
-template <int NB>
+// DRAFTS: a request may have more than one token.
+template <int NB, bool DRAFTS>
 __global__ void __launch_bounds__(WARPS * 32, Shape<NB>::CTAS_PER_SM)
     blocks_decode_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ BlocksAttn a, const __grid_constant__ Work work, uint32_t most)
 {
@@ -464,10 +465,21 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<NB>::CTAS_PER_SM)
             pt[n][1] = movmatrix_trans(pack_half2(p[2], p[3]));
         }
         // Tokens that no row sees have P = 0, but 0 times a NaN that stands there would not be: they count as 0.
-        if (tok0 < lo_any || tok0 + TILE_TOK > len) {
+        // So do NaNs in tokens that some rows see and others not: the merge puts those into the rows that see them.
+        if (tok0 < lo_all || tok0 + TILE_TOK - 1 > pos0) {
 #pragma unroll 1
             for (int t = 0; t < TILE_TOK; t++)
                 if (tok0 + t < lo_any || tok0 + t >= len) asm volatile("st.shared.u32 [%0], %1;" ::"r"(v_base + t * 128 + lane * 4), "r"(0) : "memory");
+            if (DRAFTS && rows > a.group) {
+                __syncwarp();
+#pragma unroll 1
+                for (int t = 0; t < TILE_TOK; t += 4) {
+                    const uint32_t v_at = v_base + t * 128 + lane * 16;
+                    uint4 v;
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(v_at) : "memory");
+                    if (drop_nans(v)) asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(v_at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+                }
+            }
             fence_proxy_async_smem();  // the slot's next copy comes behind these
             __syncwarp();
         }
@@ -626,7 +638,8 @@ __device__ __forceinline__ void list_units(const BlocksAttn& a, const BlocksWork
 // Warp x of W takes parts x, x + W, ...  Row and part are spread over its lanes for (m, l), and over the E sums of four dims that a lane keeps
 // for O, so that few rows go through several parts at a time; maxima and sums of the warps meet in shared memory, in a fixed order.
 // SHIFT: rows up to this power of two in all requests, or -1: each request's own (a dispatch that has prompts as well knows no more than eight).
-template <int E, int W, int SHIFT>
+// DRAFTS: a request may have more than one token.
+template <int E, int W, int SHIFT, bool DRAFTS>
 __global__ void __launch_bounds__(W * 32, W == MANY_CTAS_WARPS ? (E == 8 ? 4 : 8) : SHIFT < 0 ? 2 : 1) blocks_merge_kernel(const __grid_constant__ BlocksAttn a, const __grid_constant__ Work work)
 {
     constexpr int LEFT = SHIFT >= 0 ? 1 << SHIFT : E;  // sums that a lane leaves: one a row, where the rows are known beforehand
@@ -652,7 +665,7 @@ __global__ void __launch_bounds__(W * 32, W == MANY_CTAS_WARPS ? (E == 8 ? 4 : 8
         const Stretches cut = stretches_for(total, most);
         p0 = cut.of(at + REQUEST_WEIGHT);
         n = cut.of(end - 1) - p0 + 1;
-        if (n == 1) return;
+        if (n == 1 && (!DRAFTS || last - first == 1)) return;
     }
     if (last <= first || last > a.req.tokens || last - first > a.few || last - first > a.req.max_q) return;
     const uint32_t row0 = SHIFT < 0 ? 8 * blockIdx.z : 0, all_rows = (last - first) * a.group;
@@ -664,6 +677,41 @@ __global__ void __launch_bounds__(W * 32, W == MANY_CTAS_WARPS ? (E == 8 ? 4 : 8
     };
     if (n == 0) {
         for (uint32_t row = warp; row < rows; row += W) *out(row) = make_uint2(0u, 0u);
+        return;
+    }
+    // NaNs of V that some of the request's rows see and others not, which the decode took for 0: into the rows that see them, in their dims.
+    const auto put_nans = [&]() {
+        const Request rq = request_at(a.req, r);
+        const Tiles tiles = tiles_of(a, rq);
+        const int len = (int)rq.len, pos0 = len - (int)rq.n, window = a.req.window && a.req.window < MOST_KEYS ? (int)a.req.window : (int)MOST_KEYS;
+        // such are in the first tiles, up to the key from which on the last row sees all, and in those of the new tokens; one a warp at a time
+        const uint32_t to = tiles.lo + tiles.n, mid = min((uint32_t)(max(len - window, 0) + TILE_TOK - 1) / TILE_TOK, to), passed = mid > tiles.lo ? mid - tiles.lo : 0;
+        const uint32_t from = max((uint32_t)max(pos0 + 1, 0) / TILE_TOK, tiles.lo + passed);
+        for (uint32_t i = warp; i < passed + (to - from); i += W) {
+            const uint32_t tile = i < passed ? tiles.lo + i : from + (i - passed);
+            const size_t block = block_of_page(a.req, r, tile, ld_global(page_at(a.req, r, tile)));
+            const uint8_t* v = a.pool[1] + (block * a.n_kv + head) * TILE_BYTES + lane * 16;
+            uint32_t nans = 0;
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const uint4 y = ld_global(reinterpret_cast<const uint4*>(v + 512 * x));
+                nans |= nan_bytes(y.x) | nan_bytes(y.y) | nan_bytes(y.z) | nan_bytes(y.w);
+            }
+            if (nans == 0) continue;
+#pragma unroll 1
+            for (uint32_t x = 0; x < 64; x++) {  // byte by byte: token 4 (x / 16) + lane / 8, dim 16 (lane % 8) + x % 16
+                const int t = (int)(tile * TILE_TOK + 4 * (x / 16) + lane / 8);
+                if ((*(const volatile uint8_t*)(v + 512 * (x / 16) + x % 16) & 0x7f) != 0x7f) continue;
+#pragma unroll 1
+                for (uint32_t row = 0; row < rows; row++) {
+                    const int pos = pos0 + (int)((row0 + row) >> a.group_shift);
+                    if (t <= pos && t > pos - window) *(reinterpret_cast<__half*>(out(row) - lane) + 16 * (lane % 8) + x % 16) = __ushort_as_half(0x7fff);
+                }
+            }
+        }
+    };
+    if (DRAFTS && n == 1) {
+        put_nans();
         return;
     }
     const uint32_t shift = SHIFT >= 0 ? SHIFT : rows <= 1 ? 0 : rows <= 2 ? 1 : rows <= 4 ? 2 : 3, mask = (1u << shift) - 1;  // rows up to a power of two
@@ -736,6 +784,10 @@ __global__ void __launch_bounds__(W * 32, W == MANY_CTAS_WARPS ? (E == 8 ? 4 : 8
         const float f = 1.0f / l;  // a row that saw nothing is 0, whatever stands in V
         *out(row) = l != 0.0f ? make_uint2(pack_half2(sum.x * f, sum.y * f), pack_half2(sum.z * f, sum.w * f)) : make_uint2(0u, 0u);
     }
+    if (DRAFTS && last - first > 1) {
+        __syncthreads();  // other warps wrote some of the rows
+        put_nans();
+    }
 }
 
 // Warps that fit the GPU at once, and what every kv head gets of them.
@@ -745,7 +797,7 @@ uint32_t grid_ctas(int sm_count, uint32_t n_kv, int ctas_per_sm)
     return ctas > least ? ctas : least;
 }
 
-template <int NB>
+template <int NB, bool DRAFTS>
 int launch_decode(const LaunchArgs& a, const BlocksAttn& k, const CUtensorMap (&tm)[2], const Work& w, uint32_t ctas, uint32_t most)
 {
     const size_t smem = sizeof(DecodeSmem<NB>) + 1024;
@@ -755,13 +807,13 @@ int launch_decode(const LaunchArgs& a, const BlocksAttn& k, const CUtensorMap (&
         static bool attr_set[64] = {};
         std::lock_guard<std::mutex> lock(attr_mutex);
         if (a.device < 0 || a.device >= 64 || !attr_set[a.device]) {
-            if (int r = check_cuda(a, cudaFuncSetAttribute(blocks_decode_kernel<NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+            if (int r = check_cuda(a, cudaFuncSetAttribute(blocks_decode_kernel<NB, DRAFTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
                                    "cudaFuncSetAttribute(blocks_decode)"))
                 return r;
             if (a.device >= 0 && a.device < 64) attr_set[a.device] = true;
         }
     }
-    const cudaError_t e = launch_dependent(blocks_decode_kernel<NB>, dim3(ctas), dim3(WARPS * 32), smem, a.stream, tm[0], tm[1], k, w, most);
+    const cudaError_t e = launch_dependent(blocks_decode_kernel<NB, DRAFTS>, dim3(ctas), dim3(WARPS * 32), smem, a.stream, tm[0], tm[1], k, w, most);
     ++*a.launches;
     return check_cuda(a, e, "attn_blocks decode");
 }
@@ -792,16 +844,20 @@ int launch_blocks_decode(const LaunchArgs& a, const BlocksAttn& k, const BlocksW
     const uint32_t most_rows = k.few * k.group, ctas = grid_ctas(a.sm_count, k.n_kv, ctas_per_sm(most_rows)), most = ctas * WARPS / k.n_kv;
     Work w{head, nullptr, reinterpret_cast<float4*>(head.parts), part_rows(most_rows, k.group, k.req.max_q)};
     w.ml = reinterpret_cast<float2*>(w.acc + 2ull * most * k.n_kv * w.rows * (HD / 4));
-    if (int r = most_rows <= 8 ? launch_decode<1>(a, k, tm, w, ctas, most) : launch_decode<2>(a, k, tm, w, ctas, most)) return r;
+    const bool drafts = k.req.max_q > 1;
+    if (int r = most_rows > 8 ? launch_decode<2, true>(a, k, tm, w, ctas, most) : drafts ? launch_decode<1, true>(a, k, tm, w, ctas, most) : launch_decode<1, false>(a, k, tm, w, ctas, most))
+        return r;
     // Few CTAs have many parts each (one request of 131072 keys: 148 of every head; 9.4 us with four warps a CTA).
     const uint32_t row_blocks = (w.rows + 7) / 8;
     const bool few = (uint64_t)k.req.n * k.n_kv * row_blocks <= 2u * (uint32_t)a.sm_count;
     const dim3 grid(k.req.n + (k.req.max_q > k.few ? 1 : 0), k.n_kv, row_blocks);
-    const auto merge = [&](auto shift) {
+    const auto merge_of = [&](auto shift, auto with_drafts) {
         constexpr int SHIFT = decltype(shift)::value, WARPS_IF_FEW = SHIFT < 0 ? FEW_CTAS_WARPS / 2 : FEW_CTAS_WARPS;
-        return few ? launch_dependent(blocks_merge_kernel<8, WARPS_IF_FEW, SHIFT>, grid, dim3(WARPS_IF_FEW * 32), 0, a.stream, k, w)
-                   : launch_dependent(blocks_merge_kernel<SHIFT < 0 ? 8 : 4, MANY_CTAS_WARPS, SHIFT>, grid, dim3(MANY_CTAS_WARPS * 32), 0, a.stream, k, w);
+        constexpr bool DRAFTS = decltype(with_drafts)::value;
+        return few ? launch_dependent(blocks_merge_kernel<8, WARPS_IF_FEW, SHIFT, DRAFTS>, grid, dim3(WARPS_IF_FEW * 32), 0, a.stream, k, w)
+                   : launch_dependent(blocks_merge_kernel<SHIFT < 0 ? 8 : 4, MANY_CTAS_WARPS, SHIFT, DRAFTS>, grid, dim3(MANY_CTAS_WARPS * 32), 0, a.stream, k, w);
     };
+    const auto merge = [&](auto shift) { return drafts ? merge_of(shift, std::true_type()) : merge_of(shift, std::false_type()); };
     const cudaError_t e = w.rows <= 1 ? merge(std::integral_constant<int, 0>()) : w.rows <= 2 ? merge(std::integral_constant<int, 1>())
         : w.rows <= 4 ? merge(std::integral_constant<int, 2>()) : merge(std::integral_constant<int, -1>());
     ++*a.launches;

@@ -46,6 +46,7 @@ struct Item {
     uint32_t valid, request, head, first_tok, toks, piece, pieces, slot, slot0, counter;  // slot, slot0: of this piece's part and of piece 0's
     int first_pos, band_lo, tile0;  // position of the first query, first key that any row sees, first tile of 64 keys
     int n_tiles[2];                 // of either tile of queries; the second has none, or as many as the unit
+    uint32_t nan_met;               // the converting warps: a value that some rows see and others not may be a NaN, and counts as 0 in P V
     __device__ int unit_tiles() const { return max(n_tiles[0], n_tiles[1]); }
     __device__ int last_pos() const { return first_pos + (int)toks - 1; }
 };
@@ -97,7 +98,7 @@ __device__ __forceinline__ void fetch_item(const BlocksAttn& a, const BlocksWork
 {
     const uint32_t lane = threadIdx.x & 31;
     Item it;
-    it.valid = 0;
+    it.valid = it.nan_met = 0;
     uint32_t i = 0, rest = 0, begin = 0, n = 0;  // the item; of one that is cut: its number among those, its first tile and its tiles
     it.piece = it.slot = it.slot0 = it.counter = 0;
     it.pieces = 1;
@@ -179,6 +180,9 @@ __device__ __forceinline__ void fetch_item(const BlocksAttn& a, const BlocksWork
     }
     if (lane == 0) *out = it;
 }
+
+// Keys of a tile of 64 that some rows of the unit see and others may not.
+__device__ __forceinline__ bool crosses_edge(int key0, int first_pos, int last_lo) { return key0 + KEYS - 1 > first_pos || key0 < last_lo; }
 
 // 16 cached bytes as 16 f16 numbers, into two 16-byte chunks of a row.
 __device__ __forceinline__ void put_converted(uint32_t chunk0, uint32_t chunk1, const uint4& raw)
@@ -411,30 +415,53 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t to = half * HALF_TILE + tok * 128, at0 = to + ((c ^ (tok & 7)) << 4), at1 = to + (((c + 1) ^ (tok & 7)) << 4);
         // Keys go two tiles ahead of values: Q K^T(j + 2) is issued right behind P V(j), so the order is K(0) K(1) V(0) K(2) V(1) K(3) ...
         // (in step, a tile's K behind the V before it, the tensor pipe waited 540 cycles a tile for K; a chunk of 2048 tokens 2055 us).
+        const int window = a.req.window && a.req.window < MOST_KEYS ? (int)a.req.window : (int)MOST_KEYS;
         uint32_t key = 0;  // tiles of keys before this item
         for (; const Item* it = next_item();) {
-            const int tiles = it->unit_tiles(), tile0 = it->tile0, band_lo = it->band_lo, last_pos = it->last_pos();
+            const int tiles = it->unit_tiles(), tile0 = it->tile0, band_lo = it->band_lo, last_pos = it->last_pos(), first_pos = it->first_pos;
+            const int last_lo = max(last_pos + 1 - window, 0);
+            const uint32_t nan_met = smem_u32(&it->nan_met);  // (the softmax warps keep the item until they have read it)
             done_item();
-            auto convert = [&](int side, int j) {
-                const int key0 = (tile0 + j) * KEYS + (int)tok;
-                const bool edge = (tile0 + j + 1) * KEYS - 1 > last_pos || (tile0 + j) * KEYS < band_lo;
+            auto fetch = [&](int side, int j, uint4 (&d)[4]) {
                 const uint32_t raw = smem_u32(sm.raw[(key + j) % RAW][side][0]) + from;
-                uint4 d[4];
 #pragma unroll
-                for (int x = 0; x < 4; x++) {
+                for (int x = 0; x < 4; x++)
                     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                                  : "=r"(d[x].x), "=r"(d[x].y), "=r"(d[x].z), "=r"(d[x].w)
                                  : "r"(raw + x * TILE_BYTES)
                                  : "memory");
-                    // what no query sees counts as 0: its weight is 0, but 0 times a NaN that stands there would not be
-                    if (edge && (key0 + 16 * x > last_pos || key0 + 16 * x < band_lo)) d[x] = make_uint4(0u, 0u, 0u, 0u);
-                }
+            };
+            auto put = [&](int side, int j, const uint4 (&d)[4]) {
                 const uint32_t out = smem_u32(side ? sm.v[(key + j) & 1][0] : sm.k[(key + j) & 1][0]);
 #pragma unroll
                 for (int x = 0; x < 4; x++) put_converted(out + at0 + x * 2048, out + at1 + x * 2048, d[x]);
+            };
+            auto done = [&](int side, int j) {
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(side ? &sm.full_v[(key + j) & 1] : &sm.full_k[(key + j) & 1]);
+            };
+            auto convert = [&](int side, int j) {
+                uint4 d[4];
+                fetch(side, j, d);
+                put(side, j, d);
+                done(side, j);
+            };
+            // Of values that not every row sees: those that none sees count as 0 (their weight is 0, but 0 times a NaN that stands there would not be), and so
+            // do NaNs, which get into the rows that see them at their end.  (Keys need neither: a score that is masked is none, whatever it was.)
+            auto convert_edge = [&](int j) {
+                const int key0 = (tile0 + j) * KEYS + (int)tok;
+                uint4 d[4];
+                fetch(1, j, d);
+                bool any = false;
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    if (key0 + 16 * x > last_pos || key0 + 16 * x < band_lo) d[x] = make_uint4(0u, 0u, 0u, 0u);
+                    any |= drop_nans(d[x]);
+                }
+                if (any) asm volatile("st.shared.u32 [%0], %1;" ::"r"(nan_met), "r"(1) : "memory");
+                put(1, j, d);
+                done(1, j);
             };
             auto keys = [&](int j) {
                 mbar_wait_warp(&sm.raw_full[(key + j) % RAW], ((key + j) / RAW) & 1, status, 651, failed);
@@ -446,7 +473,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int j = 0; j < tiles && !failed; ++j) {
                 if (key + j >= 2) mbar_wait_warp(&sm.v_free[(key + j) & 1], phase(key + j - 2), status, 646, failed, 20);
                 if (failed) break;
-                convert(1, j);
+                if (crosses_edge((tile0 + j) * KEYS, first_pos, last_lo)) convert_edge(j); else convert(1, j);
                 if (lane == 0) mbar_arrive(&sm.raw_empty[(key + j) % RAW]);
                 if (j + 2 < tiles) keys(j + 2);
             }
@@ -611,6 +638,22 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                     for (int x = 0; x < 8; x++)
                         part(it.slot)[(8 * c + x) * ROWS] = make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]), __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
+                }
+            }
+            // NaNs that the converting warps took out, at keys that this row sees: into what it has written (its row by other threads of the warp).
+            if (live && *(const volatile uint32_t*)&at->nan_met) {
+                const uint32_t request = at->request;
+#pragma unroll 1
+                for (int x = max(tile0 * KEYS, row_lo); x <= min((tile0 + tiles) * KEYS - 1, pos); x++) {
+                    if (!crosses_edge(x / KEYS * KEYS, it.first_pos, last_lo)) continue;
+                    const size_t block = block_of_page(a.req, request, (uint32_t)x / TILE_TOK, ld_global(page_at(a.req, request, (uint32_t)x / TILE_TOK)));
+                    const uint8_t* v = a.pool[1] + (block * a.n_kv + it.head) * TILE_BYTES + x % TILE_TOK * HD;
+#pragma unroll 1
+                    for (uint32_t d = 0; d < (uint32_t)HD; d++) {
+                        if ((*(const volatile uint8_t*)(v + d) & 0x7f) != 0x7f) continue;
+                        if (whole) a.out[((size_t)(it.first_tok + tok) * (a.n_kv * a.group) + it.head * a.group + ((uint32_t)r & (a.group - 1))) * HD + d] = __ushort_as_half(0x7fff);
+                        else reinterpret_cast<float*>(part(it.slot) + d / 4 * ROWS)[d % 4] = __int_as_float(0x7fffffff);
+                    }
                 }
             }
             if (!whole) {

@@ -133,6 +133,15 @@ __device__ __forceinline__ uint32_t f16x2_to_e4m3x2(uint32_t x)
     asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(x));
     return r;
 }
+// The bytes of four e4m3 numbers that are a NaN (0x7f, 0xff): 0x80 in each of those.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+// Those of 16 numbers become 0: whether there are any.
+__device__ __forceinline__ bool drop_nans(uint4& v)
+{
+    const uint32_t x = nan_bytes(v.x), y = nan_bytes(v.y), z = nan_bytes(v.z), w = nan_bytes(v.w);
+    v = make_uint4(v.x & ~((x >> 7) * 0xffu), v.y & ~((y >> 7) * 0xffu), v.z & ~((z >> 7) * 0xffu), v.w & ~((w >> 7) * 0xffu));
+    return (x | y | z | w) != 0;
+}
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
 __device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
 

@@ -15,8 +15,8 @@ namespace sgb {
 constexpr uint32_t UNIT_ROWS = 256, UNIT_KEYS = 64;
 // Weights are 2^(s - m), f16 in the second product.  m is found anew where a score exceeds it by GROWTH_T, and stands LIFT below the row's
 // largest then, so that the largest weight is between 2^7 and 2^15.  f16's normal range thus reaches from 2^-21 of the largest on: V's powers of two are in
-// the weights, and a tile of small values beside one of large ones keeps its digits (with m at the maximum, values whose scale was 2^-18 of the largest
-// were off by up to a tenth and more in dims where the large tile held nothing).
+// the weights, and a tile of small values beside one of large ones keeps its digits (with m at the maximum, values whose scale was 2^-18 of the largest,
+// in dims where the large tile holds nothing, were off by a tenth or more in a tenth of the results).
 constexpr float LIFT = 7.0f, GROWTH_T = 15.0f;
 constexpr uint32_t MOST_SORTED = 2048, MOST_PLACES = 256;
 

@@ -84,3 +84,45 @@ def _outliers(b, dims):
 def test_values_beside_tiles_of_much_larger_scale(ctx, lens, new, kv, group):  # noqa: F811
     """Dims in which the tiles of the largest scale hold nothing keep what the others hold: their weights are 2^-16 to 2^-18 of the largest."""
     check(ctx, _outliers(Batch(1, lens, new, kv, group, 32), 8))
+
+
+def _nan_at(b, r, tokens, side, share):
+    """NaNs of either sign in tokens of a request: in a share of V's dims, or in all of K's."""
+    rows = ref.rows_of(b.table[r], int(b.lens[r]), b.page)[np.asarray(tokens)]
+    pool = b.vp if side == "v" else b.kp
+    at = b.rng.random((len(rows), b.kv, D)) < share
+    codes = pool[rows // TILE, :, rows % TILE]
+    pool[rows // TILE, :, rows % TILE] = np.where(at, b.rng.choice([0x7F, 0xFF], at.shape), codes)
+
+
+@pytest.mark.parametrize("side", ["v", "k"])
+@pytest.mark.parametrize("window", [0, 3, 40])
+@pytest.mark.parametrize("lens,new,kv,group", [
+    ([4, 50, 1037, 21], [4, 4, 2, 3], 3, 2), ([8, 50, 1037, 23], [8, 7, 8, 1], 2, 1), ([8, 50, 4037, 23], [8, 7, 8, 2], 3, 2), ([16, 50, 1037, 21], [16, 9, 13, 1], 2, 1),
+    ([70, 100, 900, 65], [70, 33, 64, 1], 2, 1), ([300, 333, 1000, 64], [300, 129, 200, 3], 2, 2), ([5000, 200, 1300, 60], [300, 40, 31, 40], 2, 4)])
+def test_nan_reaches_the_rows_that_see_it(ctx, lens, new, kv, group, window, side):  # noqa: F811
+    """A NaN in a token's value is in the results of the rows that see that token, in its dims; one in a key in all dims of those rows.  The
+    rows before it, and those whose window has passed it, are as they would be without."""
+    b = Batch(7, lens, new, kv, group, 16, spare_rows=2)
+    clean = b.kp.copy(), b.vp.copy()
+    tokens = []
+    for r, (n, m) in enumerate(zip(lens, new)):
+        t = {n - 1, n - m, n - 1 - m // 2, max(0, n - m - 2), max(0, n - max(window, 1) - m // 3)} if r != 2 else {n - 1, max(0, n - m - window + 1)}
+        tokens.append(sorted(t))
+        _nan_at(b, r, tokens[r], side, 0.3 if side == "v" else 1.0)
+    poisoned = b.vp if side == "v" else b.kp
+    nan = np.zeros(b.q.shape, bool)
+    for r, (n, m) in enumerate(zip(lens, new)):
+        rows = ref.rows_of(b.table[r], n, b.page)[tokens[r]]
+        pos, t = n - m + np.arange(m)[:, None], np.array(tokens[r])[None, :]
+        seen = (t <= pos) & ((t > pos - window) if window else True)
+        codes = (poisoned[rows // TILE, :, rows % TILE] & 127) == 127  # [token, kv, dim]
+        hit = np.einsum("mt,thd->mhd", seen.astype(int), codes) > 0
+        nan[int(b.starts[r]):int(b.starts[r]) + m] = np.repeat(hit, group, 1)
+    got = run(ctx, b, window)
+    n = int(b.starts[-1])
+    (b.kp, b.vp), poison = clean, (b.kp, b.vp)
+    want, bound = attend(b, window)
+    wrong = np.isnan(got[:n]) != nan[:n]
+    assert not wrong.any(), f"{wrong.sum()} of {wrong.size}, {nan[:n].sum()} are NaN; first at {np.argwhere(wrong)[0].tolist()}"
+    assert (np.abs(got - want)[:n][~nan[:n]] <= bound[:n][~nan[:n]]).all()
