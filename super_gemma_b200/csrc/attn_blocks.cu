@@ -6,7 +6,7 @@
 //
 // Requests of few rows (query tokens x heads of a group) are decoded (attn_blocks_decode.cu), the others prefilled
 // (attn_blocks_prefill.cu); a dispatch that names no request of more than 16 rows launches the decode alone.
-#include <cmath>
+#include <algorithm>
 
 #include "blocks.cuh"
 #include "blocks_work.cuh"
@@ -28,6 +28,10 @@ uint32_t rows_decoded(uint32_t group, uint32_t max_q)
     const uint64_t rows = (uint64_t)group * max_q;
     return rows <= 8 || rows > FEW_ROWS ? 8 : 16;
 }
+
+// A query with a key reaches 2^39 (128 products of f16 numbers), so below 2^-80 all scores lie within 2^-39 of each other and the weights are equal in f32
+// whatever the scale: it is taken as that.  Times a tile's power of two a smaller one could become 0, and 0 times the -inf of a masked score is a NaN.
+constexpr float LEAST_SCALE = 0x1p-80f, MOST_SCALE = 0x1p100f;
 
 }  // namespace
 
@@ -51,7 +55,7 @@ int launch_attn_blocks(const LaunchArgs& a)
     if (p.group != 1 && p.group != 2 && p.group != 4 && p.group != 8) return fail_validation(a, "attn_blocks: query heads per kv head must be 1, 2, 4 or 8");
     if (p.page < (uint32_t)TILE_TOK || (p.page & (p.page - 1))) return fail_validation(a, "attn_blocks: page must be a power of two, at least 16 tokens");
     if (p.stride == 0 || p.max_q == 0) return fail_validation(a, "attn_blocks: the table's stride and the most query tokens must be > 0");
-    if (!(p.scale > 0.0f) || !std::isfinite(p.scale)) return fail_validation(a, "attn_blocks: the softmax scale must be positive");
+    if (!(p.scale > 0.0f && p.scale <= MOST_SCALE)) return fail_validation(a, "attn_blocks: the softmax scale must be positive, and at most 2^100");
     const size_t tile_row = (size_t)n_kv * TILE_BYTES, rows = (size_t)tokens * n_kv * p.group;
     const size_t blocks = a.b[1].bytes / tile_row;
     if (blocks == 0 || a.b[3].bytes / tile_row != blocks)
@@ -72,7 +76,7 @@ int launch_attn_blocks(const LaunchArgs& a)
     const BlocksAttn k{{(const uint32_t*)a.b[5].ptr, (const uint32_t*)a.b[6].ptr, (const uint32_t*)a.b[7].ptr, n, p.stride, shift,
                         (uint32_t)(blocks >> (shift - 4)), tokens, p.max_q, p.window, a.status},
                        (const __half*)a.b[0].ptr, {(const uint8_t*)a.b[1].ptr, (const uint8_t*)a.b[3].ptr}, {(const int8_t*)a.b[2].ptr, (const int8_t*)a.b[4].ptr},
-                       (__half*)a.b[8].ptr, n_kv, p.group, (uint32_t)__builtin_ctz(p.group), (uint32_t)(blocks * n_kv), rows_decoded(p.group, p.max_q) / p.group, p.scale};
+                       (__half*)a.b[8].ptr, n_kv, p.group, (uint32_t)__builtin_ctz(p.group), (uint32_t)(blocks * n_kv), rows_decoded(p.group, p.max_q) / p.group, std::max(p.scale, LEAST_SCALE)};
     const BlocksWork work = blocks_work_at((uint8_t*)a.b[9].ptr, n, blocks_places(a.sm_count));
     if (int r = launch_blocks_decode(a, k, work)) return r;
     return (uint64_t)p.max_q * p.group > FEW_ROWS ? launch_blocks_prefill(a, k, work) : 0;

@@ -126,3 +126,14 @@ def test_nan_reaches_the_rows_that_see_it(ctx, lens, new, kv, group, window, sid
     wrong = np.isnan(got[:n]) != nan[:n]
     assert not wrong.any(), f"{wrong.sum()} of {wrong.size}, {nan[:n].sum()} are NaN; first at {np.argwhere(wrong)[0].tolist()}"
     assert (np.abs(got - want)[:n][~nan[:n]] <= bound[:n][~nan[:n]]).all()
+
+
+@pytest.mark.parametrize("scale", [1.5e-45, 1e-43, 1e-38, 1e-20])
+def test_scales_that_make_all_weights_equal(ctx, scale):  # noqa: F811
+    for new in ([1, 3, 1], [8, 5, 1], [70, 200, 1]):
+        b = Batch(3, [max(n, m) for n, m in zip([90, 200, 1000], new)], new, 2, 2, 16)
+        b.ke[b.ke != 127] = -15
+        scale = float(np.float32(scale))
+        want, bound = attend(b, 40, scale)
+        got = run(ctx, b, 40, scale)
+        assert np.isfinite(got).all() and (np.abs(got - want) <= bound).all()
