@@ -33,11 +33,15 @@ uint32_t rows_decoded(uint32_t group, uint32_t max_q)
 // whatever the scale: it is taken as that.  Times a tile's power of two a smaller one could become 0, and 0 times the -inf of a masked score is a NaN.
 constexpr float LEAST_SCALE = 0x1p-80f, MOST_SCALE = 0x1p100f;
 
+// What the grid and the push may say of heads and requests; the launcher names what it refuses.
+constexpr uint32_t MOST_KV = 1024;
+bool group_is_served(uint32_t group) { return group == 1 || group == 2 || group == 4 || group == 8; }
+
 }  // namespace
 
 size_t attn_blocks_work_bytes(int sm_count, uint32_t n_kv, uint32_t group, uint32_t requests, uint32_t tokens, uint32_t max_q)
 {
-    if (n_kv == 0 || group == 0 || group > 8 || requests == 0 || tokens == 0 || max_q == 0) return 0;
+    if (n_kv == 0 || n_kv > MOST_KV || !group_is_served(group) || requests == 0 || requests > MOST_REQUESTS || tokens == 0 || max_q == 0) return 0;
     const size_t few = blocks_decode_work(sm_count, n_kv, group, max_q);
     const size_t many = (uint64_t)max_q * group > FEW_ROWS ? blocks_prefill_work(sm_count) : 0;
     return blocks_work_header(requests, blocks_places(sm_count)) + (few > many ? few : many);
@@ -50,9 +54,9 @@ int launch_attn_blocks(const LaunchArgs& a)
     const PushAttnBlocks p = *(const PushAttnBlocks*)a.push;
     const uint32_t n_kv = a.groups[0], n = a.groups[1], tokens = a.groups[2];
     if (n_kv == 0 || n == 0 || tokens == 0) return fail_validation(a, "attn_blocks: groups must be [kv heads, requests, query tokens]");
-    if (n_kv > 1024) return fail_validation(a, "attn_blocks: at most 1024 kv heads");
+    if (n_kv > MOST_KV) return fail_validation(a, "attn_blocks: at most 1024 kv heads");
     if (n > MOST_REQUESTS) return fail_validation(a, "attn_blocks: at most 65536 requests");
-    if (p.group != 1 && p.group != 2 && p.group != 4 && p.group != 8) return fail_validation(a, "attn_blocks: query heads per kv head must be 1, 2, 4 or 8");
+    if (!group_is_served(p.group)) return fail_validation(a, "attn_blocks: query heads per kv head must be 1, 2, 4 or 8");
     if (p.page < (uint32_t)TILE_TOK || (p.page & (p.page - 1))) return fail_validation(a, "attn_blocks: page must be a power of two, at least 16 tokens");
     if (p.stride == 0 || p.max_q == 0) return fail_validation(a, "attn_blocks: the table's stride and the most query tokens must be > 0");
     if (!(p.scale > 0.0f && p.scale <= MOST_SCALE)) return fail_validation(a, "attn_blocks: the softmax scale must be positive, and at most 2^100");
