@@ -1,4 +1,4 @@
-"""GPU tests of the batched cache's attention against bounds that an output of zeros, or of another sign, misses.
+"""GPU tests of the batched cache's attention and append against bounds that an output of zeros, or of another sign, misses.
 
 ``bound`` weighs what each key's score may be off by with that key's own weight, and counts f16 weights from the largest one that a row
 has: they stand 2^7 above one where a row's maximum is found, so what f16's subnormal grid (2^-25, half a step) takes from a weight is at
@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 
 import blocks_ref as ref
-from test_gpu_blocks import Batch, D, SCALE, TILE, ctx  # noqa: F401
+from test_gpu_blocks import Batch, D, SCALE, TILE, _pool, _run_append, ctx  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -137,3 +137,74 @@ def test_scales_that_make_all_weights_equal(ctx, scale):  # noqa: F811
         want, bound = attend(b, 40, scale)
         got = run(ctx, b, 40, scale)
         assert np.isfinite(got).all() and (np.abs(got - want) <= bound).all()
+
+
+def _peaked(b, q):
+    """Scores of deviation 10 and more: few keys carry a row."""
+    b.q = (b.q * np.float16(q)).astype(np.float16)
+    return b
+
+
+@pytest.mark.parametrize("lens,new,kv,group", [([500, 33, 2000], [1, 4, 1], 2, 2), ([500, 2000, 35], [16, 16, 1], 2, 1), ([500, 2000, 35], [8, 7, 1], 2, 2),
+                                               ([500, 233, 3000], [130, 70, 300], 2, 2), ([500, 233], [130, 70], 2, 8)])
+@pytest.mark.parametrize("window", [0, 100])
+def test_peaked_softmaxes(ctx, lens, new, kv, group, window):  # noqa: F811
+    check(ctx, _peaked(Batch(2, lens, new, kv, group, 32), 4), window)
+
+
+@pytest.mark.parametrize("lens,new,kv,group", [([500, 33, 2000], [1, 4, 1], 2, 2), ([500, 2000, 35], [16, 16, 1], 2, 1), ([500, 2000, 35], [4, 4, 1], 2, 4),
+                                               ([500, 233, 3000], [130, 70, 300], 2, 2), ([500, 233], [130, 70], 2, 8)])
+def test_values_of_all_scales(ctx, lens, new, kv, group):  # noqa: F811
+    """V's exponents anywhere between the ends of the format."""
+    b = Batch(4, lens, new, kv, group, 32)
+    real = b.ve != 127
+    b.ve[real] = b.rng.integers(-15, 8, int(real.sum()))
+    check(ctx, b)
+
+
+def test_more_units_than_are_sorted(ctx):  # noqa: F811
+    """Over 2048 units a head, over 1024 requests: units stand in the requests' order.  Requests of no token, of one, and refused ones between them."""
+    rng = np.random.default_rng(21)
+    requests = 2600
+    new = rng.integers(9, 18, requests)
+    new[rng.random(requests) < 0.1] = 1
+    new[rng.random(requests) < 0.05] = 0
+    new[[700, 1900]] = 300, 513  # several units each
+    lens = np.maximum(new + rng.integers(0, 40, requests), 1)
+    dead = set(np.flatnonzero(rng.random(requests) < 0.03).tolist()) - {700, 1900}
+    assert sum(-(-int(m) // 256) for m in new if m > 8) > 2048
+    check(ctx, Batch(21, lens, new, 3, 1, 16, spare_rows=3, dead=dead))
+
+
+@pytest.mark.parametrize("many", [False, True])
+def test_heads_whose_units_stand_together(ctx, many):  # noqa: F811
+    """Prompts whose keys and values are more than 96 MiB: a head's units follow each other.  Every unit is cut, or most are whole items and more than
+    are sorted."""
+    kv = 16
+    lens, new = [25700, 700, 40], [72, 1, 40]
+    if many:
+        rng = np.random.default_rng(22)
+        new = np.concatenate([rng.integers(9, 12, 2100), new])
+        lens = np.concatenate([new[:-3] + rng.integers(0, 20, 2100), lens])
+    assert sum(int(n) // 1024 for n, m in zip(lens, new) if m > 8) * 1024 * kv * 2 * D > 96 << 20
+    check(ctx, Batch(22, lens, new, kv, 1, 64, spare_rows=1, dead=(5, 9) if many else ()))
+
+
+def test_append_of_nan_and_infinity_keeps_the_rest_of_the_tile(ctx):  # noqa: F811
+    """Rows before the run are rounded again for the exponent that infinity calls for, rows behind it are left."""
+    for kv, first, n in ((1, 4, 2), (3, 0, 5), (3, 9, 7), (2, 15, 1)):
+        rng = np.random.default_rng(first)
+        k, v = (rng.standard_normal((n, kv, D)).astype(np.float16) for _ in range(2))
+        k[0, 0, :4] = [np.nan, np.inf, -np.inf, 65504]
+        v[-1, -1, 5:8] = [-np.inf, -np.nan, 1]
+        pools = [*_pool(1, 3, kv), *_pool(2, 3, kv)]
+        for p in pools[::2]:
+            p[1, 0, 0, 0] = 0x7F  # one that was there
+        slots = np.arange(n) + TILE + first
+        got = _run_append(ctx, k, v, slots, pools, kv)
+        ref.append(k, slots, *pools[:2])
+        ref.append(v, slots, *pools[2:])
+        for g, w in zip(got, pools):
+            if g.dtype == np.uint8:  # a NaN's sign is nobody's
+                g, w = np.where((g & 127) == 127, 0x7F, g), np.where((w & 127) == 127, 0x7F, w)
+            assert np.array_equal(g, w)
