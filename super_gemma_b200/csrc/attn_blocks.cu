@@ -22,7 +22,7 @@ struct PushAttnBlocks {
 };
 
 // Rows up to which a request is decoded: 8 or 16, as the most that the dispatch names need, and 8 beside prompts, for the single tokens' sake.
-// (16 drafts of 2 to 4 tokens, four heads a group, up to 32768 keys: 97 us, as prompts 160; of two heads, 4 to 8 tokens 180 and 256.)
+// (16 drafts of 2 to 4 tokens, four heads a group, up to 32768 keys: 99 us, as prompts 160; of two heads, 4 to 8 tokens 185 and 256.)
 uint32_t rows_decoded(uint32_t group, uint32_t max_q)
 {
     const uint64_t rows = (uint64_t)group * max_q;

@@ -10,12 +10,13 @@
 // One tile: S = K Q^T with the 16 tokens as M and eight query rows (or twice eight) as N of mma.sync m16n8k16 (far below tcgen05's 64
 // rows), e4m3 -> f16 exactly on the way from shared memory (ldmatrix, one conversion a pair), O^T += V^T P^T with 16 dims as M.
 // The powers of two never touch the elements: K's multiplies the scores, V's goes into the exponent, P' = 2^(s + e_v - m),
-// and out of the sum again, l += P' 2^-e_v.  Softmax in base 2 with a running maximum that is raised when it grows by more than 2^8:
+// and out of the sum again, l += P' 2^-e_v.  P' goes into the second product as f16, 2^-11 of itself off at most in f16's normal range (LIFT says how far
+// that reaches); l takes it unrounded.  Softmax in base 2 with a running maximum that is raised when it grows by more than 2^8:
 // every lane compares its own scores with it, a row's maximum over the lanes is found only where one is that much larger (three shuffles
 // a tile and row, and the wait for them: 64 requests 114 us, 107 without).
-// Bound by the cache's bytes: 2 x 128 1/16 per token and kv head.  16 kv heads, two query heads each: 64 requests of 256 to 8192 keys 107 us
-// (5.6 TB/s; 6.2 in this kernel, the merge is 6 us), one of 131072 96 us, drafts of 2 to 4 tokens over up to 32768 keys in 16 requests 138 us
-// (5.6 TB/s), one of 1000 keys 10.3 us.  Two blocks of rows are bound by their warps' own latency: drafts of 4 to 8 tokens 180 us (4.3 TB/s).
+// Bound by the cache's bytes: 2 x 128 1/16 per token and kv head.  16 kv heads, two query heads each: 64 requests of 256 to 8192 keys 108 us
+// (5.5 TB/s; 6.3 in this kernel, the merge is 7 to 8 us by itself), one of 131072 96 to 98 us, drafts of 2 to 4 tokens over up to 32768 keys in 16 requests
+// 140 us (5.5 TB/s), one of 1000 keys 11.5 us.  Two blocks of rows are bound by their warps' own latency: drafts of 4 to 8 tokens 185 us (4.2 TB/s).
 #include <mutex>
 #include <type_traits>
 
@@ -29,9 +30,9 @@ namespace {
 
 constexpr int HD = 128;
 constexpr int WARPS = 4;
-constexpr uint32_t LEAST_TILES = 2;  // of a stretch: fewer would only mean more to merge (one request of 1000 keys: 12.3 us with 4, 10.3 with 2 and with 1)
-// A request weighs a tile more than it has: its queries to fetch, its result to write.  (256 requests of 17 to 2048 keys: a warp whose
-// stretch was of many short ones ended 11 of 52 us after the median one.)
+constexpr uint32_t LEAST_TILES = 2;  // of a stretch: fewer mean more to merge (one request of 1000 keys, 16 heads: 12.3 us with 4, 11.5 with 2, 11.1 with 1)
+// A request weighs a tile more than it has: its queries to fetch, its result to write.  (256 requests of 17 to 2048 keys: without it
+// the warps with many short ones end last, 61.9 us instead of 57.4.)
 constexpr uint32_t REQUEST_WEIGHT = 1;
 constexpr uint32_t STAGE_BYTES = 2 * TILE_BYTES;
 
@@ -124,7 +125,8 @@ __device__ __forceinline__ Tiles tiles_of(const BlocksAttn& a, const Request& q)
     return Tiles{lo, (q.len + TILE_TOK - 1) / TILE_TOK - lo};
 }
 // `total` tiles in `n` stretches, the first `longer` of them of each + 1 tiles, the others of `each`.  (A division of 64 bits costs some
-// hundred cycles, and this stands before the first copy: with one for every end of a stretch the cut took 3400 of a short call's 12000.)
+// hundred cycles, and this stands before the first copy: with one for every end of a stretch one request of 131072 keys took 102.5 us
+// instead of 98.7.)
 struct Stretches {
     uint64_t each;
     uint32_t n, longer;

@@ -15,7 +15,7 @@
 //
 // Bound by shared memory's port, 192 KB = 1536 cycles per 64 keys and 256 rows (raw bytes in and out 32, f16 tiles 32, operands of Q K^T 96, of
 // P V 32), of the 2000 or so that a tile takes; in long runs by the board's power.  1740 tokens of 65536 keys, 16 kv heads of two query heads:
-// 1835 us, 1.0 PFLOP/s (the f16 kernel reaches 1.05 to 1.1 on cached f16 keys).  128 rows a CTA and two CTAs an SM would convert every key twice
+// 1855 us, 0.99 PFLOP/s (the f16 kernel reaches 1.05 to 1.1 on cached f16 keys).  128 rows a CTA and two CTAs an SM would convert every key twice
 // as often and need 256 KB of the port.
 #include <mutex>
 
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t from = tok * 128 + half * 64 + (lane & 3) * 16;
         const uint32_t to = half * HALF_TILE + tok * 128, at0 = to + ((c ^ (tok & 7)) << 4), at1 = to + (((c + 1) ^ (tok & 7)) << 4);
         // Keys go two tiles ahead of values: Q K^T(j + 2) is issued right behind P V(j), so the order is K(0) K(1) V(0) K(2) V(1) K(3) ...
-        // (in step, a tile's K behind the V before it, the tensor pipe waited 540 cycles a tile for K; a chunk of 2048 tokens 2055 us).
+        // (in step, a tile's K behind the V before it, the tensor pipe waits for K: a chunk of 65536 keys 2055 us, 1905 this way).
         const int window = a.req.window && a.req.window < MOST_KEYS ? (int)a.req.window : (int)MOST_KEYS;
         uint32_t key = 0;  // tiles of keys before this item
         for (; const Item* it = next_item();) {
@@ -628,7 +628,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         if (blank && l_run == 0.0f) h = make_uint4(0u, 0u, 0u, 0u);  // a row that saw nothing is 0, whatever stands in V
                         sm.rows[warp][lane][x] = h;
                     }
-                    // 64 bytes of each of eight rows go out together (a thread's own row by itself met a line a thread: 4700 cycles a unit)
+                    // 64 bytes of each of eight rows go out together (a thread's own row by itself would meet a line a thread)
                     __syncwarp();
 #pragma unroll
                     for (int x = 0; x < 4; x++)

@@ -59,7 +59,7 @@ __device__ __forceinline__ void split_item(uint32_t i, uint32_t total, uint32_t 
 }
 // The first `whole` items go to the places one by one.  Those left over, fewer than there are places, are laid end to end and cut
 // into equal stretches, one per place, of eight tiles at least unless that were fewer stretches than units: a unit has its start and its end to
-// pay for (four units of two tiles in one stretch: the last CTA ended 6 us after the others).
+// pay for (24 requests with three prompts: 87.6 us with fewer stretches than units, 80.3 so).
 __device__ __forceinline__ uint32_t whole_items(uint32_t items, uint32_t places) { return items / places * places; }
 __device__ __forceinline__ uint32_t rest_stretches(uint32_t tiles, uint32_t units, uint32_t places) { return min(max((tiles + 7) / 8, units), places); }
 
