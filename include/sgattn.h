@@ -139,6 +139,19 @@ uint32_t sgb_decode_paged_splits_hint(const sgb_ctx *ctx, uint32_t n_kv_heads, u
 size_t sgb_attn_blocks_work_bytes(const sgb_ctx *ctx, uint32_t n_kv_heads, uint32_t q_per_kv, uint32_t requests, uint32_t n_tokens,
                                   uint32_t max_q);
 
+/* Frequencies of a rotary embedding, for rope_cos_sin: out[i] radians a position, i < pairs, f_i = theta^(-2 i / dims).  For contexts
+ * `factor` times as long as the `trained` tokens they are slowed down: all of them by the factor (LINEAR), or only those that turn rarely over the trained
+ * length.  BY_TURNS: f_i keeps the share clamp((turns_i - slow) / (fast - slow), 0, 1), turns_i = trained f_i / 2 pi, and the rest of it is f_i / factor.
+ * BY_PAIRS: the share falls from 1 to 0 evenly over the pairs, from the last whole pair that turns `fast` times to the first that turns `slow` times.
+ * (Published as position interpolation and as its variants by parts; the magnitude that goes with them is a push word of rope_cos_sin.)
+ * dims is the head's rotated dims (2 pairs), or all of the head's where only its first pairs turn.  Host only, once per model. */
+enum { SGB_ROPE_PLAIN = 0, SGB_ROPE_LINEAR = 1, SGB_ROPE_BY_TURNS = 2, SGB_ROPE_BY_PAIRS = 3 };
+typedef struct sgb_rope_scaling {
+    uint32_t pairs, dims, kind, reserved;
+    double theta, factor, trained, slow, fast;
+} sgb_rope_scaling;
+int sgb_rope_frequencies(const sgb_rope_scaling *scaling, double *out);
+
 /* ---- record once, replay: record_graph / submit_blocking (crates/sg-gpu/src/graph.rs:523-528, */
 /* 640-642).  Between begin and end every sgb_dispatch / sgb_step_write-free call is captured    */
 /* into a CUDA graph instead of running; the graph keeps its buffers alive.  A replay runs the   */

@@ -5,8 +5,8 @@ is the thin host-side mirror of the reference's Rust API that tests and benchmar
 """
 from .gpu import (ABI, LIB_PATH, Bounds, Buffer, BufferBinding, CommandGraph, CudaError, GpuContext, GpuError, GpuTimer,
                   Kernel, KernelBlob, NoDevice, State, StepState, Timeout, UnknownKernel, Validation, kernel_blob, kernels,
-                  lib)
+                  lib, rope_frequencies)
 
 __all__ = ["ABI", "LIB_PATH", "Bounds", "Buffer", "BufferBinding", "CommandGraph", "CudaError", "GpuContext", "GpuError",
            "GpuTimer", "Kernel", "KernelBlob", "NoDevice", "State", "StepState", "Timeout", "UnknownKernel", "Validation",
-           "kernel_blob", "kernels", "lib"]
+           "kernel_blob", "kernels", "lib", "rope_frequencies"]

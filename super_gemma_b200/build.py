@@ -12,7 +12,8 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libsgattn.so")
 SOURCES = ["sgb_runtime.cu", "sgb_registry.cu", "kv_codec.cu", "attn_generic.cu", "attn_decode_paged.cu", "attn_decode_rows.cu",
            "attn_prefill_flash.cu", "attn_prefill_wide.cu", "attn_prefill_int8.cu", "pre_attn.cu", "attn_exchange.cu", "cache2.cu", "kv_blocks.cu",
-           "attn_blocks.cu", "attn_blocks_decode.cu", "attn_blocks_prefill.cu", "mma_probe.cu"]
+           "attn_blocks.cu", "attn_blocks_decode.cu", "attn_blocks_prefill.cu", "rope_rows.cu", "pre_attn_blocks.cu",
+           "block_norms.cu", "kv_read_blocks.cu", "mma_probe.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "--use_fast_math=false",
               "-Xcompiler", "-fPIC"]
 

@@ -145,4 +145,29 @@ __device__ __forceinline__ bool drop_nans(uint4& v)
 __device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
 __device__ __forceinline__ uint32_t as_u32(__half2 x) { return *reinterpret_cast<const uint32_t*>(&x); }
 
+// The least e >= LOWEST_EXP with a <= 448 * 2^e: a = f * 2^k, 1 <= f < 2, 448 = 1.75 * 2^8.
+__device__ __forceinline__ int exponent_for(float a)
+{
+    const uint32_t bits = __float_as_uint(a);
+    const int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return max(e, LOWEST_EXP);
+}
+// 2^e as f16 pair, e in [-24, 15].
+__device__ __forceinline__ __half2 power_of_two(int e) { return __float2half2_rn(__int_as_float((e + 127) << 23)); }
+
+// 2^e in f32, e in [-126, 127].
+__device__ __forceinline__ float exp2_of(int e) { return __int_as_float((e + 127) << 23); }
+// 16 cached numbers as e4m3(q * f).
+__device__ __forceinline__ uint4 round_again(uint4 v, __half2 f)
+{
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const uint32_t lo = f16x2_to_e4m3x2(as_u32(__hmul2(as_half2(e4m3x2_to_f16x2(w[k] & 0xffffu)), f)));
+        const uint32_t hi = f16x2_to_e4m3x2(as_u32(__hmul2(as_half2(e4m3x2_to_f16x2(w[k] >> 16)), f)));
+        w[k] = lo | (hi << 16);
+    }
+    return v;
+}
+
 }  // namespace sgb

@@ -325,33 +325,12 @@ struct AppendArgs {
     uint32_t* status;
 };
 
-// The least e >= LOWEST_EXP with a <= 448 * 2^e: a = f * 2^k, 1 <= f < 2, 448 = 1.75 * 2^8.
-__device__ __forceinline__ int exponent_for(float a)
-{
-    const uint32_t bits = __float_as_uint(a);
-    const int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-    return max(e, LOWEST_EXP);
-}
-// 2^e as f16 pair, e in [-24, 15].
-__device__ __forceinline__ __half2 power_of_two(int e) { return __float2half2_rn(__int_as_float((e + 127) << 23)); }
-
-// Eight f16 numbers as e4m3(x * f); 16 cached ones as e4m3(q * f).
+// Eight f16 numbers as e4m3(x * f).
 __device__ __forceinline__ uint2 quantise(const uint4& x, __half2 f)
 {
     const __half2 top = __float2half2_rn(61440.0f), low = __float2half2_rn(-61440.0f);
     const auto pair = [&](uint32_t w) { return f16x2_to_e4m3x2(as_u32(__hmul2(__hmax2_nan(__hmin2_nan(as_half2(w), top), low), f))); };
     return make_uint2(pair(x.x) | (pair(x.y) << 16), pair(x.z) | (pair(x.w) << 16));
-}
-__device__ __forceinline__ uint4 round_again(uint4 v, __half2 f)
-{
-    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        const uint32_t lo = f16x2_to_e4m3x2(as_u32(__hmul2(as_half2(e4m3x2_to_f16x2(w[k] & 0xffffu)), f)));
-        const uint32_t hi = f16x2_to_e4m3x2(as_u32(__hmul2(as_half2(e4m3x2_to_f16x2(w[k] >> 16)), f)));
-        w[k] = lo | (hi << 16);
-    }
-    return v;
 }
 __device__ __forceinline__ __half2 largest(__half2 m, const uint4& x)  // a NaN loses against a number
 {

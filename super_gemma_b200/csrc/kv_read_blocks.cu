@@ -1,0 +1,116 @@
+// The way back out of the 8-bit cache of blocks.cuh: tokens [from_r, from_r + n_r) of every request as packed f16 rows, n_r = starts[r + 1] - starts[r].
+// value = e4m3 * 2^e is an f16 number for every tile that an append writes, so that nothing is rounded.
+//
+// One byte read and two written per value: bound by bytes.
+#include "blocks.cuh"
+#include "sgb_kernels.h"
+
+namespace sgb {
+
+namespace {
+
+constexpr int THREADS = 256;
+constexpr uint32_t MOST_ROWS = 32;  // of a CTA
+
+struct ReadArgs {
+    const uint8_t* pool[2];
+    const int8_t* exps[2];
+    const uint32_t *table, *from, *starts;
+    __half* out[2];
+    uint32_t n, tokens, n_kv, stride, page_shift, blocks, rows;  // rows of a CTA
+    uint32_t* status;
+};
+
+// Pool row of packed row i, or NO_SLOT.
+__device__ __forceinline__ uint32_t cached_row(const ReadArgs& a, uint32_t i)
+{
+    uint32_t lo = 0, hi = a.n;  // the last request with starts <= i
+    while (hi - lo > 1) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (ld_global(a.starts + mid) <= i) lo = mid; else hi = mid;
+    }
+    const uint32_t first = ld_global(a.starts + lo), end = ld_global(a.starts + lo + 1);
+    if (i < first || i >= end) return NO_SLOT;
+    const uint64_t pos = (uint64_t)ld_global(a.from + lo) + (i - first), page = pos >> a.page_shift;
+    if (page >= a.stride) {
+        report_error(a.status, DEV_ERR_BOUNDS, 641, lo, (uint32_t)pos);
+        return NO_SLOT;
+    }
+    const uint64_t row = ((uint64_t)ld_global(a.table + (size_t)lo * a.stride + page) << a.page_shift) + (pos & ((1u << a.page_shift) - 1));
+    if (row / TILE_TOK >= a.blocks) {
+        report_error(a.status, DEV_ERR_BOUNDS, 642, lo, (uint32_t)(row >> a.page_shift));
+        return NO_SLOT;
+    }
+    return (uint32_t)row;
+}
+
+// Two e4m3 numbers times 2^e as f16.  A tile of an append has e in [-15, 8] and the product is exact; others go through f32.
+__device__ __forceinline__ uint32_t scaled(uint32_t two_bytes, int e)
+{
+    const __half2 q = as_half2(e4m3x2_to_f16x2(two_bytes));
+    if (e >= -24 && e <= 15) return as_u32(__hmul2(q, power_of_two(e)));
+    const float2 f = __half22float2(q);
+    const float by = exp2_of(max(e, -126));  // 448 * 2^-126 is no f16 number either
+    return pack_half2(f.x * by, f.y * by);
+}
+
+__global__ void __launch_bounds__(THREADS) read_blocks_kernel(const __grid_constant__ ReadArgs a)
+{
+    __shared__ uint32_t where[MOST_ROWS];
+    pdl_wait();
+    pdl_launch_dependents();
+    const uint32_t i0 = blockIdx.x * a.rows;
+    if (threadIdx.x < a.rows) where[threadIdx.x] = i0 + threadIdx.x < a.tokens ? cached_row(a, i0 + threadIdx.x) : NO_SLOT;
+    __syncthreads();
+    // half a warp a row of 128: eight bytes a lane
+    const uint32_t lane = threadIdx.x & 15, units = a.rows * a.n_kv * 2;
+    for (uint32_t u = blockIdx.y * (THREADS / 16) + threadIdx.x / 16; u < units; u += gridDim.y * (THREADS / 16)) {
+        const uint32_t row = u % a.rows, rest = u / a.rows, head = rest >> 1, side = rest & 1;
+        const uint32_t at = where[row];
+        if (at == NO_SLOT) continue;
+        const size_t tile = (size_t)(at / TILE_TOK) * a.n_kv + head;
+        const uint2 q = ld_global(reinterpret_cast<const uint2*>(a.pool[side] + tile * TILE_BYTES + at % TILE_TOK * 128 + lane * 8));
+        const int e = ld_global_if(true, a.exps[side] + tile);
+        *reinterpret_cast<uint4*>(a.out[side] + ((size_t)(i0 + row) * a.n_kv + head) * 128 + lane * 8) =
+            make_uint4(scaled(q.x & 0xffffu, e), scaled(q.x >> 16, e), scaled(q.y & 0xffffu, e), scaled(q.y >> 16, e));
+    }
+}
+
+struct PushRead {
+    uint32_t page, stride;
+};
+
+}  // namespace
+
+// kv_read_blocks_e4m3_d128: k pool, k exps, v pool, v exps, table, from, starts, k, v.  push {page, stride}.  grid [KV, requests, rows].
+int launch_kv_read_blocks(const LaunchArgs& a)
+{
+    const PushRead p = *(const PushRead*)a.push;
+    const uint32_t n_kv = a.groups[0], n = a.groups[1], tokens = a.groups[2];
+    if (n_kv == 0 || n == 0 || tokens == 0) return fail_validation(a, "read_blocks: groups must be [kv heads, requests, rows]");
+    if (n_kv > 1024) return fail_validation(a, "read_blocks: at most 1024 kv heads");
+    if (n > MOST_REQUESTS) return fail_validation(a, "read_blocks: at most 65536 requests");
+    if (tokens > 0x7fffffffu) return fail_validation(a, "read_blocks: less than 2^31 rows");
+    if (p.page < (uint32_t)TILE_TOK || (p.page & (p.page - 1))) return fail_validation(a, "read_blocks: page must be a power of two, at least 16 tokens");
+    if (p.stride == 0) return fail_validation(a, "read_blocks: the table's stride must be > 0");
+    const size_t tile_row = (size_t)n_kv * TILE_BYTES, blocks = a.b[0].bytes / tile_row;
+    if (blocks == 0 || a.b[2].bytes / tile_row != blocks)
+        return fail_validation(a, "read_blocks: K and V pools must hold the same (non-zero) number of 16-token blocks");
+    if (blocks > NO_SLOT / TILE_TOK) return fail_validation(a, "read_blocks: a pool holds less than 2^32 rows");
+    if (int r = need_bytes(a, 1, blocks * n_kv, "k exponents")) return r;
+    if (int r = need_bytes(a, 3, blocks * n_kv, "v exponents")) return r;
+    if (int r = need_bytes(a, 4, 4 * (size_t)n * p.stride, "table")) return r;
+    if (int r = need_bytes(a, 5, 4 * (size_t)n, "from")) return r;
+    if (int r = need_bytes(a, 6, 4 * (size_t)n + 4, "starts")) return r;
+    if (int r = need_bytes(a, 7, 256 * (size_t)tokens * n_kv, "k")) return r;
+    if (int r = need_bytes(a, 8, 256 * (size_t)tokens * n_kv, "v")) return r;
+    if (int r = need_aligned(a, {16, 1, 16, 1, 4, 4, 4, 16, 16})) return r;
+    ReadArgs k{{(const uint8_t*)a.b[0].ptr, (const uint8_t*)a.b[2].ptr}, {(const int8_t*)a.b[1].ptr, (const int8_t*)a.b[3].ptr}, (const uint32_t*)a.b[4].ptr,
+               (const uint32_t*)a.b[5].ptr, (const uint32_t*)a.b[6].ptr, {(__half*)a.b[7].ptr, (__half*)a.b[8].ptr}, n, tokens, n_kv, p.stride,
+               (uint32_t)__builtin_ctz(p.page), (uint32_t)blocks, 16, a.status};
+    const cudaError_t e = launch_dependent(read_blocks_kernel, dim3((tokens + k.rows - 1) / k.rows), dim3(THREADS), 0, a.stream, k);
+    ++*a.launches;
+    return check_cuda(a, e, "kv_read_blocks_e4m3_d128");
+}
+
+}  // namespace sgb

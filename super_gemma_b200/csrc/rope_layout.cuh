@@ -1,0 +1,87 @@
+// Which dims of a head a rotary embedding couples, and their rotation.  pairs = rot_dims / 2, a multiple of 8:
+//   layout 0   (i, i + head_dim / 2)   halves of the head; with rot_dims < head_dim the first pairs of each half turn
+//   layout 1   (i, i + rot_dims / 2)   halves of the first rot_dims dims
+//   layout 2   (2 i, 2 i + 1)          neighbours in the first rot_dims dims
+// A head is cut into pieces of 16 dims, two octets each: of eight pairs, so that a rotation stays in a thread, or of eight pairs that do not
+// turn.  The pieces that turn come first.
+#pragma once
+
+#include "sgb_common.cuh"
+
+namespace sgb {
+
+constexpr uint32_t ROPE_LAYOUTS = 3;
+
+struct RopePiece {
+    uint32_t lo, hi;  // first dims of its octets
+    uint32_t pair;    // its first pair
+    bool turns;
+};
+__device__ __forceinline__ RopePiece rope_piece(uint32_t layout, uint32_t piece, uint32_t head_dim, uint32_t pairs)
+{
+    RopePiece p;
+    p.pair = 8 * piece;
+    p.turns = p.pair < pairs;
+    if (layout == 0) {
+        p.lo = 8 * piece;
+        p.hi = head_dim / 2 + 8 * piece;
+    } else if (layout == 1 && p.turns) {
+        p.lo = 8 * piece;
+        p.hi = pairs + 8 * piece;
+    } else {
+        p.lo = 16 * piece;
+        p.hi = 16 * piece + 8;
+    }
+    return p;
+}
+
+__device__ __forceinline__ void load_cos_sin(const float2* row, float (&c)[8], float (&s)[8])  // row on 16 bytes
+{
+    const float4* p = reinterpret_cast<const float4*>(row);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float4 v = ld_global(p + j);
+        c[2 * j] = v.x;
+        s[2 * j] = v.y;
+        c[2 * j + 1] = v.z;
+        s[2 * j + 1] = v.w;
+    }
+}
+
+// The eight pairs of a piece's octets x, y, turned.
+__device__ __forceinline__ void rope_turn(uint32_t layout, float (&x)[8], float (&y)[8], const float (&c)[8], const float (&s)[8])
+{
+    if (layout == 2) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            float(&v)[8] = j < 4 ? x : y;
+            const float a = v[2 * (j & 3)], b = v[2 * (j & 3) + 1];
+            v[2 * (j & 3)] = a * c[j] - b * s[j];
+            v[2 * (j & 3) + 1] = b * c[j] + a * s[j];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float a = x[j], b = y[j];
+            x[j] = a * c[j] - b * s[j];
+            y[j] = b * c[j] + a * s[j];
+        }
+    }
+}
+
+__device__ __forceinline__ void unpack_f16x8(const uint4& u, float (&v)[8])
+{
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float2 f = __half22float2(h[j]);
+        v[2 * j] = f.x;
+        v[2 * j + 1] = f.y;
+    }
+}
+__device__ __forceinline__ uint4 pack_f16x8(const float (&v)[8])
+{
+    return make_uint4(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]), pack_half2(v[4], v[5]), pack_half2(v[6], v[7]));
+}
+
+}  // namespace sgb

@@ -10,6 +10,8 @@
 
 #include <string>
 
+struct sgb_rope_scaling;
+
 namespace sgb {
 
 struct BufView {
@@ -48,6 +50,9 @@ int check_cuda(const LaunchArgs& a, cudaError_t e, const char* what);
 int need_bytes(const LaunchArgs& a, int binding, size_t bytes, const char* what);
 // The alignment in bytes that the kernels' accesses ask of bindings 0, 1, ... (adopted pointers carry no promise of their own).
 int need_aligned(const LaunchArgs& a, std::initializer_list<uint32_t> bytes);
+
+// Whether two tensors of `n` rows share a byte: rows of `wa` and `wb` bytes, `sa` and `sb` apart (with unequal distances: whether their spans do).
+bool rows_meet(const void* pa, size_t sa, size_t wa, const void* pb, size_t sb, size_t wb, size_t n);
 
 // Tensor-map encoder resolved at run time through the CUDA runtime (no link-time libcuda).
 // dims/strides innermost first; strides[i] is the byte stride of dimension i+1.
@@ -149,6 +154,14 @@ int launch_kv_block_tables(const LaunchArgs&);
 int launch_kv_append_blocks(const LaunchArgs&);
 int launch_attn_blocks(const LaunchArgs&);
 size_t attn_blocks_work_bytes(int sm_count, uint32_t n_kv, uint32_t group, uint32_t requests, uint32_t tokens, uint32_t max_q);
+
+// rope_rows.cu, pre_attn_blocks.cu, block_norms.cu, kv_read_blocks.cu: what stands around the attention of a batch
+int rope_frequencies(const sgb_rope_scaling& r, double* out, std::string* err);
+int launch_rope_cos_sin(const LaunchArgs&);
+int launch_rope_qk_f16(const LaunchArgs&);
+int launch_qkv_norm_rope_append_blocks(const LaunchArgs&);
+template <typename R> int launch_block_norms(const LaunchArgs&);  // R: __half, __nv_bfloat16, float
+int launch_kv_read_blocks(const LaunchArgs&);
 
 // mma_probe.cu
 int launch_diag_mma_cycles(const LaunchArgs&);

@@ -6,6 +6,8 @@
 // reference kernels do not take (page table, Q8_0 V, f32 output) get NEW names: an existing
 // binding list never changes meaning.  For those, the number of kv heads is groups[0], so a rank
 // that owns a slice of the heads dispatches the same kernel with a smaller grid.
+#include <cuda_bf16.h>
+
 #include "sgb_kernels.h"
 
 namespace sgb {
@@ -188,6 +190,34 @@ const KernelEntry REGISTRY[] = {
      "push {scale f32, page u32, stride u32, window u32 (0 = none), q_per_kv u32 (1, 2, 4, 8), max_q u32} | grid [KV, R, N]; request r's queries are its last "
      "starts[r+1] - starts[r] <= max_q tokens, causal; rows that see no key are zero, rows behind starts[R] are left",
      launch_attn_blocks, W(8) | W(9)},
+    // ---- what stands around the attention of a batch, for its packed tokens ----------------------------------------------------------
+    {"rope_cos_sin", {256, 1, 1}, 3, 8,
+     "freqs f64[rot/2] (radians a position: sgb_rope_frequencies), positions i32[N], cos_sin f32[N x rot/2 x2] | push {rot_dims u32 (multiple of 16 up to 1024), "
+     "magnitude f32} | grid [N]; cos_sin = magnitude * (cos, sin)(position * freq), angles in 64 bits; a negative position turns back",
+     launch_rope_cos_sin, W(2)},
+    {"rope_qk_f16", {256, 1, 1}, 5, 28,
+     "q f16[N x H x head_dim], k f16[N x KV x head_dim], cos_sin f32[N x rot/2 x2], q_out, k_out (may be q and k) | push {head_dim u32, rot_dims u32, layout u32 "
+     "(0: pairs (i, i + head_dim/2), 1: (i, i + rot/2), 2: (2i, 2i + 1)), token strides u32 of q, k, q_out, k_out in values (0 = dense)} | grid [H, KV (may be 0), N]; "
+     "head_dim and rot_dims multiples of 16; dims that do not turn are copied",
+     launch_rope_qk_f16, W(3) | W(4)},
+    {"qkv_norm_rope_append_blocks_e4m3_d128", {128, 1, 1}, 12, 28,
+     "q f16[N x H x128], q_w f32[128], q_out f16[N x H x128], k f16[N x KV x128], v, k_w f32[128], cos_sin f32[N x rot/2 x2], slots u32[N] (pool rows, 0xffffffff = none: "
+     "the token is left out), k_pool e4m3[row/16 x KV x16x128], k_exps i8[row/16 x KV], v_pool, v_exps | push {rot_dims u32 (multiple of 16 up to 128, 0 = none), layout u32 "
+     "(as rope_qk_f16), plus_one u32, token strides u32 of q, k, v in values (0 = dense), magnitude f32 (of cos_sin)} | grid [H, KV, N]; q: norm, rotation; k: norm, rotation, "
+     "e4m3 * 2^e, e the least >= -15 with 11.336 max|w| magnitude <= 448 * 2^e; v: weightless norm, e = -5; a tile that the call continues keeps a larger e, a smaller "
+     "one grows; slots as in kv_append_blocks_e4m3_d128",
+     launch_qkv_norm_rope_append_blocks, W(2) | W(8) | W(9) | W(10) | W(11)},
+    {"block_norms_f16", {1024, 1, 1}, 7, 20,
+     "y f16[rows x hidden] (a block's output), h f16[rows x hidden] (residual stream), w_post f32[hidden], gate f32, w_pre f32[hidden], h_out (may be h), x f16[rows x hidden] | "
+     "push {post u32 (0: y as it is, 1: normed, 2: no y, h_out not written), gate u32 (0 none, 1 f32[hidden], 2 f32[rows], 3 f32[1]), plus_one u32, scale f32, eps f32} | "
+     "grid [hidden (multiple of 8 up to 16384), rows]; h_out = (h + gate * norm(y, w_post)) * scale, x = norm of that with w_pre",
+     launch_block_norms<__half>, W(5) | W(6)},
+    {"block_norms_bf16", {1024, 1, 1}, 7, 20, "as block_norms_f16 with h and h_out bf16", launch_block_norms<__nv_bfloat16>, W(5) | W(6)},
+    {"block_norms_f32", {1024, 1, 1}, 7, 20, "as block_norms_f16 with h and h_out f32", launch_block_norms<float>, W(5) | W(6)},
+    {"kv_read_blocks_e4m3_d128", {256, 1, 1}, 9, 8,
+     "k_pool, k_exps, v_pool, v_exps (as attn_blocks_e4m3_d128), table u32[R x stride], from u32[R], starts u32[R+1], k f16[N x KV x128], v | push {page u32, stride u32} | "
+     "grid [KV, R, N]; packed row starts[r] + i = token from[r] + i of request r; rows that no request has are left",
+     launch_kv_read_blocks, W(7) | W(8)},
     // ---- measurement aid -----------------------------------------------------------------------------------------
     {"diag_mma_cycles", {64, 1, 1}, 1, 8,
      "cycles u64[2 x SMs x groups[0]] (per CTA: cycles until n_mma back-to-back tcgen05.mma completed, cycles until they were issued) | "

@@ -76,6 +76,15 @@ int need_aligned(const LaunchArgs& a, std::initializer_list<uint32_t> bytes)
     return SGB_OK;
 }
 
+bool rows_meet(const void* pa, size_t sa, size_t wa, const void* pb, size_t sb, size_t wb, size_t n)
+{
+    const uintptr_t a = reinterpret_cast<uintptr_t>(pa), b = reinterpret_cast<uintptr_t>(pb);
+    if (n == 0 || wa == 0 || wb == 0 || a + (n - 1) * sa + wa <= b || b + (n - 1) * sb + wb <= a) return false;
+    if (sa != sb) return true;  // (or not: told apart from nothing, and refused)
+    const size_t off = a <= b ? (b - a) % sa : (sa - (a - b) % sa) % sa;  // where b's rows begin in a's
+    return off < wa || sa - off < wb;
+}
+
 // cuTensorMapEncodeTiled, looked up through the runtime so the library has no link-time
 // dependency on libcuda (it must load, and export its symbols, on a machine without a driver).
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -331,6 +340,14 @@ uint32_t sgb_decode_paged_splits_hint(const sgb_ctx* c, uint32_t n_kv_heads, uin
 size_t sgb_attn_blocks_work_bytes(const sgb_ctx* c, uint32_t n_kv_heads, uint32_t q_per_kv, uint32_t requests, uint32_t n_tokens, uint32_t max_q)
 {
     return attn_blocks_work_bytes(c && c->sm_count > 0 ? c->sm_count : 148, n_kv_heads, q_per_kv, requests, n_tokens, max_q);
+}
+
+int sgb_rope_frequencies(const sgb_rope_scaling* scaling, double* out)
+{
+    if (!scaling || !out) return set_error(SGB_ERR_VALIDATION, "sgb_rope_frequencies: NULL argument");
+    std::string err;
+    const int r = rope_frequencies(*scaling, out, &err);
+    return r == SGB_OK ? r : set_error(r, err);
 }
 
 int sgb_sync(sgb_ctx* c, uint32_t timeout_ms)

@@ -79,6 +79,11 @@ class _Cache2Stats(C.Structure):
                 ("hits", C.c_uint64), ("misses", C.c_uint64), ("evictions", C.c_uint64)]
 
 
+class _RopeScaling(C.Structure):
+    _fields_ = [("pairs", C.c_uint32), ("dims", C.c_uint32), ("kind", C.c_uint32), ("reserved", C.c_uint32), ("theta", C.c_double), ("factor", C.c_double),
+                ("trained", C.c_double), ("slow", C.c_double), ("fast", C.c_double)]
+
+
 # Every symbol include/sgattn.h declares: (restype, argtypes).
 _vp, _u32, _u64, _sz, _int = C.c_void_p, C.c_uint32, C.c_uint64, C.c_size_t, C.c_int
 _PP = C.POINTER(C.c_void_p)
@@ -116,6 +121,7 @@ ABI = {
     "sgb_launch_count": (_u64, [_vp]),
     "sgb_decode_paged_splits_hint": (_u32, [_vp, _u32, _u32]),
     "sgb_attn_blocks_work_bytes": (_sz, [_vp, _u32, _u32, _u32, _u32, _u32]),
+    "sgb_rope_frequencies": (_int, [C.POINTER(_RopeScaling), C.POINTER(C.c_double)]),
     "sgb_graph_begin": (_int, [_vp]),
     "sgb_graph_end": (_int, [_vp, _PP]),
     "sgb_graph_launch": (_int, [_vp, _vp]),
@@ -183,6 +189,20 @@ def kernels() -> list[KernelBlob]:
 
 def kernel_blob(name: str) -> Optional[KernelBlob]:
     return next((k for k in kernels() if k.name == name), None)
+
+
+ROPE_KINDS = {"plain": 0, "linear": 1, "by_turns": 2, "by_pairs": 3}
+
+
+def rope_frequencies(pairs: int, theta: float, *, dims: Optional[int] = None, kind: str = "plain", factor: float = 1.0, trained: float = 0.0, slow: float = 1.0,
+                     fast: float = 32.0) -> np.ndarray:
+    """Radians a position of each pair in 64 bits, the ``freqs`` binding of ``rope_cos_sin`` (``sgb_rope_frequencies``)."""
+    if kind not in ROPE_KINDS:
+        raise Validation(f"rope_frequencies: kind must be one of {', '.join(ROPE_KINDS)}")
+    out = np.empty(max(0, operator.index(pairs)), np.float64)
+    s = _RopeScaling(operator.index(pairs) & 0xFFFFFFFF, (2 * pairs if dims is None else operator.index(dims)) & 0xFFFFFFFF, ROPE_KINDS[kind], 0, theta, factor, trained, slow, fast)
+    _check(lib().sgb_rope_frequencies(C.byref(s), out.ctypes.data_as(C.POINTER(C.c_double))))
+    return out
 
 
 @dataclass
