@@ -25,182 +25,195 @@ struct NormsArgs {
     const float *w_post, *gate, *w_pre;
     void* h_out;
     __half* x;
-    uint32_t rows, hidden, lanes;  // lanes of a row
+    uint32_t rows, hidden, lanes;  // lanes of a row: 2^k in a warp, or whole warps
     uint32_t post, gates;
     float plus, scale, eps;  // plus: 1 where weights are 1 + w
 };
+constexpr uint32_t MOST_EACH = 8;   // units of a lane
 enum : uint32_t { POST_NONE = 0, POST_NORM = 1, FIRST_NORM = 2 };
 enum : uint32_t { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_ROW = 2, GATE_ONE = 3 };
+constexpr uint32_t MOST_WARPS = 16;  // of a row
 
-// U consecutive values: 16 bytes of R.
+// Consecutive values of a unit: 16 bytes of R.
 template <typename R>
 constexpr int UNIT = 16 / sizeof(R);
 
+// A unit of f16 as it is loaded, and as pairs of f32.
 template <int U>
-__device__ __forceinline__ void load_f16(const __half* p, float (&v)[U])
-{
+struct RawHalf {
     uint32_t w[U / 2];
+};
+template <int U>
+__device__ __forceinline__ RawHalf<U> load_f16(const __half* p)
+{
+    RawHalf<U> r;
     if constexpr (U == 8) {
         const uint4 u = ld_global(reinterpret_cast<const uint4*>(p));
-        w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+        r.w[0] = u.x, r.w[1] = u.y, r.w[2] = u.z, r.w[3] = u.w;
     } else {
         const uint2 u = ld_global(reinterpret_cast<const uint2*>(p));
-        w[0] = u.x, w[1] = u.y;
+        r.w[0] = u.x, r.w[1] = u.y;
     }
-#pragma unroll
-    for (int i = 0; i < U / 2; i++) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-    }
+    return r;
 }
+__device__ __forceinline__ float2 pair_of(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 template <int U>
-__device__ __forceinline__ void store_f16(__half* p, const float (&v)[U])
+__device__ __forceinline__ void store_f16(__half* p, const float2 (&v)[U / 2])
 {
     uint32_t w[U / 2];
 #pragma unroll
-    for (int i = 0; i < U / 2; i++) w[i] = pack_half2(v[2 * i], v[2 * i + 1]);
+    for (int i = 0; i < U / 2; i++) w[i] = pack_half2(v[i].x, v[i].y);
     if constexpr (U == 8)
         *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     else
         *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
 }
 template <typename R>
-__device__ __forceinline__ void unpack(const uint4& u, float (&v)[UNIT<R>])
+__device__ __forceinline__ void unpack(const uint4& u, float2 (&v)[UNIT<R> / 2])
 {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
     if constexpr (sizeof(R) == 4) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = __uint_as_float(w[i]);
+        v[0] = make_float2(__uint_as_float(w[0]), __uint_as_float(w[1]));
+        v[1] = make_float2(__uint_as_float(w[2]), __uint_as_float(w[3]));
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            if constexpr (std::is_same_v<R, __half>) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-                v[2 * i] = f.x, v[2 * i + 1] = f.y;
-            } else {
-                v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            }
+            if constexpr (std::is_same_v<R, __half>)
+                v[i] = pair_of(w[i]);
+            else
+                v[i] = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
         }
     }
 }
 template <typename R>
-__device__ __forceinline__ uint4 pack(const float (&v)[UNIT<R>])
+__device__ __forceinline__ uint4 pack(const float2 (&v)[UNIT<R> / 2])
 {
     uint32_t w[4];
+    if constexpr (sizeof(R) == 4) {
+        w[0] = __float_as_uint(v[0].x), w[1] = __float_as_uint(v[0].y), w[2] = __float_as_uint(v[1].x), w[3] = __float_as_uint(v[1].y);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if constexpr (sizeof(R) == 4) {
-            w[i] = __float_as_uint(v[i]);
-        } else if constexpr (std::is_same_v<R, __half>) {
-            w[i] = pack_half2(v[2 * i], v[2 * i + 1]);
-        } else {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-            w[i] = *reinterpret_cast<const uint32_t*>(&b);
+        for (int i = 0; i < 4; i++) {
+            if constexpr (std::is_same_v<R, __half>) {
+                w[i] = pack_half2(v[i].x, v[i].y);
+            } else {
+                const __nv_bfloat162 b = __floats2bfloat162_rn(v[i].x, v[i].y);
+                w[i] = *reinterpret_cast<const uint32_t*>(&b);
+            }
         }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 template <int U>
-__device__ __forceinline__ void load_f32(const float* p, float (&v)[U])
+__device__ __forceinline__ void load_f32(const float* p, float2 (&v)[U / 2])
 {
 #pragma unroll
     for (int i = 0; i < U / 4; i++) {
         const float4 f = ld_global(reinterpret_cast<const float4*>(p) + i);
-        v[4 * i] = f.x, v[4 * i + 1] = f.y, v[4 * i + 2] = f.z, v[4 * i + 3] = f.w;
+        v[2 * i] = make_float2(f.x, f.y);
+        v[2 * i + 1] = make_float2(f.z, f.w);
     }
 }
 
-// The sum over a row's lanes: a butterfly in the warp, then over the row's warps in a fixed order.  Everybody calls it.
+// The sum over a row's lanes: a butterfly in the warp, then over the row's warps in their order.  Everybody calls it.
 __device__ __forceinline__ float row_sum(float v, uint32_t lanes, float* parts)
 {
-    for (uint32_t d = 1; d < min(lanes, 32u); d <<= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    if (lanes <= 32) return v;
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = lanes >> 5, first = warp - warp % warps;
-    if (lane == 0) parts[warp] = v;
-    __syncthreads();
-    v = lane < warps ? parts[first + lane] : 0.0f;
+    if (lanes >= 32) {
 #pragma unroll
-    for (uint32_t d = 1; d < 32; d <<= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+        for (uint32_t d = 1; d < 32; d <<= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    } else {
+        for (uint32_t d = 1; d < lanes; d <<= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    }
+    if (lanes <= 32) return v;
+    if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = v;  // (one row a CTA; those of warps that it has not are 0)
+    __syncthreads();
+    v = 0.0f;
+    for (uint32_t i = 0; i < lanes / 32; i += 4) {
+        const float4 f = reinterpret_cast<const float4*>(parts)[i / 4];
+        v += (f.x + f.y) + (f.z + f.w);
+    }
     return v;
 }
 
-template <typename R, int N, int THREADS>
-__global__ void __launch_bounds__(THREADS) block_norms_kernel(const __grid_constant__ NormsArgs a)
+template <typename R, int N>
+__global__ void __launch_bounds__(32 * MOST_WARPS) block_norms_kernel(const __grid_constant__ NormsArgs a)
 {
-    constexpr int U = UNIT<R>;
-    __shared__ float parts[2][32];
+    constexpr int U = UNIT<R>, P = U / 2;
+    __shared__ alignas(16) float parts[2][MOST_WARPS];
+    if (a.lanes > 32 && threadIdx.x < 2 * MOST_WARPS) parts[threadIdx.x / MOST_WARPS][threadIdx.x % MOST_WARPS] = 0.0f;
     pdl_wait();
     pdl_launch_dependents();
-    const uint32_t in_cta = threadIdx.x / a.lanes, lane = threadIdx.x - in_cta * a.lanes;
-    const uint64_t row = (uint64_t)blockIdx.x * (blockDim.x / a.lanes) + in_cta;
-    const size_t base = row * a.hidden;
+    if (a.lanes > 32) __syncthreads();  // the zeros come before the sums
+    const uint32_t shift = a.lanes <= 32 ? __ffs(a.lanes) - 1 : 31;  // a row of several warps has the CTA to itself
+    const uint32_t lane = a.lanes <= 32 ? threadIdx.x & (a.lanes - 1) : threadIdx.x;
+    const uint64_t row = a.lanes <= 32 ? (uint64_t)blockIdx.x * (blockDim.x >> shift) + (threadIdx.x >> shift) : blockIdx.x;
+    const size_t at = row * a.hidden + lane * U;  // of the first unit
+    const uint32_t step = a.lanes * U;
+    const bool live = row < a.rows;
     const float inv_n = 1.0f / (float)a.hidden;
-    uint32_t col[N];
-    bool on[N];
+    // all units but the last are within the row
+    const auto on = [&](int i) { return live && (i + 1 < N || lane * U + i * step < a.hidden); };
+    RawHalf<U> y[N];
     uint4 raw[N];
-    float v[N][U];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        col[i] = (lane + i * a.lanes) * U;
-        on[i] = row < a.rows && col[i] < a.hidden;
+        y[i] = RawHalf<U>{};
         raw[i] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int j = 0; j < U; j++) v[i][j] = 0.0f;
-        if (on[i]) {
-            if (a.post != FIRST_NORM) load_f16<U>(a.y + base + col[i], v[i]);
-            raw[i] = ld_global(reinterpret_cast<const uint4*>(static_cast<const R*>(a.h) + base + col[i]));
+        if (on(i)) {
+            if (a.post != FIRST_NORM) y[i] = load_f16<U>(a.y + at + i * step);
+            raw[i] = ld_global(reinterpret_cast<const uint4*>(static_cast<const R*>(a.h) + at + i * step));
         }
     }
     float by = 1.0f;  // of the block's output
-    if (a.gates == GATE_ROW && row < a.rows) by = ld_global(a.gate + row);
+    if (a.gates == GATE_ROW && live) by = ld_global(a.gate + row);
     if (a.gates == GATE_ONE) by = ld_global(a.gate);
     if (a.post == POST_NORM) {
-        float ss = 0.0f;
+        float2 ss = make_float2(0.0f, 0.0f);
 #pragma unroll
         for (int i = 0; i < N; i++)
 #pragma unroll
-            for (int j = 0; j < U; j++) ss = fmaf(v[i][j], v[i][j], ss);
-        by *= rsqrtf(row_sum(ss, a.lanes, parts[0]) * inv_n + a.eps);
+            for (int j = 0; j < P; j++) {
+                const float2 f = pair_of(y[i].w[j]);
+                ss = fma2_rn(f, f, ss);
+            }
+        by *= rsqrtf(row_sum(ss.x + ss.y, a.lanes, parts[0]) * inv_n + a.eps);
     }
-    float ss = 0.0f;
+    const float2 by2 = make_float2(by, by), scale2 = make_float2(a.scale, a.scale), plus2 = make_float2(a.plus, a.plus);
+    float2 ss = make_float2(0.0f, 0.0f), v[N][P];
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        float h[U];
-        unpack<R>(raw[i], h);
-        if (a.post != FIRST_NORM && on[i]) {
-            float w[U];
+        unpack<R>(raw[i], v[i]);
+        if (a.post != FIRST_NORM && on(i)) {
+            float2 n[P], w[P];
 #pragma unroll
-            for (int j = 0; j < U; j++) v[i][j] *= by;
+            for (int j = 0; j < P; j++) n[j] = pair_of(y[i].w[j]);
             if (a.post == POST_NORM) {
-                load_f32<U>(a.w_post + col[i], w);
+                load_f32<U>(a.w_post + lane * U + i * step, w);
 #pragma unroll
-                for (int j = 0; j < U; j++) v[i][j] *= w[j] + a.plus;
+                for (int j = 0; j < P; j++) n[j] = mul2_rn(n[j], add2_rn(w[j], plus2));
             }
             if (a.gates == GATE_CHANNEL) {
-                load_f32<U>(a.gate + col[i], w);
+                load_f32<U>(a.gate + lane * U + i * step, w);
 #pragma unroll
-                for (int j = 0; j < U; j++) v[i][j] *= w[j];
+                for (int j = 0; j < P; j++) n[j] = mul2_rn(n[j], w[j]);
             }
 #pragma unroll
-            for (int j = 0; j < U; j++) v[i][j] = (h[j] + v[i][j]) * a.scale;
-            *reinterpret_cast<uint4*>(static_cast<R*>(a.h_out) + base + col[i]) = pack<R>(v[i]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < U; j++) v[i][j] = h[j];
+            for (int j = 0; j < P; j++) v[i][j] = mul2_rn(fma2_rn(n[j], by2, v[i][j]), scale2);
+            *reinterpret_cast<uint4*>(static_cast<R*>(a.h_out) + at + i * step) = pack<R>(v[i]);
         }
 #pragma unroll
-        for (int j = 0; j < U; j++) ss = fmaf(v[i][j], v[i][j], ss);
+        for (int j = 0; j < P; j++) ss = fma2_rn(v[i][j], v[i][j], ss);
     }
-    const float inv = rsqrtf(row_sum(ss, a.lanes, parts[1]) * inv_n + a.eps);
+    const float inv = rsqrtf(row_sum(ss.x + ss.y, a.lanes, parts[1]) * inv_n + a.eps);
+    const float2 inv2 = make_float2(inv, inv);
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        if (!on[i]) continue;
-        float w[U];
-        load_f32<U>(a.w_pre + col[i], w);
+        if (!on(i)) continue;
+        float2 w[P];
+        load_f32<U>(a.w_pre + lane * U + i * step, w);
 #pragma unroll
-        for (int j = 0; j < U; j++) v[i][j] *= inv * (w[j] + a.plus);
-        store_f16<U>(a.x + base + col[i], v[i]);
+        for (int j = 0; j < P; j++) v[i][j] = mul2_rn(mul2_rn(v[i][j], inv2), add2_rn(w[j], plus2));
+        store_f16<U>(a.x + at + i * step, v[i]);
     }
 }
 
@@ -212,7 +225,8 @@ struct PushNorms {
 template <typename R>
 auto norms_kernel(uint32_t n)
 {
-    return n == 1 ? block_norms_kernel<R, 1, 1024> : n == 2 ? block_norms_kernel<R, 2, 1024> : block_norms_kernel<R, 4, 1024>;
+    return n == 1 ? block_norms_kernel<R, 1> : n == 2 ? block_norms_kernel<R, 2> : n == 3 ? block_norms_kernel<R, 3> : n == 4 ? block_norms_kernel<R, 4>
+         : n == 5 ? block_norms_kernel<R, 5> : n == 6 ? block_norms_kernel<R, 6> : n == 7 ? block_norms_kernel<R, 7> : block_norms_kernel<R, 8>;
 }
 
 }  // namespace
@@ -255,15 +269,17 @@ int launch_block_norms(const LaunchArgs& a)
     const uint32_t units = hidden / U;
     NormsArgs k{(const __half*)a.b[0].ptr, a.b[1].ptr, (const float*)a.b[2].ptr, (const float*)a.b[3].ptr, (const float*)a.b[4].ptr, a.b[5].ptr, (__half*)a.b[6].ptr,
                 rows, hidden, 1, p.post, p.gates, p.plus_one ? 1.0f : 0.0f, p.scale, p.eps};
+    // units a lane: eight at most
     uint32_t each = 1;
     if (units <= 32) {
         while (k.lanes < units) k.lanes <<= 1;
     } else {
-        while ((units + 31) / 32 * 32 > each * 1024) each <<= 1;
-        k.lanes = (units + 32 * each - 1) / (32 * each) * 32;
+        uint32_t warps = (units + 32 * MOST_EACH - 1) / (32 * MOST_EACH);
+        each = (units + 32 * warps - 1) / (32 * warps);
+        warps = (units + 32 * each - 1) / (32 * each);
+        k.lanes = 32 * warps;
     }
-    const uint32_t threads = k.lanes >= 128 ? k.lanes : 128 / k.lanes * k.lanes;
-    const uint32_t per_cta = threads / k.lanes;
+    const uint32_t threads = k.lanes <= 32 ? 128 : k.lanes, per_cta = threads / k.lanes;
     const cudaError_t e = launch_dependent(norms_kernel<R>(each), dim3((unsigned)((rows + per_cta - 1ull) / per_cta)), dim3(threads), 0, a.stream, k);
     ++*a.launches;
     return check_cuda(a, e, "block_norms");
