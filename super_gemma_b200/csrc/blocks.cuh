@@ -91,6 +91,14 @@ __device__ __forceinline__ uint4 ld_global_if(bool p, const uint4* at)
         : "l"(at), "r"((uint32_t)p));
     return v;
 }
+__device__ __forceinline__ uint2 ld_global_if(bool p, const uint2* at)
+{
+    uint2 v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\tmov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\t@p ld.global.v2.b32 {%0, %1}, [%2];\n\t}"
+                 : "=&r"(v.x), "=&r"(v.y)
+                 : "l"(at), "r"((uint32_t)p));
+    return v;
+}
 __device__ __forceinline__ uint32_t ld_global_if(bool p, const uint32_t* at)
 {
     uint32_t v;

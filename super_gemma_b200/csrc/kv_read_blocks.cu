@@ -10,14 +10,15 @@ namespace sgb {
 namespace {
 
 constexpr int THREADS = 256;
-constexpr uint32_t MOST_ROWS = 32;  // of a CTA
+constexpr uint32_t ROWS = THREADS / 16;  // of a CTA
+constexpr uint32_t AHEAD = 4;
 
 struct ReadArgs {
     const uint8_t* pool[2];
     const int8_t* exps[2];
     const uint32_t *table, *from, *starts;
     __half* out[2];
-    uint32_t n, tokens, n_kv, stride, page_shift, blocks, rows;  // rows of a CTA
+    uint32_t n, tokens, n_kv, stride, page_shift, blocks;
     uint32_t* status;
 };
 
@@ -54,25 +55,37 @@ __device__ __forceinline__ uint32_t scaled(uint32_t two_bytes, int e)
     return pack_half2(f.x * by, f.y * by);
 }
 
+// A CTA has ROWS packed rows, half a warp each: eight bytes in and sixteen out a lane, so that both sides move whole sectors.  Sixteen rows are
+// a tile's where a request's rows begin with one.  The heads of both sides go round, AHEAD of them asked for at a time (with gridDim.y
+// CTAs they share them).
 __global__ void __launch_bounds__(THREADS) read_blocks_kernel(const __grid_constant__ ReadArgs a)
 {
-    __shared__ uint32_t where[MOST_ROWS];
+    __shared__ uint32_t where[ROWS];
     pdl_wait();
     pdl_launch_dependents();
-    const uint32_t i0 = blockIdx.x * a.rows;
-    if (threadIdx.x < a.rows) where[threadIdx.x] = i0 + threadIdx.x < a.tokens ? cached_row(a, i0 + threadIdx.x) : NO_SLOT;
+    const uint32_t i0 = blockIdx.x * ROWS;
+    if (threadIdx.x < ROWS) where[threadIdx.x] = i0 + threadIdx.x < a.tokens ? cached_row(a, i0 + threadIdx.x) : NO_SLOT;
     __syncthreads();
-    // half a warp a row of 128: eight bytes a lane
-    const uint32_t lane = threadIdx.x & 15, units = a.rows * a.n_kv * 2;
-    for (uint32_t u = blockIdx.y * (THREADS / 16) + threadIdx.x / 16; u < units; u += gridDim.y * (THREADS / 16)) {
-        const uint32_t row = u % a.rows, rest = u / a.rows, head = rest >> 1, side = rest & 1;
-        const uint32_t at = where[row];
-        if (at == NO_SLOT) continue;
-        const size_t tile = (size_t)(at / TILE_TOK) * a.n_kv + head;
-        const uint2 q = ld_global(reinterpret_cast<const uint2*>(a.pool[side] + tile * TILE_BYTES + at % TILE_TOK * 128 + lane * 8));
-        const int e = ld_global_if(true, a.exps[side] + tile);
-        *reinterpret_cast<uint4*>(a.out[side] + ((size_t)(i0 + row) * a.n_kv + head) * 128 + lane * 8) =
-            make_uint4(scaled(q.x & 0xffffu, e), scaled(q.x >> 16, e), scaled(q.y & 0xffffu, e), scaled(q.y >> 16, e));
+    const uint32_t lane = threadIdx.x & 15, row = threadIdx.x >> 4, at = where[row];
+    if (at == NO_SLOT) return;
+    const size_t tile = (size_t)(at / TILE_TOK) * a.n_kv, in_tile = at % TILE_TOK * 128 + lane * 8, out = (size_t)(i0 + row) * a.n_kv * 128 + lane * 8;
+    for (uint32_t u0 = blockIdx.y; u0 < 2 * a.n_kv; u0 += AHEAD * gridDim.y) {
+        uint2 q[AHEAD];
+        int e[AHEAD];
+#pragma unroll
+        for (uint32_t j = 0; j < AHEAD; j++) {
+            const uint32_t u = u0 + j * gridDim.y, side = u >= a.n_kv, head = side ? u - a.n_kv : u;
+            const bool on = u < 2 * a.n_kv;
+            q[j] = ld_global_if(on, reinterpret_cast<const uint2*>(a.pool[side] + (tile + head) * TILE_BYTES + in_tile));
+            e[j] = ld_global_if(on, a.exps[side] + tile + head);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < AHEAD; j++) {
+            const uint32_t u = u0 + j * gridDim.y, side = u >= a.n_kv, head = side ? u - a.n_kv : u;
+            if (u >= 2 * a.n_kv) return;
+            *reinterpret_cast<uint4*>(a.out[side] + out + (size_t)head * 128) =
+                make_uint4(scaled(q[j].x & 0xffffu, e[j]), scaled(q[j].x >> 16, e[j]), scaled(q[j].y & 0xffffu, e[j]), scaled(q[j].y >> 16, e[j]));
+        }
     }
 }
 
@@ -107,8 +120,11 @@ int launch_kv_read_blocks(const LaunchArgs& a)
     if (int r = need_aligned(a, {16, 1, 16, 1, 4, 4, 4, 16, 16})) return r;
     ReadArgs k{{(const uint8_t*)a.b[0].ptr, (const uint8_t*)a.b[2].ptr}, {(const int8_t*)a.b[1].ptr, (const int8_t*)a.b[3].ptr}, (const uint32_t*)a.b[4].ptr,
                (const uint32_t*)a.b[5].ptr, (const uint32_t*)a.b[6].ptr, {(__half*)a.b[7].ptr, (__half*)a.b[8].ptr}, n, tokens, n_kv, p.stride,
-               (uint32_t)__builtin_ctz(p.page), (uint32_t)blocks, 16, a.status};
-    const cudaError_t e = launch_dependent(read_blocks_kernel, dim3((tokens + k.rows - 1) / k.rows), dim3(THREADS), 0, a.stream, k);
+               (uint32_t)__builtin_ctz(p.page), (uint32_t)blocks, a.status};
+    const uint32_t ctas = (tokens + ROWS - 1) / ROWS;
+    uint32_t shares = 1;  // CTAs that have the same rows: as many as fill the GPU
+    while (shares < 2 * n_kv && shares * (uint64_t)ctas < 4ull * a.sm_count) shares *= 2;
+    const cudaError_t e = launch_dependent(read_blocks_kernel, dim3(ctas, shares), dim3(THREADS), 0, a.stream, k);
     ++*a.launches;
     return check_cuda(a, e, "kv_read_blocks_e4m3_d128");
 }
