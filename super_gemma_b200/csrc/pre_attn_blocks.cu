@@ -34,14 +34,54 @@ struct PreArgs {
     uint8_t* pool[2];
     int8_t* exps[2];
     uint32_t q_stride, k_stride, v_stride;  // values from token to token
-    uint32_t n_q, n_kv, tokens, blocks, pairs, layout, slot_bits;
-    float magnitude;
+    uint32_t n_q, n_kv, tokens, blocks, pairs, layout, share_bits;
+    float plus, magnitude;  // plus: 1 where weights are 1 + w
     uint32_t* status;
 };
 
-// Sixteen normed values as e4m3 of x * 2^-e.  |x| 2^-e stays below 448 but where an exponent is at its upper end: magnitudes count up to
-// 61440 (every cached value is an f16 number), which is 240 of an exponent of 8.
-__device__ __forceinline__ uint32_t quantise4(float a, float b, float c, float d)
+// A lane's eight pairs, a[j] = (a_2j, a_2j+1) and b likewise: the two octets of its piece, or with NEXT (layout 2) their even and their odd
+// dims.  Which register a value comes to is all that the layouts differ in.
+struct Pairs {
+    float2 a[4], b[4];
+};
+template <bool NEXT>
+__device__ __forceinline__ Pairs unpack_pairs(const uint4& lo, const uint4& hi)
+{
+    const uint32_t x[4] = {lo.x, lo.y, lo.z, lo.w}, y[4] = {hi.x, hi.y, hi.z, hi.w};
+    Pairs p;
+    float2 f[4], g[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        f[j] = __half22float2(as_half2(x[j]));
+        g[j] = __half22float2(as_half2(y[j]));
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float2* from = j < 2 ? f + 2 * j : g + 2 * (j - 2);
+        p.a[j] = NEXT ? make_float2(from[0].x, from[1].x) : f[j];
+        p.b[j] = NEXT ? make_float2(from[0].y, from[1].y) : g[j];
+    }
+    return p;
+}
+template <bool NEXT>
+__device__ __forceinline__ void write_f16(__half* row, const RopePiece& at, const Pairs& p)
+{
+    uint32_t x[4], y[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if constexpr (NEXT) {
+            uint32_t* to = j < 2 ? x + 2 * j : y + 2 * (j - 2);
+            to[0] = pack_half2(p.a[j].x, p.b[j].x);
+            to[1] = pack_half2(p.a[j].y, p.b[j].y);
+        } else {
+            x[j] = pack_half2(p.a[j].x, p.a[j].y);
+            y[j] = pack_half2(p.b[j].x, p.b[j].y);
+        }
+    }
+    *reinterpret_cast<uint4*>(row + at.lo) = make_uint4(x[0], x[1], x[2], x[3]);
+    *reinterpret_cast<uint4*>(row + at.hi) = make_uint4(y[0], y[1], y[2], y[3]);
+}
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d)
 {
     uint32_t r;
     asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\tmov.b32 %0, {lo, hi};\n\t}"
@@ -49,122 +89,186 @@ __device__ __forceinline__ uint32_t quantise4(float a, float b, float c, float d
         : "f"(a), "f"(b), "f"(c), "f"(d));
     return r;
 }
-__device__ __forceinline__ void write_e4m3(uint8_t* row, const RopePiece& at, float (&x)[8], float (&y)[8], int e)
+// Values times 2^-e already.
+template <bool NEXT>
+__device__ __forceinline__ void write_e4m3(uint8_t* row, const RopePiece& at, const Pairs& p)
 {
-    const float f = exp2_of(-e);
-    if (e > 7) {  // (NaN stays)
-        const float most = 61440.0f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            x[i] = x[i] > most ? most : x[i] < -most ? -most : x[i];
-            y[i] = y[i] > most ? most : y[i] < -most ? -most : y[i];
-        }
+    const float2 *a = p.a, *b = p.b;
+    if constexpr (NEXT) {
+        *reinterpret_cast<uint2*>(row + at.lo) = make_uint2(e4m3x4(a[0].x, b[0].x, a[0].y, b[0].y), e4m3x4(a[1].x, b[1].x, a[1].y, b[1].y));
+        *reinterpret_cast<uint2*>(row + at.hi) = make_uint2(e4m3x4(a[2].x, b[2].x, a[2].y, b[2].y), e4m3x4(a[3].x, b[3].x, a[3].y, b[3].y));
+    } else {
+        *reinterpret_cast<uint2*>(row + at.lo) = make_uint2(e4m3x4(a[0].x, a[0].y, a[1].x, a[1].y), e4m3x4(a[2].x, a[2].y, a[3].x, a[3].y));
+        *reinterpret_cast<uint2*>(row + at.hi) = make_uint2(e4m3x4(b[0].x, b[0].y, b[1].x, b[1].y), e4m3x4(b[2].x, b[2].y, b[3].x, b[3].y));
     }
-    *reinterpret_cast<uint2*>(row + at.lo) = make_uint2(quantise4(x[0] * f, x[1] * f, x[2] * f, x[3] * f), quantise4(x[4] * f, x[5] * f, x[6] * f, x[7] * f));
-    *reinterpret_cast<uint2*>(row + at.hi) = make_uint2(quantise4(y[0] * f, y[1] * f, y[2] * f, y[3] * f), quantise4(y[4] * f, y[5] * f, y[6] * f, y[7] * f));
 }
 
-template <bool PLUS_ONE>
-__global__ void __launch_bounds__(THREADS) pre_attn_blocks_kernel(const __grid_constant__ PreArgs a)
+// Weight and rotation of a token's heads in one: (a, b) -> (a A - b B, b C + a E) with A = w_a c, B = w_b s, C = w_b c, E = w_a s.
+struct Turn {
+    float2 A[4], minus_B[4], C[4], E[4];
+};
+__device__ __forceinline__ void apply(const Turn& t, bool turns, Pairs& p)
+{
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float2 a = p.a[j], b = p.b[j];
+        p.a[j] = mul2_rn(a, t.A[j]);
+        p.b[j] = mul2_rn(b, t.C[j]);
+        if (turns) {  // (a partner that is no number stays out of what does not turn)
+            p.a[j] = fma2_rn(b, t.minus_B[j], p.a[j]);
+            p.b[j] = fma2_rn(a, t.E[j], p.b[j]);
+        }
+    }
+}
+
+// 2^SHARE_BITS groups of eight lanes share the rows of a token (q heads, k heads, v heads in this order), group by group one after the other.  What is the same for
+// a token's heads (the slot, the rotation with its weights, the exponents' bound) is made once a group, and a row's values are asked for one row ahead.  GROUP: its lanes in
+// the warp; groups of a warp may have different rows to do.
+template <bool NEXT>
+__global__ void __launch_bounds__(THREADS, 5) pre_attn_blocks_kernel(const __grid_constant__ PreArgs a)
 {
     pdl_wait();
     pdl_launch_dependents();
     const uint32_t lane = threadIdx.x & (ROW_LANES - 1), group = blockIdx.x * (THREADS / ROW_LANES) + threadIdx.x / ROW_LANES;
-    const uint32_t token = group >> a.slot_bits, rows = a.n_q + 2 * a.n_kv;
-    // a warp's four groups may have different tokens; those behind the last one go along without rows
-    const bool live = token < a.tokens;
+    const uint32_t mask = 0xffu << (threadIdx.x & 24);
+    const uint32_t token = group >> a.share_bits, shares = 1u << a.share_bits;
+    if (token >= a.tokens) return;
     const RopePiece at = rope_piece(a.layout, lane, 128, a.pairs);
     // The slot, and those of the fifteen tokens before it: two a lane.
-    uint32_t slot = NO_SLOT, before[2] = {NO_SLOT, NO_SLOT};
-    if (live) {
-        slot = ld_global(a.slots + token);
+    const uint32_t slot = ld_global(a.slots + token);
+    uint32_t before[2] = {NO_SLOT, NO_SLOT};
 #pragma unroll
-        for (uint32_t j = 0; j < 2; j++)
-            if (token >= 1 + lane + 8 * j) before[j] = ld_global(a.slots + token - 1 - lane - 8 * j);
-    }
-    const uint32_t in_tile = slot % TILE_TOK, previous = __shfl_sync(0xffffffffu, before[0], 0, ROW_LANES);
+    for (uint32_t j = 0; j < 2; j++)
+        if (token >= 1 + lane + 8 * j) before[j] = ld_global(a.slots + token - 1 - lane - 8 * j);
+    const uint32_t end_q = a.n_q, end_k = a.n_q + a.n_kv, end = end_k + a.n_kv;
+    uint32_t r = group & (shares - 1);
+    struct Row {
+        uint4 lo, hi;
+    };
+    const auto fetch = [&](uint32_t i) {
+        const __half* src = i < end_q   ? a.q + ((size_t)token * a.q_stride + i * 128)
+                            : i < end_k ? a.k + ((size_t)token * a.k_stride + (i - end_q) * 128)
+                                        : a.v + ((size_t)token * a.v_stride + (i - end_k) * 128);
+        return Row{ld_global_if(i < end, reinterpret_cast<const uint4*>(src + at.lo)), ld_global_if(i < end, reinterpret_cast<const uint4*>(src + at.hi))};
+    };
+    Row row = fetch(r);
+    float c[8], s[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) c[i] = 1.0f, s[i] = 0.0f;
+    if (at.turns) load_cos_sin(a.cos_sin + (size_t)token * a.pairs + at.pair, c, s);
+    float most = 0.0f;
+    const auto turn_of = [&](const float* weights) {
+        Turn t;
+        float4 u[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) u[j] = ld_global(reinterpret_cast<const float4*>(weights + (j < 2 ? at.lo : at.hi)) + (j & 1));
+        const float w[16] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w, u[2].x, u[2].y, u[2].z, u[2].w, u[3].x, u[3].y, u[3].z, u[3].w};
+        most = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float2 wa = NEXT ? make_float2(w[4 * j], w[4 * j + 2]) : make_float2(w[2 * j], w[2 * j + 1]);
+            float2 wb = NEXT ? make_float2(w[4 * j + 1], w[4 * j + 3]) : make_float2(w[8 + 2 * j], w[8 + 2 * j + 1]);
+            wa = add2_rn(wa, make_float2(a.plus, a.plus));
+            wb = add2_rn(wb, make_float2(a.plus, a.plus));
+            most = max3(most, fmaxf(fabsf(wa.x), fabsf(wa.y)), fmaxf(fabsf(wb.x), fabsf(wb.y)));
+            const float2 cc = make_float2(c[2 * j], c[2 * j + 1]), ss = make_float2(s[2 * j], s[2 * j + 1]);
+            t.A[j] = mul2_rn(wa, cc);
+            t.C[j] = mul2_rn(wb, cc);
+            t.E[j] = mul2_rn(wa, ss);
+            t.minus_B[j] = mul2_rn(wb, make_float2(-ss.x, -ss.y));
+        }
+        return t;
+    };
+    const auto inverse_rms = [&](const Pairs& p) {
+        float2 ss = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int j = 0; j < 4; j++) ss = fma2_rn(p.b[j], p.b[j], fma2_rn(p.a[j], p.a[j], ss));
+        float sum = ss.x + ss.y;
+#pragma unroll
+        for (uint32_t d = 1; d < ROW_LANES; d <<= 1) sum += __shfl_xor_sync(mask, sum, d);
+        return rsqrtf(fmaf(sum, 1.0f / 128.0f, RMS_EPS));
+    };
+    const auto scale = [&](Pairs& p, float by) {
+        const float2 f = make_float2(by, by);
+#pragma unroll
+        for (int j = 0; j < 4; j++) p.a[j] = mul2_rn(p.a[j], f), p.b[j] = mul2_rn(p.b[j], f);
+    };
+    Turn turn;
+    if (r < end_q) turn = turn_of(a.q_w);
+
+    if (slot == NO_SLOT) return;
+    const uint32_t in_tile = slot % TILE_TOK, previous = __shfl_sync(mask, before[0], 0, ROW_LANES);
     const uint32_t back = in_tile ? in_tile - 1 : 0;  // the token that would be the tile's first, counted from the one before this
-    const uint32_t opener0 = __shfl_sync(0xffffffffu, before[0], back & 7, ROW_LANES), opener1 = __shfl_sync(0xffffffffu, before[1], back & 7, ROW_LANES);
+    const uint32_t opener0 = __shfl_sync(mask, before[0], back & 7, ROW_LANES), opener1 = __shfl_sync(mask, before[1], back & 7, ROW_LANES);
     const bool fresh = in_tile == 0 || (back < 8 ? opener0 : opener1) == slot - in_tile;  // the tile begins with this run
     const bool follows = in_tile != 0 && previous != NO_SLOT && previous + 1 == slot;
-    bool placed = slot != NO_SLOT;
-    if (placed && slot / TILE_TOK >= a.blocks) {
+    bool placed = true;
+    if (slot / TILE_TOK >= a.blocks) {
         report_error(a.status, DEV_ERR_BOUNDS, 631, slot, a.blocks);
         placed = false;
-    } else if (placed && previous != NO_SLOT && previous / TILE_TOK == slot / TILE_TOK && previous + 1 != slot) {
+    } else if (previous != NO_SLOT && previous / TILE_TOK == slot / TILE_TOK && previous + 1 != slot) {
         report_error(a.status, DEV_ERR_BOUNDS, 632, previous, slot);  // a tile's tokens stand in its order
         placed = false;
     }
-    const bool some = slot != NO_SLOT;
-    float c[8], s[8];
-    if (at.turns && some) load_cos_sin(a.cos_sin + (size_t)token * a.pairs + at.pair, c, s);
-    for (uint32_t r0 = (blockIdx.y << a.slot_bits); r0 < rows; r0 += gridDim.y << a.slot_bits) {
-        const uint32_t r = r0 + (group & ((1u << a.slot_bits) - 1));
-        const bool is_q = r < a.n_q, is_v = r >= a.n_q + a.n_kv, on = some && r < rows;
-        const uint32_t head = is_q ? r : is_v ? r - a.n_q - a.n_kv : r - a.n_q;
-        const __half* src = (is_q ? a.q + (size_t)token * a.q_stride : is_v ? a.v + (size_t)token * a.v_stride : a.k + (size_t)token * a.k_stride) + (size_t)head * 128;
-        const uint4 u = ld_global_if(on, reinterpret_cast<const uint4*>(src + at.lo)), w = ld_global_if(on, reinterpret_cast<const uint4*>(src + at.hi));
-        const size_t tile = (size_t)(slot / TILE_TOK) * a.n_kv + head;
-        const int old = ld_global_if(on && placed && !is_q && !fresh, a.exps[is_v] + tile);
-        float x[8], y[8];
-        unpack_f16x8(u, x);
-        unpack_f16x8(w, y);
-        float ss = 0.0f, more = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            ss = fmaf(x[i], x[i], ss);
-            more = fmaf(y[i], y[i], more);
-        }
-        ss += more;
-#pragma unroll
-        for (uint32_t d = 1; d < ROW_LANES; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-        const float inv = rsqrtf(ss / 128.0f + RMS_EPS);
-        float most = 1.0f;
-        if (!is_v) {
-            const float* wt = is_q ? a.q_w : a.k_w;
-            float wx[8], wy[8];
-#pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const float4 f = ld_global(reinterpret_cast<const float4*>(wt + at.lo) + j), g = ld_global(reinterpret_cast<const float4*>(wt + at.hi) + j);
-                wx[4 * j] = f.x, wx[4 * j + 1] = f.y, wx[4 * j + 2] = f.z, wx[4 * j + 3] = f.w;
-                wy[4 * j] = g.x, wy[4 * j + 1] = g.y, wy[4 * j + 2] = g.z, wy[4 * j + 3] = g.w;
-            }
-            most = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                if (PLUS_ONE) wx[i] += 1.0f, wy[i] += 1.0f;
-                x[i] *= inv * wx[i];
-                y[i] *= inv * wy[i];
-                most = max3(most, fabsf(wx[i]), fabsf(wy[i]));
-            }
-            if (at.turns) rope_turn(a.layout, x, y, c, s);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] *= inv, y[i] *= inv;
-        }
-        if (is_q && on) {
-            __half* to = a.q_out + ((size_t)token * a.n_q + head) * 128;
-            *reinterpret_cast<uint4*>(to + at.lo) = pack_f16x8(x);
-            *reinterpret_cast<uint4*>(to + at.hi) = pack_f16x8(y);
-        }
-#pragma unroll
-        for (uint32_t d = 1; d < ROW_LANES; d <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-        if (is_q || !on || !placed) continue;
-        const int least = exponent_for(fminf(is_v ? ROW_REACH : most * ROW_REACH * a.magnitude, 61440.0f));
-        const int e = fresh ? least : max(least, old);
-        uint8_t* to = a.pool[is_v] + tile * TILE_BYTES;
-        if (!follows) {  // the run's first token: nobody else writes the rows before it, nor the exponent
-            if (!fresh && least > old) {
-                const __half2 f = power_of_two(max(old - least, -24));
-                for (uint32_t j = 0; j < in_tile; j++) {
-                    uint4* p = reinterpret_cast<uint4*>(to + j * 128 + lane * 16);
-                    *p = round_again(ld_global(p), f);
-                }
-            }
-            if (lane == 0) a.exps[is_v][tile] = (int8_t)e;
-        }
-        write_e4m3(to + in_tile * 128, at, x, y, e);
+
+    for (; r < end_q; r += shares) {
+        Pairs p = unpack_pairs<NEXT>(row.lo, row.hi);
+        row = fetch(r + shares);
+        const float inv = inverse_rms(p);
+        apply(turn, at.turns, p);
+        scale(p, inv);
+        write_f16<NEXT>(a.q_out + ((size_t)token * a.n_q + r) * 128, at, p);
     }
+    if (!placed) return;
+
+    // Rows [r, last) of one side into the cache; `least`: the exponent that holds them all.
+    const size_t tile0 = (size_t)(slot / TILE_TOK) * a.n_kv;
+    const auto append = [&](int side, uint32_t first, uint32_t last, int least, const auto& turned) {
+        if (r >= last) return;
+        uint8_t* const pool = a.pool[side] + tile0 * TILE_BYTES;
+        int8_t* const exps = a.exps[side] + tile0;
+        int old = ld_global_if(!fresh, exps + (r - first));
+        for (; r < last; r += shares) {
+            Pairs p = unpack_pairs<NEXT>(row.lo, row.hi);
+            row = fetch(r + shares);
+            const uint32_t head = r - first;
+            const int had = old, e = fresh ? least : max(least, had);
+            old = ld_global_if(!fresh && r + shares < last, exps + head + shares);
+            const float inv = inverse_rms(p);
+            turned(p);
+            uint8_t* to = pool + (size_t)head * TILE_BYTES;
+            if (!follows) {  // the run's first token: nobody else writes the rows before it, nor the exponent
+                if (!fresh && least > had) {
+                    const __half2 f = power_of_two(max(had - least, -24));
+                    for (uint32_t j = 0; j < in_tile; j++) {
+                        uint4* q = reinterpret_cast<uint4*>(to + j * 128 + lane * 16);
+                        *q = round_again(ld_global(q), f);
+                    }
+                }
+                if (lane == 0) exps[head] = (int8_t)e;
+            }
+            if (e > 7) {  // magnitudes count up to 61440, which is 240 of an exponent of 8 (NaN stays)
+                scale(p, inv);
+                const auto cut = [](float2& v) {
+                    v.x = v.x > 61440.0f ? 61440.0f : v.x < -61440.0f ? -61440.0f : v.x;
+                    v.y = v.y > 61440.0f ? 61440.0f : v.y < -61440.0f ? -61440.0f : v.y;
+                };
+#pragma unroll
+                for (int j = 0; j < 4; j++) cut(p.a[j]), cut(p.b[j]);
+                scale(p, exp2_of(-e));
+            } else {
+                scale(p, inv * exp2_of(-e));
+            }
+            write_e4m3<NEXT>(to + in_tile * 128, at, p);
+        }
+    };
+    if (r < end_k) {
+        turn = turn_of(a.k_w);
+#pragma unroll
+        for (uint32_t d = 1; d < ROW_LANES; d <<= 1) most = fmaxf(most, __shfl_xor_sync(mask, most, d));
+        append(0, end_q, end_k, exponent_for(fminf(most * ROW_REACH * a.magnitude, 61440.0f)), [&](Pairs& p) { apply(turn, at.turns, p); });
+    }
+    append(1, end_k, end, exponent_for(ROW_REACH), [](Pairs&) {});
 }
 
 struct PushPre {
@@ -218,14 +322,12 @@ int launch_qkv_norm_rope_append_blocks(const LaunchArgs& a)
     const uint32_t rows = n_q + 2 * n_kv;
     PreArgs k{(const __half*)a.b[0].ptr, (const __half*)a.b[3].ptr, (const __half*)a.b[4].ptr, (const float*)a.b[1].ptr, (const float*)a.b[5].ptr, (const float2*)a.b[6].ptr,
               (const uint32_t*)a.b[7].ptr, (__half*)a.b[2].ptr, {(uint8_t*)a.b[8].ptr, (uint8_t*)a.b[10].ptr}, {(int8_t*)a.b[9].ptr, (int8_t*)a.b[11].ptr},
-              p.q_stride, p.k_stride, p.v_stride, n_q, n_kv, tokens, (uint32_t)blocks, p.rot_dims / 2, p.layout, 0, p.magnitude, a.status};
-    const uint64_t per_sm = ((uint64_t)tokens * rows + a.sm_count - 1) / a.sm_count;
-    const uint32_t each = per_sm <= 64 ? 1 : per_sm <= 384 ? 2 : 4;  // rows of a group of lanes
-    while ((1u << k.slot_bits) < 32 && (each << k.slot_bits) < rows) k.slot_bits++;
-    const uint64_t groups = (uint64_t)tokens << k.slot_bits;  // < 2^31
-    const uint32_t per_token = (rows + (1u << k.slot_bits) - 1) >> k.slot_bits;
-    const dim3 grid((unsigned)((groups * ROW_LANES + THREADS - 1) / THREADS), each == 1 && per_token < 1024 ? per_token : 1);
-    const cudaError_t e = launch_dependent(p.plus_one ? pre_attn_blocks_kernel<true> : pre_attn_blocks_kernel<false>, grid, dim3(THREADS), 0, a.stream, k);
+              p.q_stride, p.k_stride, p.v_stride, n_q, n_kv, tokens, (uint32_t)blocks, p.rot_dims / 2, p.layout, 0, p.plus_one ? 1.0f : 0.0f, p.magnitude, a.status};
+    // Groups of a token: enough for two waves of the GPU, as many as rows at most.
+    while (k.share_bits < 10 && (1u << k.share_bits) < rows && ((uint64_t)tokens << k.share_bits) * ROW_LANES < 2 * 640ull * a.sm_count) k.share_bits++;
+    const uint64_t groups = (uint64_t)tokens << k.share_bits;
+    const dim3 grid((unsigned)((groups * ROW_LANES + THREADS - 1) / THREADS));
+    const cudaError_t e = launch_dependent(p.layout == 2 ? pre_attn_blocks_kernel<true> : pre_attn_blocks_kernel<false>, grid, dim3(THREADS), 0, a.stream, k);
     ++*a.launches;
     return check_cuda(a, e, "qkv_norm_rope_append_blocks_e4m3_d128");
 }
