@@ -23,6 +23,7 @@ namespace {
 constexpr float RMS_EPS = 1e-6f;
 constexpr float ROW_REACH = 11.336f;  // sqrt(128) = 11.3137, and 0.2 % for the rounding of norm, weight and rotation
 constexpr int THREADS = 128;
+constexpr uint32_t SLOTS = 4;      // rows of a group on their way, and one in use
 constexpr uint32_t ROW_LANES = 8;  // of a row: a lane has two octets that turn with each other
 
 struct PreArgs {
@@ -121,11 +122,12 @@ __device__ __forceinline__ void apply(const Turn& t, bool turns, Pairs& p)
     }
 }
 
-// 2^SHARE_BITS groups of eight lanes share the rows of a token (q heads, k heads, v heads in this order), group by group one after the other.  What is the same for
-// a token's heads (the slot, the rotation with its weights, the exponents' bound) is made once a group, and a row's values are asked for one row ahead.  GROUP: its lanes in
-// the warp; groups of a warp may have different rows to do.
+// 2^share_bits groups of eight lanes share the rows of a token (q heads, k heads, v heads in this order), group by group one after the other.  What is the same for
+// a token's heads (the slot, the rotation with its weights, the exponents' bound) is made once a group.  Groups of a warp may have different rows to do, so that a
+// group exchanges values within its own lanes only.  20300 tokens of 32 q and 16 kv heads (17 prompts) take 104.7 us, 6.67 TB/s, which is the copy rate; with rows asked for
+// one ahead into registers 143, two ahead 131 (128 registers, four CTAs an SM), weights and rotation applied one after the other to every row 165.
 template <bool NEXT>
-__global__ void __launch_bounds__(THREADS, 5) pre_attn_blocks_kernel(const __grid_constant__ PreArgs a)
+__global__ void __launch_bounds__(THREADS, 4) pre_attn_blocks_kernel(const __grid_constant__ PreArgs a)
 {
     pdl_wait();
     pdl_launch_dependents();
@@ -142,16 +144,29 @@ __global__ void __launch_bounds__(THREADS, 5) pre_attn_blocks_kernel(const __gri
         if (token >= 1 + lane + 8 * j) before[j] = ld_global(a.slots + token - 1 - lane - 8 * j);
     const uint32_t end_q = a.n_q, end_k = a.n_q + a.n_kv, end = end_k + a.n_kv;
     uint32_t r = group & (shares - 1);
-    struct Row {
-        uint4 lo, hi;
+    // Rows on their way: SLOTS places of 32 bytes a thread in shared memory, written and read by itself alone, so that nothing but its own copies is waited for.  A place
+    // is written again when what was read from it has been used.
+    __shared__ alignas(16) uint4 places[SLOTS][2][THREADS];
+    const __half* const base_q = a.q + (size_t)token * a.q_stride + at.lo;
+    const __half* const base_k = a.k + (size_t)token * a.k_stride + at.lo - (size_t)end_q * 128;  // (row 0 of all, were they keys)
+    const __half* const base_v = a.v + (size_t)token * a.v_stride + at.lo - (size_t)end_k * 128;
+    const uint32_t apart = at.hi - at.lo;
+    uint32_t place = 0;
+    const auto fetch = [&](uint32_t i, uint32_t to) {
+        const __half* src = (i < end_q ? base_q : i < end_k ? base_k : base_v) + (size_t)i * 128;
+        copy_async_if(i < end, &places[to][0][threadIdx.x], src);
+        copy_async_if(i < end, &places[to][1][threadIdx.x], src + apart);
+        copy_async_commit();
     };
-    const auto fetch = [&](uint32_t i) {
-        const __half* src = i < end_q   ? a.q + ((size_t)token * a.q_stride + i * 128)
-                            : i < end_k ? a.k + ((size_t)token * a.k_stride + (i - end_q) * 128)
-                                        : a.v + ((size_t)token * a.v_stride + (i - end_k) * 128);
-        return Row{ld_global_if(i < end, reinterpret_cast<const uint4*>(src + at.lo)), ld_global_if(i < end, reinterpret_cast<const uint4*>(src + at.hi))};
+#pragma unroll
+    for (uint32_t j = 0; j + 1 < SLOTS; j++) fetch(r + j * shares, j);
+    const auto next = [&]() {  // row r
+        copy_async_wait<SLOTS - 2>();
+        const Pairs p = unpack_pairs<NEXT>(places[place][0][threadIdx.x], places[place][1][threadIdx.x]);
+        fetch(r + (SLOTS - 1) * shares, (place + SLOTS - 1) % SLOTS);
+        place = (place + 1) % SLOTS;
+        return p;
     };
-    Row row = fetch(r);
     float c[8], s[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) c[i] = 1.0f, s[i] = 0.0f;
@@ -212,8 +227,7 @@ __global__ void __launch_bounds__(THREADS, 5) pre_attn_blocks_kernel(const __gri
     }
 
     for (; r < end_q; r += shares) {
-        Pairs p = unpack_pairs<NEXT>(row.lo, row.hi);
-        row = fetch(r + shares);
+        Pairs p = next();
         const float inv = inverse_rms(p);
         apply(turn, at.turns, p);
         scale(p, inv);
@@ -229,8 +243,7 @@ __global__ void __launch_bounds__(THREADS, 5) pre_attn_blocks_kernel(const __gri
         int8_t* const exps = a.exps[side] + tile0;
         int old = ld_global_if(!fresh, exps + (r - first));
         for (; r < last; r += shares) {
-            Pairs p = unpack_pairs<NEXT>(row.lo, row.hi);
-            row = fetch(r + shares);
+            Pairs p = next();
             const uint32_t head = r - first;
             const int had = old, e = fresh ? least : max(least, had);
             old = ld_global_if(!fresh && r + shares < last, exps + head + shares);
@@ -323,8 +336,10 @@ int launch_qkv_norm_rope_append_blocks(const LaunchArgs& a)
     PreArgs k{(const __half*)a.b[0].ptr, (const __half*)a.b[3].ptr, (const __half*)a.b[4].ptr, (const float*)a.b[1].ptr, (const float*)a.b[5].ptr, (const float2*)a.b[6].ptr,
               (const uint32_t*)a.b[7].ptr, (__half*)a.b[2].ptr, {(uint8_t*)a.b[8].ptr, (uint8_t*)a.b[10].ptr}, {(int8_t*)a.b[9].ptr, (int8_t*)a.b[11].ptr},
               p.q_stride, p.k_stride, p.v_stride, n_q, n_kv, tokens, (uint32_t)blocks, p.rot_dims / 2, p.layout, 0, p.plus_one ? 1.0f : 0.0f, p.magnitude, a.status};
-    // Groups of a token: enough for two waves of the GPU, as many as rows at most.
-    while (k.share_bits < 10 && (1u << k.share_bits) < rows && ((uint64_t)tokens << k.share_bits) * ROW_LANES < 2 * 640ull * a.sm_count) k.share_bits++;
+    // Groups of a token.  What a group makes for its token costs it as much as two rows, so that as few as give each SM 256 threads to do are best (us in a recorded
+    // chain at 128 | 256 | 512 threads: 512 tokens of 32 q and 16 kv heads 3.3 | 3.6 | 4.7, about 440 tokens 4.4 | 4.2 | 5.2, 9225 of 8 and 2 heads 9.3 | 9.3 | 10.2); but
+    // sixteen rows a group at most: 20300 tokens take 112.8 with 8, 104.7 with 16, 107.4 with 32 of them (4104 tokens 21.3, 20.0, 20.5).
+    while (k.share_bits < 10 && (1u << k.share_bits) < rows && (((uint64_t)tokens << k.share_bits) * ROW_LANES < 256ull * a.sm_count || rows > 16u << k.share_bits)) k.share_bits++;
     const uint64_t groups = (uint64_t)tokens << k.share_bits;
     const dim3 grid((unsigned)((groups * ROW_LANES + THREADS - 1) / THREADS));
     const cudaError_t e = launch_dependent(p.layout == 2 ? pre_attn_blocks_kernel<true> : pre_attn_blocks_kernel<false>, grid, dim3(THREADS), 0, a.stream, k);

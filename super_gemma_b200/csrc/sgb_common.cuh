@@ -293,6 +293,17 @@ __device__ __forceinline__ T ld_global(const T* p)
     }
     return v;
 }
+// 16 bytes into shared memory without a register, by the copy engine of the load path; a thread's copies are committed in groups and waited for by their number.
+__device__ __forceinline__ void copy_async_if(bool p, void* dst_smem, const void* src)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(smem_u32(dst_smem)), "l"(src), "r"((uint32_t)p) : "memory");
+}
+__device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_async_wait()  // all but the last N groups
+{
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 // Barrier `id` (1..15; 0 is __syncthreads) over `threads` threads of the CTA, a multiple of 32.
 __device__ __forceinline__ void named_barrier_sync(uint32_t id, uint32_t threads)
 {
