@@ -9,7 +9,9 @@
 // covers it, else whole warps with N units a lane.
 #include <cuda_bf16.h>
 
+#include <algorithm>
 #include <cmath>
+#include <mutex>
 #include <type_traits>
 
 #include "sgb_common.cuh"
@@ -29,18 +31,21 @@ struct NormsArgs {
     uint32_t post, gates;
     float plus, scale, eps;  // plus: 1 where weights are 1 + w
 };
-constexpr uint32_t MOST_EACH = 8;   // units of a lane
 enum : uint32_t { POST_NONE = 0, POST_NORM = 1, FIRST_NORM = 2 };
 enum : uint32_t { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_ROW = 2, GATE_ONE = 3 };
 constexpr uint32_t MOST_WARPS = 16;  // of a row
 
+// Shared memory of a CTA whose rows come ahead.
+constexpr size_t MOST_STAGED = 200 * 1024;
 // Consecutive values of a unit: 16 bytes of R.
 template <typename R>
 constexpr int UNIT = 16 / sizeof(R);
+template <typename R>
+constexpr int MOST_STREAMED = sizeof(R) == 4 ? 8 : 4;  // units of a lane whose rows come ahead
 
 // A unit of f16 as it is loaded, and as pairs of f32.
 template <int U>
-struct RawHalf {
+struct alignas(2 * U) RawHalf {
     uint32_t w[U / 2];
 };
 template <int U>
@@ -115,7 +120,8 @@ __device__ __forceinline__ void load_f32(const float* p, float2 (&v)[U / 2])
     }
 }
 
-// The sum over a row's lanes: a butterfly in the warp, then over the row's warps in their order.  Everybody calls it.
+// The sum over a row's lanes: a butterfly in the warp, then over the row's warps in their order.  Everybody calls it.  A row of several warps has the CTA to itself, and
+// `parts` is 0 for the warps up to the next multiple of four.
 __device__ __forceinline__ float row_sum(float v, uint32_t lanes, float* parts)
 {
     if (lanes >= 32) {
@@ -125,7 +131,7 @@ __device__ __forceinline__ float row_sum(float v, uint32_t lanes, float* parts)
         for (uint32_t d = 1; d < lanes; d <<= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     }
     if (lanes <= 32) return v;
-    if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = v;  // (one row a CTA; those of warps that it has not are 0)
+    if ((threadIdx.x & 31) == 0) parts[threadIdx.x >> 5] = v;
     __syncthreads();
     v = 0.0f;
     for (uint32_t i = 0; i < lanes / 32; i += 4) {
@@ -135,86 +141,236 @@ __device__ __forceinline__ float row_sum(float v, uint32_t lanes, float* parts)
     return v;
 }
 
+// Where a thread stands: its row's place in the CTA, its first column.
+struct Place {
+    uint32_t in_cta, per_cta, col, step;  // `step` columns from unit to unit
+};
+template <int U>
+__device__ __forceinline__ Place place_of(uint32_t lanes)
+{
+    if (lanes > 32) return Place{0, 1, threadIdx.x * U, lanes * U};
+    const uint32_t shift = __ffs(lanes) - 1;
+    return Place{threadIdx.x >> shift, blockDim.x >> shift, (threadIdx.x & (lanes - 1)) * U, lanes * U};
+}
+
+// h' = (h + y by w) s, in v (which holds h), and its sum of squares.
 template <typename R, int N>
-__global__ void __launch_bounds__(32 * MOST_WARPS) block_norms_kernel(const __grid_constant__ NormsArgs a)
+__device__ __forceinline__ void add_block(const NormsArgs& a, const RawHalf<UNIT<R>> (&y)[N], const float2 (&w)[N][UNIT<R> / 2], float by, float2 (&v)[N][UNIT<R> / 2])
+{
+    const float2 by2 = make_float2(by, by), scale2 = make_float2(a.scale, a.scale);
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int j = 0; j < UNIT<R> / 2; j++) v[i][j] = mul2_rn(fma2_rn(mul2_rn(pair_of(y[i].w[j]), w[i][j]), by2, v[i][j]), scale2);
+}
+template <int N, int P>
+__device__ __forceinline__ float squares(const float2 (&v)[N][P])
+{
+    float2 ss = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int j = 0; j < P; j++) ss = fma2_rn(v[i][j], v[i][j], ss);
+    return ss.x + ss.y;
+}
+template <int N, int U>
+__device__ __forceinline__ float squares(const RawHalf<U> (&y)[N])
+{
+    float2 ss = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int j = 0; j < U / 2; j++) {
+            const float2 f = pair_of(y[i].w[j]);
+            ss = fma2_rn(f, f, ss);
+        }
+    return ss.x + ss.y;
+}
+template <int U>
+__device__ __forceinline__ void times_f32(const float* p, float2 (&w)[U / 2])
+{
+    float2 f[U / 2];
+    load_f32<U>(p, f);
+#pragma unroll
+    for (int j = 0; j < U / 2; j++) w[j] = mul2_rn(w[j], f[j]);
+}
+template <typename R>
+__device__ __forceinline__ void write_next(__half* x, const float2 (&v)[UNIT<R> / 2], const float2 (&w)[UNIT<R> / 2], float inv)
+{
+    float2 out[UNIT<R> / 2];
+#pragma unroll
+    for (int j = 0; j < UNIT<R> / 2; j++) out[j] = mul2_rn(mul2_rn(v[j], make_float2(inv, inv)), w[j]);
+    store_f16<UNIT<R>>(x, out);
+}
+
+// One row a CTA (or a warp, or some of its lanes): nothing waits for anything that could have been asked for before it.  The block's weights come beside the row, the
+// next ones beside the second sum.
+// Three units of 16-bit values: two CTAs of twelve warps an SM, 80 registers instead of 98 (400 rows of 5376 3.6 us, else 4.1).
+template <typename R, int N>
+constexpr bool TIGHT = sizeof(R) == 2 && N == 3;
+template <typename R, int N>
+__global__ void __launch_bounds__(TIGHT<R, N> ? 384 : 512, TIGHT<R, N> ? 2 : 0) block_norms_kernel(const __grid_constant__ NormsArgs a)
 {
     constexpr int U = UNIT<R>, P = U / 2;
     __shared__ alignas(16) float parts[2][MOST_WARPS];
-    if (a.lanes > 32 && threadIdx.x < 2 * MOST_WARPS) parts[threadIdx.x / MOST_WARPS][threadIdx.x % MOST_WARPS] = 0.0f;
     pdl_wait();
     pdl_launch_dependents();
-    if (a.lanes > 32) __syncthreads();  // the zeros come before the sums
-    const uint32_t shift = a.lanes <= 32 ? __ffs(a.lanes) - 1 : 31;  // a row of several warps has the CTA to itself
-    const uint32_t lane = a.lanes <= 32 ? threadIdx.x & (a.lanes - 1) : threadIdx.x;
-    const uint64_t row = a.lanes <= 32 ? (uint64_t)blockIdx.x * (blockDim.x >> shift) + (threadIdx.x >> shift) : blockIdx.x;
-    const size_t at = row * a.hidden + lane * U;  // of the first unit
-    const uint32_t step = a.lanes * U;
+    const Place me = place_of<U>(a.lanes);
+    const uint64_t row = (uint64_t)blockIdx.x * me.per_cta + me.in_cta;
+    const size_t at = row * a.hidden + me.col;  // of the first unit
     const bool live = row < a.rows;
-    const float inv_n = 1.0f / (float)a.hidden;
-    // all units but the last are within the row
-    const auto on = [&](int i) { return live && (i + 1 < N || lane * U + i * step < a.hidden); };
+    const auto on = [&](int i) { return live && (i + 1 < N || me.col + i * me.step < a.hidden); };  // all units but the last are within the row
     RawHalf<U> y[N];
     uint4 raw[N];
+    float2 w[N][P];
 #pragma unroll
     for (int i = 0; i < N; i++) {
         y[i] = RawHalf<U>{};
         raw[i] = make_uint4(0, 0, 0, 0);
         if (on(i)) {
-            if (a.post != FIRST_NORM) y[i] = load_f16<U>(a.y + at + i * step);
-            raw[i] = ld_global(reinterpret_cast<const uint4*>(static_cast<const R*>(a.h) + at + i * step));
+            if (a.post != FIRST_NORM) y[i] = load_f16<U>(a.y + at + i * me.step);
+            raw[i] = ld_global(reinterpret_cast<const uint4*>(static_cast<const R*>(a.h) + at + i * me.step));
         }
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+#pragma unroll
+        for (int j = 0; j < P; j++) w[i][j] = make_float2(1.0f, 1.0f);
+        if (a.post == POST_NORM && on(i)) load_f32<U>(a.w_post + me.col + i * me.step, w[i]);
     }
     float by = 1.0f;  // of the block's output
     if (a.gates == GATE_ROW && live) by = ld_global(a.gate + row);
     if (a.gates == GATE_ONE) by = ld_global(a.gate);
+    if (a.lanes > 32) {
+        if (threadIdx.x < MOST_WARPS) parts[0][threadIdx.x] = parts[1][threadIdx.x] = 0.0f;
+        __syncthreads();  // the zeros come before the sums
+    }
+    const float inv_n = 1.0f / (float)a.hidden;
+    const float2 plus2 = make_float2(a.plus, a.plus);
     if (a.post == POST_NORM) {
-        float2 ss = make_float2(0.0f, 0.0f);
+        by *= rsqrtf(row_sum(squares(y), a.lanes, parts[0]) * inv_n + a.eps);
 #pragma unroll
         for (int i = 0; i < N; i++)
 #pragma unroll
-            for (int j = 0; j < P; j++) {
-                const float2 f = pair_of(y[i].w[j]);
-                ss = fma2_rn(f, f, ss);
-            }
-        by *= rsqrtf(row_sum(ss.x + ss.y, a.lanes, parts[0]) * inv_n + a.eps);
+            for (int j = 0; j < P; j++) w[i][j] = add2_rn(w[i][j], plus2);
     }
-    const float2 by2 = make_float2(by, by), scale2 = make_float2(a.scale, a.scale), plus2 = make_float2(a.plus, a.plus);
-    float2 ss = make_float2(0.0f, 0.0f), v[N][P];
+    float2 v[N][P];
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        unpack<R>(raw[i], v[i]);
-        if (a.post != FIRST_NORM && on(i)) {
-            float2 n[P], w[P];
+    for (int i = 0; i < N; i++) unpack<R>(raw[i], v[i]);
+    if (a.post != FIRST_NORM) {
+        if (a.gates == GATE_CHANNEL) {
 #pragma unroll
-            for (int j = 0; j < P; j++) n[j] = pair_of(y[i].w[j]);
-            if (a.post == POST_NORM) {
-                load_f32<U>(a.w_post + lane * U + i * step, w);
-#pragma unroll
-                for (int j = 0; j < P; j++) n[j] = mul2_rn(n[j], add2_rn(w[j], plus2));
-            }
-            if (a.gates == GATE_CHANNEL) {
-                load_f32<U>(a.gate + lane * U + i * step, w);
-#pragma unroll
-                for (int j = 0; j < P; j++) n[j] = mul2_rn(n[j], w[j]);
-            }
-#pragma unroll
-            for (int j = 0; j < P; j++) v[i][j] = mul2_rn(fma2_rn(n[j], by2, v[i][j]), scale2);
-            *reinterpret_cast<uint4*>(static_cast<R*>(a.h_out) + at + i * step) = pack<R>(v[i]);
+            for (int i = 0; i < N; i++)
+                if (on(i)) times_f32<U>(a.gate + me.col + i * me.step, w[i]);
         }
+        add_block<R, N>(a, y, w, by, v);
 #pragma unroll
-        for (int j = 0; j < P; j++) ss = fma2_rn(v[i][j], v[i][j], ss);
+        for (int i = 0; i < N; i++)
+            if (on(i)) *reinterpret_cast<uint4*>(static_cast<R*>(a.h_out) + at + i * me.step) = pack<R>(v[i]);
     }
-    const float inv = rsqrtf(row_sum(ss.x + ss.y, a.lanes, parts[1]) * inv_n + a.eps);
-    const float2 inv2 = make_float2(inv, inv);
+#pragma unroll
+    for (int i = 0; i < N; i++)
+        if (on(i)) load_f32<U>(a.w_pre + me.col + i * me.step, w[i]);
+    const float inv = rsqrtf(row_sum(squares(v), a.lanes, parts[1]) * inv_n + a.eps);
 #pragma unroll
     for (int i = 0; i < N; i++) {
         if (!on(i)) continue;
-        float2 w[P];
-        load_f32<U>(a.w_pre + lane * U + i * step, w);
 #pragma unroll
-        for (int j = 0; j < P; j++) v[i][j] = mul2_rn(mul2_rn(v[i][j], inv2), add2_rn(w[j], plus2));
-        store_f16<U>(a.x + at + i * step, v[i]);
+        for (int j = 0; j < P; j++) w[i][j] = add2_rn(w[i][j], plus2);
+        write_next<R>(a.x + at + i * me.step, v[i], w[i], inv);
     }
+}
+
+// Many rows: CTAs that stay, with the weights of their columns in registers.  Rows come ahead of their turn into shared memory, STAGES - 1 of them on their way; a thread
+// reads what it has copied itself, so that only its own copies are waited for, and a stage is written again one row after it was read.
+template <typename R, int N, int STAGES>
+__global__ void __launch_bounds__(512) block_norms_stream_kernel(const __grid_constant__ NormsArgs a)
+{
+    constexpr int U = UNIT<R>, P = U / 2;
+    __shared__ alignas(16) float parts[3][MOST_WARPS];
+    extern __shared__ uint4 stages[];
+    pdl_wait();
+    pdl_launch_dependents();
+    const Place me = place_of<U>(a.lanes);
+    const uint32_t stride = gridDim.x * me.per_cta;
+    const uint64_t first = (uint64_t)blockIdx.x * me.per_cta;
+    const auto on = [&](uint64_t row, int i) { return row < a.rows && (i + 1 < N || me.col + i * me.step < a.hidden); };
+    const auto h_place = [&](uint32_t stage, int i) { return stages + (stage * N + i) * blockDim.x + threadIdx.x; };
+    const auto y_place = [&](uint32_t stage, int i) {
+        return reinterpret_cast<RawHalf<U>*>(stages + STAGES * N * blockDim.x) + (stage * N + i) * blockDim.x + threadIdx.x;
+    };
+    const auto ask = [&](uint64_t row, uint32_t stage) {
+        const size_t at = row * a.hidden + me.col;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            copy_async_if<2 * U>(on(row, i) && a.post != FIRST_NORM, y_place(stage, i), a.y + at + i * me.step);
+            copy_async_if<16>(on(row, i), h_place(stage, i), static_cast<const R*>(a.h) + at + i * me.step);
+        }
+        copy_async_commit();
+    };
+#pragma unroll
+    for (uint32_t j = 0; j + 1 < STAGES; j++) ask(first + me.in_cta + j * (uint64_t)stride, j);
+    float2 w[N][P], next[N][P];  // what a column of the block and of the next input is multiplied by
+    const float2 plus2 = make_float2(a.plus, a.plus);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const uint32_t col = me.col + i * me.step;
+#pragma unroll
+        for (int j = 0; j < P; j++) w[i][j] = next[i][j] = make_float2(1.0f, 1.0f);
+        if (col >= a.hidden) continue;
+        if (a.post == POST_NORM) {
+            load_f32<U>(a.w_post + col, w[i]);
+#pragma unroll
+            for (int j = 0; j < P; j++) w[i][j] = add2_rn(w[i][j], plus2);
+        }
+        if (a.gates == GATE_CHANNEL) times_f32<U>(a.gate + col, w[i]);
+        load_f32<U>(a.w_pre + col, next[i]);
+#pragma unroll
+        for (int j = 0; j < P; j++) next[i][j] = add2_rn(next[i][j], plus2);
+    }
+    float one = 1.0f;
+    if (a.gates == GATE_ONE) one = ld_global(a.gate);
+    if (a.lanes > 32) {
+        if (threadIdx.x < MOST_WARPS) parts[0][threadIdx.x] = parts[1][threadIdx.x] = parts[2][threadIdx.x] = 0.0f;
+        __syncthreads();  // the zeros come before the sums
+    }
+    const float inv_n = 1.0f / (float)a.hidden;
+    uint32_t stage = 0, turn = 0;
+    for (uint64_t row0 = first; row0 < a.rows; row0 += stride) {
+        const uint64_t row = row0 + me.in_cta;
+        const size_t at = row * a.hidden + me.col;
+        float by = one;
+        if (a.gates == GATE_ROW && row < a.rows) by = ld_global(a.gate + row);
+        RawHalf<U> y[N];
+        float2 v[N][P];
+        copy_async_wait<STAGES - 2>();
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            y[i] = RawHalf<U>{};
+            uint4 raw = make_uint4(0, 0, 0, 0);
+            if (on(row, i)) {
+                if (a.post != FIRST_NORM) y[i] = *y_place(stage, i);
+                raw = *h_place(stage, i);
+            }
+            unpack<R>(raw, v[i]);
+        }
+        ask(row + (STAGES - 1) * (uint64_t)stride, stage == 0 ? STAGES - 1 : stage - 1);
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+        if (a.post == POST_NORM) by *= rsqrtf(row_sum(squares(y), a.lanes, parts[2]) * inv_n + a.eps);
+        if (a.post != FIRST_NORM) {
+            add_block<R, N>(a, y, w, by, v);
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (on(row, i)) *reinterpret_cast<uint4*>(static_cast<R*>(a.h_out) + at + i * me.step) = pack<R>(v[i]);
+        }
+        // a row's sums are read while the next one's are written where nothing is waited for in between (post 0 and 2): two places in turn
+        const float inv = rsqrtf(row_sum(squares(v), a.lanes, parts[turn]) * inv_n + a.eps);
+        turn ^= 1;
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (on(row, i)) write_next<R>(a.x + at + i * me.step, v[i], next[i], inv);
+    }
+    copy_async_wait<0>();
 }
 
 struct PushNorms {
@@ -222,11 +378,61 @@ struct PushNorms {
     float scale, eps;
 };
 
-template <typename R>
-auto norms_kernel(uint32_t n)
+struct NormsShape {
+    uint32_t lanes, each;  // of a row; units of a lane
+};
+// Eight lanes to sixteen warps a row and at most `most` units a lane, so that a row takes the fewest instructions: about 45 a unit, full or not, and 110 for the two sums.
+NormsShape norms_shape(uint32_t units, uint32_t most)
 {
-    return n == 1 ? block_norms_kernel<R, 1> : n == 2 ? block_norms_kernel<R, 2> : n == 3 ? block_norms_kernel<R, 3> : n == 4 ? block_norms_kernel<R, 4>
-         : n == 5 ? block_norms_kernel<R, 5> : n == 6 ? block_norms_kernel<R, 6> : n == 7 ? block_norms_kernel<R, 7> : block_norms_kernel<R, 8>;
+    NormsShape s{0, 0};
+    uint32_t least = ~0u;
+    const auto look = [&](uint32_t lanes) {
+        const uint32_t each = (units + lanes - 1) / lanes, cost = lanes * (each * 45 + 110);
+        if (each <= most && cost < least) s = {lanes, each}, least = cost;
+    };
+    for (uint32_t lanes = units < 8 ? 1 : 8; lanes < 32; lanes *= 2) look(lanes);
+    for (uint32_t warps = 1; warps <= MOST_WARPS; warps++) look(32 * warps);
+    if (s.lanes == 0) s = {32 * MOST_WARPS, (units + 32 * MOST_WARPS - 1) / (32 * MOST_WARPS)};  // the widest rows
+    return s;
+}
+
+template <typename R, int N, int STAGES>
+int launch_stream(const LaunchArgs& a, const NormsArgs& k, uint32_t threads, size_t smem)
+{
+    const auto kern = block_norms_stream_kernel<R, N, STAGES>;
+    static std::mutex mutex;
+    static int registers[64] = {};  // of a thread, 0: not asked yet
+    int regs = 0;
+    {
+        std::lock_guard<std::mutex> lock(mutex);
+        if (a.device < 0 || a.device >= 64 || registers[a.device] == 0) {
+            if (int r = check_cuda(a, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MOST_STAGED), "cudaFuncSetAttribute(block_norms)")) return r;
+            cudaFuncAttributes at;
+            if (int r = check_cuda(a, cudaFuncGetAttributes(&at, kern), "cudaFuncGetAttributes(block_norms)")) return r;
+            regs = at.numRegs;
+            if (a.device >= 0 && a.device < 64) registers[a.device] = regs;
+        } else {
+            regs = registers[a.device];
+        }
+    }
+    // as many CTAs as the SMs hold at once: registers come in eights a thread, an SM has 65536 of them, 2048 threads and 228 KB, of which a CTA takes 1 KB more than it asks for
+    const uint32_t by_regs = 65536 / ((regs + 7) / 8 * 8 * threads), by_smem = (uint32_t)(228 * 1024 / (smem + 2048)), by_threads = std::min(32u, 2048 / threads);
+    const uint32_t resident = std::max(1u, std::min(by_regs, std::min(by_smem, by_threads)));
+    const uint32_t per_cta = threads / k.lanes, ctas = (uint32_t)((k.rows + per_cta - 1ull) / per_cta);
+    return check_cuda(a, launch_dependent(kern, dim3(std::min(ctas, resident * a.sm_count)), dim3(threads), smem, a.stream, k), "block_norms");
+}
+
+template <typename R, int N>
+int launch_norms(const LaunchArgs& a, const NormsArgs& k, bool stream)
+{
+    const uint32_t threads = k.lanes <= 32 ? 128 : k.lanes, per_cta = threads / k.lanes;
+    if constexpr (N <= MOST_STREAMED<R>) {
+        const size_t stage = (size_t)N * threads * (16 + 2 * UNIT<R>);
+        if (stream && 3 * stage <= MOST_STAGED) return launch_stream<R, N, 3>(a, k, threads, 3 * stage);
+        if constexpr (sizeof(R) == 4)  // rows of 10248 and more
+            if (stream) return launch_stream<R, N, 2>(a, k, threads, 2 * stage);
+    }
+    return check_cuda(a, launch_dependent(block_norms_kernel<R, N>, dim3((unsigned)((k.rows + per_cta - 1ull) / per_cta)), dim3(threads), 0, a.stream, k), "block_norms");
 }
 
 }  // namespace
@@ -269,20 +475,28 @@ int launch_block_norms(const LaunchArgs& a)
     const uint32_t units = hidden / U;
     NormsArgs k{(const __half*)a.b[0].ptr, a.b[1].ptr, (const float*)a.b[2].ptr, (const float*)a.b[3].ptr, (const float*)a.b[4].ptr, a.b[5].ptr, (__half*)a.b[6].ptr,
                 rows, hidden, 1, p.post, p.gates, p.plus_one ? 1.0f : 0.0f, p.scale, p.eps};
-    // units a lane: eight at most
-    uint32_t each = 1;
-    if (units <= 32) {
-        while (k.lanes < units) k.lanes <<= 1;
-    } else {
-        uint32_t warps = (units + 32 * MOST_EACH - 1) / (32 * MOST_EACH);
-        each = (units + 32 * warps - 1) / (32 * warps);
-        warps = (units + 32 * each - 1) / (32 * each);
-        k.lanes = 32 * warps;
+    // Rows come ahead of their turn where there is enough to stream, 96 MB; below, the CTAs' start costs more than it brings.  A row of its own has lanes enough for 2048 columns
+    // at a time where all of them are on the GPU at once, else as many units a lane as registers allow.
+    const bool stream = (uint64_t)n * (4 + 2 * R_BYTES) >= 96ull << 20;
+    NormsShape shape = norms_shape(units, std::min(4u, (hidden + 2047) / 2048));
+    if (stream)
+        shape = norms_shape(units, U == 8 ? 4 : 3);
+    else if ((uint64_t)rows * shape.lanes > 1024ull * a.sm_count)
+        shape = norms_shape(units, U == 8 && units <= 192 ? 6 : 4);  // (6000 rows of 1096 in f16: 9.8 us with six units a lane, 11.2 with four; of 5376, 800 rows: 7.6 | 7.2)
+    k.lanes = shape.lanes;
+    int e = 0;
+    switch (shape.each) {
+        case 1: e = launch_norms<R, 1>(a, k, stream); break;
+        case 2: e = launch_norms<R, 2>(a, k, stream); break;
+        case 3: e = launch_norms<R, 3>(a, k, stream); break;
+        case 4: e = launch_norms<R, 4>(a, k, stream); break;
+        case 5: e = launch_norms<R, 5>(a, k, stream); break;
+        case 6: e = launch_norms<R, 6>(a, k, stream); break;
+        default:  // f32 rows of more than 12288
+            if constexpr (U == 4) e = shape.each == 7 ? launch_norms<R, 7>(a, k, stream) : launch_norms<R, 8>(a, k, stream);
     }
-    const uint32_t threads = k.lanes <= 32 ? 128 : k.lanes, per_cta = threads / k.lanes;
-    const cudaError_t e = launch_dependent(norms_kernel<R>(each), dim3((unsigned)((rows + per_cta - 1ull) / per_cta)), dim3(threads), 0, a.stream, k);
     ++*a.launches;
-    return check_cuda(a, e, "block_norms");
+    return e;
 }
 template int launch_block_norms<__half>(const LaunchArgs&);
 template int launch_block_norms<__nv_bfloat16>(const LaunchArgs&);
