@@ -17,12 +17,43 @@ constexpr int ROW_THREADS = 256;
 constexpr uint32_t MOST_ROT = 1024;
 
 // ---- rows of cosines and sines ---------------------------------------------------------------------------------------------------
-// In turns instead of radians the reduction is a subtraction: g = f / 2 pi, a = 2 pi (p g - rint(p g)).  A position has up to 31 bits and p g
-// as many before the point, so that the product is taken in 64 bits and with the 1 / 2 pi in two of them (hi + lo): what is left
-// behind the point is good to 2^-53 of a turn for every position.  The rest is f32: half a turn at most, and so an angle error of
-// 2^-25 turns, which is what an f32 cosine of it could show.
-// Written bytes bound it; a thread makes two pairs (16 bytes) of ROWS tokens and has its two frequencies in registers.
+// Angles are counted in turns, as 64-bit fractions of one: F = f / 2 pi mod 1 in units of 2^-64, made of the f64 frequency and 1 / 2 pi in two f64 (hi + lo),
+// so that the whole turns of p F fall off by themselves and what is left is good to 2^-34 of a turn for every 32-bit p.  Its upper word's nearest quarter turn goes into signs and
+// an exchange of sine and cosine, the rest, an eighth of a turn at most, into their Taylor series up to x^9 and x^10 (cut off below 2 * 10^-9).
+// Integers instead of f64 sums and reductions: those kept the units that convert between formats busy, 5.8 us for 32768 rows of 64 pairs, now 3.4.
+// A thread makes two pairs (16 bytes) of ROWS tokens.
 constexpr double INV_2PI_HI = 0.15915494309189535, INV_2PI_LO = -9.839338337591243e-18;
+
+__device__ __forceinline__ uint64_t fraction_of_turn(double f)
+{
+    const double hi = f * INV_2PI_HI, lo = fma(f, INV_2PI_HI, -hi) + f * INV_2PI_LO, unit = 18446744073709551616.0;
+    return (uint64_t)__double2ll_rn((hi - rint(hi)) * unit) + (uint64_t)__double2ll_rn(lo * unit);
+}
+// Cosines and sines of two angles of t 2^-32 turns each, times m.
+__device__ __forceinline__ float4 cos_sin_of(uint32_t t0, uint32_t t1, float2 m)
+{
+    const uint32_t quarter[2] = {(t0 + 0x20000000u) >> 30, (t1 + 0x20000000u) >> 30};
+    const float radian = 1.4629180792671596e-9f;  // 2 pi 2^-32
+    const float2 x = make_float2((float)(int)(t0 - (quarter[0] << 30)) * radian, (float)(int)(t1 - (quarter[1] << 30)) * radian), z = mul2_rn(x, x);
+    const auto both = [](float v) { return make_float2(v, v); };
+    float2 c = both(-1.0f / 3628800.0f), s = both(1.0f / 362880.0f);
+    c = fma2_rn(c, z, both(1.0f / 40320.0f));
+    c = fma2_rn(c, z, both(-1.0f / 720.0f));
+    c = fma2_rn(c, z, both(1.0f / 24.0f));
+    c = fma2_rn(c, z, both(-0.5f));
+    c = mul2_rn(fma2_rn(c, z, both(1.0f)), m);
+    s = fma2_rn(s, z, both(-1.0f / 5040.0f));
+    s = fma2_rn(s, z, both(1.0f / 120.0f));
+    s = fma2_rn(s, z, both(-1.0f / 6.0f));
+    s = mul2_rn(fma2_rn(mul2_rn(s, z), x, x), m);
+    // a quarter turn on: (c, s) -> (-s, c)
+    const auto place = [](uint32_t q, float c, float s) {
+        const float a = q & 1 ? s : c, b = q & 1 ? c : s;
+        return make_float2(__uint_as_float(__float_as_uint(a) ^ ((q + 1) >> 1 << 31)), __uint_as_float(__float_as_uint(b) ^ (q >> 1 << 31)));
+    };
+    const float2 first = place(quarter[0], c.x, s.x), second = place(quarter[1], c.y, s.y);
+    return make_float4(first.x, first.y, second.x, second.y);
+}
 
 template <int ROWS>
 __global__ void __launch_bounds__(ROW_THREADS) rope_cos_sin_kernel(const double* freqs, const int* positions, float4* __restrict__ cos_sin, float magnitude,
@@ -33,31 +64,22 @@ __global__ void __launch_bounds__(ROW_THREADS) rope_cos_sin_kernel(const double*
     const uint32_t row = threadIdx.x / per_row, at = threadIdx.x - row * per_row;
     if (row >= rows_here) return;
     const uint64_t first = (uint64_t)blockIdx.x * (rows_here * ROWS) + row;
-    double hi[2], lo[2];
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-        const double f = ld_global(freqs + 2 * at + j);
-        hi[j] = f * INV_2PI_HI;
-        lo[j] = fma(f, INV_2PI_HI, -hi[j]) + f * INV_2PI_LO;
-    }
-    int p[ROWS];
+    const double f[2] = {ld_global(freqs + 2 * at), ld_global(freqs + 2 * at + 1)};
+    uint32_t p[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
         p[i] = 0;
-        if (first + i * rows_here < tokens) p[i] = ld_global(positions + first + i * rows_here);
+        if (first + i * rows_here < tokens) p[i] = (uint32_t)ld_global(positions + first + i * rows_here);
     }
+    const uint64_t turn[2] = {fraction_of_turn(f[0]), fraction_of_turn(f[1])};
+    const float2 m = make_float2(magnitude + (float)(f[0] - f[0]), magnitude + (float)(f[1] - f[1]));  // a frequency that is no number gives rows that are none
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
         const uint64_t t = first + i * rows_here;
         if (t >= tokens) return;
-        float c[2], s[2];
-#pragma unroll
-        for (int j = 0; j < 2; j++) {
-            const double x = (double)p[i], turns = x * hi[j];
-            const double rest = (turns - rint(turns)) + fma(x, lo[j], fma(x, hi[j], -turns));
-            sincospif(2.0f * (float)rest, &s[j], &c[j]);
-        }
-        cos_sin[t * per_row + at] = make_float4(c[0] * magnitude, s[0] * magnitude, c[1] * magnitude, s[1] * magnitude);
+        // the upper word of p F, p counted as signed: sign and all fall off above 2^64 but for p's high word, all ones where it is negative
+        const auto upper = [&](uint64_t F) { return (uint32_t)((p[i] * F) >> 32) - ((int)p[i] < 0 ? (uint32_t)F : 0u); };
+        cos_sin[t * per_row + at] = cos_sin_of(upper(turn[0]), upper(turn[1]), m);
     }
 }
 
@@ -68,7 +90,8 @@ struct PushCosSin {
 
 // ---- rotation --------------------------------------------------------------------------------------------------------------------
 // A thread has one piece of 16 dims (two octets of a layout's pairs) of ROWS heads of a token, all of them asked for before the first
-// is turned; the token's eight cosines and sines stay in its registers.  Two bytes read and two written per value: bound by bytes.
+// is turned; the token's eight cosines and sines stay in its registers.  Two bytes read and two written per value: bound by bytes (8192
+// tokens of 32 and 16 heads of 128, neighbours coupled, out of packed rows: 30.1 us, 6.8 TB/s).
 struct RotateArgs {
     const __half* src[2];  // q, k
     __half* dst[2];
@@ -179,9 +202,9 @@ int launch_rope_cos_sin(const LaunchArgs& a)
     if (int r = need_bytes(a, 2, 4 * (size_t)tokens * p.rot_dims, "cos_sin")) return r;
     if (int r = need_aligned(a, {8, 4, 16})) return r;
     const uint32_t per_row = p.rot_dims / 4, rows_here = ROW_THREADS / per_row;
-    const bool many = (uint64_t)tokens * per_row > 4ull * 2048 * a.sm_count;
-    const uint32_t each = rows_here * (many ? 4 : 1);
-    const cudaError_t e = launch_dependent(many ? rope_cos_sin_kernel<4> : rope_cos_sin_kernel<1>, dim3((tokens + each - 1ull) / each), dim3(ROW_THREADS), 0, a.stream,
+    const bool many = (uint64_t)tokens * per_row > 2048ull * a.sm_count;  // (ROWS 8 | 4 | 1, 32768 rows of 64 pairs: 3.4 | 3.5 | 5.6 us)
+    const uint32_t each = rows_here * (many ? 8 : 1);
+    const cudaError_t e = launch_dependent(many ? rope_cos_sin_kernel<8> : rope_cos_sin_kernel<1>, dim3((tokens + each - 1ull) / each), dim3(ROW_THREADS), 0, a.stream,
                                            (const double*)a.b[0].ptr, (const int*)a.b[1].ptr, (float4*)a.b[2].ptr, p.magnitude, tokens, per_row, rows_here);
     ++*a.launches;
     return check_cuda(a, e, "rope_cos_sin");
@@ -226,7 +249,9 @@ int launch_rope_qk_f16(const LaunchArgs& a)
     k.pieces = (in_place ? p.rot_dims : p.head_dim) / 16;  // in place, what does not turn is not touched: a layout's turning pieces come first
     const uint32_t all = heads[0] + heads[1];
     const uint64_t rows = (uint64_t)tokens * all * k.pieces;
-    const uint32_t each = rows > 8ull * 1024 * a.sm_count ? 4 : rows > 2ull * 1024 * a.sm_count ? 2 : 1;
+    // Heads of a thread, us in a recorded chain with 1 | 2 | 4 (| 8): 64 tokens of 32 and 16 heads of 128 1.23 | 1.21 | 1.29, 256 of them 1.64 | 1.71 | 1.64, 256 of 256 dims
+    // 2.56 | 2.07 | 2.23, 5000 of 128 22.3 | 18.6 | 18.7 | 18.9, 10000 of 8 and 1 heads of 80 5.5 | 4.5 | 4.2 | 5.0.
+    const uint32_t each = rows > 8ull * 1024 * a.sm_count ? 4 : rows > 1024ull * a.sm_count ? 2 : 1;
     k.slots = (all + each - 1) / each;
     const uint64_t threads = (uint64_t)tokens * k.pieces * k.slots;
     if (threads >= 1ull << 32) return fail_validation(a, "rope_qk: more values than one dispatch takes (2^36)");
