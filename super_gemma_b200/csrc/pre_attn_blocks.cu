@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(THREADS, 4) pre_attn_blocks_kernel(const __gri
     float c[8], s[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) c[i] = 1.0f, s[i] = 0.0f;
-    if (at.turns) load_cos_sin(a.cos_sin + (size_t)token * a.pairs + at.pair, c, s);
+    if (at.turns) load_cos_sin(a.cos_sin + (size_t)token * a.pairs, at, c, s);
     float most = 0.0f;
     const auto turn_of = [&](const float* weights) {
         Turn t;

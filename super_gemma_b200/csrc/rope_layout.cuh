@@ -2,8 +2,9 @@
 //   layout 0   (i, i + head_dim / 2)   halves of the head; with rot_dims < head_dim the first pairs of each half turn
 //   layout 1   (i, i + rot_dims / 2)   halves of the first rot_dims dims
 //   layout 2   (2 i, 2 i + 1)          neighbours in the first rot_dims dims
-// A head is cut into pieces of 16 dims, two octets each: of eight pairs, so that a rotation stays in a thread, or of eight pairs that do not
-// turn.  The pieces that turn come first.
+// A head is cut into pieces of two octets of dims: of eight pairs, so that a rotation stays in a thread, or of octets that do not
+// turn.  The pieces that turn come first; the first octets of consecutive pieces lie side by side, and so do the second ones (octets of a piece that lie side by
+// side themselves leave half of a sector to each access: prompts through the pre-attention pass took 1.46 times the copy, now 1.05).
 #pragma once
 
 #include "sgb_common.cuh"
@@ -13,34 +14,35 @@ namespace sgb {
 constexpr uint32_t ROPE_LAYOUTS = 3;
 
 struct RopePiece {
-    uint32_t lo, hi;  // first dims of its octets
-    uint32_t pair;    // its first pair
+    uint32_t lo, hi;      // first dims of its octets
+    uint32_t pair[2];     // first pairs of its two fours
     bool turns;
 };
 __device__ __forceinline__ RopePiece rope_piece(uint32_t layout, uint32_t piece, uint32_t head_dim, uint32_t pairs)
 {
     RopePiece p;
-    p.pair = 8 * piece;
-    p.turns = p.pair < pairs;
+    const uint32_t turning = pairs / 8;
+    p.turns = piece < turning;
+    p.pair[0] = layout == 2 ? 4 * piece : 8 * piece;
+    p.pair[1] = layout == 2 ? 4 * (turning + piece) : 8 * piece + 4;
     if (layout == 0) {
         p.lo = 8 * piece;
         p.hi = head_dim / 2 + 8 * piece;
-    } else if (layout == 1 && p.turns) {
+    } else if (p.turns) {
         p.lo = 8 * piece;
         p.hi = pairs + 8 * piece;
     } else {
-        p.lo = 16 * piece;
-        p.hi = 16 * piece + 8;
+        p.lo = pairs + 8 * piece;  // 2 pairs + 8 (piece - turning)
+        p.hi = head_dim / 2 + 8 * piece;
     }
     return p;
 }
 
-__device__ __forceinline__ void load_cos_sin(const float2* row, float (&c)[8], float (&s)[8])  // row on 16 bytes
+__device__ __forceinline__ void load_cos_sin(const float2* row, const RopePiece& at, float (&c)[8], float (&s)[8])  // row on 16 bytes
 {
-    const float4* p = reinterpret_cast<const float4*>(row);
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const float4 v = ld_global(p + j);
+        const float4 v = ld_global(reinterpret_cast<const float4*>(row + at.pair[j / 2]) + (j & 1));
         c[2 * j] = v.x;
         s[2 * j] = v.y;
         c[2 * j + 1] = v.z;

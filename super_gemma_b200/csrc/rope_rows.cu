@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(ROW_THREADS) rope_qk_kernel(const __grid_const
         }
     }
     float c[8], s[8];
-    if (at.turns) load_cos_sin(a.cos_sin + (size_t)token * a.pairs + at.pair, c, s);
+    if (at.turns) load_cos_sin(a.cos_sin + (size_t)token * a.pairs, at, c, s);
 #pragma unroll
     for (int i = 0; i < ROWS; i++) {
         const uint32_t h = slot + i * a.slots;
