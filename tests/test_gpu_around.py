@@ -444,6 +444,29 @@ def test_norms_of_many_rows(ctx, kind, rows, hidden):
         _check_norms(got, *case, kind, post, gates, 0, 0.5, 1e-5, (post, gates))
 
 
+STREAMED = [("f16", 200_003, 72), ("bf16", 100_000, 136), ("f16", 13_001, 1096), ("bf16", 6500, 2048), ("f16", 2501, 5376), ("f32", 1700, 5376), ("bf16", 1600, 8192), ("f16", 800, 16384),
+            ("f32", 1000, 10240), ("f32", 900, 10248), ("f32", 520, 16384), ("f32", 120_001, 72), ("f32", 32_011, 264)]
+
+
+@pytest.mark.parametrize("kind,rows,hidden", STREAMED)
+def test_norms_whose_rows_come_ahead(ctx, kind, rows, hidden):
+    """From 96 MB on CTAs stay and rows come ahead of their turn: 300 rows against the plain statement, all of them against calls of a few rows each."""
+    assert rows * hidden * (4 + 2 * TYPES[kind].itemsize) >= 96 << 20
+    some = torch.cat([torch.arange(100), torch.randint(0, rows, (100,), generator=torch.Generator().manual_seed(rows)), torch.arange(rows - 100, rows)]).cuda()
+    for post, gates, plus_one, scale, in_place in ((1, 1, 1, 0.75, True), (0, 2, 0, -1.5, False), (1, 3, 0, 1.0, False), (2, 0, 1, 1.0, False), (0, 0, 0, 0.5, True)):
+        y, h, w_post, gate, w_pre = _norms_case(rows + post, kind, rows, hidden, gates)
+        y0, h0 = y.clone(), h.clone()
+        got = _norms(ctx, kind, y, h, w_post, gate, w_pre, post, gates, plus_one, scale, 1e-6, in_place)
+        rows_gate = gate[some] if gates == 2 else gate
+        _check_norms([g[some] for g in got], y0[some], h0[some], w_post, rows_gate, w_pre, kind, post, gates, plus_one, scale, 1e-6, (post, gates, in_place))
+        part = max(1, (90 << 20) // (hidden * (4 + 2 * h0.element_size())))
+        for r in range(0, rows, part):
+            few = _norms(ctx, kind, y0[r:r + part].clone(), h0[r:r + part].clone(), w_post, gate[r:r + part].clone() if gates == 2 else gate, w_pre, post, gates, plus_one, scale, 1e-6)
+            for a, b, step in ((got[0][r:r + part], few[0], HALF_STEP[kind]), (got[1][r:r + part], few[1], 2.0 ** -11)):  # the order of a sum, a few units of 2^-24 of values below 32, and with it a rounding
+                a, b = a.float(), b.float()
+                assert ((a - b).abs() <= 2.02 * step * b.abs() + 1e-5).all(), f"rows from {r}, {(post, gates)}"
+
+
 @pytest.mark.parametrize("kind", list(TYPES))
 def test_norms_of_rows_of_all_sizes(ctx, kind):
     """Rows whose squares are near or below eps, zero rows, an eps of 0."""
