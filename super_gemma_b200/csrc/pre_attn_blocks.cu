@@ -211,7 +211,10 @@ __global__ void __launch_bounds__(THREADS, 4) pre_attn_blocks_kernel(const __gri
     Turn turn;
     if (r < end_q) turn = turn_of(a.q_w);
 
-    if (slot == NO_SLOT) return;
+    if (slot == NO_SLOT) {
+        copy_async_wait<0>();  // nothing lands in the memory of whoever comes next
+        return;
+    }
     const uint32_t in_tile = slot % TILE_TOK, previous = __shfl_sync(mask, before[0], 0, ROW_LANES);
     const uint32_t back = in_tile ? in_tile - 1 : 0;  // the token that would be the tile's first, counted from the one before this
     const uint32_t opener0 = __shfl_sync(mask, before[0], back & 7, ROW_LANES), opener1 = __shfl_sync(mask, before[1], back & 7, ROW_LANES);
@@ -233,7 +236,10 @@ __global__ void __launch_bounds__(THREADS, 4) pre_attn_blocks_kernel(const __gri
         scale(p, inv);
         write_f16<NEXT>(a.q_out + ((size_t)token * a.n_q + r) * 128, at, p);
     }
-    if (!placed) return;
+    if (!placed) {
+        copy_async_wait<0>();
+        return;
+    }
 
     // Rows [r, last) of one side into the cache; `least`: the exponent that holds them all.
     const size_t tile0 = (size_t)(slot / TILE_TOK) * a.n_kv;

@@ -292,6 +292,22 @@ def test_pre_attention_of_prompts(ctx, tokens, heads, kv):
     Step(tokens, _runs(tokens, [(5, tokens)], blocks, True), heads, kv, blocks, packed=tokens == 4099, layout=tokens % 3).run(ctx)
 
 
+@pytest.mark.parametrize("tokens,heads,kv", [(3, 130, 65), (2, 1500, 700), (2, 8192, 1024), (6000, 2, 1), (1500, 20, 5)])
+def test_pre_attention_of_many_heads_and_of_few(ctx, tokens, heads, kv):
+    """More rows a token than lanes share, and tokens enough that one group of lanes has all of a token's rows."""
+    blocks = tokens // TILE + 3
+    Step(tokens, _runs(tokens, [(15, tokens)], blocks, True), heads, kv, blocks, packed=heads != 20, layout=heads % 3, rot=(128, 96, 64)[heads % 3]).run(ctx)
+
+
+def test_pre_attention_of_steps_with_room(ctx):
+    """A step with room for many more tokens than it has: what is behind them is left, wherever the slots stand."""
+    rng = np.random.default_rng(8)
+    slots = np.full(3000, NONE, np.int64)
+    slots[rng.choice(3000, 40, replace=False)] = rng.permutation(64)[:40] * TILE + rng.integers(0, TILE, 40)
+    Step(8, slots, 4, 2, 64, packed=True).run(ctx)
+    Step(8, np.full(70, NONE), 4, 2, 2).run(ctx)
+
+
 def test_pre_attention_token_by_token(ctx):
     """A tile filled one token after another holds what one call for all of them writes, but for where it grew."""
     whole = Step(3, TILE + np.arange(TILE), 2, 2, 2).run(ctx)
