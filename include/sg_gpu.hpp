@@ -46,6 +46,14 @@ constexpr uint64_t STEP_WORDS = 4;
 
 class GpuContext;
 
+// Radians a position of each pair: the frequencies of rope_cos_sin.
+inline std::vector<double> rope_frequencies(const sgb_rope_scaling& scaling)
+{
+    std::vector<double> out(scaling.pairs <= 512 ? scaling.pairs : 0);  // (more are refused)
+    check(sgb_rope_frequencies(&scaling, out.data()));
+    return out;
+}
+
 // A typed view of device memory; copies share the allocation (the reference's Arc).
 template <class T>
 class Buffer {

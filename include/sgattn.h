@@ -139,6 +139,8 @@ uint32_t sgb_decode_paged_splits_hint(const sgb_ctx *ctx, uint32_t n_kv_heads, u
 size_t sgb_attn_blocks_work_bytes(const sgb_ctx *ctx, uint32_t n_kv_heads, uint32_t q_per_kv, uint32_t requests, uint32_t n_tokens,
                                   uint32_t max_q);
 
+/* What stands around that attention (no counterpart in the reference either): rope_cos_sin, rope_qk_f16, qkv_norm_rope_append_blocks_e4m3_d128,
+ * block_norms_f16 / _bf16 / _f32 and kv_read_blocks_e4m3_d128 take the packed tokens of the same step; one launch each, no workspace. */
 /* Frequencies of a rotary embedding, for rope_cos_sin: out[i] radians a position, i < pairs, f_i = theta^(-2 i / dims).  For contexts
  * `factor` times as long as the `trained` tokens they are slowed down: all of them by the factor (LINEAR), or only those that turn rarely over the trained
  * length.  BY_TURNS: f_i keeps the share clamp((turns_i - slow) / (fast - slow), 0, 1), turns_i = trained f_i / 2 pi, and the rest of it is f_i / factor.

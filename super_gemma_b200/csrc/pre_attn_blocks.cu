@@ -124,7 +124,7 @@ __device__ __forceinline__ void apply(const Turn& t, bool turns, Pairs& p)
 
 // 2^share_bits groups of eight lanes share the rows of a token (q heads, k heads, v heads in this order), group by group one after the other.  What is the same for
 // a token's heads (the slot, the rotation with its weights, the exponents' bound) is made once a group.  Groups of a warp may have different rows to do, so that a
-// group exchanges values within its own lanes only.  20300 tokens of 32 q and 16 kv heads (17 prompts) take 104.7 us, 6.67 TB/s, which is the copy rate; with rows asked for
+// group exchanges values within its own lanes only.  23931 tokens of 32 q and 16 kv heads (17 prompts) take 104.7 us, 6.67 TB/s, which is the copy rate; with rows asked for
 // one ahead into registers 143, two ahead 131 (128 registers, four CTAs an SM), weights and rotation applied one after the other to every row 165.
 template <bool NEXT>
 __global__ void __launch_bounds__(THREADS, 4) pre_attn_blocks_kernel(const __grid_constant__ PreArgs a)
@@ -344,7 +344,7 @@ int launch_qkv_norm_rope_append_blocks(const LaunchArgs& a)
               p.q_stride, p.k_stride, p.v_stride, n_q, n_kv, tokens, (uint32_t)blocks, p.rot_dims / 2, p.layout, 0, p.plus_one ? 1.0f : 0.0f, p.magnitude, a.status};
     // Groups of a token.  What a group makes for its token costs it as much as two rows, so that as few as give each SM 256 threads to do are best (us in a recorded
     // chain at 128 | 256 | 512 threads: 512 tokens of 32 q and 16 kv heads 3.3 | 3.6 | 4.7, about 440 tokens 4.4 | 4.2 | 5.2, 9225 of 8 and 2 heads 9.3 | 9.3 | 10.2); but
-    // sixteen rows a group at most: 20300 tokens take 112.8 with 8, 104.7 with 16, 107.4 with 32 of them (4104 tokens 21.3, 20.0, 20.5).
+    // sixteen rows a group at most: 23931 tokens take 112.8 with 8, 104.7 with 16, 107.4 with 32 of them (4104 tokens 21.3, 20.0, 20.5).
     while (k.share_bits < 10 && (1u << k.share_bits) < rows && (((uint64_t)tokens << k.share_bits) * ROW_LANES < 256ull * a.sm_count || rows > 16u << k.share_bits)) k.share_bits++;
     const uint64_t groups = (uint64_t)tokens << k.share_bits;
     const dim3 grid((unsigned)((groups * ROW_LANES + THREADS - 1) / THREADS));
