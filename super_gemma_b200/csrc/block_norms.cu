@@ -35,13 +35,14 @@ enum : uint32_t { POST_NONE = 0, POST_NORM = 1, FIRST_NORM = 2 };
 enum : uint32_t { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_ROW = 2, GATE_ONE = 3 };
 constexpr uint32_t MOST_WARPS = 16;  // of a row
 
-// Shared memory of a CTA whose rows come ahead.
+// Rows of a CTA that come ahead and the one in use, and the shared memory for them.
+constexpr uint32_t STAGES = 3;
 constexpr size_t MOST_STAGED = 200 * 1024;
 // Consecutive values of a unit: 16 bytes of R.
 template <typename R>
 constexpr int UNIT = 16 / sizeof(R);
 template <typename R>
-constexpr int MOST_STREAMED = sizeof(R) == 4 ? 8 : 4;  // units of a lane whose rows come ahead
+constexpr int MOST_STREAMED = sizeof(R) == 4 ? 5 : 4;  // units of a lane whose rows come ahead
 
 // A unit of f16 as it is loaded, and as pairs of f32.
 template <int U>
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(TIGHT<R, N> ? 384 : 512, TIGHT<R, N> ? 2 : 0) 
 
 // Many rows: CTAs that stay, with the weights of their columns in registers.  Rows come ahead of their turn into shared memory, STAGES - 1 of them on their way; a thread
 // reads what it has copied itself, so that only its own copies are waited for, and a stage is written again one row after it was read.
-template <typename R, int N, int STAGES>
+template <typename R, int N>
 __global__ void __launch_bounds__(512) block_norms_stream_kernel(const __grid_constant__ NormsArgs a)
 {
     constexpr int U = UNIT<R>, P = U / 2;
@@ -335,12 +336,14 @@ __global__ void __launch_bounds__(512) block_norms_stream_kernel(const __grid_co
         __syncthreads();  // the zeros come before the sums
     }
     const float inv_n = 1.0f / (float)a.hidden;
+    const auto gate_of = [&](uint64_t row) { return a.gates == GATE_ROW && row < a.rows ? ld_global(a.gate + row) : one; };
+    float gate = gate_of(first + me.in_cta);
     uint32_t stage = 0, turn = 0;
     for (uint64_t row0 = first; row0 < a.rows; row0 += stride) {
         const uint64_t row = row0 + me.in_cta;
         const size_t at = row * a.hidden + me.col;
-        float by = one;
-        if (a.gates == GATE_ROW && row < a.rows) by = ld_global(a.gate + row);
+        float by = gate;
+        gate = gate_of(row + stride);
         RawHalf<U> y[N];
         float2 v[N][P];
         copy_async_wait<STAGES - 2>();
@@ -396,10 +399,14 @@ NormsShape norms_shape(uint32_t units, uint32_t most)
     return s;
 }
 
-template <typename R, int N, int STAGES>
+uint32_t cta_threads(uint32_t lanes) { return lanes <= 32 ? 128 : lanes; }
+template <typename R>
+size_t staged_bytes(const NormsShape& s) { return (size_t)STAGES * s.each * cta_threads(s.lanes) * (16 + 2 * UNIT<R>); }
+
+template <typename R, int N>
 int launch_stream(const LaunchArgs& a, const NormsArgs& k, uint32_t threads, size_t smem)
 {
-    const auto kern = block_norms_stream_kernel<R, N, STAGES>;
+    const auto kern = block_norms_stream_kernel<R, N>;
     static std::mutex mutex;
     static int registers[64] = {};  // of a thread, 0: not asked yet
     int regs = 0;
@@ -425,13 +432,9 @@ int launch_stream(const LaunchArgs& a, const NormsArgs& k, uint32_t threads, siz
 template <typename R, int N>
 int launch_norms(const LaunchArgs& a, const NormsArgs& k, bool stream)
 {
-    const uint32_t threads = k.lanes <= 32 ? 128 : k.lanes, per_cta = threads / k.lanes;
-    if constexpr (N <= MOST_STREAMED<R>) {
-        const size_t stage = (size_t)N * threads * (16 + 2 * UNIT<R>);
-        if (stream && 3 * stage <= MOST_STAGED) return launch_stream<R, N, 3>(a, k, threads, 3 * stage);
-        if constexpr (sizeof(R) == 4)  // rows of 10248 and more
-            if (stream) return launch_stream<R, N, 2>(a, k, threads, 2 * stage);
-    }
+    const uint32_t threads = cta_threads(k.lanes), per_cta = threads / k.lanes;
+    if constexpr (N <= MOST_STREAMED<R>)
+        if (stream) return launch_stream<R, N>(a, k, threads, staged_bytes<R>({k.lanes, N}));
     return check_cuda(a, launch_dependent(block_norms_kernel<R, N>, dim3((unsigned)((k.rows + per_cta - 1ull) / per_cta)), dim3(threads), 0, a.stream, k), "block_norms");
 }
 
@@ -475,12 +478,14 @@ int launch_block_norms(const LaunchArgs& a)
     const uint32_t units = hidden / U;
     NormsArgs k{(const __half*)a.b[0].ptr, a.b[1].ptr, (const float*)a.b[2].ptr, (const float*)a.b[3].ptr, (const float*)a.b[4].ptr, a.b[5].ptr, (__half*)a.b[6].ptr,
                 rows, hidden, 1, p.post, p.gates, p.plus_one ? 1.0f : 0.0f, p.scale, p.eps};
-    // Rows come ahead of their turn where there is enough to stream, 96 MB; below, the CTAs' start costs more than it brings.  A row of its own has lanes enough for 2048 columns
-    // at a time where all of them are on the GPU at once, else as many units a lane as registers allow.
-    const bool stream = (uint64_t)n * (4 + 2 * R_BYTES) >= 96ull << 20;
+    // Rows come ahead of their turn where there is enough to stream, 80 MB, and three of them fit a CTA (all of 16 bits, f32 up to 10240); below, the CTAs' start costs more than it brings (us, ahead | not: 2000
+    // rows of 5376 in f16, 86 MB, 15.6 | 17.8, 800 of them 8.2 | 7.3; 6000 of 1096 in f32, 79 MB, 13.3 | 13.2; 2000 of 16384 in f32, one on its way, 70.9 | 73.4).  A row of its own has lanes enough for
+    // 2048 columns at a time where all of them are on the GPU at once, else as many units a lane as registers allow.
+    const NormsShape ahead = norms_shape(units, U == 8 ? 4 : 3);
+    const bool stream = (uint64_t)n * (4 + 2 * R_BYTES) >= 80ull << 20 && staged_bytes<R>(ahead) <= MOST_STAGED;
     NormsShape shape = norms_shape(units, std::min(4u, (hidden + 2047) / 2048));
     if (stream)
-        shape = norms_shape(units, U == 8 ? 4 : 3);
+        shape = ahead;
     else if ((uint64_t)rows * shape.lanes > 1024ull * a.sm_count)
         shape = norms_shape(units, U == 8 && units <= 192 ? 6 : 4);  // (6000 rows of 1096 in f16: 9.8 us with six units a lane, 11.2 with four; of 5376, 800 rows: 7.6 | 7.2)
     k.lanes = shape.lanes;
