@@ -182,6 +182,7 @@ struct sgb_ctx {
     cudaEvent_t sync_event = nullptr;
     bool recording = false;
     std::vector<sgb_buffer*> recording_refs;
+    std::vector<void*> freed_later;            // memory of buffers released while recording: the stream cannot be waited for before the recording ends
     uint64_t recording_launches = 0;
     std::vector<RecordedOp> ops;               // dispatches recorded so far
     std::vector<cudaGraphNode_t> open_nodes;   // the capture's dependency set as the last dispatch left it
@@ -191,11 +192,31 @@ struct sgb_ctx {
     std::atomic<int> refs{1};
 };
 
+// The thread may be recording on another context, whose capture would end at a call that waits or frees; what is done in here concerns other streams.
+struct AnyCaptureMode {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    AnyCaptureMode() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~AnyCaptureMode() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+// Memory given back once the work queued on the context's stream is done with it.
+static void free_memory(sgb_ctx* c, std::vector<void*>* memory)
+{
+    if (memory->empty()) return;
+    AnyCaptureMode any;
+    cudaSetDevice(c->device);
+    cudaStreamSynchronize(c->stream);
+    for (void* p : *memory) cudaFree(p);
+    memory->clear();
+}
+
 static void ctx_release(sgb_ctx* c)
 {
     if (!c) return;
     if (c->refs.fetch_sub(1) != 1) return;
+    AnyCaptureMode any;
     cudaSetDevice(c->device);
+    free_memory(c, &c->freed_later);
     if (c->stream) cudaStreamSynchronize(c->stream);
     if (c->status_dev) cudaFree(c->status_dev);
     if (c->status_host) cudaFreeHost(c->status_host);
@@ -432,9 +453,8 @@ void sgb_buffer_release(sgb_buffer* b)
     if (!b) return;
     if (b->refs.fetch_sub(1) != 1) return;
     if (b->owned && b->base) {
-        cudaSetDevice(b->ctx->device);
-        cudaStreamSynchronize(b->ctx->stream);
-        cudaFree(b->base);
+        b->ctx->freed_later.push_back(b->base);
+        if (!b->ctx->recording) free_memory(b->ctx, &b->ctx->freed_later);
     }
     sgb_buffer* parent = b->parent;
     sgb_ctx* c = b->ctx;
@@ -707,6 +727,7 @@ int sgb_graph_end(sgb_ctx* c, sgb_graph** out)
     g->refs.swap(c->recording_refs);
     g->launches = c->recording_launches;
     cudaError_t e = cudaStreamEndCapture(c->stream, &g->graph);
+    free_memory(c, &c->freed_later);
     if (e == cudaSuccess) e = cudaGraphInstantiate(&g->exec, g->graph, 0);
     if (e != cudaSuccess) {
         std::string msg = std::string("graph capture: ") + cudaGetErrorString(e);
