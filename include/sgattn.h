@@ -70,7 +70,7 @@ int sgb_buffer_create(sgb_ctx *ctx, size_t bytes, sgb_buffer **out);
 int sgb_buffer_adopt(sgb_ctx *ctx, void *device_ptr, size_t bytes, sgb_buffer **out);
 int sgb_buffer_slice(sgb_buffer *parent, size_t offset, size_t bytes, sgb_buffer **out); /* Buffer::slice */
 void sgb_buffer_retain(sgb_buffer *buf);
-void sgb_buffer_release(sgb_buffer *buf);
+void sgb_buffer_release(sgb_buffer *buf); /* while its context records a graph: the memory goes back when that ends */
 void *sgb_buffer_device_ptr(const sgb_buffer *buf);
 size_t sgb_buffer_bytes(const sgb_buffer *buf);
 int sgb_buffer_upload(sgb_buffer *buf, size_t offset, const void *host, size_t bytes);
