@@ -317,9 +317,19 @@ class GpuTimer:
         return list(arr)
 
 
+_push_formats: dict = {}
+
+
 def _push_bytes(push) -> bytes:
     if push is None:
         return b""
+    if type(push) is tuple:  # u32 / f32 by the values' types, in declaration order
+        types = tuple(map(type, push))
+        packer = _push_formats.get(types)
+        if packer is None and all(t is int or t is float for t in types):
+            packer = _push_formats[types] = struct.Struct("<" + "".join("f" if t is float else "I" for t in types))
+        if packer is not None:
+            return packer.pack(*push)
     if isinstance(push, (bytes, bytearray)):
         return bytes(push)
     if isinstance(push, (int, np.integer)):
@@ -334,7 +344,16 @@ def _push_bytes(push) -> bytes:
 # structure per binding costs several times as much, more than the launch itself.
 _PACKED = [_vp, _vp, C.c_char_p, _u32, C.c_char_p, _sz, C.c_char_p]
 _U32 = 0xFFFFFFFF
+_GRID = struct.Struct("3I")
 _packed_fns: dict = {}
+_binding_structs: dict = {}
+
+
+def _binding_words(n: int) -> struct.Struct:
+    words = _binding_structs.get(n)
+    if words is None:
+        words = _binding_structs[n] = struct.Struct("I4xP" * n)
+    return words
 
 
 def _packed(name: str):
@@ -423,14 +442,21 @@ class GpuContext:
                                             info.signature.decode()))
 
     def _dispatch(self, fn, kernel: Kernel, bindings: Sequence[BufferBinding], push, groups: Sequence[int]) -> None:
-        flat: list = []
-        for b in bindings:
-            flat += (operator.index(b.index) & _U32, b.buf._h or 0)
         n = len(bindings)
+        try:  # the common case: plain words
+            packed = _binding_words(n).pack(*[w for b in bindings for w in (b.index, b.buf._h)])
+            grid = _GRID.pack(*groups)
+        except struct.error:
+            flat: list = []
+            for b in bindings:
+                flat += (operator.index(b.index) & _U32, b.buf._h or 0)
+            packed = _binding_words(n).pack(*flat)
+            g = (list(groups) + [1, 1, 1])[:3]
+            grid = _GRID.pack(operator.index(g[0]) & _U32, operator.index(g[1]) & _U32, operator.index(g[2]) & _U32)
         pb = _push_bytes(push)
-        g = (list(groups) + [1, 1, 1])[:3]
-        _check(fn(self._h, kernel._h, struct.pack("I4xP" * n, *flat), n, pb or None, len(pb),
-                  struct.pack("3I", operator.index(g[0]) & _U32, operator.index(g[1]) & _U32, operator.index(g[2]) & _U32)))
+        code = fn(self._h, kernel._h, packed, n, pb or None, len(pb), grid)
+        if code:
+            _check(code)
 
     def dispatch(self, kernel: Kernel, bindings: Sequence[BufferBinding], push, groups: Sequence[int]) -> None:
         """Enqueue (or, while recording, capture) one kernel (GraphRecorder::dispatch, graph.rs:203)."""
