@@ -35,7 +35,8 @@ struct PreArgs {
     uint8_t* pool[2];
     int8_t* exps[2];
     uint32_t q_stride, k_stride, v_stride;  // values from token to token
-    uint32_t n_q, n_kv, tokens, blocks, pairs, layout, share_bits;
+    uint32_t n_q, n_kv, tokens, blocks, pairs, layout;
+    uint32_t share_bits, each, step;        // groups of a token, rows of a group, from row to row of it
     float plus, magnitude;  // plus: 1 where weights are 1 + w
     uint32_t* status;
 };
@@ -122,7 +123,7 @@ __device__ __forceinline__ void apply(const Turn& t, bool turns, Pairs& p)
     }
 }
 
-// 2^share_bits groups of eight lanes share the rows of a token (q heads, k heads, v heads in this order), group by group one after the other.  What is the same for
+// 2^share_bits groups of eight lanes share the rows of a token (q heads, k heads, v heads in this order).  What is the same for
 // a token's heads (the slot, the rotation with its weights, the exponents' bound) is made once a group.  Groups of a warp may have different rows to do, so that a
 // group exchanges values within its own lanes only.  23931 tokens of 32 q and 16 kv heads (17 prompts) take 104.7 us, 6.67 TB/s, which is the copy rate; with rows asked for
 // one ahead into registers 143, two ahead 131 (128 registers, four CTAs an SM), weights and rotation applied one after the other to every row 165.
@@ -133,7 +134,7 @@ __global__ void __launch_bounds__(THREADS, 4) pre_attn_blocks_kernel(const __gri
     pdl_launch_dependents();
     const uint32_t lane = threadIdx.x & (ROW_LANES - 1), group = blockIdx.x * (THREADS / ROW_LANES) + threadIdx.x / ROW_LANES;
     const uint32_t mask = 0xffu << (threadIdx.x & 24);
-    const uint32_t token = group >> a.share_bits, shares = 1u << a.share_bits;
+    const uint32_t token = group >> a.share_bits, share = group & ((1u << a.share_bits) - 1);
     if (token >= a.tokens) return;
     const RopePiece at = rope_piece(a.layout, lane, 128, a.pairs);
     // The slot, and those of the fifteen tokens before it: two a lane.
@@ -143,7 +144,8 @@ __global__ void __launch_bounds__(THREADS, 4) pre_attn_blocks_kernel(const __gri
     for (uint32_t j = 0; j < 2; j++)
         if (token >= 1 + lane + 8 * j) before[j] = ld_global(a.slots + token - 1 - lane - 8 * j);
     const uint32_t end_q = a.n_q, end_k = a.n_q + a.n_kv, end = end_k + a.n_kv;
-    uint32_t r = group & (shares - 1);
+    uint32_t r = a.step == 1 ? share * a.each : share;
+    const uint32_t stop = a.step == 1 ? min(end, r + a.each) : end;
     // Rows on their way: SLOTS places of 32 bytes a thread in shared memory, written and read by itself alone, so that nothing but its own copies is waited for.  A place
     // is written again when what was read from it has been used.
     __shared__ alignas(16) uint4 places[SLOTS][2][THREADS];
@@ -154,23 +156,23 @@ __global__ void __launch_bounds__(THREADS, 4) pre_attn_blocks_kernel(const __gri
     uint32_t place = 0;
     const auto fetch = [&](uint32_t i, uint32_t to) {
         const __half* src = (i < end_q ? base_q : i < end_k ? base_k : base_v) + (size_t)i * 128;
-        copy_async_if(i < end, &places[to][0][threadIdx.x], src);
-        copy_async_if(i < end, &places[to][1][threadIdx.x], src + apart);
+        copy_async_if(i < stop, &places[to][0][threadIdx.x], src);
+        copy_async_if(i < stop, &places[to][1][threadIdx.x], src + apart);
         copy_async_commit();
     };
 #pragma unroll
-    for (uint32_t j = 0; j + 1 < SLOTS; j++) fetch(r + j * shares, j);
+    for (uint32_t j = 0; j + 1 < SLOTS; j++) fetch(r + j * a.step, j);
     const auto next = [&]() {  // row r
         copy_async_wait<SLOTS - 2>();
         const Pairs p = unpack_pairs<NEXT>(places[place][0][threadIdx.x], places[place][1][threadIdx.x]);
-        fetch(r + (SLOTS - 1) * shares, (place + SLOTS - 1) % SLOTS);
+        fetch(r + (SLOTS - 1) * a.step, (place + SLOTS - 1) % SLOTS);
         place = (place + 1) % SLOTS;
         return p;
     };
     float c[8], s[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) c[i] = 1.0f, s[i] = 0.0f;
-    if (at.turns) load_cos_sin(a.cos_sin + (size_t)token * a.pairs, at, c, s);
+    if (at.turns && r < end_k) load_cos_sin(a.cos_sin + (size_t)token * a.pairs, at, c, s);
     float most = 0.0f;
     const auto turn_of = [&](const float* weights) {
         Turn t;
@@ -229,7 +231,7 @@ __global__ void __launch_bounds__(THREADS, 4) pre_attn_blocks_kernel(const __gri
         placed = false;
     }
 
-    for (; r < end_q; r += shares) {
+    for (; r < min(end_q, stop); r += a.step) {
         Pairs p = next();
         const float inv = inverse_rms(p);
         apply(turn, at.turns, p);
@@ -248,11 +250,11 @@ __global__ void __launch_bounds__(THREADS, 4) pre_attn_blocks_kernel(const __gri
         uint8_t* const pool = a.pool[side] + tile0 * TILE_BYTES;
         int8_t* const exps = a.exps[side] + tile0;
         int old = ld_global_if(!fresh, exps + (r - first));
-        for (; r < last; r += shares) {
+        for (; r < last; r += a.step) {
             Pairs p = next();
             const uint32_t head = r - first;
             const int had = old, e = fresh ? least : max(least, had);
-            old = ld_global_if(!fresh && r + shares < last, exps + head + shares);
+            old = ld_global_if(!fresh && r + a.step < last, exps + head + a.step);
             const float inv = inverse_rms(p);
             turned(p);
             uint8_t* to = pool + (size_t)head * TILE_BYTES;
@@ -281,13 +283,13 @@ __global__ void __launch_bounds__(THREADS, 4) pre_attn_blocks_kernel(const __gri
             write_e4m3<NEXT>(to + in_tile * 128, at, p);
         }
     };
-    if (r < end_k) {
+    if (r < min(end_k, stop)) {
         turn = turn_of(a.k_w);
 #pragma unroll
         for (uint32_t d = 1; d < ROW_LANES; d <<= 1) most = fmaxf(most, __shfl_xor_sync(mask, most, d));
-        append(0, end_q, end_k, exponent_for(fminf(most * ROW_REACH * a.magnitude, 61440.0f)), [&](Pairs& p) { apply(turn, at.turns, p); });
+        append(0, end_q, min(end_k, stop), exponent_for(fminf(most * ROW_REACH * a.magnitude, 61440.0f)), [&](Pairs& p) { apply(turn, at.turns, p); });
     }
-    append(1, end_k, end, exponent_for(ROW_REACH), [](Pairs&) {});
+    append(1, end_k, stop, exponent_for(ROW_REACH), [](Pairs&) {});
 }
 
 struct PushPre {
@@ -341,11 +343,15 @@ int launch_qkv_norm_rope_append_blocks(const LaunchArgs& a)
     const uint32_t rows = n_q + 2 * n_kv;
     PreArgs k{(const __half*)a.b[0].ptr, (const __half*)a.b[3].ptr, (const __half*)a.b[4].ptr, (const float*)a.b[1].ptr, (const float*)a.b[5].ptr, (const float2*)a.b[6].ptr,
               (const uint32_t*)a.b[7].ptr, (__half*)a.b[2].ptr, {(uint8_t*)a.b[8].ptr, (uint8_t*)a.b[10].ptr}, {(int8_t*)a.b[9].ptr, (int8_t*)a.b[11].ptr},
-              p.q_stride, p.k_stride, p.v_stride, n_q, n_kv, tokens, (uint32_t)blocks, p.rot_dims / 2, p.layout, 0, p.plus_one ? 1.0f : 0.0f, p.magnitude, a.status};
+              p.q_stride, p.k_stride, p.v_stride, n_q, n_kv, tokens, (uint32_t)blocks, p.rot_dims / 2, p.layout, 0, 0, 0, p.plus_one ? 1.0f : 0.0f, p.magnitude, a.status};
     // Groups of a token.  What a group makes for its token costs it as much as two rows, so that as few as give each SM 256 threads to do are best (us in a recorded
     // chain at 128 | 256 | 512 threads: 512 tokens of 32 q and 16 kv heads 3.3 | 3.6 | 4.7, about 440 tokens 4.4 | 4.2 | 5.2, 9225 of 8 and 2 heads 9.3 | 9.3 | 10.2); but
     // sixteen rows a group at most: 23931 tokens take 112.8 with 8, 104.7 with 16, 107.4 with 32 of them (4104 tokens 21.3, 20.0, 20.5).
     while (k.share_bits < 10 && (1u << k.share_bits) < rows && (((uint64_t)tokens << k.share_bits) * ROW_LANES < 256ull * a.sm_count || rows > 16u << k.share_bits)) k.share_bits++;
+    // A group of few rows has them one after the other, most of them of one kind; with more, a warp's groups would read kilobytes apart at a time, and they take them in turn
+    // (512 tokens, four rows each: 3.3 us, in turn 3.7; 23931 tokens, sixteen each: 202, in turn 105).
+    k.each = (rows + (1u << k.share_bits) - 1) >> k.share_bits;
+    k.step = k.each <= 4 ? 1 : 1u << k.share_bits;
     const uint64_t groups = (uint64_t)tokens << k.share_bits;
     const dim3 grid((unsigned)((groups * ROW_LANES + THREADS - 1) / THREADS));
     const cudaError_t e = launch_dependent(p.layout == 2 ? pre_attn_blocks_kernel<true> : pre_attn_blocks_kernel<false>, grid, dim3(THREADS), 0, a.stream, k);
