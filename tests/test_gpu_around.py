@@ -682,3 +682,56 @@ def test_two_contexts_and_graphs_side_by_side(ctx):
                 s.pools[side] = np.where(keep[:, None, :, None], s.pools[side], lo)
                 s.pools[side + 1] = np.where(exps == s.pools[side + 1], s.pools[side + 1], exps)
             s.check("replayed")
+
+
+def _one_of_each(ctx, seed):
+    """A call of every operator over tensors of its own: (kernel, bindings, push, grid, the buffers it writes)."""
+    rng = np.random.default_rng(seed)
+    up = ctx.buffer_from_iter
+    n, heads, kv, hidden = 90 + seed, 6, 3, 1096
+    half = lambda *s: rng.standard_normal(s).astype(np.float16)  # noqa: E731
+    fill = lambda k: up(np.full(k, 0x5555, np.uint16))  # noqa: E731
+    freqs, positions = up(around.frequencies(64, 1e4, 128)), up(_u32(rng.integers(0, 1 << 20, n)))
+    rows = up(np.zeros(n * 128, np.float32))
+    q, k = up(half(n, heads, D)), up(half(n, kv, D))
+    q_out, k_out = fill(n * heads * D), fill(n * kv * D)
+    calls = [("rope_cos_sin", (freqs, positions, rows), (128, 1.25), [n, 1, 1], [rows]),
+             ("rope_qk_f16", (q, k, rows, q_out, k_out), (D, 128, seed % 3, 0, 0, 0, 0), [heads, kv, n], [q_out, k_out])]
+    for i, kind in enumerate(TYPES):
+        h = rng.standard_normal((n, hidden)).astype(np.float32)
+        h = up(h if kind == "f32" else h.astype(np.float16) if kind == "f16" else (h.view(np.uint32) >> 16).astype(np.uint16))
+        h_out, x = ctx.new_buffer(h.nbytes, np.uint8), fill(n * hidden)
+        w = [up(rng.standard_normal(hidden).astype(np.float32)) for _ in range(3)]
+        calls.append(("block_norms_" + kind, (up(half(n, hidden)), h, w[0], w[1], w[2], h_out, x), (1, 1, i % 2, 0.5, 1e-6), [hidden, n, 1], [h_out, x]))
+    s = Step(seed, _runs(seed, [(0, n)], 8, False), heads, kv, 8, exps=(-5, -4), magnitude=1.25)  # (tiles begin in it: nothing grows from replay to replay)
+    b = s.buffers(ctx)
+    b[6].buf = rows
+    calls.append(("qkv_norm_rope_append_blocks_e4m3_d128", tuple(x.buf for x in b), *s.call(), [s.q_out, *s.b]))
+    out = fill(n * kv * D), fill(n * kv * D)
+    calls.append(("kv_read_blocks_e4m3_d128", (*s.b, up(_u32(np.random.default_rng(seed).permutation(8))), up(_u32([0])), up(_u32([0, n])), *out), (16, 8), [kv, 1, n], list(out)))
+    return [(ctx.load_kernel(name), bind(*bufs), push, grid, written) for name, bufs, push, grid, written in calls]
+
+
+def test_all_of_them_recorded_and_side_by_side(ctx):
+    """Every operator twice in a recording with branches, replayed beside another context's: the bits of calls made one after the other."""
+    import super_gemma_b200 as sg
+
+    other = sg.GpuContext(0)
+    sides = []
+    for i, c in enumerate((ctx, other)):
+        calls = _one_of_each(c, 2 * i) + _one_of_each(c, 2 * i + 1)
+        for call in calls:
+            c.dispatch_blocking(*call[:4])
+        want = [[b.read() for b in call[4]] for call in calls]
+        for call in calls[:2] + calls[7:9]:  # (not the cache: a tile's other rows are nobody's)
+            for b in call[4]:
+                b.zero()
+        sides.append((c, calls, want, c.record_graph(lambda at, calls=calls: [at.dispatch(*call[:4]) for call in calls])))
+    for _ in range(25):
+        for c, _, _, graph in sides:
+            c.submit(graph)
+    for c, calls, want, _ in sides:
+        c.sync()
+        for n, (call, w) in enumerate(zip(calls, want)):
+            for b, x in zip(call[4], w):
+                assert np.array_equal(b.read(), x), f"{n}: {call[0].name}"
