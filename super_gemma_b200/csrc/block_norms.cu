@@ -5,8 +5,8 @@
 // and with post 2 the first norm of all, x = f16(h / rms(h) * w_pre) alone.  Both sums of squares, h' and everything between are f32; x is made of
 // h' as it is before its own rounding.
 //
-// One pass over the bytes: a row stays in the registers of its lanes between the two sums.  A row has 2^k lanes of a warp if one unit (16 bytes of h) a lane
-// covers it, else whole warps with N units a lane.
+// One pass over the bytes: a row stays in the registers of its lanes between the two sums, a unit being 16 bytes of h.  A row has eight or sixteen lanes of a warp
+// (1, 2 or 4 if it has fewer units than eight) or whole warps, each lane up to eight units.
 #include <cuda_bf16.h>
 
 #include <algorithm>

@@ -18,7 +18,7 @@ constexpr uint32_t MOST_ROT = 1024;
 
 // ---- rows of cosines and sines ---------------------------------------------------------------------------------------------------
 // Angles are counted in turns, as 64-bit fractions of one: F = f / 2 pi mod 1 in units of 2^-64, made of the f64 frequency and 1 / 2 pi in two f64 (hi + lo),
-// so that the whole turns of p F fall off by themselves and what is left is good to 2^-34 of a turn for every 32-bit p.  Its upper word's nearest quarter turn goes into signs and
+// so that the whole turns of p F fall off by themselves and the upper word is good to 2^-32 of a turn for every 32-bit p.  Its nearest quarter turn goes into signs and
 // an exchange of sine and cosine, the rest, an eighth of a turn at most, into their Taylor series up to x^9 and x^10 (cut off below 2 * 10^-9).
 // Integers instead of f64 sums and reductions: those kept the units that convert between formats busy, 5.8 us for 32768 rows of 64 pairs, now 3.4.
 // A thread makes two pairs (16 bytes) of ROWS tokens.

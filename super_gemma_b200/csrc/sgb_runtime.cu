@@ -180,9 +180,11 @@ struct sgb_ctx {
     uint32_t* status_dev = nullptr;   // 4 words
     uint32_t* status_host = nullptr;  // pinned mirror
     cudaEvent_t sync_event = nullptr;
-    bool recording = false;
+    std::atomic<bool> recording{false};
     std::vector<sgb_buffer*> recording_refs;
-    std::vector<void*> freed_later;            // memory of buffers released while recording: the stream cannot be waited for before the recording ends
+    // Buffers may be released by any thread.  While the stream is being captured it cannot be waited for, and their memory goes back when that ends.
+    std::mutex release_mutex;
+    std::vector<void*> freed_later;
     uint64_t recording_launches = 0;
     std::vector<RecordedOp> ops;               // dispatches recorded so far
     std::vector<cudaGraphNode_t> open_nodes;   // the capture's dependency set as the last dispatch left it
@@ -199,15 +201,22 @@ struct AnyCaptureMode {
     ~AnyCaptureMode() { cudaThreadExchangeStreamCaptureMode(&mode); }
 };
 
-// Memory given back once the work queued on the context's stream is done with it.
-static void free_memory(sgb_ctx* c, std::vector<void*>* memory)
+// Memory given back once the work queued on the context's stream is done with it.  The caller holds release_mutex.
+static void free_memory(sgb_ctx* c, const std::vector<void*>& memory)
 {
-    if (memory->empty()) return;
+    if (memory.empty()) return;
     AnyCaptureMode any;
     cudaSetDevice(c->device);
     cudaStreamSynchronize(c->stream);
-    for (void* p : *memory) cudaFree(p);
-    memory->clear();
+    for (void* p : memory) cudaFree(p);
+}
+static void release_memory(sgb_ctx* c, void* p)
+{
+    std::lock_guard<std::mutex> lock(c->release_mutex);
+    if (c->recording)
+        c->freed_later.push_back(p);
+    else
+        free_memory(c, {p});
 }
 
 static void ctx_release(sgb_ctx* c)
@@ -216,7 +225,7 @@ static void ctx_release(sgb_ctx* c)
     if (c->refs.fetch_sub(1) != 1) return;
     AnyCaptureMode any;
     cudaSetDevice(c->device);
-    free_memory(c, &c->freed_later);
+    free_memory(c, c->freed_later);
     if (c->stream) cudaStreamSynchronize(c->stream);
     if (c->status_dev) cudaFree(c->status_dev);
     if (c->status_host) cudaFreeHost(c->status_host);
@@ -452,10 +461,7 @@ void sgb_buffer_release(sgb_buffer* b)
 {
     if (!b) return;
     if (b->refs.fetch_sub(1) != 1) return;
-    if (b->owned && b->base) {
-        b->ctx->freed_later.push_back(b->base);
-        if (!b->ctx->recording) free_memory(b->ctx, &b->ctx->freed_later);
-    }
+    if (b->owned && b->base) release_memory(b->ctx, b->base);
     sgb_buffer* parent = b->parent;
     sgb_ctx* c = b->ctx;
     delete b;
@@ -708,8 +714,11 @@ int sgb_graph_begin(sgb_ctx* c)
     if (!c) return set_error(SGB_ERR_VALIDATION, "sgb_graph_begin: ctx is NULL");
     if (c->recording) return set_error(SGB_ERR_STATE, "sgb_graph_begin: already recording");
     CUDA_TRY(cudaSetDevice(c->device), "cudaSetDevice");
-    CUDA_TRY(cudaStreamBeginCapture(c->stream, cudaStreamCaptureModeThreadLocal), "cudaStreamBeginCapture");
-    c->recording = true;
+    {
+        std::lock_guard<std::mutex> lock(c->release_mutex);
+        CUDA_TRY(cudaStreamBeginCapture(c->stream, cudaStreamCaptureModeThreadLocal), "cudaStreamBeginCapture");
+        c->recording = true;
+    }
     c->recording_launches = 0;
     c->ops.clear();
     c->open_nodes.clear();
@@ -720,14 +729,19 @@ int sgb_graph_end(sgb_ctx* c, sgb_graph** out)
 {
     if (!c || !out) return set_error(SGB_ERR_VALIDATION, "sgb_graph_end: NULL argument");
     if (!c->recording) return set_error(SGB_ERR_STATE, "sgb_graph_end without sgb_graph_begin");
-    c->recording = false;
     c->ops.clear();
     c->open_nodes.clear();
     sgb_graph* g = new sgb_graph();
     g->refs.swap(c->recording_refs);
     g->launches = c->recording_launches;
-    cudaError_t e = cudaStreamEndCapture(c->stream, &g->graph);
-    free_memory(c, &c->freed_later);
+    cudaError_t e;
+    {
+        std::lock_guard<std::mutex> lock(c->release_mutex);
+        e = cudaStreamEndCapture(c->stream, &g->graph);
+        c->recording = false;
+        free_memory(c, c->freed_later);
+        c->freed_later.clear();
+    }
     if (e == cudaSuccess) e = cudaGraphInstantiate(&g->exec, g->graph, 0);
     if (e != cudaSuccess) {
         std::string msg = std::string("graph capture: ") + cudaGetErrorString(e);

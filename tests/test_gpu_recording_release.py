@@ -63,3 +63,30 @@ def test_releases_in_a_recording_that_fails():
     call, y = _norm(ctx, 3)
     ctx.dispatch_blocking(ctx.load_kernel("rmsnorm_256"), call, None, [3, 1, 1])
     assert (y.read() == 0x3C00).all()
+
+
+def test_releases_by_another_thread():
+    """One thread records and replays, three others make nothing but room: their buffers go at any moment of that."""
+    import threading
+
+    import super_gemma_b200 as sg
+
+    ctx = sg.GpuContext(0)
+    kernel = ctx.load_kernel("rmsnorm_256")
+    call, y = _norm(ctx, 40)
+    heaps = [[ctx.new_buffer(4096, np.uint8) for _ in range(150)] for _ in range(3)]
+    def drop(heap):
+        while heap:
+            heap.pop()
+
+    threads = [threading.Thread(target=drop, args=(heap,)) for heap in heaps]
+    for t in threads:
+        t.start()
+    graphs = []
+    for _ in range(20):
+        graphs.append(ctx.record_graph(lambda at: [at.dispatch(kernel, call, None, [40, 1, 1]) for _ in range(4)]))
+        ctx.submit(graphs[-1])
+    for t in threads:
+        t.join()
+    ctx.sync()
+    assert (y.read() == 0x3C00).all()
