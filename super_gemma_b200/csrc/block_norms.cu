@@ -36,13 +36,12 @@ enum : uint32_t { GATE_NONE = 0, GATE_CHANNEL = 1, GATE_ROW = 2, GATE_ONE = 3 };
 constexpr uint32_t MOST_WARPS = 16;  // of a row
 
 // Rows of a CTA that come ahead and the one in use, and the shared memory for them.
-constexpr uint32_t STAGES = 3;
+constexpr uint32_t STAGES = 2;
 constexpr size_t MOST_STAGED = 200 * 1024;
+constexpr uint32_t MOST_STREAMED = 4;  // units of a lane of such a row
 // Consecutive values of a unit: 16 bytes of R.
 template <typename R>
 constexpr int UNIT = 16 / sizeof(R);
-template <typename R>
-constexpr int MOST_STREAMED = sizeof(R) == 4 ? 5 : 4;  // units of a lane whose rows come ahead
 
 // A unit of f16 as it is loaded, and as pairs of f32.
 template <int U>
@@ -282,7 +281,72 @@ __global__ void __launch_bounds__(TIGHT<R, N> ? 384 : 512, TIGHT<R, N> ? 2 : 0) 
     }
 }
 
-// Many rows: CTAs that stay, with the weights of their columns in registers.  Rows come ahead of their turn into shared memory, STAGES - 1 of them on their way; a thread
+// Many rows of f32, or of 16 bits that a warp holds: weights are asked for unit by unit where they are used, which leaves registers for more rows on an SM at a time.
+// (Three units of f32 in 40 registers: 3 CTAs of fourteen warps an SM instead of 2, 8192 rows of 5376 99 -> 90 us.)
+template <typename R, int N>
+__global__ void __launch_bounds__(512, sizeof(R) == 4 && N <= 3 ? 3 : 0) block_norms_late_kernel(const __grid_constant__ NormsArgs a)
+{
+    constexpr int U = UNIT<R>, P = U / 2;
+    __shared__ alignas(16) float parts[2][MOST_WARPS];
+    pdl_wait();
+    pdl_launch_dependents();
+    const Place me = place_of<U>(a.lanes);
+    const uint64_t row = (uint64_t)blockIdx.x * me.per_cta + me.in_cta;
+    const size_t at = row * a.hidden + me.col;  // of the first unit
+    const bool live = row < a.rows;
+    const auto on = [&](int i) { return live && (i + 1 < N || me.col + i * me.step < a.hidden); };  // all units but the last are within the row
+    RawHalf<U> y[N];
+    uint4 raw[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        y[i] = RawHalf<U>{};
+        raw[i] = make_uint4(0, 0, 0, 0);
+        if (on(i)) {
+            if (a.post != FIRST_NORM) y[i] = load_f16<U>(a.y + at + i * me.step);
+            raw[i] = ld_global(reinterpret_cast<const uint4*>(static_cast<const R*>(a.h) + at + i * me.step));
+        }
+    }
+    if (a.lanes > 32) {
+        if (threadIdx.x < MOST_WARPS) parts[0][threadIdx.x] = parts[1][threadIdx.x] = 0.0f;
+        __syncthreads();  // the zeros come before the sums
+    }
+    float by = 1.0f;  // of the block's output
+    if (a.gates == GATE_ROW && live) by = ld_global(a.gate + row);
+    if (a.gates == GATE_ONE) by = ld_global(a.gate);
+    const float inv_n = 1.0f / (float)a.hidden;
+    if (a.post == POST_NORM) by *= rsqrtf(row_sum(squares(y), a.lanes, parts[0]) * inv_n + a.eps);
+    const float2 by2 = make_float2(by, by), scale2 = make_float2(a.scale, a.scale), plus2 = make_float2(a.plus, a.plus);
+    float2 v[N][P];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        unpack<R>(raw[i], v[i]);
+        if (a.post == FIRST_NORM || !on(i)) continue;
+        float2 n[P], w[P];
+#pragma unroll
+        for (int j = 0; j < P; j++) n[j] = pair_of(y[i].w[j]);
+        if (a.post == POST_NORM) {
+            load_f32<U>(a.w_post + me.col + i * me.step, w);
+#pragma unroll
+            for (int j = 0; j < P; j++) n[j] = mul2_rn(n[j], add2_rn(w[j], plus2));
+        }
+        if (a.gates == GATE_CHANNEL) times_f32<U>(a.gate + me.col + i * me.step, n);
+#pragma unroll
+        for (int j = 0; j < P; j++) v[i][j] = mul2_rn(fma2_rn(n[j], by2, v[i][j]), scale2);
+        *reinterpret_cast<uint4*>(static_cast<R*>(a.h_out) + at + i * me.step) = pack<R>(v[i]);
+    }
+    const float inv = rsqrtf(row_sum(squares(v), a.lanes, parts[1]) * inv_n + a.eps);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        if (!on(i)) continue;
+        float2 w[P];
+        load_f32<U>(a.w_pre + me.col + i * me.step, w);
+#pragma unroll
+        for (int j = 0; j < P; j++) w[j] = add2_rn(w[j], plus2);
+        write_next<R>(a.x + at + i * me.step, v[i], w, inv);
+    }
+}
+
+// Many rows of 16 bits: CTAs that stay, with the weights of their columns in registers.  Rows come ahead of their turn into shared memory, STAGES - 1 of them on their way; a thread
 // reads what it has copied itself, so that only its own copies are waited for, and a stage is written again one row after it was read.
 template <typename R, int N>
 __global__ void __launch_bounds__(512) block_norms_stream_kernel(const __grid_constant__ NormsArgs a)
@@ -304,8 +368,8 @@ __global__ void __launch_bounds__(512) block_norms_stream_kernel(const __grid_co
         const size_t at = row * a.hidden + me.col;
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            copy_async_if<2 * U>(on(row, i) && a.post != FIRST_NORM, y_place(stage, i), a.y + at + i * me.step);
-            copy_async_if<16>(on(row, i), h_place(stage, i), static_cast<const R*>(a.h) + at + i * me.step);
+            copy_async_if(on(row, i) && a.post != FIRST_NORM, y_place(stage, i), a.y + at + i * me.step);
+            copy_async_if(on(row, i), h_place(stage, i), static_cast<const R*>(a.h) + at + i * me.step);
         }
         copy_async_commit();
     };
@@ -429,13 +493,15 @@ int launch_stream(const LaunchArgs& a, const NormsArgs& k, uint32_t threads, siz
     return check_cuda(a, launch_dependent(kern, dim3(std::min(ctas, resident * a.sm_count)), dim3(threads), smem, a.stream, k), "block_norms");
 }
 
+enum class Way { EARLY, LATE, STREAM };
 template <typename R, int N>
-int launch_norms(const LaunchArgs& a, const NormsArgs& k, bool stream)
+int launch_norms(const LaunchArgs& a, const NormsArgs& k, Way way)
 {
     const uint32_t threads = cta_threads(k.lanes), per_cta = threads / k.lanes;
-    if constexpr (N <= MOST_STREAMED<R>)
-        if (stream) return launch_stream<R, N>(a, k, threads, staged_bytes<R>({k.lanes, N}));
-    return check_cuda(a, launch_dependent(block_norms_kernel<R, N>, dim3((unsigned)((k.rows + per_cta - 1ull) / per_cta)), dim3(threads), 0, a.stream, k), "block_norms");
+    if constexpr (sizeof(R) == 2 && N <= MOST_STREAMED)
+        if (way == Way::STREAM) return launch_stream<R, N>(a, k, threads, staged_bytes<R>({k.lanes, N}));
+    const auto kern = way == Way::LATE ? block_norms_late_kernel<R, N> : block_norms_kernel<R, N>;
+    return check_cuda(a, launch_dependent(kern, dim3((unsigned)((k.rows + per_cta - 1ull) / per_cta)), dim3(threads), 0, a.stream, k), "block_norms");
 }
 
 }  // namespace
@@ -478,27 +544,28 @@ int launch_block_norms(const LaunchArgs& a)
     const uint32_t units = hidden / U;
     NormsArgs k{(const __half*)a.b[0].ptr, a.b[1].ptr, (const float*)a.b[2].ptr, (const float*)a.b[3].ptr, (const float*)a.b[4].ptr, a.b[5].ptr, (__half*)a.b[6].ptr,
                 rows, hidden, 1, p.post, p.gates, p.plus_one ? 1.0f : 0.0f, p.scale, p.eps};
-    // Rows come ahead of their turn where there is enough to stream, 80 MB, and three of them fit a CTA (all of 16 bits, f32 up to 10240); below, the CTAs' start costs more than it brings (us, ahead | not: 2000
-    // rows of 5376 in f16, 86 MB, 15.6 | 17.8, 800 of them 8.2 | 7.3; 6000 of 1096 in f32, 79 MB, 13.3 | 13.2; 2000 of 16384 in f32, one on its way, 70.9 | 73.4).  A row of its own has lanes enough for
-    // 2048 columns at a time where all of them are on the GPU at once, else as many units a lane as registers allow.
-    const NormsShape ahead = norms_shape(units, U == 8 ? 4 : 3);
-    const bool stream = (uint64_t)n * (4 + 2 * R_BYTES) >= 80ull << 20 && staged_bytes<R>(ahead) <= MOST_STAGED;
+    // Where all rows are on the GPU at once each has lanes enough for 2048 columns at a time and asks for its weights beside them; else lanes have as many units as registers
+    // allow.  From 80 MB on rows of 16 bits come ahead of their turn, but for those that a warp holds.  Measured one launch after the other, us, early | late | ahead: f32, 8192 rows of 5376
+    // 102.6 | 88.9 | 96.1, 30011 of 1096 70.7 | 68.0 | 74.5, 800 of 5376 13.7 | 14.0; bf16, 30011 of 1096 51.0 | 44.5 | 48.0; f16, 6000 of 5376 54.8 | 49.0 | 45.5, 100000 of 264 46.4 | 48.5 | 40.6, 3000 of 8192
+    // 44.1 | 45.4 | 36.5.
+    const bool many = (uint64_t)n * (4 + 2 * R_BYTES) >= 80ull << 20, warp_holds = units > 64 && units <= 192;
     NormsShape shape = norms_shape(units, std::min(4u, (hidden + 2047) / 2048));
-    if (stream)
-        shape = ahead;
-    else if ((uint64_t)rows * shape.lanes > 1024ull * a.sm_count)
-        shape = norms_shape(units, U == 8 && units <= 192 ? 6 : 4);  // (6000 rows of 1096 in f16: 9.8 us with six units a lane, 11.2 with four; of 5376, 800 rows: 7.6 | 7.2)
+    Way way = Way::EARLY;
+    if ((uint64_t)rows * shape.lanes > 1024ull * a.sm_count) {
+        way = U == 4 || (many && warp_holds) ? Way::LATE : many ? Way::STREAM : Way::EARLY;
+        shape = norms_shape(units, U == 4 ? 3 : warp_holds ? 6 : MOST_STREAMED);
+    }
     k.lanes = shape.lanes;
     int e = 0;
     switch (shape.each) {
-        case 1: e = launch_norms<R, 1>(a, k, stream); break;
-        case 2: e = launch_norms<R, 2>(a, k, stream); break;
-        case 3: e = launch_norms<R, 3>(a, k, stream); break;
-        case 4: e = launch_norms<R, 4>(a, k, stream); break;
-        case 5: e = launch_norms<R, 5>(a, k, stream); break;
-        case 6: e = launch_norms<R, 6>(a, k, stream); break;
+        case 1: e = launch_norms<R, 1>(a, k, way); break;
+        case 2: e = launch_norms<R, 2>(a, k, way); break;
+        case 3: e = launch_norms<R, 3>(a, k, way); break;
+        case 4: e = launch_norms<R, 4>(a, k, way); break;
+        case 5: e = launch_norms<R, 5>(a, k, way); break;
+        case 6: e = launch_norms<R, 6>(a, k, way); break;
         default:  // f32 rows of more than 12288
-            if constexpr (U == 4) e = shape.each == 7 ? launch_norms<R, 7>(a, k, stream) : launch_norms<R, 8>(a, k, stream);
+            if constexpr (U == 4) e = shape.each == 7 ? launch_norms<R, 7>(a, k, way) : launch_norms<R, 8>(a, k, way);
     }
     ++*a.launches;
     return e;

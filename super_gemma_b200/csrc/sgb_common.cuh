@@ -293,15 +293,10 @@ __device__ __forceinline__ T ld_global(const T* p)
     }
     return v;
 }
-// 16 (or 8) bytes into shared memory without a register, by the load path; a thread's copies are committed in groups and waited for by their number.
-template <int BYTES = 16>
+// 16 bytes into shared memory without a register, by the load path; a thread's copies are committed in groups and waited for by their number.
 __device__ __forceinline__ void copy_async_if(bool p, void* dst_smem, const void* src)
 {
-    static_assert(BYTES == 16 || BYTES == 8, "one copy");
-    if constexpr (BYTES == 16)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(smem_u32(dst_smem)), "l"(src), "r"((uint32_t)p) : "memory");
-    else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p cp.async.ca.shared.global [%0], [%1], 8;\n\t}" ::"r"(smem_u32(dst_smem)), "l"(src), "r"((uint32_t)p) : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p cp.async.cg.shared.global [%0], [%1], 16;\n\t}" ::"r"(smem_u32(dst_smem)), "l"(src), "r"((uint32_t)p) : "memory");
 }
 __device__ __forceinline__ void copy_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
