@@ -282,9 +282,9 @@ __global__ void __launch_bounds__(TIGHT<R, N> ? 384 : 512, TIGHT<R, N> ? 2 : 0) 
 }
 
 // Many rows of f32, or of 16 bits that a warp holds: weights are asked for unit by unit where they are used, which leaves registers for more rows on an SM at a time.
-// (Three units of f32 in 40 registers: 3 CTAs of fourteen warps an SM instead of 2, 8192 rows of 5376 99 -> 90 us.)
+// (Three units of f32 in 40 registers: 3 CTAs of fourteen warps an SM instead of 2, 8192 rows of 5376 99 -> 90 us; eight in 64 instead of 70: 2 CTAs, 2000 rows of 16384 113 -> 85.)
 template <typename R, int N>
-__global__ void __launch_bounds__(512, sizeof(R) == 4 && N <= 3 ? 3 : 0) block_norms_late_kernel(const __grid_constant__ NormsArgs a)
+__global__ void __launch_bounds__(512, sizeof(R) == 4 ? (N <= 3 ? 3 : 2) : 0) block_norms_late_kernel(const __grid_constant__ NormsArgs a)
 {
     constexpr int U = UNIT<R>, P = U / 2;
     __shared__ alignas(16) float parts[2][MOST_WARPS];
@@ -500,7 +500,9 @@ int launch_norms(const LaunchArgs& a, const NormsArgs& k, Way way)
     const uint32_t threads = cta_threads(k.lanes), per_cta = threads / k.lanes;
     if constexpr (sizeof(R) == 2 && N <= MOST_STREAMED)
         if (way == Way::STREAM) return launch_stream<R, N>(a, k, threads, staged_bytes<R>({k.lanes, N}));
-    const auto kern = way == Way::LATE ? block_norms_late_kernel<R, N> : block_norms_kernel<R, N>;
+    auto kern = block_norms_kernel<R, N>;
+    if constexpr (sizeof(R) == 4 || N >= 4)  // (rows of 16 bits that a warp holds have four units a lane and more)
+        if (way == Way::LATE) kern = block_norms_late_kernel<R, N>;
     return check_cuda(a, launch_dependent(kern, dim3((unsigned)((k.rows + per_cta - 1ull) / per_cta)), dim3(threads), 0, a.stream, k), "block_norms");
 }
 
