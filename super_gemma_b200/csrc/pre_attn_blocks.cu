@@ -125,8 +125,8 @@ __device__ __forceinline__ void apply(const Turn& t, bool turns, Pairs& p)
 
 // 2^share_bits groups of eight lanes share the rows of a token (q heads, k heads, v heads in this order).  What is the same for
 // a token's heads (the slot, the rotation with its weights, the exponents' bound) is made once a group.  Groups of a warp may have different rows to do, so that a
-// group exchanges values within its own lanes only.  23931 tokens of 32 q and 16 kv heads (17 prompts) take 104.7 us, 6.67 TB/s, which is the copy rate; with rows asked for
-// one ahead into registers 143, two ahead 131 (128 registers, four CTAs an SM), weights and rotation applied one after the other to every row 165.
+// group exchanges values within its own lanes only.  23931 tokens of 32 q and 16 kv heads (17 prompts) take 112 to 114 us, 6.2 TB/s, 0.94 of the copy rate (side by side
+// with others of its kind 104.7); with rows asked for one ahead into registers 143, two ahead 131 (128 registers, four CTAs an SM), weights and rotation applied one after the other to every row 165.
 template <bool NEXT>
 __global__ void __launch_bounds__(THREADS, 4) pre_attn_blocks_kernel(const __grid_constant__ PreArgs a)
 {
@@ -344,12 +344,16 @@ int launch_qkv_norm_rope_append_blocks(const LaunchArgs& a)
     PreArgs k{(const __half*)a.b[0].ptr, (const __half*)a.b[3].ptr, (const __half*)a.b[4].ptr, (const float*)a.b[1].ptr, (const float*)a.b[5].ptr, (const float2*)a.b[6].ptr,
               (const uint32_t*)a.b[7].ptr, (__half*)a.b[2].ptr, {(uint8_t*)a.b[8].ptr, (uint8_t*)a.b[10].ptr}, {(int8_t*)a.b[9].ptr, (int8_t*)a.b[11].ptr},
               p.q_stride, p.k_stride, p.v_stride, n_q, n_kv, tokens, (uint32_t)blocks, p.rot_dims / 2, p.layout, 0, 0, 0, p.plus_one ? 1.0f : 0.0f, p.magnitude, a.status};
-    // Groups of a token.  What a group makes for its token costs it as much as two rows, so that as few as give each SM 256 threads to do are best (us in a recorded
-    // chain at 128 | 256 | 512 threads: 512 tokens of 32 q and 16 kv heads 3.3 | 3.6 | 4.7, about 440 tokens 4.4 | 4.2 | 5.2, 9225 of 8 and 2 heads 9.3 | 9.3 | 10.2); but
-    // sixteen rows a group at most: 23931 tokens take 112.8 with 8, 104.7 with 16, 107.4 with 32 of them (4104 tokens 21.3, 20.0, 20.5).
+    // Groups of a token.  What a group makes for its token costs it as much as two rows, so that as few as give each SM 256 threads to do are best (us, one launch after the
+    // other, at 128 | 256 | 512 threads: 512 tokens of 32 q and 16 kv heads 5.0 | 4.4 | 5.5, 440 of them 5.0 | 4.4 | 5.2, 200 3.3 | 3.5 | 4.4); but sixteen rows a group at
+    // most: 23931 tokens take 122 with 8, 112 with 16, 116 with 32 of them, about 5000 tokens 31.5, 30.5, 34.7.
     while (k.share_bits < 10 && (1u << k.share_bits) < rows && (((uint64_t)tokens << k.share_bits) * ROW_LANES < 256ull * a.sm_count || rows > 16u << k.share_bits)) k.share_bits++;
+    // An SM has 512 threads at a time; up to half as many again wait for two rounds, where shorter groups take three of half their length
+    // (us, two | three: tokens of 8 q and 2 kv heads, floor 9.4 us of bytes 20.9 | 15.7, 11.3 us 20.5 | 16.9; of 32 and 16, 12.2 us 18.9 | 18.2; of 16 and 2, 10.6 us 16.3 | 17.2).
+    const uint64_t threads = ((uint64_t)tokens << k.share_bits) * ROW_LANES;
+    if (threads > 512ull * a.sm_count && threads <= 768ull * a.sm_count && rows > 8u << k.share_bits) k.share_bits++;
     // A group of few rows has them one after the other, most of them of one kind; with more, a warp's groups would read kilobytes apart at a time, and they take them in turn
-    // (512 tokens, four rows each: 3.3 us, in turn 3.7; 23931 tokens, sixteen each: 202, in turn 105).
+    // (512 tokens, four rows each: 4.4 us, in turn 5.1; 23931 tokens, sixteen each: 202, in turn 112).
     k.each = (rows + (1u << k.share_bits) - 1) >> k.share_bits;
     k.step = k.each <= 4 ? 1 : 1u << k.share_bits;
     const uint64_t groups = (uint64_t)tokens << k.share_bits;
