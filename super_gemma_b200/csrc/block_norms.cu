@@ -205,7 +205,7 @@ __device__ __forceinline__ void write_next(__half* x, const float2 (&v)[UNIT<R> 
 
 // One row a CTA (or a warp, or some of its lanes): nothing waits for anything that could have been asked for before it.  The block's weights come beside the row, the
 // next ones beside the second sum.
-// Three units of 16-bit values: two CTAs of twelve warps an SM, 80 registers instead of 98 (400 rows of 5376 3.6 us, else 4.1).
+// Three units of 16-bit values: two CTAs of twelve warps an SM, 80 registers instead of 98 (400 rows of 5376 4.6 us, else 5.7).
 template <typename R, int N>
 constexpr bool TIGHT = sizeof(R) == 2 && N == 3;
 template <typename R, int N>
@@ -548,7 +548,7 @@ int launch_block_norms(const LaunchArgs& a)
                 rows, hidden, 1, p.post, p.gates, p.plus_one ? 1.0f : 0.0f, p.scale, p.eps};
     // Where all rows are on the GPU at once each has lanes enough for 2048 columns at a time and asks for its weights beside them; else lanes have as many units as registers
     // allow.  From 80 MB on rows of 16 bits come ahead of their turn, but for those that a warp holds.  Measured one launch after the other, us, early | late | ahead: f32, 8192 rows of 5376
-    // 102.6 | 88.9 | 96.1, 30011 of 1096 70.7 | 68.0 | 74.5, 800 of 5376 13.7 | 14.0; bf16, 30011 of 1096 51.0 | 44.5 | 48.0; f16, 6000 of 5376 54.8 | 49.0 | 45.5, 100000 of 264 46.4 | 48.5 | 40.6, 3000 of 8192
+    // 102.6 | 89 to 90 | 96.1, 30011 of 1096 70.7 | 68.0 | 74.5, 800 of 5376 13.7 | 14.0; bf16, 30011 of 1096 51.0 | 44.5 | 48.0; f16, 6000 of 5376 54.8 | 49.0 | 45.5, 100000 of 264 46.4 | 48.5 | 40.6, 3000 of 8192
     // 44.1 | 45.4 | 36.5.
     const bool many = (uint64_t)n * (4 + 2 * R_BYTES) >= 80ull << 20, warp_holds = units > 64 && units <= 192;
     NormsShape shape = norms_shape(units, std::min(4u, (hidden + 2047) / 2048));

@@ -1,8 +1,8 @@
 // The way back out of the 8-bit cache of blocks.cuh: tokens [from_r, from_r + n_r) of every request as packed f16 rows, n_r = starts[r + 1] - starts[r].
 // value = e4m3 * 2^e is an f16 number for every tile that an append writes, so that nothing is rounded.
 //
-// One byte read and two written per value: bound by bytes (119690 tokens of 40 requests, 16 heads, pages of 16: 226 us, 0.99 of the copy rate;
-// 1000 of one request 2.7).
+// One byte read and two written per value: bound by bytes (119690 tokens of 40 requests, 16 heads, pages of 16: 233 us, 0.96 of the copy rate;
+// 1000 of one request 4.0).
 #include "blocks.cuh"
 #include "sgb_kernels.h"
 
@@ -62,7 +62,8 @@ __device__ __forceinline__ uint32_t scaled(uint32_t two_bytes, int e)
 
 // A CTA has ROWS packed rows, half a warp each: eight bytes in and sixteen out a lane, so that both sides move whole sectors.  Sixteen rows are
 // a tile's where a request's rows begin with one.  The heads of both sides go round, AHEAD of them asked for at a time (gridDim.y CTAs share
-// them).  With one head at a time, or its place looked for by one thread a row, 40 requests took 289 and 231 us.
+// them).  With one head at a time, or its place looked for by one thread a row, 40 requests took 289 and 231 us where they now take
+// 226 (launches side by side).
 __global__ void __launch_bounds__(THREADS) read_blocks_kernel(const __grid_constant__ ReadArgs a)
 {
     pdl_wait();

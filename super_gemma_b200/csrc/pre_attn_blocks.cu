@@ -125,7 +125,7 @@ __device__ __forceinline__ void apply(const Turn& t, bool turns, Pairs& p)
 
 // 2^share_bits groups of eight lanes share the rows of a token (q heads, k heads, v heads in this order).  What is the same for
 // a token's heads (the slot, the rotation with its weights, the exponents' bound) is made once a group.  Groups of a warp may have different rows to do, so that a
-// group exchanges values within its own lanes only.  23931 tokens of 32 q and 16 kv heads (17 prompts) take 112 to 114 us, 6.2 TB/s, 0.94 of the copy rate (side by side
+// group exchanges values within its own lanes only.  23931 tokens of 32 q and 16 kv heads (17 prompts) take 112 to 115 us, 6.2 TB/s, 0.94 of the copy rate (side by side
 // with others of its kind 104.7); with rows asked for one ahead into registers 143, two ahead 131 (128 registers, four CTAs an SM), weights and rotation applied one after the other to every row 165.
 template <bool NEXT>
 __global__ void __launch_bounds__(THREADS, 4) pre_attn_blocks_kernel(const __grid_constant__ PreArgs a)

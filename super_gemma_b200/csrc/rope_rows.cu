@@ -20,7 +20,7 @@ constexpr uint32_t MOST_ROT = 1024;
 // Angles are counted in turns, as 64-bit fractions of one: F = f / 2 pi mod 1 in units of 2^-64, made of the f64 frequency and 1 / 2 pi in two f64 (hi + lo),
 // so that the whole turns of p F fall off by themselves and the upper word is good to 2^-32 of a turn for every 32-bit p.  Its nearest quarter turn goes into signs and
 // an exchange of sine and cosine, the rest, an eighth of a turn at most, into their Taylor series up to x^9 and x^10 (cut off below 2 * 10^-9).
-// Integers instead of f64 sums and reductions: those kept the units that convert between formats busy, 5.8 us for 32768 rows of 64 pairs, now 3.4.
+// Integers instead of f64 sums and reductions: those kept the units that convert between formats busy, 5.8 us for 32768 rows of 64 pairs where these take 3.4 (launches side by side; 4.3 one after the other).
 // A thread makes two pairs (16 bytes) of ROWS tokens.
 constexpr double INV_2PI_HI = 0.15915494309189535, INV_2PI_LO = -9.839338337591243e-18;
 
@@ -91,7 +91,7 @@ struct PushCosSin {
 // ---- rotation --------------------------------------------------------------------------------------------------------------------
 // A thread has one piece of 16 dims (two octets of a layout's pairs) of ROWS heads of a token, all of them asked for before the first
 // is turned; the token's eight cosines and sines stay in its registers.  Two bytes read and two written per value: bound by bytes (8192
-// tokens of 32 and 16 heads of 128, neighbours coupled, out of packed rows: 30.1 us, 6.8 TB/s).
+// tokens of 32 and 16 heads of 128, neighbours coupled, out of packed rows: 31.8 us, 6.5 TB/s).
 struct RotateArgs {
     const __half* src[2];  // q, k
     __half* dst[2];
@@ -202,7 +202,7 @@ int launch_rope_cos_sin(const LaunchArgs& a)
     if (int r = need_bytes(a, 2, 4 * (size_t)tokens * p.rot_dims, "cos_sin")) return r;
     if (int r = need_aligned(a, {8, 4, 16})) return r;
     const uint32_t per_row = p.rot_dims / 4, rows_here = ROW_THREADS / per_row;
-    const bool many = (uint64_t)tokens * per_row > 2048ull * a.sm_count;  // (ROWS 8 | 4 | 1, 32768 rows of 64 pairs: 3.4 | 3.5 | 5.6 us)
+    const bool many = (uint64_t)tokens * per_row > 2048ull * a.sm_count;  // (ROWS 8 | 4 | 1, 32768 rows of 64 pairs: 4.2 | 4.2 | 6.2 us)
     const uint32_t each = rows_here * (many ? 8 : 1);
     const cudaError_t e = launch_dependent(many ? rope_cos_sin_kernel<8> : rope_cos_sin_kernel<1>, dim3((tokens + each - 1ull) / each), dim3(ROW_THREADS), 0, a.stream,
                                            (const double*)a.b[0].ptr, (const int*)a.b[1].ptr, (float4*)a.b[2].ptr, p.magnitude, tokens, per_row, rows_here);
@@ -249,9 +249,11 @@ int launch_rope_qk_f16(const LaunchArgs& a)
     k.pieces = (in_place ? p.rot_dims : p.head_dim) / 16;  // in place, what does not turn is not touched: a layout's turning pieces come first
     const uint32_t all = heads[0] + heads[1];
     const uint64_t rows = (uint64_t)tokens * all * k.pieces;
-    // Heads of a thread, us in a recorded chain with 1 | 2 | 4 (| 8): 64 tokens of 32 and 16 heads of 128 1.23 | 1.21 | 1.29, 256 of them 1.64 | 1.71 | 1.64, 256 of 256 dims
-    // 2.56 | 2.07 | 2.23, 5000 of 128 22.3 | 18.6 | 18.7 | 18.9, 10000 of 8 and 1 heads of 80 5.5 | 4.5 | 4.2 | 5.0.
-    const uint32_t each = rows > 8ull * 1024 * a.sm_count ? 4 : rows > 1024ull * a.sm_count ? 2 : 1;
+    // Heads of a thread: few threads start sooner, but one head of each is best while an SM has 256 or fewer.  Places that four heads leave empty cost where there are many
+    // (us, one launch after the other, 1 | 2 | 4: 64 tokens of 32 and 16 heads of 128 1.71 | 1.88 | 2.23, 128 of them 2.13 | 1.89 | 2.23, 256 3.16 | 2.40 | 2.31, 1000 5.5 | 4.4 | 4.0, 5000
+    // 23.5 | 20.1 | 20.4; 64 of 32 and 4 heads of 512, 64 pairs, 1.89 | 1.80 | 2.14; 2500 of 8 and 4 heads of 64 2.91 | 2.31 | 2.31; 10000 of 8 and 1 heads of 80 6.8 | 5.9 | 6.5).
+    const bool empty_places = rows > 2048ull * a.sm_count && (all + 3) / 4 * 20 > all * 6;
+    const uint32_t each = rows > 512ull * a.sm_count && !empty_places ? 4 : rows > 256ull * a.sm_count ? 2 : 1;
     k.slots = (all + each - 1) / each;
     const uint64_t threads = (uint64_t)tokens * k.pieces * k.slots;
     if (threads >= 1ull << 32) return fail_validation(a, "rope_qk: more values than one dispatch takes (2^36)");
