@@ -466,7 +466,7 @@ STREAMED = [("f16", 200_003, 72), ("bf16", 100_000, 136), ("f16", 13_001, 1096),
 
 @pytest.mark.parametrize("kind,rows,hidden", STREAMED)
 def test_norms_whose_rows_come_ahead(ctx, kind, rows, hidden):
-    """From 80 MB on CTAs stay and rows come ahead of their turn: 300 rows against the plain statement, all of them against calls of a few rows each."""
+    """From 80 MB on rows come ahead of their turn or ask late for their weights: 300 rows against the plain statement, all of them against calls of a few rows each."""
     assert rows * hidden * (4 + 2 * TYPES[kind].itemsize) >= 96 << 20
     some = torch.cat([torch.arange(100), torch.randint(0, rows, (100,), generator=torch.Generator().manual_seed(rows)), torch.arange(rows - 100, rows)]).cuda()
     for post, gates, plus_one, scale, in_place in ((1, 1, 1, 0.75, True), (0, 2, 0, -1.5, False), (1, 3, 0, 1.0, False), (2, 0, 1, 1.0, False), (0, 0, 0, 0.5, True)):
