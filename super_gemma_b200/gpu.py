@@ -199,8 +199,14 @@ def rope_frequencies(pairs: int, theta: float, *, dims: Optional[int] = None, ki
     """Radians a position of each pair in 64 bits, the ``freqs`` binding of ``rope_cos_sin`` (``sgb_rope_frequencies``)."""
     if kind not in ROPE_KINDS:
         raise Validation(f"rope_frequencies: kind must be one of {', '.join(ROPE_KINDS)}")
-    out = np.empty(max(0, operator.index(pairs)), np.float64)
-    s = _RopeScaling(operator.index(pairs) & 0xFFFFFFFF, (2 * pairs if dims is None else operator.index(dims)) & 0xFFFFFFFF, ROPE_KINDS[kind], 0, theta, factor, trained, slow, fast)
+    pairs = operator.index(pairs)
+    dims = 2 * pairs if dims is None else operator.index(dims)
+    if not 1 <= pairs <= 512:  # (checked here too: the library writes as many numbers as its 32-bit word says)
+        raise Validation("rope_frequencies: pairs must be 1..512")
+    if not 2 * pairs <= dims <= 0xFFFFFFFF:
+        raise Validation("rope_frequencies: dims must be at least twice the pairs, in 32 bits")
+    out = np.empty(pairs, np.float64)
+    s = _RopeScaling(pairs, dims, ROPE_KINDS[kind], 0, theta, factor, trained, slow, fast)
     _check(lib().sgb_rope_frequencies(C.byref(s), out.ctypes.data_as(C.POINTER(C.c_double))))
     return out
 

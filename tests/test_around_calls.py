@@ -1,0 +1,26 @@
+"""CPU checks of calls around the batched attention that nobody should make: what they are answered before anything is launched or written."""
+import pytest
+
+
+@pytest.fixture(scope="module")
+def sg():
+    from super_gemma_b200 import build
+
+    build.build()
+    import super_gemma_b200 as sg
+
+    return sg
+
+
+# Numbers whose lower 32 bits would be good ones among them: the array is as long as `pairs` says and the library writes as many numbers as its word says.
+@pytest.mark.parametrize("change", [{"dims": -2}, {"dims": 2 ** 32}, {"dims": 2 ** 32 + 128}, {"dims": -2 ** 32 + 128}, {"pairs": 2 ** 32 + 64, "dims": 128}, {"pairs": -2 ** 32 + 64, "dims": 128},
+                                    {"pairs": -2 ** 32 + 64}, {"pairs": 513, "dims": 2 ** 31}])
+def test_frequencies_beyond_32_bits_are_refused(sg, monkeypatch, change):
+    monkeypatch.setattr(sg.gpu, "lib", lambda: pytest.fail("the library was called"))
+    call = {"pairs": 64, "theta": 1e4, **change}
+    with pytest.raises(sg.Validation):
+        sg.rope_frequencies(call.pop("pairs"), call.pop("theta"), **call)
+
+
+def test_frequencies_at_the_limits(sg):
+    assert sg.rope_frequencies(512, 1e4).shape == (512,) and sg.rope_frequencies(1, 1e4, dims=2 ** 32 - 1).tolist() == [1.0]
