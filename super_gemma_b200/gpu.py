@@ -448,7 +448,7 @@ class GpuContext:
                                             info.signature.decode()))
 
     def _dispatch(self, fn, kernel: Kernel, bindings: Sequence[BufferBinding], push, groups: Sequence[int]) -> None:
-        n = len(bindings)
+        n, groups = len(bindings), tuple(groups)  # (groups may be an iterator, and are read twice below)
         try:  # the common case: plain words
             packed = _binding_words(n).pack(*[w for b in bindings for w in (b.index, b.buf._h)])
             grid = _GRID.pack(*groups)
@@ -457,7 +457,7 @@ class GpuContext:
             for b in bindings:
                 flat += (operator.index(b.index) & _U32, b.buf._h or 0)
             packed = _binding_words(n).pack(*flat)
-            g = (list(groups) + [1, 1, 1])[:3]
+            g = (groups + (1, 1, 1))[:3]
             grid = _GRID.pack(operator.index(g[0]) & _U32, operator.index(g[1]) & _U32, operator.index(g[2]) & _U32)
         pb = _push_bytes(push)
         code = fn(self._h, kernel._h, packed, n, pb or None, len(pb), grid)

@@ -24,3 +24,23 @@ def test_frequencies_beyond_32_bits_are_refused(sg, monkeypatch, change):
 
 def test_frequencies_at_the_limits(sg):
     assert sg.rope_frequencies(512, 1e4).shape == (512,) and sg.rope_frequencies(1, 1e4, dims=2 ** 32 - 1).tolist() == [1.0]
+
+
+def test_groups_of_any_kind(sg):
+    """Grids shorter or longer than three words, out of lists, tuples, arrays and iterators, reach the library as the same three words."""
+    import struct
+
+    import numpy as np
+
+    ctx, seen = object.__new__(sg.GpuContext), []
+    ctx._h = None  # (no context: nothing is called but the stand-in below)
+    kernel = type("K", (), {"_h": None})()
+
+    def dispatch(_ctx, _kernel, bindings, n, push, push_bytes, groups):
+        seen.append(struct.unpack("3I", groups))
+        return 0
+
+    for want, words in (((5, 1, 1), [5]), ((5, 7, 1), [5, 7]), ((5, 7, 9), [5, 7, 9]), ((5, 7, 9), [5, 7, 9, 11])):
+        for groups in (words, tuple(words), np.array(words), iter(words), (w for w in words)):
+            ctx._dispatch(dispatch, kernel, [], None, groups)
+            assert seen.pop() == want, (words, type(groups))
