@@ -4,14 +4,16 @@
 //
 // The exponent of a tile needs no look at its values: a normed row of 128 has a 2-norm of at most sqrt(128), so that with weights w and
 // a rotation whose (cos, sin) have length m
-//   |v_i| <= sqrt(128),     |k_i| <= sqrt(128) max|w| m,
-// and e is the least >= -15 with that bound <= 448 * 2^e.  The bound is loose by 2 to 8 where values are spread evenly, which costs nothing: e4m3
+//   |v_i| <= sqrt(128),     |k_i| <= sqrt(128) max|w| m   where dim i turns,     sqrt(128) max|w|   where it does not
+// (so that m counts as 1 at least unless the whole head turns), and e is the least >= -15 with that bound <= 448 * 2^e.  The bound is loose by 2 to 8 where values are spread evenly, which costs nothing: e4m3
 // keeps its four significant bits down to 2^-6 2^e, for values 2^-11 below the rows' root mean square (|w| of one size), and what
 // is smaller is off by at most 2^-10 2^e.  So every token is written by itself, where kv_append_blocks_e4m3_d128 has to see a tile's tokens together and to
 // round the earlier ones again as the maximum grows.  Its tiles may stand in the same pool: a tile that this call continues keeps its exponent if that is
 // larger; if it is smaller (a tile of the other append with small values), the rows before are rounded again, once.
 //
 // Three bytes a value of k and v and four of q move: bound by bytes when there are many tokens, by a launch and the chain slots -> exponents when few.
+#include <algorithm>
+
 #include "blocks.cuh"
 #include "rope_layout.cuh"
 #include "sgb_kernels.h"
@@ -37,7 +39,7 @@ struct PreArgs {
     uint32_t q_stride, k_stride, v_stride;  // values from token to token
     uint32_t n_q, n_kv, tokens, blocks, pairs, layout;
     uint32_t share_bits, each, step;        // groups of a token, rows of a group, from row to row of it
-    float plus, magnitude;  // plus: 1 where weights are 1 + w
+    float plus, longest;  // plus: 1 where weights are 1 + w; longest: what a rotation, or a dim's staying, multiplies a row's bound by
     uint32_t* status;
 };
 
@@ -287,7 +289,7 @@ __global__ void __launch_bounds__(THREADS, 4) pre_attn_blocks_kernel(const __gri
         turn = turn_of(a.k_w);
 #pragma unroll
         for (uint32_t d = 1; d < ROW_LANES; d <<= 1) most = fmaxf(most, __shfl_xor_sync(mask, most, d));
-        append(0, end_q, min(end_k, stop), exponent_for(fminf(most * ROW_REACH * a.magnitude, 61440.0f)), [&](Pairs& p) { apply(turn, at.turns, p); });
+        append(0, end_q, min(end_k, stop), exponent_for(fminf(most * ROW_REACH * a.longest, 61440.0f)), [&](Pairs& p) { apply(turn, at.turns, p); });
     }
     append(1, end_k, stop, exponent_for(ROW_REACH), [](Pairs&) {});
 }
@@ -343,7 +345,8 @@ int launch_qkv_norm_rope_append_blocks(const LaunchArgs& a)
     const uint32_t rows = n_q + 2 * n_kv;
     PreArgs k{(const __half*)a.b[0].ptr, (const __half*)a.b[3].ptr, (const __half*)a.b[4].ptr, (const float*)a.b[1].ptr, (const float*)a.b[5].ptr, (const float2*)a.b[6].ptr,
               (const uint32_t*)a.b[7].ptr, (__half*)a.b[2].ptr, {(uint8_t*)a.b[8].ptr, (uint8_t*)a.b[10].ptr}, {(int8_t*)a.b[9].ptr, (int8_t*)a.b[11].ptr},
-              p.q_stride, p.k_stride, p.v_stride, n_q, n_kv, tokens, (uint32_t)blocks, p.rot_dims / 2, p.layout, 0, 0, 0, p.plus_one ? 1.0f : 0.0f, p.magnitude, a.status};
+              p.q_stride, p.k_stride, p.v_stride, n_q, n_kv, tokens, (uint32_t)blocks, p.rot_dims / 2, p.layout, 0, 0, 0, p.plus_one ? 1.0f : 0.0f,
+              p.rot_dims == 128 ? p.magnitude : std::max(p.magnitude, 1.0f), a.status};
     // Groups of a token.  What a group makes for its token costs it as much as two rows, so that as few as give each SM 256 threads to do are best (us, one launch after the
     // other, at 128 | 256 | 512 threads: 512 tokens of 32 q and 16 kv heads 5.0 | 4.4 | 5.5, 440 of them 5.0 | 4.4 | 5.2, 200 3.3 | 3.5 | 4.4); but sixteen rows a group at
     // most: 23931 tokens take 122 with 8, 112 with 16, 116 with 32 of them, about 5000 tokens 31.5, 30.5, 34.7.

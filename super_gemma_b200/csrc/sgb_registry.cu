@@ -204,7 +204,7 @@ const KernelEntry REGISTRY[] = {
      "q f16[N x H x128], q_w f32[128], q_out f16[N x H x128], k f16[N x KV x128], v, k_w f32[128], cos_sin f32[N x rot/2 x2], slots u32[N] (pool rows, 0xffffffff = none: "
      "the token is left out), k_pool e4m3[row/16 x KV x16x128], k_exps i8[row/16 x KV], v_pool, v_exps | push {rot_dims u32 (multiple of 16 up to 128, 0 = none), layout u32 "
      "(as rope_qk_f16), plus_one u32, token strides u32 of q, k, v in values (0 = dense), magnitude f32 (of cos_sin)} | grid [H, KV, N]; q: norm, rotation; k: norm, rotation, "
-     "e4m3 * 2^e, e the least >= -15 with 11.336 max|w| magnitude <= 448 * 2^e; v: weightless norm, e = -5; a tile that the call continues keeps a larger e, a smaller "
+     "e4m3 * 2^e, e the least >= -15 with 11.336 max|w| magnitude <= 448 * 2^e (magnitude counts as 1 at least where rot_dims < 128); v: weightless norm, e = -5; a tile that the call continues keeps a larger e, a smaller "
      "one grows; slots as in kv_append_blocks_e4m3_d128",
      launch_qkv_norm_rope_append_blocks, W(2) | W(8) | W(9) | W(10) | W(11)},
     {"block_norms_f16", {1024, 1, 1}, 7, 20,
