@@ -18,9 +18,11 @@ constexpr uint32_t MOST_ROT = 1024;
 
 // ---- rows of cosines and sines ---------------------------------------------------------------------------------------------------
 // Angles are counted in turns, as 64-bit fractions of one: F = f / 2 pi mod 1 in units of 2^-64, made of the f64 frequency and 1 / 2 pi in two f64 (hi + lo),
-// so that the whole turns of p F fall off by themselves and the upper word is good to 2^-32 of a turn for every 32-bit p.  Its nearest quarter turn goes into signs and
-// an exchange of sine and cosine, the rest, an eighth of a turn at most, into their Taylor series up to x^9 and x^10 (cut off below 2 * 10^-9).
-// Integers instead of f64 sums and reductions: those kept the units that convert between formats busy, 5.8 us for 32768 rows of 64 pairs where these take 3.4 (launches side by side; 4.3 one after the other).
+// so that the whole turns of p F fall off by themselves for every 32-bit p.  The nearest quarter turn goes into signs and an exchange of sine and cosine, the rest, an
+// eighth of a turn at most, into their Taylor series up to x^9 and x^10 (cut off below 2 * 10^-9).  The rest becomes an f32 number with the digits of both of its words: the upper one alone is
+// good to 2^-32 of a turn, which is 10^-3 of the sine of a slow pair (theta 1e6) in the first tokens.
+// Integers instead of f64 sums and reductions: those kept the units that convert between formats busy, 5.8 us for 32768 rows of 64 pairs where these took 3.4 (launches side by side; 4.3 one after the
+// other, 4.5 since the lower words count too).
 // A thread makes two pairs (16 bytes) of ROWS tokens.
 constexpr double INV_2PI_HI = 0.15915494309189535, INV_2PI_LO = -9.839338337591243e-18;
 
@@ -29,12 +31,16 @@ __device__ __forceinline__ uint64_t fraction_of_turn(double f)
     const double hi = f * INV_2PI_HI, lo = fma(f, INV_2PI_HI, -hi) + f * INV_2PI_LO, unit = 18446744073709551616.0;
     return (uint64_t)__double2ll_rn((hi - rint(hi)) * unit) + (uint64_t)__double2ll_rn(lo * unit);
 }
-// Cosines and sines of two angles of t 2^-32 turns each, times m.
-__device__ __forceinline__ float4 cos_sin_of(uint32_t t0, uint32_t t1, float2 m)
+// Cosines and sines of two angles of t 2^-64 turns each, times m.
+__device__ __forceinline__ float4 cos_sin_of(uint64_t t0, uint64_t t1, float2 m)
 {
-    const uint32_t quarter[2] = {(t0 + 0x20000000u) >> 30, (t1 + 0x20000000u) >> 30};
+    const uint32_t upper[2] = {(uint32_t)(t0 >> 32), (uint32_t)(t1 >> 32)};
+    const uint32_t quarter[2] = {(upper[0] + 0x20000000u) >> 30, (upper[1] + 0x20000000u) >> 30};
+    // what lies beyond the quarter, in 2^-32 turns: the upper word less 1, and 1 to 2 with the lower word's first 23 bits behind the point
+    const float2 whole = make_float2((float)(int)(upper[0] - (quarter[0] << 30) - 1), (float)(int)(upper[1] - (quarter[1] << 30) - 1));
+    const float2 part = make_float2(__uint_as_float(__funnelshift_r((uint32_t)t0, 0x7f, 9)), __uint_as_float(__funnelshift_r((uint32_t)t1, 0x7f, 9)));
     const float radian = 1.4629180792671596e-9f;  // 2 pi 2^-32
-    const float2 x = make_float2((float)(int)(t0 - (quarter[0] << 30)) * radian, (float)(int)(t1 - (quarter[1] << 30)) * radian), z = mul2_rn(x, x);
+    const float2 x = mul2_rn(add2_rn(whole, part), make_float2(radian, radian)), z = mul2_rn(x, x);
     const auto both = [](float v) { return make_float2(v, v); };
     float2 c = both(-1.0f / 3628800.0f), s = both(1.0f / 362880.0f);
     c = fma2_rn(c, z, both(1.0f / 40320.0f));
@@ -77,9 +83,8 @@ __global__ void __launch_bounds__(ROW_THREADS) rope_cos_sin_kernel(const double*
     for (int i = 0; i < ROWS; i++) {
         const uint64_t t = first + i * rows_here;
         if (t >= tokens) return;
-        // the upper word of p F, p counted as signed: sign and all fall off above 2^64 but for p's high word, all ones where it is negative
-        const auto upper = [&](uint64_t F) { return (uint32_t)((p[i] * F) >> 32) - ((int)p[i] < 0 ? (uint32_t)F : 0u); };
-        cos_sin[t * per_row + at] = cos_sin_of(upper(turn[0]), upper(turn[1]), m);
+        const uint64_t turns = (uint64_t)(int64_t)(int)p[i];  // a negative position's sign falls off above 2^64 too
+        cos_sin[t * per_row + at] = cos_sin_of(turns * turn[0], turns * turn[1], m);
     }
 }
 

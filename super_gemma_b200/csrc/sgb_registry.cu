@@ -193,7 +193,7 @@ const KernelEntry REGISTRY[] = {
     // ---- what stands around the attention of a batch, for its packed tokens ----------------------------------------------------------
     {"rope_cos_sin", {256, 1, 1}, 3, 8,
      "freqs f64[rot/2] (radians a position: sgb_rope_frequencies), positions i32[N], cos_sin f32[N x rot/2 x2] | push {rot_dims u32 (multiple of 16 up to 1024), "
-     "magnitude f32} | grid [N]; cos_sin = magnitude * (cos, sin)(position * freq), angles in 64 bits; a negative position turns back",
+     "magnitude f32} | grid [N]; cos_sin = magnitude * (cos, sin)(position * freq), angles in 64 bits (fractions of a turn), cosine and sine from an f32 eighth of a turn; a negative position turns back",
      launch_rope_cos_sin, W(2)},
     {"rope_qk_f16", {256, 1, 1}, 5, 28,
      "q f16[N x H x head_dim], k f16[N x KV x head_dim], cos_sin f32[N x rot/2 x2], q_out, k_out (may be q and k) | push {head_dim u32, rot_dims u32, layout u32 "
