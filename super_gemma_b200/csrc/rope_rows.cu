@@ -206,6 +206,8 @@ int launch_rope_cos_sin(const LaunchArgs& a)
     if (int r = need_bytes(a, 1, 4 * (size_t)tokens, "positions")) return r;
     if (int r = need_bytes(a, 2, 4 * (size_t)tokens * p.rot_dims, "cos_sin")) return r;
     if (int r = need_aligned(a, {8, 4, 16})) return r;
+    const size_t rows = 4 * (size_t)tokens * p.rot_dims;
+    if (int r = need_apart(a, "rope_cos_sin", 2, "cos_sin", rows, rows, 1, {{0, 4 * (size_t)p.rot_dims, "frequencies"}, {1, 4 * (size_t)tokens, "positions"}})) return r;
     const uint32_t per_row = p.rot_dims / 4, rows_here = ROW_THREADS / per_row;
     const bool many = (uint64_t)tokens * per_row > 2048ull * a.sm_count;  // (ROWS 8 | 4 | 1, 32768 rows of 64 pairs: 4.2 | 4.2 | 6.2 us)
     const uint32_t each = rows_here * (many ? 8 : 1);
@@ -249,6 +251,8 @@ int launch_rope_qk_f16(const LaunchArgs& a)
         in_place = in_place && (same || heads[i] == 0);
     }
     if (meet(2, 3)) return fail_validation(a, "rope_qk: q_out and k_out overlap");
+    for (int i = 2; i < 4; i++)
+        if (int r = need_apart(a, "rope_qk", at[i], names[i], 2 * (size_t)p.stride[i], 2 * (size_t)heads[i & 1] * p.head_dim, tokens, {{2, 4 * (size_t)tokens * p.rot_dims, "cos_sin"}})) return r;
     RotateArgs k{{(const __half*)a.b[0].ptr, (const __half*)a.b[1].ptr}, {(__half*)a.b[3].ptr, (__half*)a.b[4].ptr}, {p.stride[0], p.stride[1]}, {p.stride[2], p.stride[3]},
                  {heads[0], heads[1]}, (const float2*)a.b[2].ptr, tokens, p.head_dim, p.rot_dims / 2, p.layout, 0, 0};
     k.pieces = (in_place ? p.rot_dims : p.head_dim) / 16;  // in place, what does not turn is not touched: a layout's turning pieces come first

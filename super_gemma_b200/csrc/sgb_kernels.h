@@ -54,6 +54,14 @@ int need_aligned(const LaunchArgs& a, std::initializer_list<uint32_t> bytes);
 // Whether two tensors of `n` rows share a byte: rows of `wa` and `wb` bytes, `sa` and `sb` apart (with unequal distances: whether their spans do).
 bool rows_meet(const void* pa, size_t sa, size_t wa, const void* pb, size_t sb, size_t wb, size_t n);
 
+// `n` rows of `width` bytes, `step` apart, of binding `at` share no byte with the first `bytes` of any of the others.
+struct Other {
+    int binding;
+    size_t bytes;
+    const char* name;
+};
+int need_apart(const LaunchArgs& a, const char* kernel, int at, const char* name, size_t step, size_t width, size_t n, std::initializer_list<Other> others);
+
 // Tensor-map encoder resolved at run time through the CUDA runtime (no link-time libcuda).
 // dims/strides innermost first; strides[i] is the byte stride of dimension i+1.
 int encode_tensor_map(const LaunchArgs& a, void* out_map /*CUtensorMap*/, int elem_kind /*0 = u8, 1 = f16*/, int rank,

@@ -85,6 +85,18 @@ bool rows_meet(const void* pa, size_t sa, size_t wa, const void* pb, size_t sb, 
     return off < wa || sa - off < wb;
 }
 
+int need_apart(const LaunchArgs& a, const char* kernel, int at, const char* name, size_t step, size_t width, size_t n, std::initializer_list<Other> others)
+{
+    const uintptr_t first = reinterpret_cast<uintptr_t>(a.b[at].ptr);
+    for (const Other& o : others) {
+        const uintptr_t b = reinterpret_cast<uintptr_t>(a.b[o.binding].ptr);
+        if (width == 0 || n == 0 || o.bytes == 0) continue;
+        const size_t row = b < first + width ? 0 : (b - first - width) / step + 1;  // the first one that ends behind b
+        if (row < n && first + row * step < b + o.bytes) return fail_validation(a, std::string(kernel) + ": " + name + " overlaps " + o.name);
+    }
+    return SGB_OK;
+}
+
 // cuTensorMapEncodeTiled, looked up through the runtime so the library has no link-time
 // dependency on libcuda (it must load, and export its symbols, on a machine without a driver).
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,

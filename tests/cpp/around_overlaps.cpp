@@ -1,0 +1,94 @@
+// Calls of the launchers around the batched attention in which something that is written shares memory with something else.  The first part asks the comparison itself;
+// every call behind it differs from a good one in the place of one binding and has to be refused (SGB_ERR_VALIDATION, 3) before a device is touched.  No good call is
+// made: its tensors are no memory.
+#include <cstdio>
+#include <cstring>
+#include <string>
+#include <vector>
+
+#include "sgb_kernels.h"
+
+using namespace sgb;
+
+static int failures = 0, calls = 0;
+
+struct Call {
+    std::vector<BufView> b;
+    std::vector<uint32_t> push;
+    uint32_t groups[3];
+    LaunchFn fn;
+    // binding i moved onto the last byte of the `bytes` at binding j (down to a multiple of 16), and onto its first
+    void refused(int i, int j, size_t bytes, const char* text) const
+    {
+        for (size_t off : {(bytes - 1) / 16 * 16, (size_t)0}) {
+            Call c = *this;
+            c.b[i].ptr = (char*)b[j].ptr + off;
+            std::string err;
+            uint64_t launches = 0;
+            LaunchArgs a{nullptr, c.b.data(), c.push.data(), {groups[0], groups[1], groups[2]}, nullptr, 148, 0, &err, &launches};
+            const int r = fn(a);
+            calls++;
+            if (r != 3 || launches != 0 || err.find("overlap") == std::string::npos || err.find(text) == std::string::npos) {
+                printf("%d on %d: returned %d, %llu launches, \"%s\", not \"%s\"\n", i, j, r, (unsigned long long)launches, err.c_str(), text);
+                failures++;
+            }
+        }
+    }
+};
+
+static uint32_t bits(float f)
+{
+    uint32_t u;
+    memcpy(&u, &f, 4);
+    return u;
+}
+static size_t next = 0x100000;
+static BufView at(size_t bytes)
+{
+    const size_t p = next;
+    next += (bytes + 4095) / 4096 * 4096 * 4;
+    return BufView{(void*)p, bytes};
+}
+
+static void comparison()
+{
+    // 3 rows of 32 bytes, 100 apart, against every stretch of 1, 7 or 150 bytes around them, byte by byte
+    std::string err;
+    for (size_t bytes : {0, 1, 7, 150})
+        for (size_t p = 700; p < 1400; p++) {
+            bool meets = false;
+            for (size_t row = 0; row < 3; row++)
+                for (size_t x = 1000 + 100 * row; x < 1032 + 100 * row; x++) meets = meets || (x >= p && x < p + bytes);
+            const BufView b[2] = {{(void*)1000, 232}, {(void*)p, bytes}};
+            LaunchArgs a{nullptr, b, nullptr, {1, 1, 1}, nullptr, 148, 0, &err, nullptr};
+            calls++;
+            if ((need_apart(a, "k", 0, "out", 100, 32, 3, {{1, bytes, "in"}}) != 0) != meets) failures++, printf("rows against %zu bytes at %zu\n", bytes, p);
+            if (need_apart(a, "k", 0, "out", 100, 32, 0, {{1, bytes, "in"}}) != 0 || need_apart(a, "k", 0, "out", 100, 0, 3, {{1, bytes, "in"}}) != 0) failures++, printf("nothing overlaps\n");
+        }
+}
+
+static void rope()
+{
+    // 5 tokens, 48 dims that turn
+    const Call angles{{at(24 * 8), at(20), at(5 * 48 * 4)}, {48, bits(1.0f)}, {5, 1, 1}, launch_rope_cos_sin};
+    angles.refused(2, 0, 24 * 8, "frequencies");
+    angles.refused(2, 1, 20, "positions");
+    angles.refused(0, 2, 5 * 48 * 4, "frequencies");
+    angles.refused(1, 2, 5 * 48 * 4, "positions");
+
+    // 5 tokens, 6 and 2 heads of 80 dims, 48 of them turn; outputs with room behind a token's heads, which cos_sin may not begin in either as it is longer
+    const Call rotate{{at(5 * 640 * 2), at(4 * 640 * 2 + 320), at(5 * 48 * 4), at(5 * 500 * 2), at(5 * 168 * 2)}, {80, 48, 1, 640, 640, 488, 168}, {6, 2, 5}, launch_rope_qk_f16};
+    rotate.refused(2, 3, (4 * 488 + 480) * 2, "q_out overlaps cos_sin");
+    rotate.refused(2, 4, (4 * 168 + 160) * 2, "k_out overlaps cos_sin");
+    rotate.refused(3, 2, 5 * 48 * 4, "q_out overlaps cos_sin");
+    rotate.refused(4, 2, 5 * 48 * 4, "k_out overlaps cos_sin");
+}
+
+int main()
+{
+    comparison();
+    rope();
+    if (failures) return 1;
+    printf("%d comparisons and calls as they should be\n", calls);
+    return 0;
+}

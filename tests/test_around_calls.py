@@ -44,3 +44,17 @@ def test_groups_of_any_kind(sg):
         for groups in (words, tuple(words), np.array(words), iter(words), (w for w in words)):
             ctx._dispatch(dispatch, kernel, [], None, groups)
             assert seen.pop() == want, (words, type(groups))
+
+
+def test_overlaps_that_are_refused(sg, tmp_path):
+    import os
+    import subprocess
+
+    from super_gemma_b200 import build
+
+    root, lib, exe = os.path.dirname(os.path.dirname(os.path.abspath(__file__))), build.build(), str(tmp_path / "overlaps")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(build._nvcc())), "include")
+    subprocess.run(["g++", "-std=c++17", "-I", cuda, "-I", os.path.join(root, "super_gemma_b200", "csrc"), os.path.join(root, "tests", "cpp", "around_overlaps.cpp"),
+                    lib, "-Wl,-rpath," + os.path.dirname(lib), "-o", exe], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout + r.stderr
