@@ -342,6 +342,18 @@ int launch_qkv_norm_rope_append_blocks(const LaunchArgs& a)
     if (int r = need_bytes(a, 9, blocks * n_kv, "k exponents")) return r;
     if (int r = need_bytes(a, 11, blocks * n_kv, "v exponents")) return r;
     if (int r = need_aligned(a, {16, 16, 16, 16, 16, 16, 16, 4, 16, 1, 16, 1})) return r;
+    // nothing else that is written stands over anything else either
+    const char* kernel = "qkv_append_blocks";
+    const Other q_w{1, 512, "q_w"}, k_w{5, 512, "k_w"}, cos_sin{6, 4 * (size_t)tokens * p.rot_dims, "cos_sin"}, slots{7, 4 * (size_t)tokens, "slots"}, k_pool{8, blocks * tile_row, "k pool"},
+        k_exps{9, blocks * n_kv, "k exponents"}, v_pool{10, blocks * tile_row, "v pool"}, v_exps{11, blocks * n_kv, "v exponents"};
+    const auto dense = [&](const Other& out, std::initializer_list<Other> others) { return need_apart(a, kernel, out.binding, out.name, out.bytes, out.bytes, 1, others); };
+    if (int r = dense({2, 256 * (size_t)tokens * n_q, "q_out"}, {q_w, k_w, cos_sin, slots, k_pool, k_exps, v_pool, v_exps})) return r;
+    for (int i = 0; i < 3; i++)
+        if (int r = need_apart(a, kernel, at[i], names[i], 2 * (size_t)*strides[i], 256 * (size_t)heads[i], tokens, {k_pool, k_exps, v_pool, v_exps})) return r;
+    if (int r = dense(k_pool, {q_w, k_w, cos_sin, slots, k_exps, v_pool, v_exps})) return r;
+    if (int r = dense(v_pool, {q_w, k_w, cos_sin, slots, k_exps, v_exps})) return r;
+    if (int r = dense(k_exps, {q_w, k_w, cos_sin, slots, v_exps})) return r;
+    if (int r = dense(v_exps, {q_w, k_w, cos_sin, slots})) return r;
     const uint32_t rows = n_q + 2 * n_kv;
     PreArgs k{(const __half*)a.b[0].ptr, (const __half*)a.b[3].ptr, (const __half*)a.b[4].ptr, (const float*)a.b[1].ptr, (const float*)a.b[5].ptr, (const float2*)a.b[6].ptr,
               (const uint32_t*)a.b[7].ptr, (__half*)a.b[2].ptr, {(uint8_t*)a.b[8].ptr, (uint8_t*)a.b[10].ptr}, {(int8_t*)a.b[9].ptr, (int8_t*)a.b[11].ptr},

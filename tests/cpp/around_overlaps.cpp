@@ -84,10 +84,29 @@ static void rope()
     rotate.refused(4, 2, 5 * 48 * 4, "k_out overlaps cos_sin");
 }
 
+static void pre_attention()
+{
+    // 5 tokens, 6 and 3 heads, 4 blocks, rows of 12 * 128 side by side
+    const size_t pool = 4 * 3 * 2048, q_out = 5 * 6 * 256;
+    const uint32_t row = 12 * 128;
+    const Call pre{{at((4 * row + 768) * 2), at(512), at(q_out), at((4 * row + 384) * 2), at((4 * row + 384) * 2), at(512), at(5 * 64 * 4), at(20), at(pool), at(12), at(pool), at(12)},
+                   {64, 0, 0, row, row, row, bits(1.0f)}, {6, 3, 5}, launch_qkv_norm_rope_append_blocks};
+    const size_t sizes[12] = {(4 * row + 768) * 2, 512, q_out, (4 * row + 384) * 2, (4 * row + 384) * 2, 512, 5 * 64 * 4, 20, pool, 12, pool, 12};
+    const char* names[12] = {"q", "q_w", "q_out", "k", "v", "k_w", "cos_sin", "slots", "k pool", "k exponents", "v pool", "v exponents"};
+    for (int out : {2, 8, 9, 10, 11})
+        for (int in = 0; in < 12; in++) {
+            if (in == out) continue;
+            pre.refused(in, out, sizes[out], names[in]);
+            // an output onto what is read, or onto another output; a 12-byte one may stand between the rows of q, k and v
+            if (out != 9 && out != 11) pre.refused(out, in, sizes[in], names[out]);
+        }
+}
+
 int main()
 {
     comparison();
     rope();
+    pre_attention();
     if (failures) return 1;
     printf("%d comparisons and calls as they should be\n", calls);
     return 0;
