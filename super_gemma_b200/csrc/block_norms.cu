@@ -543,6 +543,10 @@ int launch_block_norms(const LaunchArgs& a)
     if (block && a.b[1].ptr != a.b[5].ptr && meet(1, R_BYTES, 5, R_BYTES)) return fail_validation(a, "block_norms: h_out overlaps h and is not h");
     if (block && a.b[0].ptr != a.b[6].ptr && meet(0, 2, 6, 2)) return fail_validation(a, "block_norms: x overlaps y and is not y");
     if (meet(1, R_BYTES, 6, 2) || (block && (meet(0, 2, 5, R_BYTES) || meet(5, R_BYTES, 6, 2)))) return fail_validation(a, "block_norms: x or h_out overlaps another tensor");
+    const Other w_post{2, p.post == POST_NORM ? 4 * (size_t)hidden : 0, "w_post"}, gates{3, 4 * gate, "gate"}, w_pre{4, 4 * (size_t)hidden, "w_pre"};
+    if (block)
+        if (int r = need_apart(a, "block_norms", 5, "h_out", sizeof(R) * n, sizeof(R) * n, 1, {w_post, gates, w_pre})) return r;
+    if (int r = need_apart(a, "block_norms", 6, "x", 2 * n, 2 * n, 1, {w_post, gates, w_pre})) return r;
     const uint32_t units = hidden / U;
     NormsArgs k{(const __half*)a.b[0].ptr, a.b[1].ptr, (const float*)a.b[2].ptr, (const float*)a.b[3].ptr, (const float*)a.b[4].ptr, a.b[5].ptr, (__half*)a.b[6].ptr,
                 rows, hidden, 1, p.post, p.gates, p.plus_one ? 1.0f : 0.0f, p.scale, p.eps};

@@ -1,8 +1,11 @@
 // Calls of the launchers around the batched attention in which something that is written shares memory with something else.  The first part asks the comparison itself;
 // every call behind it differs from a good one in the place of one binding and has to be refused (SGB_ERR_VALIDATION, 3) before a device is touched.  No good call is
 // made: its tensors are no memory.
+#include <cuda_bf16.h>
+
 #include <cstdio>
 #include <cstring>
+#include <functional>
 #include <string>
 #include <vector>
 
@@ -48,6 +51,11 @@ static BufView at(size_t bytes)
     const size_t p = next;
     next += (bytes + 4095) / 4096 * 4096 * 4;
     return BufView{(void*)p, bytes};
+}
+static Call with(Call c, const std::function<void(Call&)>& change)
+{
+    change(c);
+    return c;
 }
 
 static void comparison()
@@ -102,11 +110,30 @@ static void pre_attention()
         }
 }
 
+static void norms()
+{
+    for (int type = 0; type < 3; type++) {
+        // 5 rows of 40
+        const size_t n = 200, size = type == 2 ? 4 : 2;
+        const Call block{{at(2 * n), at(size * n), at(160), at(160), at(160), at(size * n), at(2 * n)}, {1, 1, 0, bits(0.5f), bits(1e-6f)}, {40, 5, 1},
+                         type == 0 ? launch_block_norms<__half> : type == 1 ? launch_block_norms<__nv_bfloat16> : launch_block_norms<float>};
+        for (int out : {5, 6})
+            for (int w : {2, 3, 4}) {
+                block.refused(w, out, out == 5 ? size * n : 2 * n, w == 2 ? "w_post" : w == 3 ? "gate" : "w_pre");
+                block.refused(out, w, 160, out == 5 ? "h_out" : "x");
+            }
+        with(block, [](Call& c) { c.push[1] = 2; }).refused(3, 6, 2 * n, "gate");
+        with(block, [](Call& c) { c.push[1] = 3; }).refused(3, 5, size * n, "gate");
+        with(block, [](Call& c) { c.push[0] = 2; c.push[1] = 0; c.push[3] = bits(1.0f); }).refused(4, 6, 2 * n, "w_pre");
+    }
+}
+
 int main()
 {
     comparison();
     rope();
     pre_attention();
+    norms();
     if (failures) return 1;
     printf("%d comparisons and calls as they should be\n", calls);
     return 0;
