@@ -122,6 +122,12 @@ int launch_kv_read_blocks(const LaunchArgs& a)
     if (int r = need_bytes(a, 7, 256 * (size_t)tokens * n_kv, "k")) return r;
     if (int r = need_bytes(a, 8, 256 * (size_t)tokens * n_kv, "v")) return r;
     if (int r = need_aligned(a, {16, 1, 16, 1, 4, 4, 4, 16, 16})) return r;
+    const size_t out = 256 * (size_t)tokens * n_kv;
+    for (int i = 7; i < 9; i++)
+        if (int r = need_apart(a, "read_blocks", i, i == 7 ? "k" : "v", out, out, 1,
+                               {{0, blocks * tile_row, "k pool"}, {1, blocks * n_kv, "k exponents"}, {2, blocks * tile_row, "v pool"}, {3, blocks * n_kv, "v exponents"},
+                                {4, 4 * (size_t)n * p.stride, "table"}, {5, 4 * (size_t)n, "from"}, {6, 4 * (size_t)n + 4, "starts"}, {8, i == 7 ? out : 0, "v"}}))
+            return r;
     ReadArgs k{{(const uint8_t*)a.b[0].ptr, (const uint8_t*)a.b[2].ptr}, {(const int8_t*)a.b[1].ptr, (const int8_t*)a.b[3].ptr}, (const uint32_t*)a.b[4].ptr,
                (const uint32_t*)a.b[5].ptr, (const uint32_t*)a.b[6].ptr, {(__half*)a.b[7].ptr, (__half*)a.b[8].ptr}, n, tokens, n_kv, p.stride,
                (uint32_t)__builtin_ctz(p.page), (uint32_t)blocks, a.status};

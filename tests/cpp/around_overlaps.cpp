@@ -128,12 +128,27 @@ static void norms()
     }
 }
 
+static void read()
+{
+    // 3 kv heads, 2 requests, 5 rows, pages of 16, stride 2
+    const size_t pool = 4 * 3 * 2048, sizes[9] = {pool, 12, pool, 12, 16, 8, 12, 5 * 768, 5 * 768};
+    const Call back{{at(pool), at(12), at(pool), at(12), at(16), at(8), at(12), at(5 * 768), at(5 * 768)}, {16, 2}, {3, 2, 5}, launch_kv_read_blocks};
+    const char* names[9] = {"k pool", "k exponents", "v pool", "v exponents", "table", "from", "starts", "k", "v"};
+    for (int out : {7, 8})
+        for (int in = 0; in < 9; in++) {
+            if (in == out) continue;
+            back.refused(in, out, sizes[out], names[in]);
+            back.refused(out, in, sizes[in], names[out]);
+        }
+}
+
 int main()
 {
     comparison();
     rope();
     pre_attention();
     norms();
+    read();
     if (failures) return 1;
     printf("%d comparisons and calls as they should be\n", calls);
     return 0;
