@@ -341,7 +341,7 @@ int launch_qkv_norm_rope_append_blocks(const LaunchArgs& a)
     if (blocks > NO_SLOT / TILE_TOK) return fail_validation(a, "qkv_append_blocks: a pool holds less than 2^32 rows");
     if (int r = need_bytes(a, 9, blocks * n_kv, "k exponents")) return r;
     if (int r = need_bytes(a, 11, blocks * n_kv, "v exponents")) return r;
-    if (int r = need_aligned(a, {16, 16, 16, 16, 16, 16, 16, 4, 16, 1, 16, 1})) return r;
+    if (int r = need_aligned(a, {16, 16, 16, 16, 16, 16, p.rot_dims ? 16u : 1u, 4, 16, 1, 16, 1})) return r;
     // nothing else that is written stands over anything else either
     const char* kernel = "qkv_append_blocks";
     const Other q_w{1, 512, "q_w"}, k_w{5, 512, "k_w"}, cos_sin{6, 4 * (size_t)tokens * p.rot_dims, "cos_sin"}, slots{7, 4 * (size_t)tokens, "slots"}, k_pool{8, blocks * tile_row, "k pool"},

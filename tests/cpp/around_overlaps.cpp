@@ -108,6 +108,9 @@ static void pre_attention()
             // an output onto what is read, or onto another output; a 12-byte one may stand between the rows of q, k and v
             if (out != 9 && out != 11) pre.refused(out, in, sizes[in], names[out]);
         }
+    // where nothing turns, cos_sin is not looked at: what is refused here is the overlap
+    with(pre, [](Call& c) { c.push[0] = 0; c.b[6].ptr = (char*)c.b[6].ptr + 4; }).refused(1, 2, q_out, "q_w");
+    with(pre, [&](Call& c) { c.push[0] = 0; c.b[6] = c.b[2]; }).refused(1, 2, q_out, "q_w");
 }
 
 static void norms()
