@@ -208,8 +208,9 @@ __device__ __forceinline__ void write_next(__half* x, const float2 (&v)[UNIT<R> 
 // Three units of 16-bit values: two CTAs of twelve warps an SM, 80 registers instead of 98 (400 rows of 5376 4.6 us, else 5.7).
 template <typename R, int N>
 constexpr bool TIGHT = sizeof(R) == 2 && N == 3;
+constexpr uint32_t TIGHT_LANES = 384;  // (norms_shape keeps to it)
 template <typename R, int N>
-__global__ void __launch_bounds__(TIGHT<R, N> ? 384 : 512, TIGHT<R, N> ? 2 : 0) block_norms_kernel(const __grid_constant__ NormsArgs a)
+__global__ void __launch_bounds__(TIGHT<R, N> ? TIGHT_LANES : 512, TIGHT<R, N> ? 2 : 0) block_norms_kernel(const __grid_constant__ NormsArgs a)
 {
     constexpr int U = UNIT<R>, P = U / 2;
     __shared__ alignas(16) float parts[2][MOST_WARPS];
@@ -449,13 +450,15 @@ struct NormsShape {
     uint32_t lanes, each;  // of a row; units of a lane
 };
 // Eight lanes to sixteen warps a row and at most `most` units a lane, so that a row takes the fewest instructions: about 45 a unit, full or not, and 110 for the two sums.
+template <typename R>
 NormsShape norms_shape(uint32_t units, uint32_t most)
 {
     NormsShape s{0, 0};
     uint32_t least = ~0u;
     const auto look = [&](uint32_t lanes) {
         const uint32_t each = (units + lanes - 1) / lanes, cost = lanes * (each * 45 + 110);
-        if (each <= most && cost < least) s = {lanes, each}, least = cost;
+        if ((sizeof(R) == 2 && each == 3 && lanes > TIGHT_LANES) || each > most) return;
+        if (cost < least) s = {lanes, each}, least = cost;
     };
     for (uint32_t lanes = units < 8 ? 1 : 8; lanes < 32; lanes *= 2) look(lanes);
     for (uint32_t warps = 1; warps <= MOST_WARPS; warps++) look(32 * warps);
@@ -555,11 +558,11 @@ int launch_block_norms(const LaunchArgs& a)
     // 102.6 | 89 to 90 | 96.1, 30011 of 1096 70.7 | 68.0 | 74.5, 800 of 5376 13.7 | 14.0; bf16, 30011 of 1096 51.0 | 44.5 | 48.0; f16, 6000 of 5376 54.8 | 49.0 | 45.5, 100000 of 264 46.4 | 48.5 | 40.6, 3000 of 8192
     // 44.1 | 45.4 | 36.5.
     const bool many = (uint64_t)n * (4 + 2 * R_BYTES) >= 80ull << 20, warp_holds = units > 64 && units <= 192;
-    NormsShape shape = norms_shape(units, std::min(4u, (hidden + 2047) / 2048));
+    NormsShape shape = norms_shape<R>(units, std::min(4u, (hidden + 2047) / 2048));
     Way way = Way::EARLY;
     if ((uint64_t)rows * shape.lanes > 1024ull * a.sm_count) {
         way = U == 4 || (many && warp_holds) ? Way::LATE : many ? Way::STREAM : Way::EARLY;
-        shape = norms_shape(units, U == 4 ? 3 : warp_holds ? 6 : MOST_STREAMED);
+        shape = norms_shape<R>(units, U == 4 ? 3 : warp_holds ? 6 : MOST_STREAMED);
     }
     k.lanes = shape.lanes;
     int e = 0;
