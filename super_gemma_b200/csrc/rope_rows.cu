@@ -209,7 +209,7 @@ int launch_rope_cos_sin(const LaunchArgs& a)
     const size_t rows = 4 * (size_t)tokens * p.rot_dims;
     if (int r = need_apart(a, "rope_cos_sin", 2, "cos_sin", rows, rows, 1, {{0, 4 * (size_t)p.rot_dims, "frequencies"}, {1, 4 * (size_t)tokens, "positions"}})) return r;
     const uint32_t per_row = p.rot_dims / 4, rows_here = ROW_THREADS / per_row;
-    const bool many = (uint64_t)tokens * per_row > 2048ull * a.sm_count;  // (ROWS 8 | 4 | 1, 32768 rows of 64 pairs: 4.2 | 4.2 | 6.2 us)
+    const bool many = (uint64_t)tokens * per_row > 2048ull * a.sm_count;  // (ROWS 8 | 4 | 1, 20000 rows of 64 pairs: 4.4 | 3.7 us, 32768 4.5 | 4.2 | 6.2, 62500 7.5 | 7.9)
     const uint32_t each = rows_here * (many ? 8 : 1);
     const cudaError_t e = launch_dependent(many ? rope_cos_sin_kernel<8> : rope_cos_sin_kernel<1>, dim3((tokens + each - 1ull) / each), dim3(ROW_THREADS), 0, a.stream,
                                            (const double*)a.b[0].ptr, (const int*)a.b[1].ptr, (float4*)a.b[2].ptr, p.magnitude, tokens, per_row, rows_here);
